@@ -1,6 +1,6 @@
 /*
  * laplacianformer_amd.h - C ABI of the MI355X (gfx950) LaplaceSubtraction and
- * NewtonInverse operators.
+ * NewtonInverse operators, and of the transformer-block operators beside them.
  *
  * Every entry point takes plain device pointers, sizes and a HIP stream
  * (passed as void*, a hipStream_t; NULL means the null stream). Nothing here
@@ -297,6 +297,107 @@ int lfamd_landmark_pool(int dtype, const void* k, void* km, void* km_cm, int64_t
 int lfamd_landmark_pool_backward(int dtype, void* dk, const void* dkm, const void* dcm0, const void* dcm1,
                                  const void* dcm2, int64_t B, int64_t H, int gh, int gw, int pool, int d,
                                  void* stream);
+
+/* ---- Transformer-block operators ---------------------------------------- */
+
+/* What stands around the attention in a transformer block, and exact softmax
+ * attention for the stages whose tokens are few enough for it. No reference
+ * counterparts (the reference ships the two operators above only). Element types
+ * F32, F16 and BF16 (LFAMD_ERR_DTYPE for F64); arithmetic and statistics in fp32. */
+
+/* sum = x + residual (stored with one rounding; residual and sum NULL: sum is x),
+ * rstd = 1 / sqrt(mean(sum^2) + eps) over each row's fp32 sum, y = sum * rstd * weight.
+ * x and residual [rows][width] with rows x_stride / residual_stride elements apart, y and
+ * sum contiguous, weight [width] of type w_dtype (dtype or F32), rstd [rows] fp32 or NULL
+ * (the backward reads it). 1 <= width <= 16384 (LFAMD_ERR_UNSUPPORTED beyond). */
+int lfamd_add_rms_norm(int dtype, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                       int w_dtype, const void* weight, void* y, void* sum, float* rstd, int64_t rows, int64_t width,
+                       float eps, void* stream);
+
+/* The same with y in e4m3 (OCP, largest value 448) and one fp32 scale per row:
+ * scale = max|y| / 448 (1 for a row of zeros), y8 = e4m3(y / scale), to nearest even. */
+int lfamd_add_rms_norm_fp8(int dtype, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                           int w_dtype, const void* weight, void* y, float* scale, void* sum, int64_t rows,
+                           int64_t width, float eps, void* stream);
+
+/* Gradients of lfamd_add_rms_norm: with gn = grad_y * weight and n = sum * rstd,
+ * grad_x = grad_sum + rstd * (gn - n * mean(gn * n)) (the gradient of both addends;
+ * grad_sum NULL: taken as zero), grad_weight = sum over the rows of grad_y * n (type
+ * w_dtype, or NULL to skip it). `sum` is the stored sum, rows sum_stride apart; grad_x is
+ * contiguous. The workspace (4-byte aligned) is needed for grad_weight only. Deterministic. */
+size_t lfamd_add_rms_norm_backward_workspace_size(int dtype, int64_t rows, int64_t width);
+int lfamd_add_rms_norm_backward(int dtype, const void* grad_y, int64_t grad_y_stride, const void* grad_sum,
+                                int64_t grad_sum_stride, const void* sum, int64_t sum_stride, int w_dtype,
+                                const void* weight, const float* rstd, void* grad_x, void* grad_weight, int64_t rows,
+                                int64_t width, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary positions of q [batch][q_heads][tokens][head_dim] and k (k_heads; either may have
+ * no heads) over num_axes <= 8 axes: sections[a] channel pairs belong to axis a, in order;
+ * pair j of axis a turns by position_a * base^(-j / sections[a]); the first 2 * (all pairs)
+ * channels of a head are rotated, the rest copied. Pair p is channels (p, p + pairs), or
+ * (2p, 2p + 1) if interleaved. inverse != 0: by the negative angle (the backward pass).
+ * Strides (elements): batch, head, token, channels adjacent; output may be the input.
+ * positions: int32, or int64 if positions_64, element strides {axis, batch, token}; the
+ * angle is reduced exactly for any position. At most 128 pairs, head_dim <= 1024. */
+int lfamd_rotary(int dtype, const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
+                 int64_t q_heads, const void* k, const int64_t* k_strides, void* k_out, const int64_t* k_out_strides,
+                 int64_t k_heads, int64_t batch, int64_t tokens, int64_t head_dim, const void* positions,
+                 int positions_64, const int64_t* position_strides, int num_axes, const int64_t* sections, double base,
+                 int interleaved, int inverse, void* stream);
+
+/* Masks of lfamd_attention: none, truth values (a byte each, non-zero: attends), or an
+ * additive term of that element type (-inf removes the key). */
+#define LFAMD_MASK_NONE 0
+#define LFAMD_MASK_BOOL 1
+#define LFAMD_MASK_F32 2
+#define LFAMD_MASK_F16 3
+#define LFAMD_MASK_BF16 4
+
+/* One softmax attention: query [batch][heads][q_len][head_dim], key and value
+ * [batch][kv_heads][k_len][head_dim], heads a multiple of kv_heads (query head i reads key
+ * head i / (heads / kv_heads)). Strides in elements for batch, head and row; channels are
+ * adjacent. head_dim <= 128, q_len * heads / kv_heads and k_len <= 2^30.
+ *   k_lengths  [batch] or NULL: keys at or behind it do not take part and are not read
+ *   q_lengths  [batch] or NULL: queries at or behind it are not read, their output is 0
+ *   causal     query n sees keys j <= start + n, start = q_starts[b], or k_len - q_len if NULL
+ *   mask       mask_kind above, strides for batch, head, query, key (0: broadcast); a key
+ *              that it removes for every head and query (both strides 0) is not read
+ *   scale      positive and finite
+ * A query without keys gives 0 and has no gradient. Lengths are clamped to the buffers. */
+typedef struct {
+  int64_t batch, heads, kv_heads, q_len, k_len, head_dim;
+  int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];
+  const int32_t* k_lengths;
+  const int32_t* q_lengths;
+  const int32_t* q_starts;
+  const void* mask;
+  int64_t mask_strides[4];
+  int mask_kind, causal;
+  float scale;
+} lfamd_attention;
+
+/* out[b,h,n,:] = sum_j softmax_j(scale * q.k_j + mask) v_j. stats (fp32, may be NULL): what
+ * the backward reads of each row, batch * heads * q_len values, twice as many with a mask.
+ * The workspace (16-byte aligned; 0 bytes where the rows alone fill the chip) holds fp32
+ * results of key ranges. Deterministic. */
+size_t lfamd_softmax_attention_workspace_size(int dtype, const lfamd_attention* desc);
+int lfamd_softmax_attention(int dtype, const lfamd_attention* desc, const void* q, const void* k, const void* v, void* out,
+                            float* stats, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of q, k and v from the forward's inputs, output and stats; the probabilities are
+ * recomputed. Each gradient has strides of its own; grad_q, or grad_k and grad_v together, may be
+ * NULL. The workspace is 16-byte aligned. Deterministic, without atomics. */
+typedef struct {
+  const void* grad_out;
+  void* grad_q;
+  void* grad_k;
+  void* grad_v;
+  int64_t grad_out_strides[3], grad_q_strides[3], grad_k_strides[3], grad_v_strides[3];
+} lfamd_attention_grads;
+size_t lfamd_softmax_attention_backward_workspace_size(int dtype, const lfamd_attention* desc);
+int lfamd_softmax_attention_backward(int dtype, const lfamd_attention* desc, const void* q, const void* k, const void* v,
+                                     const void* out, const float* stats, const lfamd_attention_grads* grads,
+                                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- Runtime ------------------------------------------------------------ */
 

@@ -26,8 +26,10 @@ EXT_NAME = "Laplace_subtraction_cuda"
 EXT_PATH = os.path.join(PKG_DIR, EXT_NAME + ".so")
 
 HIP_SOURCES = ["laplace_kernels.hip", "laplace_bwd2.hip", "laplace_fwd2.hip", "newton_kernels.hip", "mix_kernels.hip",
-               "layer_kernels.hip", "lf_runtime.hip", "laplace_noalloc.hip"]
-TORCH_SOURCES = ["wrapper.cpp", "LaplaceSubtraction_hip.cpp", "NewtonInverse_hip.cpp", "LaplacianAttention_hip.cpp"]
+               "layer_kernels.hip", "norm_kernels.hip", "rotary_kernels.hip", "attn_fwd.hip", "attn_bwd.hip",
+               "attn_host.hip", "lf_runtime.hip", "laplace_noalloc.hip"]
+TORCH_SOURCES = ["wrapper.cpp", "LaplaceSubtraction_hip.cpp", "NewtonInverse_hip.cpp", "LaplacianAttention_hip.cpp",
+                 "Block_hip.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

@@ -55,10 +55,39 @@ CAPI_PROTOTYPES = [
                                                 _I, _P, _SZ, _P]),
     ("lfamd_landmark_pool", _I, [_I, _P, _P, _P, _I64, _I64, _I, _I, _I, _I, _P]),
     ("lfamd_landmark_pool_backward", _I, [_I, _P, _P, _P, _P, _P, _I64, _I64, _I, _I, _I, _I, _P]),
+    ("lfamd_add_rms_norm", _I, [_I, _P, _I64, _P, _I64, _I, _P, _P, _P, _P, _I64, _I64, ctypes.c_float, _P]),
+    ("lfamd_add_rms_norm_fp8", _I, [_I, _P, _I64, _P, _I64, _I, _P, _P, _P, _P, _I64, _I64, ctypes.c_float, _P]),
+    ("lfamd_add_rms_norm_backward_workspace_size", _SZ, [_I, _I64, _I64]),
+    ("lfamd_add_rms_norm_backward", _I, [_I, _P, _I64, _P, _I64, _P, _I64, _I, _P, _P, _P, _P, _I64, _I64, _P, _SZ,
+                                         _P]),
+    ("lfamd_rotary", _I, [_I, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I, _P, _I, _P,
+                          ctypes.c_double, _I, _I, _P]),
+    ("lfamd_softmax_attention_workspace_size", _SZ, [_I, _P]),
+    ("lfamd_softmax_attention", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    ("lfamd_softmax_attention_backward_workspace_size", _SZ, [_I, _P]),
+    ("lfamd_softmax_attention_backward", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     ("lfamd_runtime_version", _I, []),
     ("lfamd_status_string", ctypes.c_char_p, [_I]),
     ("lfamd_last_error", ctypes.c_char_p, []),
 ]
+
+
+
+class Attention(ctypes.Structure):
+    """lfamd_attention of include/laplacianformer_amd.h."""
+
+    _fields_ = [(n, _I64) for n in ("batch", "heads", "kv_heads", "q_len", "k_len", "head_dim")] + \
+        [(n, _I64 * 3) for n in ("q_strides", "k_strides", "v_strides", "out_strides")] + \
+        [(n, _P) for n in ("k_lengths", "q_lengths", "q_starts", "mask")] + \
+        [("mask_strides", _I64 * 4), ("mask_kind", _I), ("causal", _I), ("scale", ctypes.c_float)]
+
+
+class AttentionGrads(ctypes.Structure):
+    """lfamd_attention_grads of include/laplacianformer_amd.h."""
+
+    _fields_ = [(n, _P) for n in ("grad_out", "grad_q", "grad_k", "grad_v")] + \
+        [(n, _I64 * 3) for n in ("grad_out_strides", "grad_q_strides", "grad_k_strides", "grad_v_strides")]
+
 
 # Element type codes (LFAMD_F32, ...).
 DTYPE_CODES = {"float32": 0, "float16": 1, "bfloat16": 2, "float64": 3}

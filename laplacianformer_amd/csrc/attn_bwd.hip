@@ -1,0 +1,584 @@
+// softmax_attention, backward. With p_ij recomputed from the forward's row statistics,
+//   delta_i = g_i . o_i
+//   dv_j = sum_i p_ij g_i
+//   dz_ij = p_ij (g_i . v_j - delta_i)
+//   dk_j = scale sum_i dz_ij q_i,   dq_i = scale sum_j dz_ij k_j.
+//
+// Two kernels without atomics, each owning its outputs: attn_dkdv_kernel a block of
+// keys (over every query of the heads that share them, so that shared heads' sums
+// need no second pass), attn_dq_kernel a block of queries. The scores and g . v are
+// formed in both: seven products instead of five, and the same bits on every run.
+// Both form the scores with the owned rows as columns, so that p and dz leave the
+// accumulators as the next product's operand (attn_common.h).
+//
+// fp16: dz follows the gradient's magnitude (a scaled loss overflows 65504, a mean
+// over many keys falls below 2^-14), so it is rounded after a multiplication by a power of
+// two f per key head, with |dz| <= |g_i| |v_j| + |delta_i| <= bound and f bound <= 2^14,
+// which the result is divided by; p <= 1 likewise carries 2^15 into the product for
+// dv. bf16 and fp32 have the exponents and take f = 1.
+#include "attn_common.h"
+
+#include <algorithm>
+
+namespace lfamd {
+
+namespace {
+
+constexpr float kPShift = 15.0f;
+
+// Streamed rows per LDS tile, taken in blocks of 32.
+template <typename T, int DP> constexpr int stream_tile() { return sizeof(T) == 2 || DP == 32 ? 64 : 32; }
+
+// delta_i, and for fp16 the maxima over 64 rows of |g_i| and |delta_i|, or over 64
+// keys of |v_j|. A workgroup takes 64 rows of one head: four threads per row.
+template <typename T, bool BOUND>
+__global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
+  constexpr int CE = 16 / (int)sizeof(T);
+  const int qt = (a.N + 63) / 64, kt = (a.M + 63) / 64;
+  const int64_t nq = (int64_t)a.B * a.H * qt;
+  const bool keys = BOUND && blockIdx.x >= nq;
+  const int64_t id = keys ? blockIdx.x - nq : blockIdx.x;
+  const int tiles = keys ? kt : qt, heads = keys ? a.Hk : a.H;
+  const int64_t bh = id / tiles;
+  const int tile = (int)(id % tiles), b = (int)(bh / heads), hd = (int)(bh % heads);
+  const int row = tile * 64 + threadIdx.x / 4, part = threadIdx.x % 4;
+  float dot = 0.0f, sq = 0.0f;
+  if (keys) {
+    const bool in = row < key_count(a, b);
+    const T* p = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hd * a.vs[1] + (int64_t)row * a.vs[2];
+    bool live = in;
+    if (in && a.keyMask) {
+      const int64_t off = (int64_t)b * a.ms[0] + (int64_t)row * a.ms[3];
+      live = a.maskKind == kMaskBool ? ((const uint8_t*)a.mask)[off] != 0 : mask_bias(a, off) != kNegInf;
+    }
+    for (int c = part * CE; c < a.D; c += 4 * CE) {
+      const u32x4 x = load_chunk<T>(p, live, c, a.D, a.vecV);
+#pragma unroll
+      for (int j = 0; j < CE; ++j) {
+        const float v = to_acc(((const T*)&x)[j]);
+        sq = fmaf(v, v, sq);
+      }
+    }
+  } else {
+    const bool in = row < query_count(a, b);
+    const T* po = (const T*)a.o + (int64_t)b * a.os[0] + (int64_t)hd * a.os[1] + (int64_t)row * a.os[2];
+    const T* pg = (const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)hd * a.gs[1] + (int64_t)row * a.gs[2];
+    for (int c = part * CE; c < a.D; c += 4 * CE) {
+      const u32x4 x = load_chunk<T>(po, in, c, a.D, a.vecO), y = load_chunk<T>(pg, in, c, a.D, a.vecG);
+#pragma unroll
+      for (int j = 0; j < CE; ++j) {
+        const float u = to_acc(((const T*)&x)[j]), v = to_acc(((const T*)&y)[j]);
+        dot = fmaf(u, v, dot);
+        if (BOUND) sq = fmaf(v, v, sq);
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 1; s < 4; s <<= 1) {
+    dot += __shfl_xor(dot, s);
+    sq += __shfl_xor(sq, s);
+  }
+  if (!keys && part == 0 && row < a.N) a.delta[bh * a.N + row] = dot;
+  if constexpr (BOUND) {
+    __shared__ float w[2][4];
+    float nrm = sqrtf(sq), del = fabsf(dot);
+#pragma unroll
+    for (int s = 4; s < 64; s <<= 1) {
+      nrm = fmaxf(nrm, __shfl_xor(nrm, s));
+      del = fmaxf(del, __shfl_xor(del, s));
+    }
+    if ((threadIdx.x & 63) == 0) {
+      w[0][threadIdx.x >> 6] = nrm;
+      w[1][threadIdx.x >> 6] = del;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      nrm = fmaxf(fmaxf(w[0][0], w[0][1]), fmaxf(w[0][2], w[0][3]));
+      del = fmaxf(fmaxf(w[1][0], w[1][1]), fmaxf(w[1][2], w[1][3]));
+      if (keys) {
+        a.bounds[2 * nq + id] = nrm;
+      } else {
+        a.bounds[2 * id] = nrm;
+        a.bounds[2 * id + 1] = del;
+      }
+    }
+  }
+}
+
+// The power of two that dz of key head (b, hk) is multiplied by before it is rounded to fp16.
+__device__ __forceinline__ float dz_factor(const AttnArgs& a, int b, int hk) {
+  const int qt = (a.N + 63) / 64, kt = (a.M + 63) / 64, lane = threadIdx.x & 63;
+  const int64_t q0 = ((int64_t)b * a.H + (int64_t)hk * a.G) * qt;
+  float g = 0.0f, d = 0.0f, v = 0.0f;
+  for (int64_t i = lane; i < (int64_t)a.G * qt; i += 64) {
+    g = fmaxf(g, a.bounds[2 * (q0 + i)]);
+    d = fmaxf(d, a.bounds[2 * (q0 + i) + 1]);
+  }
+  const float* vb = a.bounds + 2 * (int64_t)a.B * a.H * qt + ((int64_t)b * a.Hk + hk) * kt;
+  for (int i = lane; i < kt; i += 64) v = fmaxf(v, vb[i]);
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    g = fmaxf(g, __shfl_xor(g, s));
+    d = fmaxf(d, __shfl_xor(d, s));
+    v = fmaxf(v, __shfl_xor(v, s));
+  }
+  const float bound = fmaf(g, v, d);
+  // A bound of zero, infinity or NaN leaves dz as it is.
+  if (!(bound > 0.0f && bound < 1e37f)) return 1.0f;
+  return exp2f(fminf(fmaxf(13.0f - floorf(log2f(bound)), -120.0f), 60.0f));
+}
+
+// p of one score. x0, x1: the row's statistics.
+template <bool MASK> __device__ __forceinline__ float prob(float s, float c, float x0, float x1) {
+  return MASK ? exp2_fast((s - x0) * kLog2e) * x1 : exp2_fast(fmaf(s, c, -x0));
+}
+
+// The masked score of key j for a row (natural units).
+__device__ __forceinline__ float masked(const AttnArgs& a, float s, int j, int lim, int64_t moff) {
+  if (j >= lim) return kNegInf;
+  const int64_t off = moff + (int64_t)j * a.ms[3];
+  if (a.maskKind == kMaskBool) return ((const uint8_t*)a.mask)[off] ? s * a.scale : kNegInf;
+  const float bias = mask_bias(a, off);
+  return bias == kNegInf ? kNegInf : fmaf(s, a.scale, bias);
+}
+
+// Whether key j of sequence b takes part at all.
+template <bool MASK> __device__ __forceinline__ bool key_live(const AttnArgs& a, int b, int j, int klen) {
+  if (j >= klen) return false;
+  if (!MASK || !a.keyMask) return true;
+  const int64_t off = (int64_t)b * a.ms[0] + (int64_t)j * a.ms[3];
+  return a.maskKind == kMaskBool ? ((const uint8_t*)a.mask)[off] != 0 : mask_bias(a, off) != kNegInf;
+}
+
+// Loads of K or V rows that leave out what key_live does.
+template <typename T, int DP, int ROWS, bool MASK>
+__device__ __forceinline__ void load_keys(const AttnArgs& a, Stage<T, DP, ROWS, 256>& s, const T* base, int64_t stride,
+                                          int b, int row0, int limit, bool vec) {
+  if (MASK && a.keyMask) {
+    using L = Tile<T, DP>;
+    const int c = threadIdx.x % L::CPR, rr = threadIdx.x / L::CPR;
+#pragma unroll
+    for (int i = 0; i < s.NIT; ++i) {
+      const int row = row0 + rr + i * s.RPI;
+      s.r[i] = load_chunk<T>(base + (int64_t)row * stride, key_live<MASK>(a, b, row, limit), c * L::CE, a.D, vec);
+    }
+  } else {
+    s.load(base, stride, row0, limit, a.D, vec);
+  }
+}
+
+// dk and dv of 128 keys, 32 per wave; queries stream through LDS in tiles of QT.
+template <typename T, int DP, bool MASK>
+__global__ void __launch_bounds__(256, DP >= 128 || sizeof(T) == 4 ? 1 : 2) attn_dkdv_kernel(const AttnArgs a) {
+  constexpr int QT = stream_tile<T, DP>(), NT = DP / 16, ND = DP / 32;
+  constexpr bool F16 = std::is_same<T, f16s>::value;
+  using L = Tile<T, DP>;
+  constexpr int TB = QT * L::ROW, SB = QT * 16;  // bytes of a tile, and of its rows' statistics
+  extern __shared__ __align__(16) char smem[];   // [2][q tile, g tile], [2][lse, delta, 1 / sum, last key]
+
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  const uint32_t place = xcd_place(blockIdx.x, gridDim.x);
+  const int split = place % a.nsplit, t0 = place / a.nsplit, bh = t0 / a.tiles, ktile = t0 % a.tiles;
+  const int b = bh / a.Hk, hk = bh % a.Hk;
+  const int klen = key_count(a, b), qlen = query_count(a, b), qstart = query_start(a, b);
+  const int key0 = ktile * 128, mykey = key0 + wave * 32 + (lane & 31);
+
+  // Query tiles of one head that can see a key of the block.
+  const int firstRow = a.causal ? min(max(key0 - qstart, 0), qlen) : 0;
+  const int tb = key0 < klen ? firstRow / QT : 0, te = key0 < klen ? (qlen + QT - 1) / QT : 0;
+  const int perHead = max(te - tb, 0), total = perHead * a.G;
+  const int share = (total + a.nsplit - 1) / a.nsplit;
+  const int beg = min(split * share, total), end = min(beg + share, total);
+
+  const bool live = key_live<MASK>(a, b, mykey, klen);
+  Frag<T> kf[NT], vf[NT];
+  {
+    const int kr = live ? mykey : 0;
+    const T* kp = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1] + (int64_t)kr * a.ks[2];
+    const T* vp = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1] + (int64_t)kr * a.vs[2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      kf[t] = global_frag<T>(kp, live, t, h, a.D, a.vecK);
+      vf[t] = global_frag<T>(vp, live, t, h, a.D, a.vecV);
+    }
+  }
+  const float f = F16 ? dz_factor(a, b, hk) : 1.0f;
+  // fp16: p carries 2^15 and dz the factor f: dz = (p 2^15) ((g.v) f' - delta f'), f' = f 2^-15.
+  const float fd = F16 ? f * exp2f(-kPShift) : 1.0f;
+
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
+
+  Stage<T, DP, QT, 256> sq, sg;
+  float st0 = 0.0f, st1 = 0.0f, st2 = 0.0f;
+  int st3 = 0;
+  auto load = [&](int step) {
+    const int g = step / perHead, row0 = (tb + step % perHead) * QT, hq = hk * a.G + g;
+    sq.load((const T*)a.q + (int64_t)b * a.qs[0] + (int64_t)hq * a.qs[1], a.qs[2], row0, qlen, a.D, a.vecQ);
+    sg.load((const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)hq * a.gs[1], a.gs[2], row0, qlen, a.D, a.vecG);
+    if (threadIdx.x < QT) {
+      const int n = row0 + threadIdx.x;
+      const bool in = n < qlen;
+      const int64_t so = ((int64_t)b * a.H + hq) * a.N + n;
+      st0 = in ? a.stat[so] : MASK ? 0.0f : __builtin_inff();
+      st1 = in ? a.delta[so] * fd : 0.0f;
+      st2 = MASK && in ? a.stat[(int64_t)a.B * a.H * a.N + so] : 0.0f;
+      st3 = !in ? 0 : a.causal ? min(klen, qstart + n + 1) : klen;
+      if (F16) {
+        if (MASK) st2 *= exp2f(kPShift);
+        else st0 -= kPShift;
+      }
+    }
+  };
+  auto store = [&](int buf) {
+    sq.store(smem + buf * 2 * TB);
+    sg.store(smem + buf * 2 * TB + TB);
+    if (threadIdx.x < QT) {
+      float* s = (float*)(smem + 4 * TB + buf * SB);
+      s[threadIdx.x] = st0;
+      s[QT + threadIdx.x] = st1;
+      s[2 * QT + threadIdx.x] = st2;
+      ((int*)s)[3 * QT + threadIdx.x] = st3;
+    }
+  };
+
+  if (beg < end) {
+    load(beg);
+    store(0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int step = beg; step < end; ++step) {
+    const bool more = step + 1 < end;
+    if (more) load(step + 1);
+    const char* tq = smem + buf * 2 * TB;
+    const char* tg = tq + TB;
+    const float* stats = (const float*)(smem + 4 * TB + buf * SB);
+    const int g = step / perHead, row0 = (tb + step % perHead) * QT, hq = hk * a.G + g;
+#pragma unroll
+    for (int qb = 0; qb < QT; qb += 32) {
+      f32x16 s{}, dp{};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s = mma<T>(L::row_frag(tq, qb + (lane & 31), t, h), kf[t], s);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) dp = mma<T>(L::row_frag(tg, qb + (lane & 31), t, h), vf[t], dp);
+      // Every row sees every key of the wave: nothing to leave out.
+      const int wlast = key0 + wave * 32 + 31;
+      const bool check = MASK || wlast >= klen || row0 + qb + 32 > qlen || (a.causal && wlast > qstart + row0 + qb);
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const int rr = qb + 8 * rq + 4 * h;
+        const f32x4 x0 = *(const f32x4*)(stats + rr), de = *(const f32x4*)(stats + QT + rr);
+        f32x4 x1 = {1, 1, 1, 1};
+        if constexpr (MASK) x1 = *(const f32x4*)(stats + 2 * QT + rr);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * rq + i;
+          float x = s[r];
+          if constexpr (MASK) {
+            const int n = min(row0 + rr + i, a.N - 1);
+            x = masked(a, x, mykey, ((const int*)stats)[3 * QT + rr + i],
+                       (int64_t)b * a.ms[0] + (int64_t)hq * a.ms[1] + (int64_t)n * a.ms[2]);
+          }
+          float p = prob<MASK>(x, a.c, x0[i], x1[i]);
+          float z = p * (F16 ? fmaf(dp[r], fd, -de[i]) : dp[r] - de[i]);
+          if (check) {
+            const bool out = MASK ? x == kNegInf : mykey >= ((const int*)stats)[3 * QT + rr + i];
+            p = out ? 0.0f : p;
+            z = out ? 0.0f : z;
+          }
+          s[r] = p;
+          dp[r] = z;
+        }
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const Frag<T> pf = acc_frag<T>(s, st), zf = acc_frag<T>(dp, st);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          dv[d] = mma<T>(L::col_frag(tg, qb, st, d, lane), pf, dv[d]);
+          dk[d] = mma<T>(L::col_frag(tq, qb, st, d, lane), zf, dk[d]);
+        }
+      }
+    }
+    if (more) store(buf ^ 1);
+    buf ^= 1;
+    __syncthreads();
+  }
+
+  if (mykey >= a.M) return;
+  const float kScale = a.scale / f, vScale = F16 ? exp2f(-kPShift) : 1.0f;
+  T* dkp = (T*)a.dk + (int64_t)b * a.dks[0] + (int64_t)hk * a.dks[1] + (int64_t)mykey * a.dks[2];
+  T* dvp = (T*)a.dv + (int64_t)b * a.dvs[0] + (int64_t)hk * a.dvs[1] + (int64_t)mykey * a.dvs[2];
+  float* pk = a.part + ((((int64_t)split * 2) * a.B * a.Hk + bh) * a.M + mykey) * DP;
+  float* pv = pk + (int64_t)a.B * a.Hk * a.M * DP;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      const int c0 = 32 * d + 8 * gq + 4 * h;
+      f32x4 x = {dk[d][4 * gq], dk[d][4 * gq + 1], dk[d][4 * gq + 2], dk[d][4 * gq + 3]};
+      f32x4 y = {dv[d][4 * gq], dv[d][4 * gq + 1], dv[d][4 * gq + 2], dv[d][4 * gq + 3]};
+      x *= kScale;
+      y *= vScale;
+      if (a.nsplit > 1) {
+        *(f32x4*)(pk + c0) = x;
+        *(f32x4*)(pv + c0) = y;
+      } else {
+        store4<T>(dkp, c0, a.D, a.vecDk, x[0], x[1], x[2], x[3]);
+        store4<T>(dvp, c0, a.D, a.vecDv, y[0], y[1], y[2], y[3]);
+      }
+    }
+}
+
+// dq of 128 queries of one head, 32 per wave; keys stream through LDS in tiles of KT.
+template <typename T, int DP, bool MASK>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn_dq_kernel(const AttnArgs a) {
+  constexpr int KT = stream_tile<T, DP>(), NT = DP / 16, ND = DP / 32;
+  constexpr bool F16 = std::is_same<T, f16s>::value;
+  using L = Tile<T, DP>;
+  constexpr int TB = KT * L::ROW;
+  extern __shared__ __align__(16) char smem[];  // [2][k tile, v tile]
+
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  const uint32_t place = xcd_place(blockIdx.x, gridDim.x);
+  const int split = place % a.nsplit, t0 = place / a.nsplit, bhq = t0 / a.tiles, qtile = a.tiles - 1 - t0 % a.tiles;
+  const int b = bhq / a.H, hq = bhq % a.H, hk = hq / a.G;
+  const int klen = key_count(a, b), qlen = query_count(a, b), qstart = query_start(a, b);
+  const int row0 = qtile * 128 + wave * 32, n = row0 + (lane & 31);
+  const bool alive = n < qlen;
+  const int nr = alive ? n : 0;
+  const int lim = !alive ? 0 : a.causal ? min(klen, qstart + n + 1) : klen;
+  const int lastAll = min(qtile * 128 + 128, qlen) - 1;
+  const int kendAll = lastAll < qtile * 128 ? 0 : a.causal ? max(min(klen, qstart + lastAll + 1), 0) : klen;
+  const int kbeg = split * a.chunk * KT, kend = min(kendAll, kbeg + a.chunk * KT);
+  const int wend = row0 >= qlen ? 0 : a.causal ? min(kend, qstart + row0 + 32) : kend;
+  const int full = a.causal ? min(klen, qstart + row0 + 1) : klen;
+
+  Frag<T> qf[NT], gf[NT];
+  {
+    const T* qp = (const T*)a.q + (int64_t)b * a.qs[0] + (int64_t)hq * a.qs[1] + (int64_t)nr * a.qs[2];
+    const T* gp = (const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)hq * a.gs[1] + (int64_t)nr * a.gs[2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      qf[t] = global_frag<T>(qp, alive, t, h, a.D, a.vecQ);
+      gf[t] = global_frag<T>(gp, alive, t, h, a.D, a.vecG);
+    }
+  }
+  const float f = F16 ? dz_factor(a, b, hk) : 1.0f;
+  const int64_t so = ((int64_t)b * a.H + hq) * a.N + nr;
+  const float x0 = alive ? a.stat[so] : MASK ? 0.0f : __builtin_inff();
+  const float x1 = MASK && alive ? a.stat[(int64_t)a.B * a.H * a.N + so] : 0.0f;
+  const float de = alive ? a.delta[so] * f : 0.0f;
+  const int64_t moff = (int64_t)b * a.ms[0] + (int64_t)hq * a.ms[1] + (int64_t)nr * a.ms[2];
+
+  f32x16 dq[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) dq[d] = f32x16{};
+
+  const T* kbase = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1];
+  const T* vbase = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1];
+  Stage<T, DP, KT, 256> sk, sv;
+  auto load = [&](int k0) {
+    load_keys<T, DP, KT, MASK>(a, sk, kbase, a.ks[2], b, k0, kend, a.vecK);
+    load_keys<T, DP, KT, MASK>(a, sv, vbase, a.vs[2], b, k0, kend, a.vecV);
+  };
+  auto store = [&](int buf) {
+    sk.store(smem + buf * 2 * TB);
+    sv.store(smem + buf * 2 * TB + TB);
+  };
+  if (kbeg < kend) {
+    load(kbeg);
+    store(0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int key0 = kbeg; key0 < kend; key0 += KT) {
+    const bool more = key0 + KT < kend;
+    if (more) load(key0 + KT);
+    const char* tk = smem + buf * 2 * TB;
+    const char* tv = tk + TB;
+#pragma unroll
+    for (int kb = 0; kb < KT; kb += 32) {
+      if (key0 + kb >= wend) break;
+      f32x16 s{}, dp{};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s = mma<T>(L::row_frag(tk, kb + (lane & 31), t, h), qf[t], s);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) dp = mma<T>(L::row_frag(tv, kb + (lane & 31), t, h), gf[t], dp);
+      const bool check = MASK || key0 + kb + 32 > full;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = key0 + kb + 8 * (r >> 2) + 4 * h + (r & 3);
+        float x = s[r];
+        if constexpr (MASK) x = masked(a, x, j, lim, moff);
+        const float p = prob<MASK>(x, a.c, x0, x1);
+        float z = p * (F16 ? fmaf(dp[r], f, -de) : dp[r] - de);
+        if (check) z = (MASK ? x == kNegInf : j >= lim) ? 0.0f : z;
+        dp[r] = z;
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const Frag<T> zf = acc_frag<T>(dp, st);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dq[d] = mma<T>(L::col_frag(tk, kb, st, d, lane), zf, dq[d]);
+      }
+    }
+    if (more) store(buf ^ 1);
+    buf ^= 1;
+    __syncthreads();
+  }
+
+  if (n >= a.N) return;
+  const float scale = a.scale / f;
+  T* dqp = (T*)a.dq + (int64_t)b * a.dqs[0] + (int64_t)hq * a.dqs[1] + (int64_t)n * a.dqs[2];
+  float* pq = a.part + (((int64_t)split * a.B * a.H + bhq) * a.N + n) * DP;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      const int c0 = 32 * d + 8 * gq + 4 * h;
+      f32x4 x = {dq[d][4 * gq], dq[d][4 * gq + 1], dq[d][4 * gq + 2], dq[d][4 * gq + 3]};
+      x *= scale;
+      if (a.nsplit > 1) *(f32x4*)(pq + c0) = x;
+      else store4<T>(dqp, c0, a.D, a.vecDq, x[0], x[1], x[2], x[3]);
+    }
+}
+
+// Sums the splits' partial gradients of `rows` rows of heads x batch matrices in their order.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) attn_sum_kernel(const float* part, int nsplit, int64_t splitStride, T* out,
+                                                       int64_t s0, int64_t s1, int64_t s2, int heads, int rows,
+                                                       int64_t total, int D, int vec) {
+  constexpr int TPR = DP / 4, RPB = 256 / TPR;
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int c0 = (threadIdx.x % TPR) * 4;
+  if (row >= total) return;
+  f32x4 x = {0, 0, 0, 0};
+  for (int s = 0; s < nsplit; ++s) x += *(const f32x4*)(part + s * splitStride + row * DP + c0);
+  const int64_t bh = row / rows, n = row % rows;
+  store4<T>(out + bh / heads * s0 + bh % heads * s1 + n * s2, c0, D, vec, x[0], x[1], x[2], x[3]);
+}
+
+struct BwdPlan {
+  int dp, ktiles, ksplit, qtiles, qsplit, qchunk;
+  size_t deltaBytes, boundBytes, partBytes;
+};
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+BwdPlan bwd_plan(int dtype, const AttnArgs& a, int cus) {
+  BwdPlan p{};
+  p.dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
+  p.ktiles = (a.M + 127) / 128;
+  p.qtiles = (a.N + 127) / 128;
+  // The other axis is split where a kernel's own blocks leave CUs without work, into
+  // shares of four tiles at least.
+  const int64_t kw = (int64_t)a.B * a.Hk * p.ktiles, qw = (int64_t)a.B * a.H * p.qtiles;
+  const int tile = dtype != LFAMD_F32 || p.dp == 32 ? 64 : 32;  // stream_tile
+  const int64_t ksteps = (int64_t)a.G * ((a.N + tile - 1) / tile), qsteps = (a.M + tile - 1) / tile;
+  auto splits = [&](int64_t wgs, int64_t steps) {
+    if (wgs >= cus || steps < 8) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + wgs - 1) / wgs, steps / 4, 64}));
+  };
+  p.ksplit = kw ? splits(kw, ksteps) : 1;
+  p.qsplit = qw ? splits(qw, qsteps) : 1;
+  p.qchunk = (int)((qsteps + p.qsplit - 1) / p.qsplit);
+  if (p.qchunk < 1) p.qchunk = 1;
+  p.qsplit = (int)std::max<int64_t>(1, (qsteps + p.qchunk - 1) / p.qchunk);
+  p.deltaBytes = up256((size_t)a.B * a.H * a.N * sizeof(float));
+  if (dtype == LFAMD_F16)
+    p.boundBytes = up256(((size_t)a.B * a.H * ((a.N + 63) / 64) * 2 + (size_t)a.B * a.Hk * ((a.M + 63) / 64)) * sizeof(float));
+  const size_t kp = p.ksplit > 1 ? (size_t)p.ksplit * 2 * a.B * a.Hk * a.M * p.dp * sizeof(float) : 0;
+  const size_t qp = p.qsplit > 1 ? (size_t)p.qsplit * a.B * a.H * a.N * p.dp * sizeof(float) : 0;
+  p.partBytes = std::max(kp, qp);
+  return p;
+}
+
+int launch(const void* fn, int64_t grid, size_t lds, const AttnArgs& a, hipStream_t st) {
+  const char* what = "softmax_attention backward";
+  if (int e = set_dyn_lds(fn, lds, what)) return e;
+  if (int e = check_fit(fn, 256, lds, what)) return e;
+  AttnArgs args = a;
+  void* params[] = {&args};
+  if (hipLaunchKernel(fn, dim3((unsigned)grid), dim3(256), params, lds, st) != hipSuccess) return check_launch(what);
+  return check_launch(what);
+}
+
+template <typename T, int DP, bool MASK> int bwd_launch(AttnArgs a, const BwdPlan& p, hipStream_t st) {
+  constexpr bool F16 = std::is_same<T, f16s>::value;
+  const int qt = (a.N + 63) / 64, kt = (a.M + 63) / 64;
+  int64_t grid = (int64_t)a.B * a.H * qt + (F16 ? (int64_t)a.B * a.Hk * kt : 0);
+  if (grid)
+    if (int e = launch((const void*)attn_delta_kernel<T, F16>, grid, 0, a, st)) return e;
+  constexpr int RPB = 256 / (DP / 4);
+  if (a.dk) {
+    a.nsplit = p.ksplit;
+    a.tiles = p.ktiles;
+    const size_t lds = (size_t)2 * stream_tile<T, DP>() * (2 * DP * sizeof(T) + 16);
+    if (int e = launch((const void*)attn_dkdv_kernel<T, DP, MASK>, (int64_t)a.B * a.Hk * p.ktiles * p.ksplit, lds, a, st))
+      return e;
+    if (p.ksplit > 1) {
+      const int64_t rows = (int64_t)a.B * a.Hk * a.M;
+      for (int i = 0; i < 2; ++i) {
+        const int64_t* s = i ? a.dvs : a.dks;
+        attn_sum_kernel<T, DP><<<dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(256), 0, st>>>(
+            a.part + i * rows * DP, p.ksplit, 2 * rows * DP, (T*)(i ? a.dv : a.dk), s[0], s[1], s[2], a.Hk, a.M, rows, a.D,
+            i ? a.vecDv : a.vecDk);
+        if (int e = check_launch("softmax_attention backward (sums)")) return e;
+      }
+    }
+  }
+  if (a.dq) {
+    a.nsplit = p.qsplit;
+    a.tiles = p.qtiles;
+    a.chunk = p.qchunk;
+    const size_t lds = (size_t)2 * stream_tile<T, DP>() * 2 * DP * sizeof(T);
+    if (int e = launch((const void*)attn_dq_kernel<T, DP, MASK>, (int64_t)a.B * a.H * p.qtiles * p.qsplit, lds, a, st))
+      return e;
+    if (p.qsplit > 1) {
+      const int64_t rows = (int64_t)a.B * a.H * a.N;
+      attn_sum_kernel<T, DP><<<dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(256), 0, st>>>(
+          a.part, p.qsplit, rows * DP, (T*)a.dq, a.dqs[0], a.dqs[1], a.dqs[2], a.H, a.N, rows, a.D, a.vecDq);
+      if (int e = check_launch("softmax_attention backward (sums)")) return e;
+    }
+  }
+  return ok();
+}
+
+template <typename T, int DP> int bwd_mask(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
+  return a.maskKind ? bwd_launch<T, DP, true>(a, p, st) : bwd_launch<T, DP, false>(a, p, st);
+}
+
+template <typename T> int bwd_dim(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
+  switch (p.dp) {
+    case 32: return bwd_mask<T, 32>(a, p, st);
+    case 64: return bwd_mask<T, 64>(a, p, st);
+    default: return bwd_mask<T, 128>(a, p, st);
+  }
+}
+
+}  // namespace
+
+size_t attn_bwd_workspace(int dtype, const AttnArgs& a) {
+  const BwdPlan p = bwd_plan(dtype, a, num_cus());
+  return p.deltaBytes + p.boundBytes + p.partBytes;
+}
+
+int attn_bwd(int dtype, AttnArgs a, void* workspace, hipStream_t st) {
+  const BwdPlan p = bwd_plan(dtype, a, num_cus());
+  a.delta = (float*)workspace;
+  a.bounds = (float*)((char*)workspace + p.deltaBytes);
+  a.part = (float*)((char*)workspace + p.deltaBytes + p.boundBytes);
+  const int64_t most = std::max({(int64_t)a.B * a.Hk * p.ktiles * p.ksplit, (int64_t)a.B * a.H * p.qtiles * p.qsplit,
+                                 (int64_t)a.B * a.H * ((a.N + 63) / 64) + (int64_t)a.B * a.Hk * ((a.M + 63) / 64)});
+  if (most > INT32_MAX) return fail(LFAMD_ERR_UNSUPPORTED, "softmax_attention backward: too many workgroups");
+  switch (dtype) {
+    case LFAMD_F32: return bwd_dim<float>(a, p, st);
+    case LFAMD_F16: return bwd_dim<f16s>(a, p, st);
+    default: return bwd_dim<bf16s>(a, p, st);
+  }
+}
+
+}  // namespace lfamd

@@ -1,0 +1,297 @@
+// Shared by the softmax-attention kernels: matrix-core fragments, the LDS tile
+// and its loader, and the arguments of a call.
+//
+// Every product runs on 32 x 32 accumulators (v_mfma_f32_32x32x16 for the 16-bit
+// types, eight v_mfma_f32_32x32x2_f32 for fp32, which take the same fragments: the
+// contraction index may be dealt to the lanes in any order that both operands
+// share). With h = lane / 32 and i = lane % 32:
+//   operand     row (A) or column (B) i, contraction elements 8h .. 8h+7 of 16
+//   accumulator column i, rows 8 (r / 4) + 4 h + r % 4 for r = 0 .. 15
+// The scores are formed transposed where their columns are to be a product's
+// right operand: the eight accumulator values r = 8s .. 8s+7 of a lane are then
+// already its operand for contraction step s, if that step's rows are dealt as
+//   slot j of half h  <->  row 16 s + 8 (j / 4) + 4 h + j % 4,
+// which col_frag() reads the other operand by. No value crosses lanes.
+#pragma once
+
+#include "lf_common.h"
+#include "lf_internal.h"
+
+namespace lfamd {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <typename T> struct Frag { u32x4 v; };       // eight 16-bit elements
+template <> struct Frag<float> { f32x8 v; };
+
+template <typename T> __device__ __forceinline__ f32x16 mma(const Frag<T>& a, const Frag<T>& b, f32x16 c);
+template <> __device__ __forceinline__ f32x16 mma<f16s>(const Frag<f16s>& a, const Frag<f16s>& b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a.v), __builtin_bit_cast(h16x8, b.v), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x16 mma<bf16s>(const Frag<bf16s>& a, const Frag<bf16s>& b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, a.v), __builtin_bit_cast(b16x8, b.v), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x16 mma<float>(const Frag<float>& a, const Frag<float>& b, f32x16 c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[j], b.v[j], c, 0, 0, 0);
+  return c;
+}
+
+// Two fp32 values rounded to nearest even and packed.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<f16s>(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, h16x2));
+}
+template <> __device__ __forceinline__ uint32_t pack2<bf16s>(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, b16x2));
+}
+
+// Accumulator values 8s .. 8s+7 as an operand of contraction step s.
+template <typename T> __device__ __forceinline__ Frag<T> acc_frag(const f32x16& c, int s) {
+  Frag<T> f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f.v[j] = pack2<T>(c[8 * s + 2 * j], c[8 * s + 2 * j + 1]);
+  return f;
+}
+template <> __device__ __forceinline__ Frag<float> acc_frag<float>(const f32x16& c, int s) {
+  Frag<float> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f.v[j] = c[8 * s + j];
+  return f;
+}
+
+// The other half's value of a lane pair (lane, lane ^ 32), combined.
+__device__ __forceinline__ float half_max(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)p[0]), __builtin_bit_cast(float, (uint32_t)p[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (uint32_t)p[0]) + __builtin_bit_cast(float, (uint32_t)p[1]);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// A tile of rows of DP elements in LDS, in 16-byte chunks. A row's chunks are
+// exchanged (xor with f(row)) so that both ways it is read spread over the 64
+// banks: row_frag (32 rows, one chunk each) and col_frag (four rows x 32 bytes
+// for every 16 lanes: rows that share banks differ in f's upper bits first).
+template <typename T, int DP> struct Tile {
+  static constexpr int CE = 16 / (int)sizeof(T);         // elements per chunk
+  static constexpr int CPR = DP / CE;                    // chunks per row
+  static constexpr int ROW = DP * (int)sizeof(T);        // bytes per row
+  static constexpr int RPB = ROW >= 256 ? 1 : 256 / ROW; // rows per pass over the banks
+
+  static __device__ __forceinline__ int swz(int row) {
+    const int x = row / RPB;
+    if constexpr (CPR >= 16) return ((x & 3) << 2) | ((x >> 2) & 3);
+    else if constexpr (CPR == 8) return ((x & 1) << 2) | ((x >> 1) & 3);
+    else return x & (CPR - 1);
+  }
+  static __device__ __forceinline__ int at(int row, int chunk) { return row * ROW + ((chunk ^ swz(row)) << 4); }
+
+  // Elements 16 t + 8 h .. + 7 of row `row`.
+  static __device__ __forceinline__ Frag<T> row_frag(const char* tile, int row, int t, int h) {
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) {
+      f.v = *(const u32x4*)(tile + at(row, 2 * t + h));
+    } else {
+      const f32x4 a = *(const f32x4*)(tile + at(row, 4 * t + 2 * h));
+      const f32x4 b = *(const f32x4*)(tile + at(row, 4 * t + 2 * h + 1));
+      f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    return f;
+  }
+
+  // Column 32 db + lane % 32 of the rows of contraction step s (rows 16 s ..
+  // 16 s + 15 from row0, dealt as acc_frag deals them). 16-bit: the transposing
+  // LDS read, which gives lane i of 16 the i-th element of four rows.
+  static __device__ __forceinline__ Frag<T> col_frag(const char* tile, int row0, int s, int db, int lane) {
+    Frag<T> f;
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1), off = (i & 1) * 8;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = row0 + 16 * s + 8 * u + 4 * h + (i >> 2);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)(tile + at(row, chunk) + off));
+        const u32x2 y = __builtin_bit_cast(u32x2, x);
+        f.v[2 * u] = y[0];
+        f.v[2 * u + 1] = y[1];
+      }
+    } else {
+      const int d = 32 * db + (lane & 31);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = row0 + 16 * s + 8 * (j >> 2) + 4 * h + (j & 3);
+        f.v[j] = *(const float*)(tile + at(row, d / CE) + (d % CE) * 4);
+      }
+    }
+    return f;
+  }
+};
+
+// 16 bytes of a row from element c0 on, zero where row or column is outside.
+// vec: the row is 16-byte aligned and D a multiple of the chunk.
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T* row, bool inside, int c0, int D, bool vec) {
+  constexpr int CE = 16 / (int)sizeof(T);
+  u32x4 r = {0, 0, 0, 0};
+  if (!inside || c0 >= D) return r;
+  if (vec) return *(const u32x4*)(row + c0);
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t* p = (const uint16_t*)(row + c0);
+#pragma unroll
+    for (int j = 0; j < CE; ++j)
+      if (c0 + j < D) r[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
+  } else {
+    const uint32_t* p = (const uint32_t*)(row + c0);
+#pragma unroll
+    for (int j = 0; j < CE; ++j)
+      if (c0 + j < D) r[j] = p[j];
+  }
+  return r;
+}
+
+// Rows row0 .. row0 + ROWS - 1 of a matrix, held in the workgroup's registers
+// between their global loads and their LDS stores.
+template <typename T, int DP, int ROWS, int THREADS> struct Stage {
+  using L = Tile<T, DP>;
+  static constexpr int RPI = THREADS / L::CPR, NIT = ROWS / RPI;
+  static_assert(THREADS % L::CPR == 0 && ROWS % RPI == 0, "tile shape");
+  u32x4 r[NIT];
+  // Rows at or behind `limit` are zero and not read.
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int limit, int D, bool vec) {
+    const int tid = threadIdx.x, c = tid % L::CPR, rr = tid / L::CPR;
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+      const int row = row0 + rr + i * RPI;
+      r[i] = load_chunk<T>(base + (int64_t)row * stride, row < limit, c * L::CE, D, vec);
+    }
+  }
+  __device__ __forceinline__ void store(char* tile) const {
+    const int tid = threadIdx.x, c = tid % L::CPR, rr = tid / L::CPR;
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) *(u32x4*)(tile + L::at(rr + i * RPI, c)) = r[i];
+  }
+};
+
+// The eight elements 16 t + 8 h .. + 7 of a row in memory.
+template <typename T>
+__device__ __forceinline__ Frag<T> global_frag(const T* row, bool inside, int t, int h, int D, bool vec) {
+  Frag<T> f;
+  const int c0 = 16 * t + 8 * h;
+  if constexpr (sizeof(T) == 2) {
+    f.v = load_chunk<T>(row, inside, c0, D, vec);
+  } else {
+    const f32x4 a = __builtin_bit_cast(f32x4, load_chunk<T>(row, inside, c0, D, vec));
+    const f32x4 b = __builtin_bit_cast(f32x4, load_chunk<T>(row, inside, c0 + 4, D, vec));
+    f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  return f;
+}
+
+// Four consecutive elements of a row from c0 on, rounded from fp32.
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int c0, int D, bool vec, float a, float b, float c, float d) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t lo = pack2<T>(a, b), hi = pack2<T>(c, d);
+    if (vec) {
+      if (c0 < D) *(u32x2*)(row + c0) = (u32x2){lo, hi};
+      return;
+    }
+    uint16_t* p = (uint16_t*)(row + c0);
+    if (c0 < D) p[0] = (uint16_t)lo;
+    if (c0 + 1 < D) p[1] = (uint16_t)(lo >> 16);
+    if (c0 + 2 < D) p[2] = (uint16_t)hi;
+    if (c0 + 3 < D) p[3] = (uint16_t)(hi >> 16);
+  } else {
+    if (vec) {
+      if (c0 < D) *(f32x4*)(row + c0) = (f32x4){a, b, c, d};
+      return;
+    }
+    if (c0 < D) row[c0] = a;
+    if (c0 + 1 < D) row[c0 + 1] = b;
+    if (c0 + 2 < D) row[c0 + 2] = c;
+    if (c0 + 3 < D) row[c0 + 3] = d;
+  }
+}
+
+// n / d for 0 <= n < 2^31 by a multiplication (d >= 1).
+struct FastDiv {
+  uint32_t mul = 0, shift = 0, d = 1;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t div) : d(div) {
+    while ((1u << shift) < div && shift < 31) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - div)) / div + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    const uint32_t t = __umulhi(n, mul);
+    return (uint32_t)(((uint64_t)t + n) >> shift);
+  }
+};
+
+enum MaskKind { kMaskNone = 0, kMaskBool = 1, kMaskF32 = 2, kMaskF16 = 3, kMaskBF16 = 4 };
+
+struct AttnArgs {
+  const void *q, *k, *v, *o, *g;       // o: forward output (backward reads it); g: its gradient
+  void *out, *dq, *dk, *dv;
+  float *stat;                         // forward statistics of each row, see attn_fwd.hip
+  float *part;                         // fp32 partial results of split work
+  float *delta;                        // rowsum(g o), [B][H][N]
+  float *bounds;                       // fp16: per 64 rows max |g_i| and max |delta_i|; per 64 keys max |v_j|
+  const void* mask;
+  const int32_t *klen, *qlen, *qstart;
+  int64_t qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];  // element strides of batch, head, row
+  int64_t ms[4];                       // mask strides: batch, head, row, key (0 where broadcast)
+  int B, H, Hk, G, N, M, D;
+  int maskKind, causal, keyMask;       // keyMask: the mask is the same for every head and row
+  int vecQ, vecK, vecV, vecO, vecG, vecDq, vecDk, vecDv;
+  int nsplit, tiles, chunk;            // work split along the other axis; tiles along the own one; steps per split
+  float scale, c;                      // c = scale * log2(e)
+  FastDiv divN;
+};
+
+// Keys of sequence b that exist, and queries.
+__device__ __forceinline__ int key_count(const AttnArgs& a, int b) {
+  return a.klen ? min(max(a.klen[b], 0), a.M) : a.M;
+}
+__device__ __forceinline__ int query_count(const AttnArgs& a, int b) {
+  return a.qlen ? min(max(a.qlen[b], 0), a.N) : a.N;
+}
+// The key position of query 0.
+__device__ __forceinline__ int query_start(const AttnArgs& a, int b) {
+  return a.qstart ? min(max(a.qstart[b], -a.N), a.M) : a.M - a.N;
+}
+
+// mask element (b, h, n, j) as an additive term in natural units.
+__device__ __forceinline__ float mask_bias(const AttnArgs& a, int64_t off) {
+  if (a.maskKind == kMaskF32) return ((const float*)a.mask)[off];
+  if (a.maskKind == kMaskF16) return to_acc(((const f16s*)a.mask)[off]);
+  return to_acc(((const bf16s*)a.mask)[off]);
+}
+
+// The workgroup's place: consecutive places on one XCD (workgroups are dealt to
+// the eight XCDs in turn), so that a head's keys stay in one XCD's L2.
+__device__ __forceinline__ uint32_t xcd_place(uint32_t id, uint32_t n) {
+  const uint32_t q = n / 8, r = n % 8, x = id % 8, y = id / 8;
+  return x * q + min(x, r) + y;
+}
+
+}  // namespace lfamd

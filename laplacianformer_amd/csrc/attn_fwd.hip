@@ -1,0 +1,470 @@
+// softmax_attention, forward:  o_i = sum_j p_ij v_j,  p_i = softmax_j(scale q_i . k_j + mask_ij).
+//
+// One pass over the keys with the running maximum and sum of each row. The query
+// heads that share a key head are laid end to end, so that a workgroup's rows are
+// taken from G * N rows, whatever their number. Scores are formed as S^T = K Q^T
+// and the output as O^T = V^T P^T: a lane owns one query in both, so that the
+// softmax needs one exchange between lane halves per tile and P goes from the one
+// product's accumulators to the other's operand within the lane's registers.
+//
+// Units: without a mask the scores stay unscaled in the accumulators and the row
+// reference m is in log2 units, p = exp2(c S - m) with c = scale log2 e (one fma and
+// one exp2 per score). With a mask, x = scale S + mask in natural units, as an
+// additive mask may hold the type's lowest value, and p = exp2((x - m) log2 e).
+// P is rounded to the element type for the product with V; its sum is of the
+// unrounded values.
+//
+// Row statistics for the backward pass, [B][H][N] planes: without a mask one plane,
+// m + log2(sum) (+inf for a row without keys: its p is then 0); with a mask two, m
+// and 1 / sum, since m + log(sum) loses the sum where m is the type's lowest value.
+#include "attn_common.h"
+
+#include <algorithm>
+
+namespace lfamd {
+
+namespace {
+
+template <int KS> constexpr int key_tile() { return KS == 1 ? 64 : 128; }
+
+template <typename T, int DP, int KS> constexpr int num_buffers() {
+  return 4 * key_tile<KS>() * DP * (int)sizeof(T) <= 128 * 1024 ? 2 : 1;
+}
+
+// QB: 32-query blocks per wave. KS: 1, the four waves take different queries; 4,
+// they take different keys of each tile and their results are joined at the end.
+template <typename T, int DP, int QB, int KS, bool MASK>
+__global__ void __launch_bounds__(256, 2) attn_fwd_kernel(const AttnArgs a) {
+  constexpr int KT = key_tile<KS>(), NBUF = num_buffers<T, DP, KS>(), NT = DP / 16, ND = DP / 32;
+  constexpr int KB = KS == 1 ? KT / 32 : 1;  // 32-key blocks per wave and tile
+  constexpr int ROWS = KS == 1 ? 128 * QB : 32 * QB;
+  using L = Tile<T, DP>;
+  constexpr int TB = KT * L::ROW;  // bytes of one tile
+  extern __shared__ __align__(16) char smem[];
+
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  const uint32_t place = xcd_place(blockIdx.x, gridDim.x);
+  const int split = place % a.nsplit, t0 = place / a.nsplit;
+  const int bh = t0 / a.tiles, tile = a.tiles - 1 - t0 % a.tiles;  // the longest rows of a causal mask first
+  const int b = bh / a.Hk, hk = bh % a.Hk;
+  const int R = a.G * a.N, row0 = tile * ROWS + (KS == 1 ? wave * 32 * QB : 0);
+  const int klen = key_count(a, b), qlen = query_count(a, b), qstart = query_start(a, b);
+
+  // Bounds of the keys that any row of the workgroup, or every row of the wave, sees.
+  auto last_key = [&](int first, int count) {
+    if (!a.causal) return klen;
+    const int end = min(first + count, R) - 1;
+    const int n = end < first || a.divN.div(end) != a.divN.div(first) ? a.N - 1 : end - (int)a.divN.div(end) * a.N;
+    return min(klen, qstart + n + 1);
+  };
+  const int kendAll = max(last_key(tile * ROWS, ROWS), 0);
+  const int kbeg = split * a.chunk * KT, kend = min(kendAll, kbeg + a.chunk * KT);
+  const int wend = row0 < R ? min(kend, last_key(row0, 32 * QB)) : 0;
+
+  // This lane's queries.
+  int qrow[QB], lim[QB], full = klen;
+  int64_t qoff[QB], ooff[QB], soff[QB], moff[QB];
+  bool stored[QB], alive[QB];
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    const int r = row0 + 32 * i + (lane & 31);
+    stored[i] = r < R;
+    qrow[i] = stored[i] ? r : 0;
+    const int g = a.divN.div(qrow[i]), n = qrow[i] - g * a.N, hq = hk * a.G + g;
+    alive[i] = stored[i] && n < qlen;
+    lim[i] = !alive[i] ? 0 : a.causal ? min(klen, qstart + n + 1) : klen;
+    qoff[i] = (int64_t)b * a.qs[0] + (int64_t)hq * a.qs[1] + (int64_t)n * a.qs[2];
+    ooff[i] = (int64_t)b * a.os[0] + (int64_t)hq * a.os[1] + (int64_t)n * a.os[2];
+    soff[i] = ((int64_t)b * a.H + hq) * a.N + n;
+    if constexpr (MASK) moff[i] = (int64_t)b * a.ms[0] + (int64_t)hq * a.ms[1] + (int64_t)n * a.ms[2];
+  }
+  if (a.causal) {  // a row behind R or qlen needs no check: what it computes is not used
+    int m = klen;
+#pragma unroll
+    for (int i = 0; i < QB; ++i) m = min(m, alive[i] ? lim[i] : klen);
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) m = min(m, __shfl_xor(m, s));
+    full = uniform(m);
+  }
+
+  Frag<T> qf[QB][NT];
+#pragma unroll
+  for (int i = 0; i < QB; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) qf[i][t] = global_frag<T>((const T*)a.q + qoff[i], alive[i], t, h, a.D, a.vecQ);
+
+  f32x16 o[ND][QB];
+  float m[QB], l[QB];
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    m[i] = kNegInf;
+    l[i] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d][i] = f32x16{};
+  }
+
+  const T* kbase = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1];
+  const T* vbase = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1];
+  Stage<T, DP, KT, 256> sk, sv;
+  // Keys that a mask takes from every query are not read either: what they hold is nobody's.
+  auto load = [&](int key0) {
+    if (MASK && a.keyMask) {
+      const int c = threadIdx.x % L::CPR, rr = threadIdx.x / L::CPR;
+#pragma unroll
+      for (int i = 0; i < sk.NIT; ++i) {
+        const int row = key0 + rr + i * sk.RPI;
+        bool in = row < kend;
+        if (in) {
+          const int64_t off = (int64_t)b * a.ms[0] + (int64_t)row * a.ms[3];
+          in = a.maskKind == kMaskBool ? ((const uint8_t*)a.mask)[off] != 0 : mask_bias(a, off) != kNegInf;
+        }
+        sk.r[i] = load_chunk<T>(kbase + (int64_t)row * a.ks[2], in, c * L::CE, a.D, a.vecK);
+        sv.r[i] = load_chunk<T>(vbase + (int64_t)row * a.vs[2], in, c * L::CE, a.D, a.vecV);
+      }
+    } else {
+      sk.load(kbase, a.ks[2], key0, kend, a.D, a.vecK);
+      sv.load(vbase, a.vs[2], key0, kend, a.D, a.vecV);
+    }
+  };
+  auto store = [&](int buf) {
+    sk.store(smem + buf * 2 * TB);
+    sv.store(smem + buf * 2 * TB + TB);
+  };
+
+  if (kbeg < kend) {
+    load(kbeg);
+    store(0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int key0 = kbeg; key0 < kend; key0 += KT) {
+    const bool more = key0 + KT < kend;
+    if (more) load(key0 + KT);
+    const char* tk = smem + buf * 2 * TB;
+    const char* tv = tk + TB;
+    const int wkey = key0 + (KS == 1 ? 0 : 32 * wave);
+    if (wkey < wend) {
+      f32x16 s[KB][QB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+        for (int i = 0; i < QB; ++i) s[kb][i] = f32x16{};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const Frag<T> kf = L::row_frag(tk, (KS == 1 ? 32 * kb : 32 * wave) + (lane & 31), t, h);
+#pragma unroll
+          for (int i = 0; i < QB; ++i) s[kb][i] = mma<T>(kf, qf[i][t], s[kb][i]);
+        }
+      }
+      // The mask, and what lies behind the row's last key.
+      if (MASK || wkey + 32 * KB > full) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < QB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int j = wkey + 32 * kb + 8 * (r >> 2) + 4 * h + (r & 3);
+              if constexpr (MASK) {
+                float x = kNegInf;
+                if (j < lim[i]) {
+                  const int64_t off = moff[i] + (int64_t)j * a.ms[3];
+                  if (a.maskKind == kMaskBool) {
+                    if (((const uint8_t*)a.mask)[off]) x = s[kb][i][r] * a.scale;
+                  } else {
+                    // -inf removes the key, whatever its score
+                    const float bias = mask_bias(a, off);
+                    if (bias != kNegInf) x = fmaf(s[kb][i][r], a.scale, bias);
+                  }
+                }
+                s[kb][i][r] = x;
+              } else {
+                s[kb][i][r] = j < lim[i] ? s[kb][i][r] : kNegInf;
+              }
+            }
+      }
+#pragma unroll
+      for (int i = 0; i < QB; ++i) {
+        float mx = s[0][i][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][i][r]);
+        mx = half_max(mx);
+        if (!MASK) mx *= a.c;
+        // The reference follows the maximum only when that has grown by 2^8: p stays
+        // below 2^8, which every element type holds at full precision, and the
+        // accumulators are rescaled in few tiles.
+        const float slack = MASK ? 8.0f / kLog2e : 8.0f;
+        if (__any(mx > m[i] + slack)) {
+          const float mn = fmaxf(m[i], mx), ms = mn == kNegInf ? 0.0f : mn;
+          const float alpha = exp2_fast(MASK ? (m[i] - ms) * kLog2e : m[i] - ms);
+          m[i] = mn;
+          l[i] *= alpha;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][i][r] *= alpha;
+        }
+        const float ref = m[i] == kNegInf ? 0.0f : m[i];
+        float sum = 0.0f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float p = exp2_fast(MASK ? (s[kb][i][r] - ref) * kLog2e : fmaf(s[kb][i][r], a.c, -ref));
+            s[kb][i][r] = p;
+            sum += p;
+          }
+        l[i] += sum;
+      }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          Frag<T> pf[QB];
+#pragma unroll
+          for (int i = 0; i < QB; ++i) pf[i] = acc_frag<T>(s[kb][i], st);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            const Frag<T> vf = L::col_frag(tv, KS == 1 ? 32 * kb : 32 * wave, st, d, lane);
+#pragma unroll
+            for (int i = 0; i < QB; ++i) o[d][i] = mma<T>(vf, pf[i], o[d][i]);
+          }
+        }
+    }
+    if (NBUF == 1) __syncthreads();
+    if (more) store(NBUF == 2 ? buf ^ 1 : 0);
+    if (NBUF == 2) buf ^= 1;
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < QB; ++i) l[i] = half_sum(l[i]);
+
+  constexpr float kUnit = MASK ? kLog2e : 1.0f;
+  if constexpr (KS == 4) {
+    // Join the four waves' results through LDS (the loop's last barrier has passed).
+    constexpr int PS = DP + 4;  // floats per row: rows start four banks apart
+    static_assert(QB == 1, "one query block where the waves share it");
+    static_assert(4 * 32 * (PS + 2) * 4 <= 2 * NBUF * TB, "the tiles' LDS holds the partial results");
+    float* po = (float*)smem;
+    float* pm = po + 4 * 32 * PS;
+    float* pl = pm + 128;
+    const int q = lane & 31;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq)
+        *(f32x4*)(po + (wave * 32 + q) * PS + 32 * d + 8 * gq + 4 * h) =
+            (f32x4){o[d][0][4 * gq], o[d][0][4 * gq + 1], o[d][0][4 * gq + 2], o[d][0][4 * gq + 3]};
+    if (h == 0) {
+      pm[wave * 32 + q] = m[0];
+      pl[wave * 32 + q] = l[0];
+    }
+    __syncthreads();
+    // Wave w takes columns 8 w + 4 h of every 32.
+    float mt = kNegInf;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, pm[w * 32 + q]);
+    const float ref = mt == kNegInf ? 0.0f : mt;
+    float lt = 0.0f, f[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      f[w] = exp2_fast((pm[w * 32 + q] - ref) * kUnit);
+      lt += f[w] * pl[w * 32 + q];
+    }
+    if (!stored[0]) return;
+    const float inv = a.nsplit > 1 ? 1.0f : lt == 0.0f ? 0.0f : 1.0f / lt;
+    const bool live = alive[0];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const int c0 = 32 * d + 8 * wave + 4 * h;
+      f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) x += f[w] * *(const f32x4*)(po + (w * 32 + q) * PS + c0);
+      x *= inv;
+      if (!live) x = f32x4{0, 0, 0, 0};
+      if (a.nsplit > 1) {
+        *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[0]) * DP + c0) = x;
+      } else {
+        store4<T>((T*)a.out + ooff[0], c0, a.D, a.vecO, x[0], x[1], x[2], x[3]);
+      }
+    }
+    if (wave == 0 && h == 0) {
+      if (a.nsplit > 1) {
+        float* ps = a.part + (int64_t)a.nsplit * a.B * a.Hk * R * DP + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[0]) * 2;
+        ps[0] = live ? mt : kNegInf;
+        ps[1] = live ? lt : 0.0f;
+      } else if (a.stat) {
+        const bool none = !live || lt == 0.0f;
+        if (MASK) {
+          a.stat[soff[0]] = none ? 0.0f : mt;
+          a.stat[(int64_t)a.B * a.H * a.N + soff[0]] = none ? 0.0f : 1.0f / lt;
+        } else {
+          a.stat[soff[0]] = none ? __builtin_inff() : mt + log2f(lt);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+      if (!stored[i]) continue;
+      const bool none = !alive[i] || l[i] == 0.0f;
+      const float inv = a.nsplit > 1 ? 1.0f : none ? 0.0f : 1.0f / l[i];
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int gq = 0; gq < 4; ++gq) {
+          const int c0 = 32 * d + 8 * gq + 4 * h;
+          f32x4 x = {o[d][i][4 * gq], o[d][i][4 * gq + 1], o[d][i][4 * gq + 2], o[d][i][4 * gq + 3]};
+          x *= inv;
+          if (none) x = f32x4{0, 0, 0, 0};
+          if (a.nsplit > 1) {
+            *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[i]) * DP + c0) = x;
+          } else {
+            store4<T>((T*)a.out + ooff[i], c0, a.D, a.vecO, x[0], x[1], x[2], x[3]);
+          }
+        }
+      if (h == 0) {
+        if (a.nsplit > 1) {
+          float* ps = a.part + (int64_t)a.nsplit * a.B * a.Hk * R * DP +
+                      (((int64_t)split * a.B * a.Hk + bh) * R + qrow[i]) * 2;
+          ps[0] = none ? kNegInf : m[i];
+          ps[1] = none ? 0.0f : l[i];
+        } else if (a.stat) {
+          if (MASK) {
+            a.stat[soff[i]] = none ? 0.0f : m[i];
+            a.stat[(int64_t)a.B * a.H * a.N + soff[i]] = none ? 0.0f : 1.0f / l[i];
+          } else {
+            a.stat[soff[i]] = none ? __builtin_inff() : m[i] + log2f(l[i]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// Joins the key splits' partial results: one row of DP columns per DP / 4 threads.
+template <typename T, int DP, bool MASK>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
+  constexpr int TPR = DP / 4, RPB = 256 / TPR;
+  constexpr float kUnit = MASK ? kLog2e : 1.0f;
+  const int64_t R = (int64_t)a.G * a.N, total = (int64_t)a.B * a.Hk * R;
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int c0 = (threadIdx.x % TPR) * 4;
+  if (row >= total) return;
+  const float* ps = a.part + (int64_t)a.nsplit * total * DP;
+  float m = kNegInf;
+  for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, ps[(s * total + row) * 2]);
+  const float ref = m == kNegInf ? 0.0f : m;
+  float l = 0.0f;
+  f32x4 x = {0, 0, 0, 0};
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float f = exp2_fast((ps[(s * total + row) * 2] - ref) * kUnit);
+    l += f * ps[(s * total + row) * 2 + 1];
+    x += f * *(const f32x4*)(a.part + (s * total + row) * DP + c0);
+  }
+  const bool none = l == 0.0f;
+  x *= none ? 0.0f : 1.0f / l;
+  if (none) x = f32x4{0, 0, 0, 0};
+  const int bh = (int)(row / R), r = (int)(row % R), b = bh / a.Hk, hk = bh % a.Hk;
+  const int g = a.divN.div(r), n = r - g * a.N, hq = hk * a.G + g;
+  T* out = (T*)a.out + (int64_t)b * a.os[0] + (int64_t)hq * a.os[1] + (int64_t)n * a.os[2];
+  store4<T>(out, c0, a.D, a.vecO, x[0], x[1], x[2], x[3]);
+  if (a.stat && c0 == 0) {
+    const int64_t so = ((int64_t)b * a.H + hq) * a.N + n;
+    if (MASK) {
+      a.stat[so] = none ? 0.0f : m;
+      a.stat[(int64_t)a.B * a.H * a.N + so] = none ? 0.0f : 1.0f / l;
+    } else {
+      a.stat[so] = none ? __builtin_inff() : m + log2f(l);
+    }
+  }
+}
+
+// How a call is laid over the chip.
+struct FwdPlan {
+  int ks, qb, rows, kt, tiles, nsplit, chunk, dp;
+};
+
+FwdPlan fwd_plan(const AttnArgs& a, int cus) {
+  FwdPlan p;
+  const int64_t R = (int64_t)a.G * a.N;
+  p.dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
+  // Up to 32 rows per key head fill one wave's block: the four waves then share the
+  // rows and divide each tile's keys.
+  p.ks = R <= 32 ? 4 : 1;
+  p.qb = 1;
+  p.rows = p.ks == 4 ? 32 : 128 * p.qb;
+  p.kt = p.ks == 4 ? 128 : 64;
+  p.tiles = (int)((R + p.rows - 1) / p.rows);
+  const int64_t wgs = (int64_t)a.B * a.Hk * p.tiles;
+  const int steps = (a.M + p.kt - 1) / p.kt;
+  // The keys are split where the rows alone leave CUs without work, into pieces of
+  // four tiles at least, so that the join stays small beside them.
+  int64_t ns = 1;
+  if (wgs < cus && steps >= 8) ns = std::min<int64_t>((2 * cus + wgs - 1) / wgs, steps / 4);
+  ns = std::max<int64_t>(1, std::min<int64_t>(ns, 64));
+  p.chunk = (int)((steps + ns - 1) / ns);
+  if (p.chunk < 1) p.chunk = 1;
+  p.nsplit = std::max(1, (steps + p.chunk - 1) / p.chunk);
+  return p;
+}
+
+template <typename T, int DP, bool MASK> int fwd_launch(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
+  const void* fn = p.ks == 4 ? (const void*)attn_fwd_kernel<T, DP, 1, 4, MASK> : (const void*)attn_fwd_kernel<T, DP, 1, 1, MASK>;
+  const int nbuf = p.ks == 4 ? num_buffers<T, DP, 4>() : num_buffers<T, DP, 1>();
+  const size_t lds = (size_t)2 * nbuf * p.kt * DP * sizeof(T);
+  if (int e = set_dyn_lds(fn, lds, "softmax_attention")) return e;
+  if (int e = check_fit(fn, 256, lds, "softmax_attention")) return e;
+  const unsigned grid = (unsigned)((int64_t)a.B * a.Hk * p.tiles * p.nsplit);
+  AttnArgs args = a;
+  void* params[] = {&args};
+  if (hipLaunchKernel(fn, dim3(grid), dim3(256), params, lds, st) != hipSuccess)
+    return check_launch("softmax_attention");
+  if (int e = check_launch("softmax_attention")) return e;
+  if (p.nsplit > 1) {
+    const int64_t rows = (int64_t)a.B * a.Hk * a.G * a.N;
+    constexpr int RPB = 256 / (DP / 4);
+    attn_join_kernel<T, DP, MASK><<<dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(256), 0, st>>>(a);
+    return check_launch("softmax_attention (join)");
+  }
+  return ok();
+}
+
+template <typename T, int DP> int fwd_mask(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
+  return a.maskKind ? fwd_launch<T, DP, true>(a, p, st) : fwd_launch<T, DP, false>(a, p, st);
+}
+
+template <typename T> int fwd_dim(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
+  switch (p.dp) {
+    case 32: return fwd_mask<T, 32>(a, p, st);
+    case 64: return fwd_mask<T, 64>(a, p, st);
+    default: return fwd_mask<T, 128>(a, p, st);
+  }
+}
+
+}  // namespace
+
+size_t attn_fwd_workspace(const AttnArgs& a) {
+  const FwdPlan p = fwd_plan(a, num_cus());
+  if (p.nsplit <= 1) return 0;
+  return (size_t)p.nsplit * a.B * a.Hk * a.G * a.N * (p.dp + 2) * sizeof(float);
+}
+
+int attn_fwd(int dtype, AttnArgs a, hipStream_t st) {
+  const FwdPlan p = fwd_plan(a, num_cus());
+  a.nsplit = p.nsplit;
+  a.tiles = p.tiles;
+  a.chunk = p.chunk;
+  if ((int64_t)a.B * a.Hk * p.tiles * p.nsplit > INT32_MAX)
+    return fail(LFAMD_ERR_UNSUPPORTED, "softmax_attention: too many workgroups");
+  switch (dtype) {
+    case LFAMD_F32: return fwd_dim<float>(a, p, st);
+    case LFAMD_F16: return fwd_dim<f16s>(a, p, st);
+    default: return fwd_dim<bf16s>(a, p, st);
+  }
+}
+
+}  // namespace lfamd

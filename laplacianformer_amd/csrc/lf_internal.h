@@ -90,6 +90,14 @@ int mix_rows_trio(int dtype, const void* const* A, const float* const* B, void* 
                   const int* P, const int* Q, const int64_t* sq, const int64_t* sp, const int64_t* bStride,
                   hipStream_t st, int first = 0);
 
+// softmax_attention on a filled-in call (attn_fwd.hip, attn_bwd.hip; the C entries
+// that check and fill it in are in attn_host.hip).
+struct AttnArgs;
+size_t attn_fwd_workspace(const AttnArgs& a);
+int attn_fwd(int dtype, AttnArgs a, hipStream_t st);
+size_t attn_bwd_workspace(int dtype, const AttnArgs& a);
+int attn_bwd(int dtype, AttnArgs a, void* workspace, hipStream_t st);
+
 inline bool valid_dtype(int dt) {
   return dt == LFAMD_F32 || dt == LFAMD_F16 || dt == LFAMD_BF16 || dt == LFAMD_F64;
 }

@@ -1,0 +1,436 @@
+// add_rms_norm: s = x + residual, rstd = 1 / sqrt(mean(s^2) + eps), y = s rstd w, and its backward pass
+//   gn = gy w,  n = s rstd,  ds = gs + rstd (gn - n mean(gn n)),  dw = sum over rows of gy n.
+//
+// Memory-bound: every element is read and written once. A row stays in the registers
+// of the threads that own it (one wave, or a workgroup of 256 or 1024 threads, chosen
+// by the width so that a thread holds at most 4 vectors of 16 bytes or 16 single
+// elements) between the sum of squares and the scaling. The forward normalises the
+// fp32 sum, not its stored rounding. The backward's workgroups walk the rows with a
+// fixed stride, keep their share of dw in registers, and write one fp32 partial row
+// each; a second kernel adds those in their order, so the same call gives the same bits.
+#include "lf_common.h"
+#include "lf_internal.h"
+
+#include <algorithm>
+
+namespace lfamd {
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct NormArgs {
+  const void *x, *res, *w, *gy, *gs;
+  void *y, *sum, *dx;
+  float *rstd, *scale, *part;
+  int64_t xs, rs, gys, gss;  // row strides of x, residual, gy, gs (y, sum, dx: contiguous)
+  int64_t rows;
+  int width, wf32, e4m3;
+  float eps;
+};
+
+// V consecutive elements of a row: one 16-byte access, or a single element.
+template <typename T, int V> struct Pack {
+  T e[V];
+  __device__ __forceinline__ static Pack load(const T* p) {
+    Pack r;
+    if constexpr (V == 1) r.e[0] = *p;
+    else *(u32x4*)r.e = *(const u32x4*)p;
+    return r;
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (V == 1) *p = e[0];
+    else *(u32x4*)p = *(const u32x4*)e;
+  }
+};
+
+template <typename T, int V> __device__ __forceinline__ void load_weight(const NormArgs& a, int c, float* w) {
+  if (a.wf32) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[j] = ((const float*)a.w)[c + j];
+  } else {
+    const Pack<T, V> p = Pack<T, V>::load((const T*)a.w + c);
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[j] = to_acc(p.e[j]);
+  }
+}
+
+// Sum over the TPR threads of a row, in every one of them. lds: one float per wave.
+template <int TPR, bool MAX> __device__ __forceinline__ float row_reduce(float v, float* lds) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) v = MAX ? fmaxf(v, __shfl_xor(v, s)) : v + __shfl_xor(v, s);
+  if constexpr (TPR > 64) {
+    __syncthreads();  // the values of the reduction before have been read
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll
+    for (int i = 1; i < TPR / 64; ++i) v = MAX ? fmaxf(v, lds[i]) : v + lds[i];
+  }
+  return v;
+}
+
+template <typename T, int V, int TPR, int NV, bool F8>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(const NormArgs a) {
+  constexpr int THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR;
+  __shared__ float lds[16];
+  const int t = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  if (RPB > 1 && row >= a.rows) return;  // whole waves; no barrier where RPB > 1
+  float s[NV][V], sq = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (t + i * TPR) * V;
+    if (c < a.width) {
+      const Pack<T, V> px = Pack<T, V>::load((const T*)a.x + row * a.xs + c);
+      if (a.res) {
+        const Pack<T, V> pr = Pack<T, V>::load((const T*)a.res + row * a.rs + c);
+        Pack<T, V> ps;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          s[i][j] = to_acc(px.e[j]) + to_acc(pr.e[j]);
+          ps.e[j] = from_acc<T>(s[i][j]);
+        }
+        ps.store((T*)a.sum + row * a.width + c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[i][j] = to_acc(px.e[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) sq = fmaf(s[i][j], s[i][j], sq);
+    }
+  }
+  sq = row_reduce<TPR, false>(sq, lds);
+  const float r = 1.0f / sqrtf(sq / (float)a.width + a.eps);
+  if (t == 0 && a.rstd) a.rstd[row] = r;
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (t + i * TPR) * V;
+    if (c < a.width) {
+      float w[V];
+      load_weight<T, V>(a, c, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        s[i][j] = s[i][j] * r * w[j];
+        if (F8) top = fmaxf(top, fabsf(s[i][j]));
+      }
+      if constexpr (!F8) {
+        Pack<T, V> py;
+#pragma unroll
+        for (int j = 0; j < V; ++j) py.e[j] = from_acc<T>(s[i][j]);
+        py.store((T*)a.y + row * a.width + c);
+      }
+    }
+  }
+  if constexpr (F8) {
+    top = row_reduce<TPR, true>(top, lds);
+    // An all-zero row keeps scale 1: its zeros need none.
+    const float scale = top == 0.0f ? 1.0f : top / 448.0f;
+    if (t == 0) a.scale[row] = scale;
+    uint8_t* y = (uint8_t*)a.y + row * a.width;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (t + i * TPR) * V;
+      if (c < a.width) {
+        // |y / scale| <= 448 (1 + 2^-23), which rounds to at most 448: nothing saturates.
+        float z[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] = s[i][j] / scale;
+        if constexpr (V == 1) {
+          y[c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[0], 0, false);
+        } else {
+          uint32_t o[V / 4];
+#pragma unroll
+          for (int j = 0; j < V / 4; ++j) {
+            int p = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * j], z[4 * j + 1], 0, false);
+            o[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[4 * j + 2], z[4 * j + 3], p, true);
+          }
+          if constexpr (V == 8) *(uint64_t*)(y + c) = (uint64_t)o[1] << 32 | o[0];
+          else *(uint32_t*)(y + c) = o[0];
+        }
+      }
+    }
+  }
+}
+
+// a.sum: the stored sum (x itself without a residual). part: [gridDim.x][width].
+template <typename T, int V, int TPR, int NV>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_bwd_kernel(const NormArgs a) {
+  constexpr int THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR;
+  __shared__ float lds[16];
+  const int t = threadIdx.x % TPR;
+  float w[NV][V], dw[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (t + i * TPR) * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[i][j] = dw[i][j] = 0.0f;
+    if (c < a.width) load_weight<T, V>(a, c, w[i]);
+  }
+  // Without barriers in the loop (RPB > 1) the waves of a workgroup walk their rows alone.
+  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < a.rows; row += (int64_t)gridDim.x * RPB) {
+    const float r = a.rstd[row];
+    float n[NV][V], g[NV][V], dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (t + i * TPR) * V;
+      if (c < a.width) {
+        const Pack<T, V> ps = Pack<T, V>::load((const T*)a.sum + row * a.xs + c);
+        const Pack<T, V> pg = Pack<T, V>::load((const T*)a.gy + row * a.gys + c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          n[i][j] = to_acc(ps.e[j]) * r;
+          const float gy = to_acc(pg.e[j]);
+          dw[i][j] = fmaf(gy, n[i][j], dw[i][j]);
+          g[i][j] = gy * w[i][j];
+          dot = fmaf(g[i][j], n[i][j], dot);
+        }
+      }
+    }
+    dot = row_reduce<TPR, false>(dot, lds) / (float)a.width;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (t + i * TPR) * V;
+      if (c < a.width) {
+        Pack<T, V> pd;
+        float d[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] = r * fmaf(-n[i][j], dot, g[i][j]);
+        if (a.gs) {
+          const Pack<T, V> pg = Pack<T, V>::load((const T*)a.gs + row * a.gss + c);
+#pragma unroll
+          for (int j = 0; j < V; ++j) d[j] += to_acc(pg.e[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) pd.e[j] = from_acc<T>(d[j]);
+        pd.store((T*)a.dx + row * a.width + c);
+      }
+    }
+  }
+  if (!a.part) return;
+  if constexpr (RPB > 1) {
+    // The four waves' shares, added in their order.
+    extern __shared__ float share[];  // [width]
+    for (int k = 0; k < RPB; ++k) {
+      if ((int)threadIdx.x / TPR == k) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int c = (t + i * TPR) * V;
+          if (c < a.width)
+#pragma unroll
+            for (int j = 0; j < V; ++j) share[c + j] = k ? share[c + j] + dw[i][j] : dw[i][j];
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < a.width; c += THREADS) a.part[(int64_t)blockIdx.x * a.width + c] = share[c];
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (t + i * TPR) * V;
+      if (c < a.width)
+#pragma unroll
+        for (int j = 0; j < V; ++j) a.part[(int64_t)blockIdx.x * a.width + c + j] = dw[i][j];
+    }
+  }
+}
+
+// dw[c] = sum over the partial rows: 32 columns x 32 row groups per workgroup, then the
+// groups' sums in their order.
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_dw_kernel(const float* part, int n, int width, T* dw, int f32) {
+  __shared__ float s[32][33];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+  float x = 0.0f;
+  if (c < width)
+    for (int i = k; i < n; i += 32) x += part[(int64_t)i * width + c];
+  s[k][threadIdx.x & 31] = x;
+  __syncthreads();
+  if (k == 0 && c < width) {
+    x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x += s[i][threadIdx.x];
+    if (f32) ((float*)dw)[c] = x;
+    else dw[c] = from_acc<T>(x);
+  }
+}
+
+constexpr int kNormMaxWidth = 16384;
+
+struct NormPlan {
+  bool vec;
+  int tpr, nv;
+};
+
+// Threads per row and vectors per thread. One wave per row while a lane's share is at
+// most four vectors (16 single elements), as a wave reduces without barriers; then the
+// smallest workgroup that does.
+NormPlan norm_plan(int width, int V) {
+  NormPlan p{V > 1, 64, 1};
+  const int units = width / V, most = V > 1 ? 4 : 16;
+  for (int tpr : {64, 256, 1024}) {
+    p.tpr = tpr;
+    if (units <= tpr * most) break;
+  }
+  const int need = (units + p.tpr - 1) / p.tpr;
+  p.nv = V > 1 ? (need <= 1 ? 1 : need <= 2 ? 2 : 4) : (need <= 4 ? 4 : 16);
+  return p;
+}
+
+// Calls f.template go<V, TPR, NV>() for a plan.
+template <int V, int TPR, typename F> int with_nv(const NormPlan& p, F&& f) {
+  if constexpr (V > 1) return p.nv == 1 ? f.template go<V, TPR, 1>() : p.nv == 2 ? f.template go<V, TPR, 2>() : f.template go<V, TPR, 4>();
+  else return p.nv == 4 ? f.template go<V, TPR, 4>() : f.template go<V, TPR, 16>();
+}
+template <int V, typename F> int with_tpr(const NormPlan& p, F&& f) {
+  return p.tpr == 64 ? with_nv<V, 64>(p, f) : p.tpr == 256 ? with_nv<V, 256>(p, f) : with_nv<V, 1024>(p, f);
+}
+template <typename T, typename F> int with_plan(const NormPlan& p, F&& f) {
+  return p.vec ? with_tpr<16 / (int)sizeof(T)>(p, f) : with_tpr<1>(p, f);
+}
+
+template <typename T, bool F8> struct NormFwd {
+  NormArgs a;
+  hipStream_t st;
+  template <int V, int TPR, int NV> int go() {
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+    add_rms_norm_kernel<T, V, TPR, NV, F8>
+        <<<dim3((unsigned)((a.rows + RPB - 1) / RPB)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(a);
+    return check_launch("add_rms_norm");
+  }
+};
+
+int bwd_grid(const NormPlan& p, int64_t rows) {
+  const int rpb = p.tpr < 256 ? 256 / p.tpr : 1;
+  // Eight resident workgroups of 256 threads per CU, two of 1024.
+  const int64_t most = (int64_t)num_cus() * (p.tpr > 256 ? 2 : 4);
+  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rpb - 1) / rpb, most));
+}
+
+template <typename T> struct NormBwd {
+  NormArgs a;
+  hipStream_t st;
+  int grid;
+  template <int V, int TPR, int NV> int go() {
+    const size_t lds = TPR < 256 && a.part ? (size_t)a.width * sizeof(float) : 0;
+    add_rms_norm_bwd_kernel<T, V, TPR, NV><<<dim3(grid), dim3(TPR < 256 ? 256 : TPR), lds, st>>>(a);
+    return check_launch("add_rms_norm backward");
+  }
+};
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int check_sizes(const char* who, int dtype, int w_dtype, int64_t rows, int64_t width) {
+  if (dtype != LFAMD_F32 && dtype != LFAMD_F16 && dtype != LFAMD_BF16)
+    return fail(LFAMD_ERR_DTYPE, "%s: unsupported dtype %d", who, dtype);
+  if (w_dtype != dtype && w_dtype != LFAMD_F32)
+    return fail(LFAMD_ERR_DTYPE, "%s: the weight must have the input's dtype or fp32", who);
+  if (rows < 0 || width < 0) return fail(LFAMD_ERR_ARG, "%s: negative size", who);
+  if (width < 1 || width > kNormMaxWidth)
+    return fail(LFAMD_ERR_UNSUPPORTED, "%s: width %lld is outside 1 .. %d", who, (long long)width, kNormMaxWidth);
+  if (rows > INT32_MAX) return fail(LFAMD_ERR_UNSUPPORTED, "%s: too many rows", who);
+  return LFAMD_OK;
+}
+
+template <bool F8> int norm_forward(int dtype, const NormArgs& a, hipStream_t st) {
+  const int V = dtype == LFAMD_F32 ? 4 : 8;
+  const bool vec = a.width % V == 0 && a.xs % V == 0 && (!a.res || a.rs % V == 0) && aligned16(a.x) && aligned16(a.res) &&
+                   aligned16(a.y) && aligned16(a.sum) && aligned16(a.w);
+  const NormPlan p = norm_plan(a.width, vec ? V : 1);
+  switch (dtype) {
+    case LFAMD_F32: return with_plan<float>(p, NormFwd<float, F8>{a, st});
+    case LFAMD_F16: return with_plan<f16s>(p, NormFwd<f16s, F8>{a, st});
+    default: return with_plan<bf16s>(p, NormFwd<bf16s, F8>{a, st});
+  }
+}
+
+}  // namespace
+
+}  // namespace lfamd
+
+using namespace lfamd;
+
+extern "C" {
+
+int lfamd_add_rms_norm(int dtype, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                       int w_dtype, const void* weight, void* y, void* sum, float* rstd, int64_t rows, int64_t width,
+                       float eps, void* stream) {
+  if (int e = check_sizes("add_rms_norm", dtype, w_dtype, rows, width)) return e;
+  if (rows == 0) return ok();
+  if (!x || !weight || !y || (residual && !sum)) return fail(LFAMD_ERR_ARG, "add_rms_norm: null pointer");
+  NormArgs a{};
+  a.x = x, a.res = residual, a.w = weight, a.y = y, a.sum = sum, a.rstd = rstd;
+  a.xs = x_stride, a.rs = residual_stride, a.rows = rows, a.width = (int)width, a.wf32 = w_dtype == LFAMD_F32, a.eps = eps;
+  return norm_forward<false>(dtype, a, (hipStream_t)stream);
+}
+
+int lfamd_add_rms_norm_fp8(int dtype, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                           int w_dtype, const void* weight, void* y, float* scale, void* sum, int64_t rows,
+                           int64_t width, float eps, void* stream) {
+  if (int e = check_sizes("add_rms_norm_fp8", dtype, w_dtype, rows, width)) return e;
+  if (rows == 0) return ok();
+  if (!x || !weight || !y || !scale || (residual && !sum)) return fail(LFAMD_ERR_ARG, "add_rms_norm_fp8: null pointer");
+  NormArgs a{};
+  a.x = x, a.res = residual, a.w = weight, a.y = y, a.sum = sum, a.scale = scale;
+  a.xs = x_stride, a.rs = residual_stride, a.rows = rows, a.width = (int)width, a.wf32 = w_dtype == LFAMD_F32, a.eps = eps;
+  return norm_forward<true>(dtype, a, (hipStream_t)stream);
+}
+
+size_t lfamd_add_rms_norm_backward_workspace_size(int dtype, int64_t rows, int64_t width) {
+  if (rows <= 0 || width < 1 || width > kNormMaxWidth || rows > INT32_MAX) return 0;
+  // Whichever of the two layouts the tensors' alignment selects.
+  const int V = dtype == LFAMD_F32 ? 4 : 8;
+  int grid = bwd_grid(norm_plan((int)width, 1), rows);
+  if (width % V == 0) grid = std::max(grid, bwd_grid(norm_plan((int)width, V), rows));
+  return (size_t)grid * width * sizeof(float);
+}
+
+int lfamd_add_rms_norm_backward(int dtype, const void* grad_y, int64_t grad_y_stride, const void* grad_sum,
+                                int64_t grad_sum_stride, const void* sum, int64_t sum_stride, int w_dtype,
+                                const void* weight, const float* rstd, void* grad_x, void* grad_weight, int64_t rows,
+                                int64_t width, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "add_rms_norm backward";
+  if (int e = check_sizes(who, dtype, w_dtype, rows, width)) return e;
+  hipStream_t st = (hipStream_t)stream;
+  if (rows > 0 && (!grad_y || !sum || !weight || !rstd || !grad_x)) return fail(LFAMD_ERR_ARG, "%s: null pointer", who);
+  if (rows == 0 && !grad_weight) return ok();
+  NormArgs a{};
+  a.gy = grad_y, a.gs = grad_sum, a.sum = (void*)sum, a.w = weight, a.rstd = (float*)rstd, a.dx = grad_x;
+  a.gys = grad_y_stride, a.gss = grad_sum_stride, a.xs = sum_stride, a.rows = rows, a.width = (int)width;
+  a.wf32 = w_dtype == LFAMD_F32;
+  int grid = 0;
+  if (rows > 0) {
+    const int V = dtype == LFAMD_F32 ? 4 : 8;
+    const bool vec = width % V == 0 && sum_stride % V == 0 && grad_y_stride % V == 0 &&
+                     (!grad_sum || grad_sum_stride % V == 0) && aligned16(sum) && aligned16(grad_y) && aligned16(grad_sum) &&
+                     aligned16(grad_x) && aligned16(weight);
+    const NormPlan p = norm_plan((int)width, vec ? V : 1);
+    grid = bwd_grid(p, rows);
+    if (grad_weight) {
+      if (!workspace || workspace_bytes < lfamd_add_rms_norm_backward_workspace_size(dtype, rows, width))
+        return fail(LFAMD_ERR_ARG, "%s: workspace too small", who);
+      if ((uintptr_t)workspace & 3) return fail(LFAMD_ERR_ARG, "%s: workspace must be 4-byte aligned", who);
+      a.part = (float*)workspace;
+    }
+    int e;
+    switch (dtype) {
+      case LFAMD_F32: e = with_plan<float>(p, NormBwd<float>{a, st, grid}); break;
+      case LFAMD_F16: e = with_plan<f16s>(p, NormBwd<f16s>{a, st, grid}); break;
+      default: e = with_plan<bf16s>(p, NormBwd<bf16s>{a, st, grid}); break;
+    }
+    if (e) return e;
+  }
+  if (grad_weight) {
+    const dim3 g((unsigned)((width + 31) / 32)), b(1024);
+    switch (w_dtype) {
+      case LFAMD_F32: norm_dw_kernel<float><<<g, b, 0, st>>>(a.part, grid, (int)width, (float*)grad_weight, 1); break;
+      case LFAMD_F16: norm_dw_kernel<f16s><<<g, b, 0, st>>>(a.part, grid, (int)width, (f16s*)grad_weight, 0); break;
+      default: norm_dw_kernel<bf16s><<<g, b, 0, st>>>(a.part, grid, (int)width, (bf16s*)grad_weight, 0); break;
+    }
+    return check_launch(who);
+  }
+  return ok();
+}
+
+}  // extern "C"

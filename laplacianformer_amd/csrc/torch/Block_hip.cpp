@@ -1,0 +1,287 @@
+// Host adapters of the transformer-block operators: shape, type and device checks, then
+// the C ABI of include/laplacianformer_amd.h on the tensors' device and current stream.
+#include "Block.h"
+
+#include <ATen/ATen.h>
+
+#include <cmath>
+
+#include "torch_common.h"
+
+namespace laplace {
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<at::Tensor>;
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// Rows of `width` elements at one stride: the tensor itself where its leading
+// dimensions collapse, else a contiguous copy. Returns the row stride.
+int64_t row_view(Tensor& t) {
+  const int nd = (int)t.dim();
+  const int64_t w = t.size(nd - 1);
+  if (t.stride(nd - 1) != 1 && w != 1) t = t.contiguous();
+  int64_t stride = 0, span = 1;
+  for (int i = nd - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (span == 1) stride = t.stride(i);
+    else if (t.stride(i) != stride * span) {
+      t = t.contiguous();
+      return w;
+    }
+    span *= t.size(i);
+  }
+  return span == 1 ? w : stride;
+}
+
+struct NormIn {
+  Tensor x, res;
+  int64_t xs = 0, rs = 0, rows = 0, width = 0;
+  int dt = 0, wt = 0;
+};
+
+NormIn norm_in(const char* op, const Tensor& x, const Tensor& weight, const OptTensor& residual) {
+  TORCH_CHECK(x.is_cuda(), op, ": tensors must be on GPU");
+  TORCH_CHECK(x.dim() >= 1, op, ": x needs at least one dimension");
+  NormIn n;
+  n.dt = detail::abi_dtype(x, op);
+  n.wt = detail::abi_dtype(weight, op);
+  TORCH_CHECK(weight.is_cuda() && weight.device() == x.device(), op, ": weight must be on the same GPU as x");
+  TORCH_CHECK(weight.dim() == 1 && weight.size(0) == x.size(-1), op, ": weight must have x's last size, ", x.size(-1));
+  n.width = x.size(-1);
+  n.rows = n.width ? x.numel() / n.width : 0;
+  n.x = x;
+  n.xs = row_view(n.x);
+  if (given(residual)) {
+    TORCH_CHECK(residual->sizes() == x.sizes(), op, ": residual and x must have the same shape");
+    detail::same_type(x, *residual, "residual");
+    n.res = *residual;
+    n.rs = row_view(n.res);
+  }
+  return n;
+}
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+}  // namespace
+
+std::vector<Tensor> AddRmsNorm_forward(const Tensor x, const Tensor weight, const OptTensor residual, double eps,
+                                       bool need_rstd) {
+  const Tensor w = weight.contiguous();
+  NormIn n = norm_in("add_rms_norm", x, weight, residual);
+  at::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  Tensor y = at::empty(x.sizes(), x.options()), sum, rstd;
+  if (n.res.defined()) sum = at::empty(x.sizes(), x.options());
+  if (need_rstd) rstd = at::empty({n.rows}, x.options().dtype(at::kFloat));
+  detail::check_status(lfamd_add_rms_norm(n.dt, ptr(n.x), n.xs, ptr(n.res), n.rs, n.wt, ptr(w), ptr(y), ptr(sum),
+                                          (float*)ptr(rstd), n.rows, n.width, (float)eps, detail::stream_of(x)));
+  return {y, sum.defined() ? sum : x, rstd.defined() ? rstd : at::empty({0}, x.options().dtype(at::kFloat))};
+}
+
+std::vector<Tensor> AddRmsNorm_forward_fp8(const Tensor x, const Tensor weight, const OptTensor residual, double eps) {
+  const Tensor w = weight.contiguous();
+  NormIn n = norm_in("add_rms_norm_fp8", x, weight, residual);
+  at::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  std::vector<int64_t> ss(x.sizes().begin(), x.sizes().end());
+  ss.back() = 1;
+  Tensor y = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)), scale = at::empty(ss, x.options().dtype(at::kFloat)), sum;
+  if (n.res.defined()) sum = at::empty(x.sizes(), x.options());
+  detail::check_status(lfamd_add_rms_norm_fp8(n.dt, ptr(n.x), n.xs, ptr(n.res), n.rs, n.wt, ptr(w), ptr(y),
+                                              (float*)ptr(scale), ptr(sum), n.rows, n.width, (float)eps,
+                                              detail::stream_of(x)));
+  return {y, scale, sum.defined() ? sum : x};
+}
+
+std::vector<Tensor> AddRmsNorm_backward(const Tensor grad_y, const OptTensor grad_sum, const Tensor sum,
+                                        const Tensor weight, const Tensor rstd, bool need_weight) {
+  const char* op = "add_rms_norm backward";
+  const Tensor w = weight.contiguous();
+  NormIn n = norm_in(op, sum, weight, std::nullopt);
+  TORCH_CHECK(grad_y.sizes() == sum.sizes(), op, ": grad_y and the sum must have the same shape");
+  detail::same_type(sum, grad_y, "grad_y");
+  TORCH_CHECK(rstd.scalar_type() == at::kFloat && rstd.numel() == n.rows && rstd.is_contiguous() && rstd.device() == sum.device(),
+              op, ": rstd must be the forward's");
+  Tensor gy = grad_y, gs;
+  const int64_t gys = row_view(gy);
+  int64_t gss = 0;
+  if (given(grad_sum)) {
+    TORCH_CHECK(grad_sum->sizes() == sum.sizes(), op, ": grad_sum and the sum must have the same shape");
+    detail::same_type(sum, *grad_sum, "grad_sum");
+    gs = *grad_sum;
+    gss = row_view(gs);
+  }
+  at::hip::HIPGuardMasqueradingAsCUDA guard(sum.device());
+  Tensor dx = at::empty(sum.sizes(), sum.options()), dw, ws;
+  size_t wsb = 0;
+  if (need_weight) {
+    dw = at::empty_like(w);
+    wsb = lfamd_add_rms_norm_backward_workspace_size(n.dt, n.rows, n.width);
+    ws = at::empty({(int64_t)wsb}, sum.options().dtype(at::kByte));
+  }
+  detail::check_status(lfamd_add_rms_norm_backward(n.dt, ptr(gy), gys, ptr(gs), gss, ptr(n.x), n.xs, n.wt, ptr(w),
+                                                   rstd.data_ptr<float>(), ptr(dx), ptr(dw), n.rows, n.width, ptr(ws), wsb,
+                                                   detail::stream_of(sum)));
+  return {dx, need_weight ? dw : Tensor()};
+}
+
+namespace {
+
+// [B, heads, tokens, channels] with adjacent channels.
+Tensor unit_last(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+}  // namespace
+
+std::vector<Tensor> Rotary(const Tensor q, const OptTensor k, const Tensor positions, const std::vector<int64_t> sections,
+                           double base, bool interleaved, bool inverse) {
+  const char* op = "rotary";
+  TORCH_CHECK(q.is_cuda(), op, ": tensors must be on GPU");
+  TORCH_CHECK(q.dim() == 4, op, ": q must be [batch, heads, tokens, channels]");
+  const int dt = detail::abi_dtype(q, op);
+  const int64_t B = q.size(0), N = q.size(2), D = q.size(3);
+  const bool has_k = given(k);
+  if (has_k) {
+    TORCH_CHECK(k->dim() == 4 && k->size(0) == B && k->size(2) == N && k->size(3) == D, op,
+                ": q and k may differ in their heads only, got ", q.sizes(), " and ", k->sizes());
+    detail::same_type(q, *k, "k");
+  }
+  const int64_t A = (int64_t)sections.size();
+  TORCH_CHECK(positions.is_cuda() && positions.device() == q.device(), op, ": positions must be on the same GPU as q");
+  TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, op,
+              ": positions must be int32 or int64");
+  TORCH_CHECK((positions.dim() == 2 && positions.size(0) == A && positions.size(1) == N) ||
+                  (positions.dim() == 3 && positions.size(0) == A && positions.size(1) == B && positions.size(2) == N),
+              op, ": positions must be [axes, tokens] or [axes, batch, tokens] with ", A, " axes and ", N, " tokens, got ",
+              positions.sizes());
+  const int64_t ps[3] = {positions.stride(0), positions.dim() == 3 ? positions.stride(1) : 0, positions.stride(-1)};
+  at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  const Tensor qi = unit_last(q), ki = has_k ? unit_last(*k) : Tensor();
+  Tensor qo = at::empty_like(qi), ko = has_k ? at::empty_like(ki) : Tensor();
+  detail::check_status(lfamd_rotary(dt, ptr(qi), qi.strides().data(), ptr(qo), qo.strides().data(), q.size(1), ptr(ki),
+                                    has_k ? ki.strides().data() : nullptr, ptr(ko), has_k ? ko.strides().data() : nullptr,
+                                    has_k ? k->size(1) : 0, B, N, D, ptr(positions), positions.scalar_type() == at::kLong,
+                                    ps, (int)A, sections.data(), base, interleaved, inverse, detail::stream_of(q)));
+  return {qo, ko};
+}
+
+namespace {
+
+struct AttnIn {
+  Tensor q, k, v, mask;
+  lfamd_attention d{};
+  int dt = 0;
+};
+
+const int32_t* per_batch(const char* op, const Tensor& q, const OptTensor& t, const char* name) {
+  if (!given(t)) return nullptr;
+  TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == q.size(0) && t->is_contiguous(), op, ": ", name,
+              " must be a contiguous int32 tensor of one value per sequence");
+  TORCH_CHECK(t->is_cuda() && t->device() == q.device(), op, ": ", name, " must be on the same GPU as q");
+  return t->data_ptr<int32_t>();
+}
+
+void set_strides(int64_t* to, const Tensor& t) {
+  for (int i = 0; i < 3; ++i) to[i] = t.stride(i);
+}
+
+AttnIn attn_in(const char* op, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask, bool causal,
+               const OptTensor& k_lengths, const OptTensor& q_lengths, const OptTensor& q_starts, double scale) {
+  TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda(), op, ": tensors must be on GPU");
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, op, ": q, k and v must be [batch, heads, tokens, channels]");
+  AttnIn in;
+  in.dt = detail::abi_dtype(q, op);
+  detail::same_type(q, k, "k");
+  detail::same_type(q, v, "v");
+  TORCH_CHECK(k.sizes() == v.sizes(), op, ": k and v must have the same shape, got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(3) == q.size(3), op, ": q ", q.sizes(), " and k ", k.sizes(),
+              " differ in batch or channels");
+  in.q = unit_last(q), in.k = unit_last(k), in.v = unit_last(v);
+  lfamd_attention& d = in.d;
+  d.batch = q.size(0), d.heads = q.size(1), d.kv_heads = k.size(1), d.q_len = q.size(2), d.k_len = k.size(2);
+  d.head_dim = q.size(3);
+  set_strides(d.q_strides, in.q);
+  set_strides(d.k_strides, in.k);
+  set_strides(d.v_strides, in.v);
+  d.k_lengths = per_batch(op, q, k_lengths, "k_lengths");
+  d.q_lengths = per_batch(op, q, q_lengths, "q_lengths");
+  d.q_starts = per_batch(op, q, q_starts, "q_starts");
+  if (given(mask)) {
+    TORCH_CHECK(mask->is_cuda() && mask->device() == q.device(), op, ": mask must be on the same GPU as q");
+    switch (mask->scalar_type()) {
+      case at::kBool: d.mask_kind = LFAMD_MASK_BOOL; break;
+      case at::kFloat: d.mask_kind = LFAMD_MASK_F32; break;
+      case at::kHalf: d.mask_kind = LFAMD_MASK_F16; break;
+      case at::kBFloat16: d.mask_kind = LFAMD_MASK_BF16; break;
+      default: TORCH_CHECK(false, op, ": mask must be bool, float32, float16 or bfloat16");
+    }
+    const int64_t full[4] = {d.batch, d.heads, d.q_len, d.k_len};
+    TORCH_CHECK(mask->dim() <= 4, op, ": mask must broadcast to [batch, heads, queries, keys]");
+    for (int i = 0; i < 4; ++i) {
+      const int j = i - (4 - (int)mask->dim());
+      const int64_t size = j < 0 ? 1 : mask->size(j);
+      TORCH_CHECK(size == full[i] || size == 1, op, ": mask ", mask->sizes(), " does not broadcast to [", d.batch, ", ", d.heads,
+                  ", ", d.q_len, ", ", d.k_len, "]");
+      d.mask_strides[i] = size == 1 ? 0 : mask->stride(j);
+    }
+    in.mask = *mask;
+    d.mask = mask->data_ptr();
+  }
+  d.causal = causal;
+  d.scale = (float)scale;
+  return in;
+}
+
+}  // namespace
+
+std::vector<Tensor> SoftmaxAttention_forward(const Tensor q, const Tensor k, const Tensor v, const OptTensor mask,
+                                             bool causal, const OptTensor k_lengths, const OptTensor q_lengths,
+                                             const OptTensor q_starts, double scale, bool need_stats) {
+  AttnIn in = attn_in("softmax_attention", q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale);
+  at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  Tensor out = at::empty_like(in.q), stats, ws;
+  set_strides(in.d.out_strides, out);
+  if (need_stats)
+    stats = at::empty({in.d.mask_kind ? 2 : 1, in.d.batch, in.d.heads, in.d.q_len}, q.options().dtype(at::kFloat));
+  const size_t wsb = lfamd_softmax_attention_workspace_size(in.dt, &in.d);
+  if (wsb) ws = at::empty({(int64_t)wsb}, q.options().dtype(at::kByte));
+  detail::check_status(lfamd_softmax_attention(in.dt, &in.d, ptr(in.q), ptr(in.k), ptr(in.v), ptr(out),
+                                               (float*)ptr(stats), ptr(ws), wsb, detail::stream_of(q)));
+  return {out, stats};
+}
+
+std::vector<Tensor> SoftmaxAttention_backward(const Tensor grad_out, const Tensor q, const Tensor k, const Tensor v,
+                                              const Tensor out, const Tensor stats, const OptTensor mask, bool causal,
+                                              const OptTensor k_lengths, const OptTensor q_lengths,
+                                              const OptTensor q_starts, double scale, bool need_q, bool need_kv) {
+  const char* op = "softmax_attention backward";
+  AttnIn in = attn_in(op, q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale);
+  TORCH_CHECK(grad_out.sizes() == q.sizes() && out.sizes() == q.sizes(), op, ": grad_out, out and q must have the same shape");
+  detail::same_type(q, grad_out, "grad_out");
+  detail::same_type(q, out, "out");
+  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.device() == q.device() &&
+                  stats.numel() == (in.d.mask_kind ? 2 : 1) * in.d.batch * in.d.heads * in.d.q_len,
+              op, ": stats must be the forward's");
+  at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  const Tensor o = unit_last(out), g = unit_last(grad_out);
+  set_strides(in.d.out_strides, o);
+  Tensor dq, dk, dv;
+  lfamd_attention_grads gr{};
+  if (need_q) dq = at::empty_like(in.q);
+  if (need_kv) dk = at::empty_like(in.k), dv = at::empty_like(in.v);
+  gr.grad_out = ptr(g);
+  set_strides(gr.grad_out_strides, g);
+  if (need_q) gr.grad_q = ptr(dq), set_strides(gr.grad_q_strides, dq);
+  if (need_kv) {
+    gr.grad_k = ptr(dk), gr.grad_v = ptr(dv);
+    set_strides(gr.grad_k_strides, dk);
+    set_strides(gr.grad_v_strides, dv);
+  }
+  const size_t wsb = lfamd_softmax_attention_backward_workspace_size(in.dt, &in.d);
+  const Tensor ws = at::empty({(int64_t)wsb}, q.options().dtype(at::kByte));
+  detail::check_status(lfamd_softmax_attention_backward(in.dt, &in.d, ptr(in.q), ptr(in.k), ptr(in.v), ptr(o),
+                                                        stats.data_ptr<float>(), &gr, ptr(ws), wsb, detail::stream_of(q)));
+  return {dq, dk, dv};
+}
+
+}  // namespace laplace
