@@ -26,8 +26,18 @@ namespace {
 
 constexpr float kPShift = 15.0f;
 
-// Streamed rows per LDS tile, taken in blocks of 32.
-template <typename T, int DP> constexpr int stream_tile() { return sizeof(T) == 2 || DP == 32 ? 64 : 32; }
+// Streamed rows per LDS tile, taken in blocks of 32: queries (dk, dv), keys (dq).
+template <typename T, int DP> constexpr int query_tile() { return DP < 128 && (sizeof(T) == 2 || DP == 32) ? 64 : 32; }
+template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 2 || DP == 32 ? 64 : 32; }
+
+// At 128 channels the accumulators of dk and dv and both owned operands are more than a lane's
+// registers at two waves per SIMD (128 + 64 + 64 with the scores): V is read from LDS then.
+template <int DP> constexpr bool v_in_lds() { return DP >= 128; }
+
+template <typename T, int DP> constexpr size_t dkdv_lds() {
+  return (size_t)2 * query_tile<T, DP>() * (2 * DP * sizeof(T) + 16) + (v_in_lds<DP>() ? 128 * DP * sizeof(T) : 0);
+}
+template <typename T, int DP> constexpr size_t dq_lds() { return (size_t)2 * key_tile<T, DP>() * 2 * DP * sizeof(T); }
 
 // delta_i, and for fp16 the maxima over 64 rows of |g_i| and |delta_i|, or over 64
 // keys of |v_j|. A workgroup takes 64 rows of one head: four threads per row.
@@ -49,10 +59,10 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
     bool live = in;
     if (in && a.keyMask) {
       const int64_t off = (int64_t)b * a.ms[0] + (int64_t)row * a.ms[3];
-      live = a.maskKind == kMaskBool ? ((const uint8_t*)a.mask)[off] != 0 : mask_bias(a, off) != kNegInf;
+      live = mask_bias(a, off) != kNegInf;
     }
     for (int c = part * CE; c < a.D; c += 4 * CE) {
-      const u32x4 x = load_chunk<T>(p, live, c, a.D, a.vecV);
+      const u32x4 x = load_chunk<T>(p, live, c, a.D, a.modeV != kElements);
 #pragma unroll
       for (int j = 0; j < CE; ++j) {
         const float v = to_acc(((const T*)&x)[j]);
@@ -64,7 +74,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
     const T* po = (const T*)a.o + (int64_t)b * a.os[0] + (int64_t)hd * a.os[1] + (int64_t)row * a.os[2];
     const T* pg = (const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)hd * a.gs[1] + (int64_t)row * a.gs[2];
     for (int c = part * CE; c < a.D; c += 4 * CE) {
-      const u32x4 x = load_chunk<T>(po, in, c, a.D, a.vecO), y = load_chunk<T>(pg, in, c, a.D, a.vecG);
+      const u32x4 x = load_chunk<T>(po, in, c, a.D, a.vecO), y = load_chunk<T>(pg, in, c, a.D, a.modeG != kElements);
 #pragma unroll
       for (int j = 0; j < CE; ++j) {
         const float u = to_acc(((const T*)&x)[j]), v = to_acc(((const T*)&y)[j]);
@@ -133,48 +143,23 @@ template <bool MASK> __device__ __forceinline__ float prob(float s, float c, flo
   return MASK ? exp2_fast((s - x0) * kLog2e) * x1 : exp2_fast(fmaf(s, c, -x0));
 }
 
-// The masked score of key j for a row (natural units).
-__device__ __forceinline__ float masked(const AttnArgs& a, float s, int j, int lim, int64_t moff) {
-  if (j >= lim) return kNegInf;
-  const int64_t off = moff + (int64_t)j * a.ms[3];
-  if (a.maskKind == kMaskBool) return ((const uint8_t*)a.mask)[off] ? s * a.scale : kNegInf;
-  const float bias = mask_bias(a, off);
-  return bias == kNegInf ? kNegInf : fmaf(s, a.scale, bias);
-}
-
 // Whether key j of sequence b takes part at all.
 template <bool MASK> __device__ __forceinline__ bool key_live(const AttnArgs& a, int b, int j, int klen) {
   if (j >= klen) return false;
   if (!MASK || !a.keyMask) return true;
   const int64_t off = (int64_t)b * a.ms[0] + (int64_t)j * a.ms[3];
-  return a.maskKind == kMaskBool ? ((const uint8_t*)a.mask)[off] != 0 : mask_bias(a, off) != kNegInf;
-}
-
-// Loads of K or V rows that leave out what key_live does.
-template <typename T, int DP, int ROWS, bool MASK>
-__device__ __forceinline__ void load_keys(const AttnArgs& a, Stage<T, DP, ROWS, 256>& s, const T* base, int64_t stride,
-                                          int b, int row0, int limit, bool vec) {
-  if (MASK && a.keyMask) {
-    using L = Tile<T, DP>;
-    const int c = threadIdx.x % L::CPR, rr = threadIdx.x / L::CPR;
-#pragma unroll
-    for (int i = 0; i < s.NIT; ++i) {
-      const int row = row0 + rr + i * s.RPI;
-      s.r[i] = load_chunk<T>(base + (int64_t)row * stride, key_live<MASK>(a, b, row, limit), c * L::CE, a.D, vec);
-    }
-  } else {
-    s.load(base, stride, row0, limit, a.D, vec);
-  }
+  return mask_bias(a, off) != kNegInf;
 }
 
 // dk and dv of 128 keys, 32 per wave; queries stream through LDS in tiles of QT.
 template <typename T, int DP, bool MASK>
-__global__ void __launch_bounds__(256, DP >= 128 || sizeof(T) == 4 ? 1 : 2) attn_dkdv_kernel(const AttnArgs a) {
-  constexpr int QT = stream_tile<T, DP>(), NT = DP / 16, ND = DP / 32;
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2) attn_dkdv_kernel(const AttnArgs a) {
+  constexpr int QT = query_tile<T, DP>(), NT = DP / 16, ND = DP / 32;
   constexpr bool F16 = std::is_same<T, f16s>::value;
   using L = Tile<T, DP>;
   constexpr int TB = QT * L::ROW, SB = QT * 16;  // bytes of a tile, and of its rows' statistics
-  extern __shared__ __align__(16) char smem[];   // [2][q tile, g tile], [2][lse, delta, 1 / sum, last key]
+  constexpr bool VL = v_in_lds<DP>();
+  extern __shared__ __align__(16) char smem[];   // [2][q tile, g tile], [2][lse, delta, 1 / sum, last key], [v tile]
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
   const uint32_t place = xcd_place(blockIdx.x, gridDim.x);
@@ -191,32 +176,42 @@ __global__ void __launch_bounds__(256, DP >= 128 || sizeof(T) == 4 ? 1 : 2) attn
   const int beg = min(split * share, total), end = min(beg + share, total);
 
   const bool live = key_live<MASK>(a, b, mykey, klen);
-  Frag<T> kf[NT], vf[NT];
+  Frag<T> kf[NT], vf[VL ? 1 : NT];
+  const char* tv = smem + 4 * TB + 2 * SB + wave * 32 * L::ROW;
   {
     const int kr = live ? mykey : 0;
     const T* kp = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1] + (int64_t)kr * a.ks[2];
     const T* vp = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1] + (int64_t)kr * a.vs[2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      kf[t] = global_frag<T>(kp, live, t, h, a.D, a.vecK);
-      vf[t] = global_frag<T>(vp, live, t, h, a.D, a.vecV);
+      kf[t] = global_frag<T>(kp, live, t, h, a.D, a.modeK != kElements);
+      if constexpr (!VL) vf[t] = global_frag<T>(vp, live, t, h, a.D, a.modeV != kElements);
+    }
+    if constexpr (VL) {
+      using LV = Loader<T, DP, 128>;
+      const uint32_t bits = MASK && a.keyMask && klen > 0 ? live_keys<LV>(a, b, key0) : ~0u;
+      LV::fill(smem + 4 * TB + 2 * SB, (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1], a.vs[2], key0, klen, a.D,
+               a.modeV, bits);
     }
   }
   const float f = F16 ? dz_factor(a, b, hk) : 1.0f;
   // fp16: p carries 2^15 and dz the factor f: dz = (p 2^15) ((g.v) f' - delta f'), f' = f 2^-15.
   const float fd = F16 ? f * exp2f(-kPShift) : 1.0f;
 
+  const int64_t moff = (int64_t)b * a.ms[0] + (int64_t)min(mykey, a.M - 1) * a.ms[3];
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
 
-  Stage<T, DP, QT, 256> sq, sg;
+  using LD = Loader<T, DP, QT>;
   float st0 = 0.0f, st1 = 0.0f, st2 = 0.0f;
   int st3 = 0;
-  auto load = [&](int step) {
+  auto fill = [&](int buf, int step) {
     const int g = step / perHead, row0 = (tb + step % perHead) * QT, hq = hk * a.G + g;
-    sq.load((const T*)a.q + (int64_t)b * a.qs[0] + (int64_t)hq * a.qs[1], a.qs[2], row0, qlen, a.D, a.vecQ);
-    sg.load((const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)hq * a.gs[1], a.gs[2], row0, qlen, a.D, a.vecG);
+    LD::fill(smem + buf * 2 * TB, (const T*)a.q + (int64_t)b * a.qs[0] + (int64_t)hq * a.qs[1], a.qs[2], row0, qlen, a.D,
+             a.modeQ);
+    LD::fill(smem + buf * 2 * TB + TB, (const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)hq * a.gs[1], a.gs[2], row0, qlen,
+             a.D, a.modeG);
     if (threadIdx.x < QT) {
       const int n = row0 + threadIdx.x;
       const bool in = n < qlen;
@@ -231,9 +226,7 @@ __global__ void __launch_bounds__(256, DP >= 128 || sizeof(T) == 4 ? 1 : 2) attn
       }
     }
   };
-  auto store = [&](int buf) {
-    sq.store(smem + buf * 2 * TB);
-    sg.store(smem + buf * 2 * TB + TB);
+  auto store = [&](int buf) {  // the rows' statistics, through registers
     if (threadIdx.x < QT) {
       float* s = (float*)(smem + 4 * TB + buf * SB);
       s[threadIdx.x] = st0;
@@ -244,25 +237,29 @@ __global__ void __launch_bounds__(256, DP >= 128 || sizeof(T) == 4 ? 1 : 2) attn
   };
 
   if (beg < end) {
-    load(beg);
+    fill(0, beg);
     store(0);
   }
+  land();
   __syncthreads();
+  const int rl0 = L::row_lane(lane), cl0 = L::col_lane(lane);
   int buf = 0;
   for (int step = beg; step < end; ++step) {
     const bool more = step + 1 < end;
-    if (more) load(step + 1);
+    if (more) fill(buf ^ 1, step + 1);
     const char* tq = smem + buf * 2 * TB;
     const char* tg = tq + TB;
     const float* stats = (const float*)(smem + 4 * TB + buf * SB);
     const int g = step / perHead, row0 = (tb + step % perHead) * QT, hq = hk * a.G + g;
-#pragma unroll
+#pragma unroll 1
     for (int qb = 0; qb < QT; qb += 32) {
-      f32x16 s{}, dp{};
+      const int rl = launder(rl0), cl = launder(cl0);
+      f32x16 s{}, dp{}, bias;
+      if constexpr (MASK) mask_of_queries(a, moff + (int64_t)hq * a.ms[1], row0 + qb, h, bias);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) s = mma<T>(L::row_frag(tq, qb + (lane & 31), t, h), kf[t], s);
+      for (int t = 0; t < NT; ++t) s = mma<T>(L::row_frag(tq + qb * L::ROW, rl, t), kf[t], s);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) dp = mma<T>(L::row_frag(tg, qb + (lane & 31), t, h), vf[t], dp);
+      for (int t = 0; t < NT; ++t) dp = mma<T>(L::row_frag(tg + qb * L::ROW, rl, t), VL ? L::row_frag(tv, rl, t) : vf[VL ? 0 : t], dp);
       // Every row sees every key of the wave: nothing to leave out.
       const int wlast = key0 + wave * 32 + 31;
       const bool check = MASK || wlast >= klen || row0 + qb + 32 > qlen || (a.causal && wlast > qstart + row0 + qb);
@@ -276,11 +273,8 @@ __global__ void __launch_bounds__(256, DP >= 128 || sizeof(T) == 4 ? 1 : 2) attn
         for (int i = 0; i < 4; ++i) {
           const int r = 4 * rq + i;
           float x = s[r];
-          if constexpr (MASK) {
-            const int n = min(row0 + rr + i, a.N - 1);
-            x = masked(a, x, mykey, ((const int*)stats)[3 * QT + rr + i],
-                       (int64_t)b * a.ms[0] + (int64_t)hq * a.ms[1] + (int64_t)n * a.ms[2]);
-          }
+          if constexpr (MASK)
+            x = mykey < ((const int*)stats)[3 * QT + rr + i] ? masked_score(a, x, bias[r]) : kNegInf;
           float p = prob<MASK>(x, a.c, x0[i], x1[i]);
           float z = p * (F16 ? fmaf(dp[r], fd, -de[i]) : dp[r] - de[i]);
           if (check) {
@@ -297,13 +291,14 @@ __global__ void __launch_bounds__(256, DP >= 128 || sizeof(T) == 4 ? 1 : 2) attn
         const Frag<T> pf = acc_frag<T>(s, st), zf = acc_frag<T>(dp, st);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-          dv[d] = mma<T>(L::col_frag(tg, qb, st, d, lane), pf, dv[d]);
-          dk[d] = mma<T>(L::col_frag(tq, qb, st, d, lane), zf, dk[d]);
+          dv[d] = mma<T>(L::col_frag(tg + qb * L::ROW, cl, st, d), pf, dv[d]);
+          dk[d] = mma<T>(L::col_frag(tq + qb * L::ROW, cl, st, d), zf, dk[d]);
         }
       }
     }
     if (more) store(buf ^ 1);
     buf ^= 1;
+    land();
     __syncthreads();
   }
 
@@ -335,7 +330,7 @@ __global__ void __launch_bounds__(256, DP >= 128 || sizeof(T) == 4 ? 1 : 2) attn
 // dq of 128 queries of one head, 32 per wave; keys stream through LDS in tiles of KT.
 template <typename T, int DP, bool MASK>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn_dq_kernel(const AttnArgs a) {
-  constexpr int KT = stream_tile<T, DP>(), NT = DP / 16, ND = DP / 32;
+  constexpr int KT = key_tile<T, DP>(), NT = DP / 16, ND = DP / 32;
   constexpr bool F16 = std::is_same<T, f16s>::value;
   using L = Tile<T, DP>;
   constexpr int TB = KT * L::ROW;
@@ -362,8 +357,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
     const T* gp = (const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)hq * a.gs[1] + (int64_t)nr * a.gs[2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      qf[t] = global_frag<T>(qp, alive, t, h, a.D, a.vecQ);
-      gf[t] = global_frag<T>(gp, alive, t, h, a.D, a.vecG);
+      qf[t] = global_frag<T>(qp, alive, t, h, a.D, a.modeQ != kElements);
+      gf[t] = global_frag<T>(gp, alive, t, h, a.D, a.modeG != kElements);
     }
   }
   const float f = F16 ? dz_factor(a, b, hk) : 1.0f;
@@ -379,40 +374,44 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
 
   const T* kbase = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1];
   const T* vbase = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1];
-  Stage<T, DP, KT, 256> sk, sv;
-  auto load = [&](int k0) {
-    load_keys<T, DP, KT, MASK>(a, sk, kbase, a.ks[2], b, k0, kend, a.vecK);
-    load_keys<T, DP, KT, MASK>(a, sv, vbase, a.vs[2], b, k0, kend, a.vecV);
+  using LD = Loader<T, DP, KT>;
+  const bool byKey = MASK && a.keyMask;
+  auto fill = [&](int buf, int k0, uint32_t live) {
+    LD::fill(smem + buf * 2 * TB, kbase, a.ks[2], k0, kend, a.D, a.modeK, live);
+    LD::fill(smem + buf * 2 * TB + TB, vbase, a.vs[2], k0, kend, a.D, a.modeV, live);
   };
-  auto store = [&](int buf) {
-    sk.store(smem + buf * 2 * TB);
-    sv.store(smem + buf * 2 * TB + TB);
-  };
+  uint32_t live = ~0u;  // of the next tile to fill
   if (kbeg < kend) {
-    load(kbeg);
-    store(0);
+    if (byKey) live = live_keys<LD>(a, b, kbeg);
+    fill(0, kbeg, live);
+    if (byKey) live = live_keys<LD>(a, b, kbeg + KT);
   }
+  land();
   __syncthreads();
+  const int rl0 = L::row_lane(lane), cl0 = L::col_lane(lane);
   int buf = 0;
   for (int key0 = kbeg; key0 < kend; key0 += KT) {
     const bool more = key0 + KT < kend;
-    if (more) load(key0 + KT);
+    if (more) fill(buf ^ 1, key0 + KT, live);
+    if (byKey) live = live_keys<LD>(a, b, key0 + 2 * KT);
     const char* tk = smem + buf * 2 * TB;
     const char* tv = tk + TB;
-#pragma unroll
+#pragma unroll 1
     for (int kb = 0; kb < KT; kb += 32) {
       if (key0 + kb >= wend) break;
-      f32x16 s{}, dp{};
+      const int rl = launder(rl0), cl = launder(cl0);
+      f32x16 s{}, dp{}, bias;
+      if constexpr (MASK) mask_of_keys(a, moff, key0 + kb, h, bias);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) s = mma<T>(L::row_frag(tk, kb + (lane & 31), t, h), qf[t], s);
+      for (int t = 0; t < NT; ++t) s = mma<T>(L::row_frag(tk + kb * L::ROW, rl, t), qf[t], s);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) dp = mma<T>(L::row_frag(tv, kb + (lane & 31), t, h), gf[t], dp);
+      for (int t = 0; t < NT; ++t) dp = mma<T>(L::row_frag(tv + kb * L::ROW, rl, t), gf[t], dp);
       const bool check = MASK || key0 + kb + 32 > full;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int j = key0 + kb + 8 * (r >> 2) + 4 * h + (r & 3);
         float x = s[r];
-        if constexpr (MASK) x = masked(a, x, j, lim, moff);
+        if constexpr (MASK) x = j < lim ? masked_score(a, x, bias[r]) : kNegInf;
         const float p = prob<MASK>(x, a.c, x0, x1);
         float z = p * (F16 ? fmaf(dp[r], f, -de) : dp[r] - de);
         if (check) z = (MASK ? x == kNegInf : j >= lim) ? 0.0f : z;
@@ -422,11 +421,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
       for (int st = 0; st < 2; ++st) {
         const Frag<T> zf = acc_frag<T>(dp, st);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) dq[d] = mma<T>(L::col_frag(tk, kb, st, d, lane), zf, dq[d]);
+        for (int d = 0; d < ND; ++d) dq[d] = mma<T>(L::col_frag(tk + kb * L::ROW, cl, st, d), zf, dq[d]);
       }
     }
-    if (more) store(buf ^ 1);
     buf ^= 1;
+    land();
     __syncthreads();
   }
 
@@ -476,8 +475,9 @@ BwdPlan bwd_plan(int dtype, const AttnArgs& a, int cus) {
   // The other axis is split where a kernel's own blocks leave CUs without work, into
   // shares of four tiles at least.
   const int64_t kw = (int64_t)a.B * a.Hk * p.ktiles, qw = (int64_t)a.B * a.H * p.qtiles;
-  const int tile = dtype != LFAMD_F32 || p.dp == 32 ? 64 : 32;  // stream_tile
-  const int64_t ksteps = (int64_t)a.G * ((a.N + tile - 1) / tile), qsteps = (a.M + tile - 1) / tile;
+  const bool wide = dtype != LFAMD_F32 || p.dp == 32;
+  const int qt = wide && p.dp < 128 ? 64 : 32, kt = wide ? 64 : 32;  // query_tile, key_tile
+  const int64_t ksteps = (int64_t)a.G * ((a.N + qt - 1) / qt), qsteps = (a.M + kt - 1) / kt;
   auto splits = [&](int64_t wgs, int64_t steps) {
     if (wgs >= cus || steps < 8) return 1;
     return (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + wgs - 1) / wgs, steps / 4, 64}));
@@ -516,7 +516,7 @@ template <typename T, int DP, bool MASK> int bwd_launch(AttnArgs a, const BwdPla
   if (a.dk) {
     a.nsplit = p.ksplit;
     a.tiles = p.ktiles;
-    const size_t lds = (size_t)2 * stream_tile<T, DP>() * (2 * DP * sizeof(T) + 16);
+    const size_t lds = dkdv_lds<T, DP>();
     if (int e = launch((const void*)attn_dkdv_kernel<T, DP, MASK>, (int64_t)a.B * a.Hk * p.ktiles * p.ksplit, lds, a, st))
       return e;
     if (p.ksplit > 1) {
@@ -534,7 +534,7 @@ template <typename T, int DP, bool MASK> int bwd_launch(AttnArgs a, const BwdPla
     a.nsplit = p.qsplit;
     a.tiles = p.qtiles;
     a.chunk = p.qchunk;
-    const size_t lds = (size_t)2 * stream_tile<T, DP>() * 2 * DP * sizeof(T);
+    const size_t lds = dq_lds<T, DP>();
     if (int e = launch((const void*)attn_dq_kernel<T, DP, MASK>, (int64_t)a.B * a.H * p.qtiles * p.qsplit, lds, a, st))
       return e;
     if (p.qsplit > 1) {

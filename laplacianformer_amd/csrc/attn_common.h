@@ -105,47 +105,71 @@ template <typename T, int DP> struct Tile {
   }
   static __device__ __forceinline__ int at(int row, int chunk) { return row * ROW + ((chunk ^ swz(row)) << 4); }
 
-  // Elements 16 t + 8 h .. + 7 of row `row`.
-  static __device__ __forceinline__ Frag<T> row_frag(const char* tile, int row, int t, int h) {
+  // A lane's byte offset into a tile for row_frag and col_frag; the terms of t, db, s and the
+  // block of rows are exclusive-ors and sums of constants on it (`tile` may point at any multiple
+  // of 16 rows). Kernels pass it through launder() once per tile: one exclusive-or in front of a
+  // read costs less than the registers that its hoisted address would hold.
+  static __device__ __forceinline__ int row_lane(int lane) {
+    const int r = lane & 31, h = lane >> 5;
+    return r * ROW + (((sizeof(T) == 2 ? h : 2 * h) ^ swz(r)) << 4);
+  }
+  static __device__ __forceinline__ int col_lane(int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, row = 4 * h + (i >> 2);
+      return row * ROW + (((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ swz(row)) << 4) + (i & 1) * 8;
+    } else {
+      return lane;
+    }
+  }
+
+  // Elements 16 t + 8 h .. + 7 of row lane % 32.
+  static __device__ __forceinline__ Frag<T> row_frag(const char* tile, int rl, int t) {
     Frag<T> f;
     if constexpr (sizeof(T) == 2) {
-      f.v = *(const u32x4*)(tile + at(row, 2 * t + h));
+      f.v = *(const u32x4*)(tile + (rl ^ (t << 5)));
     } else {
-      const f32x4 a = *(const f32x4*)(tile + at(row, 4 * t + 2 * h));
-      const f32x4 b = *(const f32x4*)(tile + at(row, 4 * t + 2 * h + 1));
+      const f32x4 a = *(const f32x4*)(tile + (rl ^ (t << 6)));
+      const f32x4 b = *(const f32x4*)(tile + (rl ^ (t << 6) ^ 16));
       f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     return f;
   }
 
-  // Column 32 db + lane % 32 of the rows of contraction step s (rows 16 s ..
-  // 16 s + 15 from row0, dealt as acc_frag deals them). 16-bit: the transposing
-  // LDS read, which gives lane i of 16 the i-th element of four rows.
-  static __device__ __forceinline__ Frag<T> col_frag(const char* tile, int row0, int s, int db, int lane) {
+  // Column 32 db + lane % 32 of the rows of contraction step s (rows 16 s .. 16 s + 15, dealt as
+  // acc_frag deals them). 16-bit: the transposing LDS read, which gives lane i of 16 the i-th
+  // element of four rows; rows 8 further on differ by 2 in the exchange.
+  static __device__ __forceinline__ Frag<T> col_frag(const char* tile, int cl, int s, int db) {
     Frag<T> f;
-    const int h = lane >> 5;
     if constexpr (sizeof(T) == 2) {
-      const int i = lane & 15, chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1), off = (i & 1) * 8;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int row = row0 + 16 * s + 8 * u + 4 * h + (i >> 2);
         const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)(tile + at(row, chunk) + off));
+            (__attribute__((address_space(3))) s16x4*)(tile + (cl ^ (db << 6) ^ (u << 5)) + (16 * s + 8 * u) * ROW));
         const u32x2 y = __builtin_bit_cast(u32x2, x);
         f.v[2 * u] = y[0];
         f.v[2 * u + 1] = y[1];
       }
     } else {
-      const int d = 32 * db + (lane & 31);
+      const int lane = cl, h = lane >> 5, d = 32 * db + (lane & 31);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int row = row0 + 16 * s + 8 * (j >> 2) + 4 * h + (j & 3);
+        const int row = 16 * s + 8 * (j >> 2) + 4 * h + (j & 3);
         f.v[j] = *(const float*)(tile + at(row, d / CE) + (d % CE) * 4);
       }
     }
     return f;
   }
 };
+
+// Hides a value's origin from the compiler.
+__device__ __forceinline__ int launder(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// How a tensor's rows are read: to LDS directly, by 16-byte vectors, by elements.
+enum LoadMode { kElements = 0, kVector = 1, kAsync = 2 };
 
 // 16 bytes of a row from element c0 on, zero where row or column is outside.
 // vec: the row is 16-byte aligned and D a multiple of the chunk.
@@ -169,28 +193,53 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, bool inside, int c0, i
   return r;
 }
 
-// Rows row0 .. row0 + ROWS - 1 of a matrix, held in the workgroup's registers
-// between their global loads and their LDS stores.
-template <typename T, int DP, int ROWS, int THREADS> struct Stage {
+// Rows of a matrix into an LDS tile by a workgroup of 256 threads. Thread t fills the
+// tile's t-th chunk of every 4 KiB, whose place in the row the tile's exchange gives:
+// the loads go to LDS without passing through registers, a wave's 64 chunks side by side.
+// Rows at or behind `limit`, columns behind D and rows whose bit in `live` is 0 are zero
+// and not read. fill() issues; land() waits for this wave's loads, before the barrier
+// behind which the tile may be read.
+template <typename T, int DP, int ROWS> struct Loader {
   using L = Tile<T, DP>;
-  static constexpr int RPI = THREADS / L::CPR, NIT = ROWS / RPI;
-  static_assert(THREADS % L::CPR == 0 && ROWS % RPI == 0, "tile shape");
-  u32x4 r[NIT];
-  // Rows at or behind `limit` are zero and not read.
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int limit, int D, bool vec) {
-    const int tid = threadIdx.x, c = tid % L::CPR, rr = tid / L::CPR;
+  static constexpr int RPI = 256 / L::CPR, NIT = ROWS / RPI;
+  static_assert(256 % L::CPR == 0 && ROWS % RPI == 0 && NIT <= 32, "tile shape");
+
+  static __device__ __forceinline__ int row_of(int i) { return (int)threadIdx.x / L::CPR + i * RPI; }
+
+  // mode: kAsync, 16-byte aligned rows whose tile spans less than 2 GiB; kVector, 16-byte
+  // aligned; kElements, neither.
+  static __device__ __forceinline__ void fill(char* tile, const T* base, int64_t stride, int row0, int limit, int D,
+                                              int mode, uint32_t live = ~0u) {
+    const int slot = threadIdx.x % L::CPR;
+    if (mode == kAsync) {
+      const char* from = (const char*)(base + (int64_t)row0 * stride);  // uniform
+      const uint32_t rowBytes = (uint32_t)stride * (uint32_t)sizeof(T);
+      char* to = tile + uniform(threadIdx.x >> 6) * 1024;
+      const bool whole = row0 + ROWS <= limit && D == DP && live == ~0u;
 #pragma unroll
-    for (int i = 0; i < NIT; ++i) {
-      const int row = row0 + rr + i * RPI;
-      r[i] = load_chunk<T>(base + (int64_t)row * stride, row < limit, c * L::CE, D, vec);
+      for (int i = 0; i < NIT; ++i) {
+        const int r = row_of(i), c = slot ^ L::swz(r);
+        const uint32_t off = (uint32_t)r * rowBytes + (uint32_t)c * 16;
+        if (whole || (row0 + r < limit && c * L::CE < D && (live >> i & 1))) {
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + off),
+                                           (__attribute__((address_space(3))) void*)(to + i * 4096), 16, 0, 0);
+        } else {
+          *(u32x4*)(tile + i * 4096 + threadIdx.x * 16) = (u32x4){0, 0, 0, 0};
+        }
+      }
+    } else {
+      // Not unrolled: few registers beside the kernel's accumulators.
+#pragma unroll 1
+      for (int i = 0; i < NIT; ++i) {
+        const int r = row_of(i), c = slot ^ L::swz(r);
+        *(u32x4*)(tile + i * 4096 + threadIdx.x * 16) =
+            load_chunk<T>(base + (int64_t)(row0 + r) * stride, row0 + r < limit && (live >> i & 1), c * L::CE, D, mode == kVector);
+      }
     }
   }
-  __device__ __forceinline__ void store(char* tile) const {
-    const int tid = threadIdx.x, c = tid % L::CPR, rr = tid / L::CPR;
-#pragma unroll
-    for (int i = 0; i < NIT; ++i) *(u32x4*)(tile + L::at(rr + i * RPI, c)) = r[i];
-  }
 };
+// Waits for every load into LDS that the wave has issued (vmcnt(0); the other counters stay free).
+__device__ __forceinline__ void land() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 // The eight elements 16 t + 8 h .. + 7 of a row in memory.
 template <typename T>
@@ -262,7 +311,8 @@ struct AttnArgs {
   int64_t ms[4];                       // mask strides: batch, head, row, key (0 where broadcast)
   int B, H, Hk, G, N, M, D;
   int maskKind, causal, keyMask;       // keyMask: the mask is the same for every head and row
-  int vecQ, vecK, vecV, vecO, vecG, vecDq, vecDk, vecDv;
+  int modeQ, modeK, modeV, modeG;       // LoadMode of the streamed tensors
+  int vecO, vecDq, vecDk, vecDv;
   int nsplit, tiles, chunk;            // work split along the other axis; tiles along the own one; steps per split
   float scale, c;                      // c = scale * log2(e)
   FastDiv divN;
@@ -280,11 +330,96 @@ __device__ __forceinline__ int query_start(const AttnArgs& a, int b) {
   return a.qstart ? min(max(a.qstart[b], -a.N), a.M) : a.M - a.N;
 }
 
-// mask element (b, h, n, j) as an additive term in natural units.
+// An additive mask element in natural units.
 __device__ __forceinline__ float mask_bias(const AttnArgs& a, int64_t off) {
+  if (a.maskKind == kMaskBool) return ((const uint8_t*)a.mask)[off] ? 0.0f : kNegInf;
   if (a.maskKind == kMaskF32) return ((const float*)a.mask)[off];
   if (a.maskKind == kMaskF16) return to_acc(((const f16s*)a.mask)[off]);
   return to_acc(((const bf16s*)a.mask)[off]);
+}
+
+// The mask of a lane's 16 scores of one query: keys j0 + 8 (r / 4) + 4 h + r % 4. off: the
+// query's row. Keys at or behind M give -inf and are not read. Four adjacent keys are one
+// (unaligned) load where the mask's keys are adjacent.
+__device__ __forceinline__ void mask_of_keys(const AttnArgs& a, int64_t off, int j0, int h, f32x16& x) {
+  if (a.ms[3] == 1 && j0 + 32 <= a.M) {
+    const int64_t at = off + j0 + 4 * h;
+    if (a.maskKind == kMaskBool) {
+      uint32_t w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) __builtin_memcpy(&w[q], (const uint8_t*)a.mask + at + 8 * q, 4);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = (w[r >> 2] >> (8 * (r & 3)) & 0xff) ? 0.0f : kNegInf;
+    } else if (a.maskKind == kMaskF32) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f32x4 y;
+        __builtin_memcpy(&y, (const float*)a.mask + at + 8 * q, 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[4 * q + i] = y[i];
+      }
+    } else {
+      u32x2 w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) __builtin_memcpy(&w[q], (const uint16_t*)a.mask + at + 8 * q, 8);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const uint16_t bits = (uint16_t)(w[r >> 2][(r >> 1) & 1] >> (16 * (r & 1)));
+        x[r] = a.maskKind == kMaskF16 ? to_acc(f16s{bits}) : to_acc(bf16s{bits});
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int j = j0 + 8 * (r >> 2) + 4 * h + (r & 3);
+    x[r] = j < a.M ? mask_bias(a, off + (int64_t)j * a.ms[3]) : kNegInf;
+  }
+}
+
+// The same for one key and the queries n0 + 8 (r / 4) + 4 h + r % 4; off: the key's column.
+__device__ __forceinline__ void mask_of_queries(const AttnArgs& a, int64_t off, int n0, int h, f32x16& x) {
+  const int64_t at = off + (int64_t)(n0 + 4 * h) * a.ms[2];
+  if (n0 + 32 <= a.N) {
+    if (a.maskKind == kMaskBool) {
+      uint8_t w[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) w[r] = ((const uint8_t*)a.mask)[at + (8 * (r >> 2) + (r & 3)) * a.ms[2]];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = w[r] ? 0.0f : kNegInf;
+    } else if (a.maskKind == kMaskF32) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = ((const float*)a.mask)[at + (8 * (r >> 2) + (r & 3)) * a.ms[2]];
+    } else {
+      uint16_t w[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) w[r] = ((const uint16_t*)a.mask)[at + (8 * (r >> 2) + (r & 3)) * a.ms[2]];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = a.maskKind == kMaskF16 ? to_acc(f16s{w[r]}) : to_acc(bf16s{w[r]});
+    }
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int n = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
+    x[r] = n < a.N ? mask_bias(a, off + (int64_t)n * a.ms[2]) : kNegInf;
+  }
+}
+
+// A score under a mask in natural units; -inf removes the key, whatever its score.
+__device__ __forceinline__ float masked_score(const AttnArgs& a, float s, float bias) {
+  return bias == kNegInf ? kNegInf : fmaf(s, a.scale, bias);
+}
+
+// Bit i: row row0 + row_of(i) of the keys takes part, as far as a mask over keys alone says.
+template <typename LD> __device__ __forceinline__ uint32_t live_keys(const AttnArgs& a, int b, int row0) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < LD::NIT; ++i) {
+    const int j = min(row0 + LD::row_of(i), a.M - 1);
+    bits |= (uint32_t)(mask_bias(a, (int64_t)b * a.ms[0] + (int64_t)j * a.ms[3]) != kNegInf) << i;
+  }
+  return LD::NIT == 32 || bits != (1u << (LD::NIT & 31)) - 1 ? bits : ~0u;
 }
 
 // The workgroup's place: consecutive places on one XCD (workgroups are dealt to

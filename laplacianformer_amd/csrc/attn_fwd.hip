@@ -34,7 +34,7 @@ template <typename T, int DP, int KS> constexpr int num_buffers() {
 // QB: 32-query blocks per wave. KS: 1, the four waves take different queries; 4,
 // they take different keys of each tile and their results are joined at the end.
 template <typename T, int DP, int QB, int KS, bool MASK>
-__global__ void __launch_bounds__(256, 2) attn_fwd_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn_fwd_kernel(const AttnArgs a) {
   constexpr int KT = key_tile<KS>(), NBUF = num_buffers<T, DP, KS>(), NT = DP / 16, ND = DP / 32;
   constexpr int KB = KS == 1 ? KT / 32 : 1;  // 32-key blocks per wave and tile
   constexpr int ROWS = KS == 1 ? 128 * QB : 32 * QB;
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(const AttnArgs a) {
 #pragma unroll
   for (int i = 0; i < QB; ++i)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) qf[i][t] = global_frag<T>((const T*)a.q + qoff[i], alive[i], t, h, a.D, a.vecQ);
+    for (int t = 0; t < NT; ++t) qf[i][t] = global_frag<T>((const T*)a.q + qoff[i], alive[i], t, h, a.D, a.modeQ != kElements);
 
   f32x16 o[ND][QB];
   float m[QB], l[QB];
@@ -105,45 +105,40 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(const AttnArgs a) {
 
   const T* kbase = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1];
   const T* vbase = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1];
-  Stage<T, DP, KT, 256> sk, sv;
+  using LD = Loader<T, DP, KT>;
   // Keys that a mask takes from every query are not read either: what they hold is nobody's.
-  auto load = [&](int key0) {
-    if (MASK && a.keyMask) {
-      const int c = threadIdx.x % L::CPR, rr = threadIdx.x / L::CPR;
-#pragma unroll
-      for (int i = 0; i < sk.NIT; ++i) {
-        const int row = key0 + rr + i * sk.RPI;
-        bool in = row < kend;
-        if (in) {
-          const int64_t off = (int64_t)b * a.ms[0] + (int64_t)row * a.ms[3];
-          in = a.maskKind == kMaskBool ? ((const uint8_t*)a.mask)[off] != 0 : mask_bias(a, off) != kNegInf;
-        }
-        sk.r[i] = load_chunk<T>(kbase + (int64_t)row * a.ks[2], in, c * L::CE, a.D, a.vecK);
-        sv.r[i] = load_chunk<T>(vbase + (int64_t)row * a.vs[2], in, c * L::CE, a.D, a.vecV);
-      }
-    } else {
-      sk.load(kbase, a.ks[2], key0, kend, a.D, a.vecK);
-      sv.load(vbase, a.vs[2], key0, kend, a.D, a.vecV);
-    }
-  };
-  auto store = [&](int buf) {
-    sk.store(smem + buf * 2 * TB);
-    sv.store(smem + buf * 2 * TB + TB);
+  const bool byKey = MASK && a.keyMask;
+  auto fill = [&](int buf, int key0, uint32_t live) {
+    LD::fill(smem + buf * 2 * TB, kbase, a.ks[2], key0, kend, a.D, a.modeK, live);
+    LD::fill(smem + buf * 2 * TB + TB, vbase, a.vs[2], key0, kend, a.D, a.modeV, live);
   };
 
+  uint32_t live = ~0u;  // of the next tile to fill
   if (kbeg < kend) {
-    load(kbeg);
-    store(0);
+    if (byKey) live = live_keys<LD>(a, b, kbeg);
+    fill(0, kbeg, live);
+    if (NBUF == 2 && byKey) live = live_keys<LD>(a, b, kbeg + KT);
   }
+  land();
   __syncthreads();
+  const int rl0 = L::row_lane(lane), cl0 = L::col_lane(lane);
   int buf = 0;
   for (int key0 = kbeg; key0 < kend; key0 += KT) {
     const bool more = key0 + KT < kend;
-    if (more) load(key0 + KT);
+    if (NBUF == 2 && more) fill(buf ^ 1, key0 + KT, live);
+    if (byKey) live = live_keys<LD>(a, b, key0 + (NBUF == 2 ? 2 : 1) * KT);
+    const int rl = launder(rl0), cl = launder(cl0);
     const char* tk = smem + buf * 2 * TB;
     const char* tv = tk + TB;
     const int wkey = key0 + (KS == 1 ? 0 : 32 * wave);
     if (wkey < wend) {
+      f32x16 bias[MASK ? KB : 1][QB];
+      if constexpr (MASK) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < QB; ++i) mask_of_keys(a, moff[i], wkey + 32 * kb, h, bias[kb][i]);
+      }
       f32x16 s[KB][QB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
@@ -151,7 +146,7 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(const AttnArgs a) {
         for (int i = 0; i < QB; ++i) s[kb][i] = f32x16{};
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const Frag<T> kf = L::row_frag(tk, (KS == 1 ? 32 * kb : 32 * wave) + (lane & 31), t, h);
+          const Frag<T> kf = L::row_frag(tk + (KS == 1 ? 32 * kb : 32 * wave) * L::ROW, rl, t);
 #pragma unroll
           for (int i = 0; i < QB; ++i) s[kb][i] = mma<T>(kf, qf[i][t], s[kb][i]);
         }
@@ -166,18 +161,7 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(const AttnArgs a) {
             for (int r = 0; r < 16; ++r) {
               const int j = wkey + 32 * kb + 8 * (r >> 2) + 4 * h + (r & 3);
               if constexpr (MASK) {
-                float x = kNegInf;
-                if (j < lim[i]) {
-                  const int64_t off = moff[i] + (int64_t)j * a.ms[3];
-                  if (a.maskKind == kMaskBool) {
-                    if (((const uint8_t*)a.mask)[off]) x = s[kb][i][r] * a.scale;
-                  } else {
-                    // -inf removes the key, whatever its score
-                    const float bias = mask_bias(a, off);
-                    if (bias != kNegInf) x = fmaf(s[kb][i][r], a.scale, bias);
-                  }
-                }
-                s[kb][i][r] = x;
+                s[kb][i][r] = j < lim[i] ? masked_score(a, s[kb][i][r], bias[kb][i][r]) : kNegInf;
               } else {
                 s[kb][i][r] = j < lim[i] ? s[kb][i][r] : kNegInf;
               }
@@ -227,15 +211,19 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(const AttnArgs a) {
           for (int i = 0; i < QB; ++i) pf[i] = acc_frag<T>(s[kb][i], st);
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
-            const Frag<T> vf = L::col_frag(tv, KS == 1 ? 32 * kb : 32 * wave, st, d, lane);
+            const Frag<T> vf = L::col_frag(tv + (KS == 1 ? 32 * kb : 32 * wave) * L::ROW, cl, st, d);
 #pragma unroll
             for (int i = 0; i < QB; ++i) o[d][i] = mma<T>(vf, pf[i], o[d][i]);
           }
         }
     }
-    if (NBUF == 1) __syncthreads();
-    if (more) store(NBUF == 2 ? buf ^ 1 : 0);
-    if (NBUF == 2) buf ^= 1;
+    if (NBUF == 1) {
+      __syncthreads();
+      if (more) fill(0, key0 + KT, live);
+    } else {
+      buf ^= 1;
+    }
+    land();
     __syncthreads();
   }
 

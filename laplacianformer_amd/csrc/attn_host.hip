@@ -15,6 +15,12 @@ bool vec_ok(const void* p, const int64_t* strides, int64_t d, int64_t ce) {
   return ((uintptr_t)p & 15) == 0 && d % ce == 0 && strides[0] % ce == 0 && strides[1] % ce == 0 && strides[2] % ce == 0;
 }
 
+// The offsets inside a tile of at most 128 rows are 32-bit where loads go to LDS directly.
+int load_mode(const void* p, const int64_t* strides, int64_t d, int64_t ce) {
+  if (!vec_ok(p, strides, d, ce)) return kElements;
+  return strides[2] >= 0 && strides[2] < ((int64_t)1 << 22) ? kAsync : kVector;
+}
+
 // Sizes, types and what else needs no tensor pointer. *empty: there is no head.
 int check_desc(const char* who, int dtype, const lfamd_attention* d, bool* empty) {
   if (dtype != LFAMD_F32 && dtype != LFAMD_F16 && dtype != LFAMD_BF16)
@@ -85,7 +91,7 @@ int lfamd_softmax_attention(int dtype, const lfamd_attention* desc, const void* 
   if (need && ((uintptr_t)workspace & 15)) return fail(LFAMD_ERR_ARG, "%s: workspace must be 16-byte aligned", who);
   const int64_t ce = chunk_elems(dtype);
   a.q = q, a.k = k, a.v = v, a.out = out, a.stat = stats, a.part = (float*)workspace;
-  a.vecQ = vec_ok(q, a.qs, a.D, ce), a.vecK = vec_ok(k, a.ks, a.D, ce), a.vecV = vec_ok(v, a.vs, a.D, ce);
+  a.modeQ = load_mode(q, a.qs, a.D, ce), a.modeK = load_mode(k, a.ks, a.D, ce), a.modeV = load_mode(v, a.vs, a.D, ce);
   a.vecO = vec_ok(out, a.os, a.D, ce);
   return attn_fwd(dtype, a, (hipStream_t)stream);
 }
@@ -121,8 +127,8 @@ int lfamd_softmax_attention_backward(int dtype, const lfamd_attention* desc, con
   const int64_t ce = chunk_elems(dtype);
   a.q = q, a.k = k, a.v = v, a.o = out, a.g = grads->grad_out, a.stat = (float*)stats;
   a.dq = a.N ? grads->grad_q : nullptr, a.dk = a.M ? grads->grad_k : nullptr, a.dv = a.M ? grads->grad_v : nullptr;
-  a.vecQ = vec_ok(q, a.qs, a.D, ce), a.vecK = vec_ok(k, a.ks, a.D, ce), a.vecV = vec_ok(v, a.vs, a.D, ce);
-  a.vecO = vec_ok(out, a.os, a.D, ce), a.vecG = vec_ok(a.g, a.gs, a.D, ce), a.vecDq = vec_ok(a.dq, a.dqs, a.D, ce);
+  a.modeQ = load_mode(q, a.qs, a.D, ce), a.modeK = load_mode(k, a.ks, a.D, ce), a.modeV = load_mode(v, a.vs, a.D, ce);
+  a.vecO = vec_ok(out, a.os, a.D, ce), a.modeG = load_mode(a.g, a.gs, a.D, ce), a.vecDq = vec_ok(a.dq, a.dqs, a.D, ce);
   a.vecDk = vec_ok(a.dk, a.dks, a.D, ce), a.vecDv = vec_ok(a.dv, a.dvs, a.D, ce);
   return attn_bwd(dtype, a, workspace, (hipStream_t)stream);
 }
