@@ -8,8 +8,8 @@ transformer block around it (norm, rotary positions, softmax attention).
 """
 from ._lib import EXT_PATH, LIB_PATH, capi, check, dtype_code, ext
 from .attention import LaplacianAttention, laplacian_attention
-from .block import (AddRmsNormFunction, AttentionBlock, RotaryFunction, SoftmaxAttentionFunction, add_rms_norm,
-                    add_rms_norm_fp8, grid_positions, rotary, rotary_sections, softmax_attention)
+from .block import (AttentionBlock, add_rms_norm, add_rms_norm_fp8, grid_positions, rotary, rotary_sections,
+                    softmax_attention)
 from .graphs import GraphedStep
 from .functional import (LaplaceKernelFunction, LaplaceSubtractionFunction, NewtonInverseFunction,
                          TallMixFunction, TallProductFunction, laplace_kernel, laplace_subtraction, mix_rows,
@@ -20,6 +20,6 @@ __all__ = [
     "LaplaceSubtractionFunction", "NewtonInverseFunction", "LaplacianAttention", "laplace_kernel",
     "laplace_subtraction", "laplacian_attention", "newton_inverse", "TallMixFunction", "TallProductFunction",
     "mix_rows", "tall_mix", "tall_product", "tall_t", "GraphedStep",
-    "AddRmsNormFunction", "AttentionBlock", "RotaryFunction", "SoftmaxAttentionFunction", "add_rms_norm",
-    "add_rms_norm_fp8", "grid_positions", "rotary", "rotary_sections", "softmax_attention",
+    "AttentionBlock", "add_rms_norm", "add_rms_norm_fp8", "grid_positions", "rotary", "rotary_sections",
+    "softmax_attention",
 ]

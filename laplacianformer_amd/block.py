@@ -6,7 +6,7 @@ addition, rotary positions on the token grid, exact softmax attention, and
 All run on hand-written HIP kernels in float32, float16 and bfloat16 (float64 and CPU
 tensors are refused), take strided inputs where the last dimension's elements are
 adjacent, and record into a HIP graph. Results do not depend on the launch: the same
-call gives the same bits.
+call gives the same bits. Gradients are of first order (no create_graph).
 """
 from __future__ import annotations
 
@@ -14,35 +14,9 @@ import math
 from typing import Sequence
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._lib import ext
 from .attention import laplacian_attention
-
-
-class AddRmsNormFunction(torch.autograd.Function):
-    """(y, sum) of add_rms_norm; one gradient tensor serves both addends."""
-
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        ctx.set_materialize_grads(False)
-        need = any(ctx.needs_input_grad[:3])
-        y, total, rstd = ext().AddRmsNorm_forward(x, weight, residual, float(eps), need)
-        if need:
-            ctx.save_for_backward(total, weight, rstd)
-        return (y, total) if residual is not None else (y, None)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gy, gs):
-        total, weight, rstd = ctx.saved_tensors
-        if gy is None and gs is None:
-            return None, None, None, None
-        if gy is None:
-            gy = torch.zeros_like(total)
-        dx, dw = ext().AddRmsNorm_backward(gy, gs, total, weight, rstd, ctx.needs_input_grad[1])
-        need_x, _, need_r, _ = ctx.needs_input_grad
-        return dx if need_x else None, dw, dx if need_r else None, None
 
 
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6):
@@ -52,8 +26,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     float32 sum). Returns ``(y, sum)`` in x's type, or ``y`` alone without a residual.
     ``weight`` has x's type or float32; the last dimension is at most 16384. With autograd.
     """
-    y, total = AddRmsNormFunction.apply(x, weight, residual, eps)
-    return y if residual is None else (y, total)
+    out = ext().AddRmsNorm(x, weight, residual, eps)
+    return out[0] if residual is None else tuple(out)
 
 
 def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6):
@@ -65,32 +39,8 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     """
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("add_rms_norm_fp8 has no gradient: call it under torch.no_grad()")
-    y, scale, total = ext().AddRmsNorm_forward_fp8(x, weight, residual, float(eps))
+    y, scale, total = ext().AddRmsNorm_fp8(x, weight, residual, eps)
     return (y, scale) if residual is None else (y, scale, total)
-
-
-class RotaryFunction(torch.autograd.Function):
-    """Rotation of q and k; the backward pass rotates the gradients back."""
-
-    @staticmethod
-    def forward(ctx, q, k, positions, sections, base, interleaved):
-        ctx.set_materialize_grads(False)
-        ctx.rest = (sections, base, interleaved)
-        ctx.save_for_backward(positions)
-        q2, k2 = ext().Rotary(q, k, positions, sections, base, interleaved, False)
-        return q2, k2
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gq, gk):
-        (positions,) = ctx.saved_tensors
-        if gq is None and gk is None:
-            return (None,) * 6
-        if gq is None:  # one tensor takes q's place where only one is there
-            gk, _ = ext().Rotary(gk, None, positions, *ctx.rest, True)
-        else:
-            gq, gk = ext().Rotary(gq, gk, positions, *ctx.rest, True)
-        return gq, gk, None, None, None, None
 
 
 def rotary_sections(head_dim: int, axes: int) -> list[int]:
@@ -117,29 +67,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, sec
     ``(2 p, 2 p + 1)`` if ``interleaved``; channels behind the pairs are copied. At most 128
     pairs. Returns ``(q', k')``. With autograd.
     """
-    return RotaryFunction.apply(q, k, positions, [int(s) for s in sections], float(base), bool(interleaved))
-
-
-class SoftmaxAttentionFunction(torch.autograd.Function):
-    """softmax_attention; the backward pass recomputes the probabilities from row statistics."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale):
-        need = any(ctx.needs_input_grad[:3])
-        out, stats = ext().SoftmaxAttention_forward(q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale, need)
-        if need:
-            ctx.causal, ctx.scale = causal, scale
-            ctx.save_for_backward(q, k, v, out, stats, mask, k_lengths, q_lengths, q_starts)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        q, k, v, out, stats, mask, k_lengths, q_lengths, q_starts = ctx.saved_tensors
-        need_q, need_k, need_v = ctx.needs_input_grad[:3]
-        dq, dk, dv = ext().SoftmaxAttention_backward(g, q, k, v, out, stats, mask, ctx.causal, k_lengths, q_lengths,
-                                                     q_starts, ctx.scale, need_q, need_k or need_v)
-        return (dq, dk if need_k else None, dv if need_v else None) + (None,) * 6
+    return tuple(ext().Rotary(q, k, positions, sections, base, interleaved))
 
 
 def softmax_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: torch.Tensor | None = None,
@@ -162,11 +90,9 @@ def softmax_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: t
     finite, as its probability of 0 is multiplied by it. 16-bit types round the
     probabilities to that type in front of the product with v. With autograd.
     """
-    if mask is not None and mask.requires_grad:
-        raise RuntimeError("softmax_attention: the mask has no gradient")
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.shape[-1] else 1.0
-    return SoftmaxAttentionFunction.apply(q, k, v, mask, bool(causal), k_lengths, q_lengths, q_starts, float(scale))
+    return ext().SoftmaxAttention(q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale)
 
 
 class AttentionBlock(torch.nn.Module):

@@ -153,7 +153,8 @@ template <bool MASK> __device__ __forceinline__ bool key_live(const AttnArgs& a,
 
 // dk and dv of 128 keys, 32 per wave; queries stream through LDS in tiles of QT.
 template <typename T, int DP, bool MASK>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2) attn_dkdv_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2)
+    __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP >= 64 ? 1 : 2, 2))) attn_dkdv_kernel(const AttnArgs a) {
   constexpr int QT = query_tile<T, DP>(), NT = DP / 16, ND = DP / 32;
   constexpr bool F16 = std::is_same<T, f16s>::value;
   using L = Tile<T, DP>;
@@ -263,6 +264,18 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2) attn_
       // Every row sees every key of the wave: nothing to leave out.
       const int wlast = key0 + wave * 32 + 31;
       const bool check = MASK || wlast >= klen || row0 + qb + 32 > qlen || (a.causal && wlast > qstart + row0 + qb);
+      // Pairs that are left out: score -inf, so that p = 0, and g.v = 0, so that dz = 0 (delta - 0).
+      if (check) {
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 4 * rq + i;
+            const bool in = mykey < ((const int*)stats)[3 * QT + qb + 8 * rq + 4 * h + i];
+            s[r] = !in ? kNegInf : MASK ? masked_score(a, s[r], bias[r]) : s[r];
+            dp[r] = s[r] == kNegInf ? 0.0f : dp[r];
+          }
+      }
 #pragma unroll
       for (int rq = 0; rq < 4; ++rq) {
         const int rr = qb + 8 * rq + 4 * h;
@@ -272,18 +285,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2) attn_
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = 4 * rq + i;
-          float x = s[r];
-          if constexpr (MASK)
-            x = mykey < ((const int*)stats)[3 * QT + rr + i] ? masked_score(a, x, bias[r]) : kNegInf;
-          float p = prob<MASK>(x, a.c, x0[i], x1[i]);
-          float z = p * (F16 ? fmaf(dp[r], fd, -de[i]) : dp[r] - de[i]);
-          if (check) {
-            const bool out = MASK ? x == kNegInf : mykey >= ((const int*)stats)[3 * QT + rr + i];
-            p = out ? 0.0f : p;
-            z = out ? 0.0f : z;
-          }
+          const float p = prob<MASK>(s[r], a.c, x0[i], x1[i]);
           s[r] = p;
-          dp[r] = z;
+          dp[r] = p * (F16 ? fmaf(dp[r], fd, -de[i]) : dp[r] - de[i]);
         }
       }
 #pragma unroll
@@ -407,16 +411,16 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
 #pragma unroll
       for (int t = 0; t < NT; ++t) dp = mma<T>(L::row_frag(tv + kb * L::ROW, rl, t), gf[t], dp);
       const bool check = MASK || key0 + kb + 32 > full;
+      if (check) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = key0 + kb + 8 * (r >> 2) + 4 * h + (r & 3);
-        float x = s[r];
-        if constexpr (MASK) x = j < lim ? masked_score(a, x, bias[r]) : kNegInf;
-        const float p = prob<MASK>(x, a.c, x0, x1);
-        float z = p * (F16 ? fmaf(dp[r], f, -de) : dp[r] - de);
-        if (check) z = (MASK ? x == kNegInf : j >= lim) ? 0.0f : z;
-        dp[r] = z;
+        for (int r = 0; r < 16; ++r) {
+          const int j = key0 + kb + 8 * (r >> 2) + 4 * h + (r & 3);
+          s[r] = j >= lim ? kNegInf : MASK ? masked_score(a, s[r], bias[r]) : s[r];
+          dp[r] = s[r] == kNegInf ? 0.0f : dp[r];
+        }
       }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = prob<MASK>(s[r], a.c, x0, x1) * (F16 ? fmaf(dp[r], f, -de) : dp[r] - de);
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         const Frag<T> zf = acc_frag<T>(dp, st);

@@ -193,6 +193,19 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, bool inside, int c0, i
   return r;
 }
 
+// 16 bytes per lane from base + off (base uniform) to LDS at `lds` + 16 lane, without registers in between.
+// In asm because the compiler puts a wait for every such load in front of the next transposing LDS read,
+// whichever tile that reads; there is no output register that it could reuse early, and land() is the wait.
+// M0 takes the LDS address, one wait state in front of its use, and gets its value back (the compiler does not
+// take it as a clobber).
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0)
+               : "v"(off), "s"(base), "s"(lds)
+               : "memory");
+}
+
 // Rows of a matrix into an LDS tile by a workgroup of 256 threads. Thread t fills the
 // tile's t-th chunk of every 4 KiB, whose place in the row the tile's exchange gives:
 // the loads go to LDS without passing through registers, a wave's 64 chunks side by side.
@@ -214,15 +227,14 @@ template <typename T, int DP, int ROWS> struct Loader {
     if (mode == kAsync) {
       const char* from = (const char*)(base + (int64_t)row0 * stride);  // uniform
       const uint32_t rowBytes = (uint32_t)stride * (uint32_t)sizeof(T);
-      char* to = tile + uniform(threadIdx.x >> 6) * 1024;
+      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tile + uniform(threadIdx.x >> 6) * 1024;
       const bool whole = row0 + ROWS <= limit && D == DP && live == ~0u;
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
         const int r = row_of(i), c = slot ^ L::swz(r);
         const uint32_t off = (uint32_t)r * rowBytes + (uint32_t)c * 16;
         if (whole || (row0 + r < limit && c * L::CE < D && (live >> i & 1))) {
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + off),
-                                           (__attribute__((address_space(3))) void*)(to + i * 4096), 16, 0, 0);
+          load_to_lds(from, off, to + i * 4096);
         } else {
           *(u32x4*)(tile + i * 4096 + threadIdx.x * 16) = (u32x4){0, 0, 0, 0};
         }
@@ -238,8 +250,13 @@ template <typename T, int DP, int ROWS> struct Loader {
     }
   }
 };
-// Waits for every load into LDS that the wave has issued (vmcnt(0); the other counters stay free).
-__device__ __forceinline__ void land() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// Waits for every load into LDS that the wave has issued .
+// The builtin, so that the compiler knows its own loads to have landed as well (0x0f70: vmcnt(0) alone).
+__device__ __forceinline__ void land() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);
+  asm volatile("" ::: "memory");
+}
 
 // The eight elements 16 t + 8 h .. + 7 of a row in memory.
 template <typename T>

@@ -1,10 +1,11 @@
 // Host adapters of the transformer-block operators: shape, type and device checks, then
-// the C ABI of include/laplacianformer_amd.h on the tensors' device and current stream.
+// the C ABI of include/laplacianformer_amd.h on the tensors' device and current stream; and
+// their autograd nodes, in C++ because a small call's time is its host time (a training
+// step of softmax attention at B2 H2 N196 d32: 89 us with nodes in Python).
 #include "Block.h"
 
 #include <ATen/ATen.h>
-
-#include <cmath>
+#include <torch/csrc/autograd/custom_function.h>
 
 #include "torch_common.h"
 
@@ -77,7 +78,7 @@ std::vector<Tensor> AddRmsNorm_forward(const Tensor x, const Tensor weight, cons
   if (need_rstd) rstd = at::empty({n.rows}, x.options().dtype(at::kFloat));
   detail::check_status(lfamd_add_rms_norm(n.dt, ptr(n.x), n.xs, ptr(n.res), n.rs, n.wt, ptr(w), ptr(y), ptr(sum),
                                           (float*)ptr(rstd), n.rows, n.width, (float)eps, detail::stream_of(x)));
-  return {y, sum.defined() ? sum : x, rstd.defined() ? rstd : at::empty({0}, x.options().dtype(at::kFloat))};
+  return {y, sum.defined() ? sum : x, rstd};
 }
 
 std::vector<Tensor> AddRmsNorm_forward_fp8(const Tensor x, const Tensor weight, const OptTensor residual, double eps) {
@@ -282,6 +283,128 @@ std::vector<Tensor> SoftmaxAttention_backward(const Tensor grad_out, const Tenso
   detail::check_status(lfamd_softmax_attention_backward(in.dt, &in.d, ptr(in.q), ptr(in.k), ptr(in.v), ptr(o),
                                                         stats.data_ptr<float>(), &gr, ptr(ws), wsb, detail::stream_of(q)));
   return {dq, dk, dv};
+}
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// The backward passes are kernels without a derivative of their own.
+void once(const char* op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), op, " has no second derivative: call backward without create_graph");
+}
+
+struct AddRmsNormNode : torch::autograd::Function<AddRmsNormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& residual,
+                               double eps) {
+    ctx->set_materialize_grads(false);
+    const auto r = AddRmsNorm_forward(x, weight, residual, eps, true);
+    ctx->save_for_backward({r[1], weight, r[2]});
+    if (given(residual)) return {r[0], r[1]};
+    return {r[0]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("add_rms_norm");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor gs = g.size() > 1 ? g[1] : Tensor();
+    if (!g[0].defined() && !gs.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const Tensor gy = g[0].defined() ? g[0] : at::zeros_like(saved[0]);
+    const auto d = AddRmsNorm_backward(gy, gs.defined() ? OptTensor(gs) : std::nullopt, saved[0], saved[1], saved[2],
+                                       ctx->needs_input_grad(1));
+    return {d[0], d[1], g.size() > 1 ? d[0] : Tensor(), Tensor()};
+  }
+};
+
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k, const Tensor& positions,
+                               std::vector<int64_t> sections, double base, bool interleaved) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({positions});
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["base"] = base;
+    ctx->saved_data["interleaved"] = interleaved;
+    auto r = Rotary(q, k, positions, sections, base, interleaved, false);
+    if (!given(k)) r.pop_back();
+    return r;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("rotary");
+    const Tensor positions = ctx->get_saved_variables()[0];
+    const auto sections = ctx->saved_data["sections"].toIntVector();
+    const double base = ctx->saved_data["base"].toDouble();
+    const bool inter = ctx->saved_data["interleaved"].toBool();
+    variable_list out(6);
+    const bool has_k = g.size() > 1 && g[1].defined();
+    if (g[0].defined()) {
+      const auto r = Rotary(g[0], has_k ? OptTensor(g[1]) : std::nullopt, positions, sections, base, inter, true);
+      out[0] = r[0], out[1] = r[1];
+    } else if (has_k) {
+      out[1] = Rotary(g[1], std::nullopt, positions, sections, base, inter, true)[0];
+    }
+    return out;
+  }
+};
+
+struct SoftmaxAttentionNode : torch::autograd::Function<SoftmaxAttentionNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask,
+                        bool causal, const OptTensor& k_lengths, const OptTensor& q_lengths, const OptTensor& q_starts,
+                        double scale) {
+    const auto r = SoftmaxAttention_forward(q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale, true);
+    auto or_none = [](const OptTensor& t) { return given(t) ? *t : Tensor(); };
+    ctx->save_for_backward({q, k, v, r[0], r[1], or_none(mask), or_none(k_lengths), or_none(q_lengths), or_none(q_starts)});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("softmax_attention");
+    const auto s = ctx->get_saved_variables();
+    auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+    const bool need_k = ctx->needs_input_grad(1), need_v = ctx->needs_input_grad(2);
+    const auto d = SoftmaxAttention_backward(g[0], s[0], s[1], s[2], s[3], s[4], opt(s[5]), ctx->saved_data["causal"].toBool(),
+                                             opt(s[6]), opt(s[7]), opt(s[8]), ctx->saved_data["scale"].toDouble(),
+                                             ctx->needs_input_grad(0), need_k || need_v);
+    variable_list out(9);
+    out[0] = d[0];
+    if (need_k) out[1] = d[1];
+    if (need_v) out[2] = d[2];
+    return out;
+  }
+};
+
+bool records(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+
+}  // namespace
+
+std::vector<Tensor> AddRmsNorm(const Tensor x, const Tensor weight, const OptTensor residual, double eps) {
+  if (records({&x, &weight, given(residual) ? &*residual : nullptr})) return AddRmsNormNode::apply(x, weight, residual, eps);
+  auto r = AddRmsNorm_forward(x, weight, residual, eps, false);
+  r.resize(given(residual) ? 2 : 1);
+  return r;
+}
+
+std::vector<Tensor> RotaryPositions(const Tensor q, const OptTensor k, const Tensor positions,
+                                    const std::vector<int64_t> sections, double base, bool interleaved) {
+  if (records({&q, given(k) ? &*k : nullptr})) {
+    auto r = RotaryNode::apply(q, k, positions, sections, base, interleaved);
+    r.resize(2);
+    return r;
+  }
+  return Rotary(q, k, positions, sections, base, interleaved, false);
+}
+
+Tensor SoftmaxAttention(const Tensor q, const Tensor k, const Tensor v, const OptTensor mask, bool causal,
+                        const OptTensor k_lengths, const OptTensor q_lengths, const OptTensor q_starts, double scale) {
+  TORCH_CHECK(!given(mask) || !mask->requires_grad(), "softmax_attention: the mask has no gradient");
+  if (records({&q, &k, &v}))
+    return SoftmaxAttentionNode::apply(q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale);
+  return SoftmaxAttention_forward(q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale, false)[0];
 }
 
 }  // namespace laplace

@@ -31,4 +31,14 @@ std::vector<at::Tensor> SoftmaxAttention_backward(const at::Tensor grad_out, con
                                                   const std::optional<at::Tensor> q_starts, double scale, bool need_q,
                                                   bool need_kv);
 
+// The three with autograd: [y] or [y, sum]; [q', k' or undefined]; out.
+std::vector<at::Tensor> AddRmsNorm(const at::Tensor x, const at::Tensor weight, const std::optional<at::Tensor> residual,
+                                   double eps);
+std::vector<at::Tensor> RotaryPositions(const at::Tensor q, const std::optional<at::Tensor> k, const at::Tensor positions,
+                                        const std::vector<int64_t> sections, double base, bool interleaved);
+at::Tensor SoftmaxAttention(const at::Tensor q, const at::Tensor k, const at::Tensor v, const std::optional<at::Tensor> mask,
+                            bool causal, const std::optional<at::Tensor> k_lengths,
+                            const std::optional<at::Tensor> q_lengths, const std::optional<at::Tensor> q_starts,
+                            double scale);
+
 }  // namespace laplace

@@ -77,20 +77,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("TallT", &TallT,
         "TallT (a, b, c): c[..., p, q] = sum_n a[..., n, p] * b[..., n, q], a and c float32, widths <= 64 "
         "(the attention layer's K^T V products)");
-  m.def("AddRmsNorm_forward", &AddRmsNorm_forward,
-        "AddRmsNorm_forward (x, weight, residual or None, eps, need_rstd) -> [y, sum, rstd]");
-  m.def("AddRmsNorm_forward_fp8", &AddRmsNorm_forward_fp8,
-        "AddRmsNorm_forward_fp8 (x, weight, residual or None, eps) -> [y e4m3, scale, sum]");
-  m.def("AddRmsNorm_backward", &AddRmsNorm_backward,
-        "AddRmsNorm_backward (grad_y, grad_sum or None, sum, weight, rstd, need_weight) -> [grad_x, grad_weight]");
-  m.def("Rotary", &Rotary,
-        "Rotary (q, k or None, positions, sections, base, interleaved, inverse) -> [q', k']");
-  m.def("SoftmaxAttention_forward", &SoftmaxAttention_forward,
-        "SoftmaxAttention_forward (q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale, need_stats) -> "
-        "[out, stats]");
-  m.def("SoftmaxAttention_backward", &SoftmaxAttention_backward,
-        "SoftmaxAttention_backward (grad_out, q, k, v, out, stats, mask, causal, k_lengths, q_lengths, q_starts, "
-        "scale, need_q, need_kv) -> [grad_q, grad_k, grad_v]");
+  m.def("AddRmsNorm", &AddRmsNorm, "AddRmsNorm (x, weight, residual or None, eps) -> [y] or [y, sum], with autograd");
+  m.def("AddRmsNorm_fp8", &AddRmsNorm_forward_fp8,
+        "AddRmsNorm_fp8 (x, weight, residual or None, eps) -> [y e4m3, scale, sum]");
+  m.def("Rotary", &RotaryPositions,
+        "Rotary (q, k or None, positions, sections, base, interleaved) -> [q', k'], with autograd");
+  m.def("SoftmaxAttention", &SoftmaxAttention,
+        "SoftmaxAttention (q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale) -> out, with autograd");
 }
 
 }  // namespace laplace
