@@ -261,6 +261,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2)
       for (int t = 0; t < NT; ++t) s = mma<T>(L::row_frag(tq + qb * L::ROW, rl, t), kf[t], s);
 #pragma unroll
       for (int t = 0; t < NT; ++t) dp = mma<T>(L::row_frag(tg + qb * L::ROW, rl, t), VL ? L::row_frag(tv, rl, t) : vf[VL ? 0 : t], dp);
+      if constexpr (sizeof(T) == 2 && !VL) reads_ahead<2 * NT, 4>();
       // Every row sees every key of the wave: nothing to leave out.
       const int wlast = key0 + wave * 32 + 31;
       const bool check = MASK || wlast >= klen || row0 + qb + 32 > qlen || (a.causal && wlast > qstart + row0 + qb);

@@ -168,6 +168,18 @@ __device__ __forceinline__ int launder(int x) {
   return x;
 }
 
+// Asks the scheduler to keep AHEAD fragment reads in flight in front of N matrix instructions that take
+// one each: left alone it reads, waits and multiplies in turn, to save registers that are free.
+template <int N, int AHEAD> __device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
 // How a tensor's rows are read: to LDS directly, by 16-byte vectors, by elements.
 enum LoadMode { kElements = 0, kVector = 1, kAsync = 2 };
 

@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
           for (int i = 0; i < QB; ++i) s[kb][i] = mma<T>(kf, qf[i][t], s[kb][i]);
         }
       }
+      if constexpr (sizeof(T) == 2 && QB == 1) reads_ahead<KB * NT, (KB * NT < 4 ? KB * NT : 4)>();
       // The mask, and what lies behind the row's last key.
       if (MASK || wkey + 32 * KB > full) {
 #pragma unroll
