@@ -27,17 +27,18 @@ namespace {
 constexpr float kPShift = 15.0f;
 
 // Streamed rows per LDS tile, taken in blocks of 32: queries (dk, dv), keys (dq).
-template <typename T, int DP> constexpr int query_tile() { return DP < 128 && (sizeof(T) == 2 || DP == 32) ? 64 : 32; }
-template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 2 || DP == 32 ? 64 : 32; }
+template <typename T, int DC> constexpr int query_tile() { return DC < 96 && (sizeof(T) == 2 || DC == 32) ? 64 : 32; }
+template <typename T, int DC> constexpr int key_tile() { return sizeof(T) == 2 || DC == 32 ? 64 : 32; }
 
 // At 128 channels the accumulators of dk and dv and both owned operands are more than a lane's
 // registers at two waves per SIMD (128 + 64 + 64 with the scores): V is read from LDS then.
-template <int DP> constexpr bool v_in_lds() { return DP >= 128; }
+template <int DC> constexpr bool v_in_lds() { return DC >= 128; }
 
-template <typename T, int DP> constexpr size_t dkdv_lds() {
-  return (size_t)2 * query_tile<T, DP>() * (2 * DP * sizeof(T) + 16) + (v_in_lds<DP>() ? 128 * DP * sizeof(T) : 0);
+template <typename T, int DC> constexpr size_t dkdv_lds() {
+  constexpr int DP = row_pitch(DC);
+  return (size_t)2 * query_tile<T, DC>() * (2 * DP * sizeof(T) + 16) + (v_in_lds<DC>() ? 128 * DP * sizeof(T) : 0);
 }
-template <typename T, int DP> constexpr size_t dq_lds() { return (size_t)2 * key_tile<T, DP>() * 2 * DP * sizeof(T); }
+template <typename T, int DC> constexpr size_t dq_lds() { return (size_t)2 * key_tile<T, DC>() * 2 * row_pitch(DC) * sizeof(T); }
 
 // delta_i, and for fp16 the maxima over 64 rows of |g_i| and |delta_i|, or over 64
 // keys of |v_j|. A workgroup takes 64 rows of one head: four threads per row.
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
       live = mask_bias(a, off) != kNegInf;
     }
     for (int c = part * CE; c < a.D; c += 4 * CE) {
-      const u32x4 x = load_chunk<T>(p, live, c, a.D, a.modeV != kElements);
+      const u32x4 x = load_chunk<T>(p, live, c, a.D);
 #pragma unroll
       for (int j = 0; j < CE; ++j) {
         const float v = to_acc(((const T*)&x)[j]);
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
     const T* po = (const T*)a.o + (int64_t)b * a.os[0] + (int64_t)hd * a.os[1] + (int64_t)row * a.os[2];
     const T* pg = (const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)hd * a.gs[1] + (int64_t)row * a.gs[2];
     for (int c = part * CE; c < a.D; c += 4 * CE) {
-      const u32x4 x = load_chunk<T>(po, in, c, a.D, a.vecO), y = load_chunk<T>(pg, in, c, a.D, a.modeG != kElements);
+      const u32x4 x = load_chunk<T>(po, in, c, a.D), y = load_chunk<T>(pg, in, c, a.D);
 #pragma unroll
       for (int j = 0; j < CE; ++j) {
         const float u = to_acc(((const T*)&x)[j]), v = to_acc(((const T*)&y)[j]);
@@ -152,14 +153,14 @@ template <bool MASK> __device__ __forceinline__ bool key_live(const AttnArgs& a,
 }
 
 // dk and dv of 128 keys, 32 per wave; queries stream through LDS in tiles of QT.
-template <typename T, int DP, bool MASK>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2)
-    __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP >= 64 ? 1 : 2, 2))) attn_dkdv_kernel(const AttnArgs a) {
-  constexpr int QT = query_tile<T, DP>(), NT = DP / 16, ND = DP / 32;
+template <typename T, int DC, bool MASK>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
+    __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DC >= 64 ? 1 : 2, 2))) attn_dkdv_kernel(const AttnArgs a) {
+  constexpr int DP = row_pitch(DC), QT = query_tile<T, DC>(), NT = DC / 16, ND = DC / 32;
   constexpr bool F16 = std::is_same<T, f16s>::value;
   using L = Tile<T, DP>;
   constexpr int TB = QT * L::ROW, SB = QT * 16;  // bytes of a tile, and of its rows' statistics
-  constexpr bool VL = v_in_lds<DP>();
+  constexpr bool VL = v_in_lds<DC>();
   extern __shared__ __align__(16) char smem[];   // [2][q tile, g tile], [2][lse, delta, 1 / sum, last key], [v tile]
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
@@ -185,11 +186,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2)
     const T* vp = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1] + (int64_t)kr * a.vs[2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      kf[t] = global_frag<T>(kp, live, t, h, a.D, a.modeK != kElements);
-      if constexpr (!VL) vf[t] = global_frag<T>(vp, live, t, h, a.D, a.modeV != kElements);
+      kf[t] = global_frag<T>(kp, live, t, h, a.D);
+      if constexpr (!VL) vf[t] = global_frag<T>(vp, live, t, h, a.D);
     }
     if constexpr (VL) {
-      using LV = Loader<T, DP, 128>;
+      using LV = Loader<T, DP, DC, 128>;
       const uint32_t bits = MASK && a.keyMask && klen > 0 ? live_keys<LV>(a, b, key0) : ~0u;
       LV::fill(smem + 4 * TB + 2 * SB, (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1], a.vs[2], key0, klen, a.D,
                a.modeV, bits);
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2)
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
 
-  using LD = Loader<T, DP, QT>;
+  using LD = Loader<T, DP, DC, QT>;
   float st0 = 0.0f, st1 = 0.0f, st2 = 0.0f;
   int st3 = 0;
   auto fill = [&](int buf, int step) {
@@ -257,11 +258,22 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2)
       const int rl = launder(rl0), cl = launder(cl0);
       f32x16 s{}, dp{}, bias;
       if constexpr (MASK) mask_of_queries(a, moff + (int64_t)hq * a.ms[1], row0 + qb, h, bias);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) s = mma<T>(L::row_frag(tq + qb * L::ROW, rl, t), kf[t], s);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) dp = mma<T>(L::row_frag(tg + qb * L::ROW, rl, t), VL ? L::row_frag(tv, rl, t) : vf[VL ? 0 : t], dp);
-      if constexpr (sizeof(T) == 2 && !VL) reads_ahead<2 * NT, 4>();
+      struct Pair { Frag<T> a, b; };
+      {
+        auto read = [&](auto n) {
+          Pair p;
+          p.a = L::row_frag((n < NT ? tq : tg) + qb * L::ROW, rl, n % NT);
+          if constexpr (VL && n >= NT) p.b = L::row_frag(tv, rl, n % NT);
+          return p;
+        };
+        Ring<Pair, VL ? 2 : 4> ring;
+        first_reads<2 * NT>(ring, read);
+        read_and_use<2 * NT>(ring, read, [&](auto n, const Pair& p) {
+          if constexpr (n < NT) s = mma<T>(p.a, kf[n], s);
+          else if constexpr (VL) dp = mma<T>(p.a, p.b, dp);
+          else dp = mma<T>(p.a, vf[n - NT], dp);
+        });
+      }
       // Every row sees every key of the wave: nothing to leave out.
       const int wlast = key0 + wave * 32 + 31;
       const bool check = MASK || wlast >= klen || row0 + qb + 32 > qlen || (a.causal && wlast > qstart + row0 + qb);
@@ -277,6 +289,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2)
             dp[r] = s[r] == kNegInf ? 0.0f : dp[r];
           }
       }
+      // The first columns of g and q are read while the exponentials run.
+      auto cread = [&](auto n) {
+        return Pair{L::col_frag(tg + qb * L::ROW, cl, n / ND, n % ND), L::col_frag(tq + qb * L::ROW, cl, n / ND, n % ND)};
+      };
+      Ring<Pair, (sizeof(T) == 2 && DC <= 64 ? 2 : 1)> cring;
+      first_reads<2 * ND>(cring, cread);
 #pragma unroll
       for (int rq = 0; rq < 4; ++rq) {
         const int rr = qb + 8 * rq + 4 * h;
@@ -291,15 +309,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2)
           dp[r] = p * (F16 ? fmaf(dp[r], fd, -de[i]) : dp[r] - de[i]);
         }
       }
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const Frag<T> pf = acc_frag<T>(s, st), zf = acc_frag<T>(dp, st);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          dv[d] = mma<T>(L::col_frag(tg + qb * L::ROW, cl, st, d), pf, dv[d]);
-          dk[d] = mma<T>(L::col_frag(tq + qb * L::ROW, cl, st, d), zf, dk[d]);
-        }
-      }
+      Frag<T> pf, zf;
+      read_and_use<2 * ND>(cring, cread, [&](auto n, const Pair& p) {
+        if constexpr (n % ND == 0) pf = acc_frag<T>(s, n / ND), zf = acc_frag<T>(dp, n / ND);
+        dv[n % ND] = mma<T>(p.a, pf, dv[n % ND]);
+        dk[n % ND] = mma<T>(p.b, zf, dk[n % ND]);
+      });
     }
     if (more) store(buf ^ 1);
     buf ^= 1;
@@ -311,8 +326,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2)
   const float kScale = a.scale / f, vScale = F16 ? exp2f(-kPShift) : 1.0f;
   T* dkp = (T*)a.dk + (int64_t)b * a.dks[0] + (int64_t)hk * a.dks[1] + (int64_t)mykey * a.dks[2];
   T* dvp = (T*)a.dv + (int64_t)b * a.dvs[0] + (int64_t)hk * a.dvs[1] + (int64_t)mykey * a.dvs[2];
-  float* pk = a.part + ((((int64_t)split * 2) * a.B * a.Hk + bh) * a.M + mykey) * DP;
-  float* pv = pk + (int64_t)a.B * a.Hk * a.M * DP;
+  float* pk = a.part + ((((int64_t)split * 2) * a.B * a.Hk + bh) * a.M + mykey) * DC;
+  float* pv = pk + (int64_t)a.B * a.Hk * a.M * DC;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -326,16 +341,16 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 64 ? 1 : 2)
         *(f32x4*)(pk + c0) = x;
         *(f32x4*)(pv + c0) = y;
       } else {
-        store4<T>(dkp, c0, a.D, a.vecDk, x[0], x[1], x[2], x[3]);
-        store4<T>(dvp, c0, a.D, a.vecDv, y[0], y[1], y[2], y[3]);
+        store4<T>(dkp, c0, a.D, x[0], x[1], x[2], x[3]);
+        store4<T>(dvp, c0, a.D, y[0], y[1], y[2], y[3]);
       }
     }
 }
 
 // dq of 128 queries of one head, 32 per wave; keys stream through LDS in tiles of KT.
-template <typename T, int DP, bool MASK>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn_dq_kernel(const AttnArgs a) {
-  constexpr int KT = key_tile<T, DP>(), NT = DP / 16, ND = DP / 32;
+template <typename T, int DC, bool MASK>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_dq_kernel(const AttnArgs a) {
+  constexpr int DP = row_pitch(DC), KT = key_tile<T, DC>(), NT = DC / 16, ND = DC / 32;
   constexpr bool F16 = std::is_same<T, f16s>::value;
   using L = Tile<T, DP>;
   constexpr int TB = KT * L::ROW;
@@ -362,8 +377,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
     const T* gp = (const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)hq * a.gs[1] + (int64_t)nr * a.gs[2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      qf[t] = global_frag<T>(qp, alive, t, h, a.D, a.modeQ != kElements);
-      gf[t] = global_frag<T>(gp, alive, t, h, a.D, a.modeG != kElements);
+      qf[t] = global_frag<T>(qp, alive, t, h, a.D);
+      gf[t] = global_frag<T>(gp, alive, t, h, a.D);
     }
   }
   const float f = F16 ? dz_factor(a, b, hk) : 1.0f;
@@ -379,7 +394,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
 
   const T* kbase = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1];
   const T* vbase = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1];
-  using LD = Loader<T, DP, KT>;
+  using LD = Loader<T, DP, DC, KT>;
   const bool byKey = MASK && a.keyMask;
   auto fill = [&](int buf, int k0, uint32_t live) {
     LD::fill(smem + buf * 2 * TB, kbase, a.ks[2], k0, kend, a.D, a.modeK, live);
@@ -407,10 +422,15 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
       const int rl = launder(rl0), cl = launder(cl0);
       f32x16 s{}, dp{}, bias;
       if constexpr (MASK) mask_of_keys(a, moff, key0 + kb, h, bias);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) s = mma<T>(L::row_frag(tk + kb * L::ROW, rl, t), qf[t], s);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) dp = mma<T>(L::row_frag(tv + kb * L::ROW, rl, t), gf[t], dp);
+      {
+        auto read = [&](auto n) { return L::row_frag((n < NT ? tk : tv) + kb * L::ROW, rl, n % NT); };
+        Ring<Frag<T>, 4> ring;
+        first_reads<2 * NT>(ring, read);
+        read_and_use<2 * NT>(ring, read, [&](auto n, const Frag<T>& x) {
+          if constexpr (n < NT) s = mma<T>(x, qf[n], s);
+          else dp = mma<T>(x, gf[n - NT], dp);
+        });
+      }
       const bool check = MASK || key0 + kb + 32 > full;
       if (check) {
 #pragma unroll
@@ -420,14 +440,17 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
           dp[r] = s[r] == kNegInf ? 0.0f : dp[r];
         }
       }
+      // The first columns of k are read while the exponentials run.
+      auto cread = [&](auto n) { return L::col_frag(tk + kb * L::ROW, cl, n / ND, n % ND); };
+      Ring<Frag<T>, (sizeof(T) == 2 && DC <= 64 ? 4 : 2)> cring;
+      first_reads<2 * ND>(cring, cread);
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = prob<MASK>(s[r], a.c, x0, x1) * (F16 ? fmaf(dp[r], f, -de) : dp[r] - de);
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const Frag<T> zf = acc_frag<T>(dp, st);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) dq[d] = mma<T>(L::col_frag(tk + kb * L::ROW, cl, st, d), zf, dq[d]);
-      }
+      Frag<T> zf;
+      read_and_use<2 * ND>(cring, cread, [&](auto n, const Frag<T>& x) {
+        if constexpr (n % ND == 0) zf = acc_frag<T>(dp, n / ND);
+        dq[n % ND] = mma<T>(x, zf, dq[n % ND]);
+      });
     }
     buf ^= 1;
     land();
@@ -437,7 +460,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
   if (n >= a.N) return;
   const float scale = a.scale / f;
   T* dqp = (T*)a.dq + (int64_t)b * a.dqs[0] + (int64_t)hq * a.dqs[1] + (int64_t)n * a.dqs[2];
-  float* pq = a.part + (((int64_t)split * a.B * a.H + bhq) * a.N + n) * DP;
+  float* pq = a.part + (((int64_t)split * a.B * a.H + bhq) * a.N + n) * DC;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -446,27 +469,37 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
       f32x4 x = {dq[d][4 * gq], dq[d][4 * gq + 1], dq[d][4 * gq + 2], dq[d][4 * gq + 3]};
       x *= scale;
       if (a.nsplit > 1) *(f32x4*)(pq + c0) = x;
-      else store4<T>(dqp, c0, a.D, a.vecDq, x[0], x[1], x[2], x[3]);
+      else store4<T>(dqp, c0, a.D, x[0], x[1], x[2], x[3]);
     }
 }
 
-// Sums the splits' partial gradients of `rows` rows of heads x batch matrices in their order.
-template <typename T, int DP>
-__global__ void __launch_bounds__(256) attn_sum_kernel(const float* part, int nsplit, int64_t splitStride, T* out,
-                                                       int64_t s0, int64_t s1, int64_t s2, int heads, int rows,
-                                                       int64_t total, int D, int vec) {
-  constexpr int TPR = DP / 4, RPB = 256 / TPR;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+// One gradient whose splits' partial rows are to be added.
+struct SumOf {
+  const float* part;
+  int64_t splitStride, s0, s1, s2, rows;  // rows: heads x batch x `len`
+  void* out;
+  int nsplit, heads, len;
+};
+
+// Adds the splits' partial gradients in their order: DC / 4 threads per row, up to two gradients.
+template <typename T, int DC>
+__global__ void __launch_bounds__(256) attn_sum_kernel(const SumOf a0, const SumOf a1, int D) {
+  constexpr int TPR = DC == 96 ? 32 : DC / 4, RPB = 256 / TPR;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const bool second = row >= a0.rows;
+  const SumOf& a = second ? a1 : a0;
+  if (second) row -= a0.rows;
   const int c0 = (threadIdx.x % TPR) * 4;
-  if (row >= total) return;
+  if (row >= a.rows || c0 >= DC) return;
   f32x4 x = {0, 0, 0, 0};
-  for (int s = 0; s < nsplit; ++s) x += *(const f32x4*)(part + s * splitStride + row * DP + c0);
-  const int64_t bh = row / rows, n = row % rows;
-  store4<T>(out + bh / heads * s0 + bh % heads * s1 + n * s2, c0, D, vec, x[0], x[1], x[2], x[3]);
+#pragma unroll 8
+  for (int s = 0; s < a.nsplit; ++s) x += *(const f32x4*)(a.part + s * a.splitStride + row * DC + c0);
+  const int64_t bh = row / a.len, n = row % a.len;
+  store4<T>((T*)a.out + bh / a.heads * a.s0 + bh % a.heads * a.s1 + n * a.s2, c0, D, x[0], x[1], x[2], x[3]);
 }
 
 struct BwdPlan {
-  int dp, ktiles, ksplit, qtiles, qsplit, qchunk;
+  int dc, ktiles, ksplit, qtiles, qsplit, qchunk;
   size_t deltaBytes, boundBytes, partBytes;
 };
 
@@ -474,29 +507,25 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 BwdPlan bwd_plan(int dtype, const AttnArgs& a, int cus) {
   BwdPlan p{};
-  p.dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
+  p.dc = compute_dim(a.D);
   p.ktiles = (a.M + 127) / 128;
   p.qtiles = (a.N + 127) / 128;
-  // The other axis is split where a kernel's own blocks leave CUs without work, into
-  // shares of four tiles at least.
   const int64_t kw = (int64_t)a.B * a.Hk * p.ktiles, qw = (int64_t)a.B * a.H * p.qtiles;
-  const bool wide = dtype != LFAMD_F32 || p.dp == 32;
-  const int qt = wide && p.dp < 128 ? 64 : 32, kt = wide ? 64 : 32;  // query_tile, key_tile
+  const bool wide = dtype != LFAMD_F32 || p.dc == 32;
+  const int qt = wide && p.dc < 96 ? 64 : 32, kt = wide ? 64 : 32;  // query_tile, key_tile
   const int64_t ksteps = (int64_t)a.G * ((a.N + qt - 1) / qt), qsteps = (a.M + kt - 1) / kt;
-  auto splits = [&](int64_t wgs, int64_t steps) {
-    if (wgs >= cus || steps < 8) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + wgs - 1) / wgs, steps / 4, 64}));
-  };
-  p.ksplit = kw ? splits(kw, ksteps) : 1;
-  p.qsplit = qw ? splits(qw, qsteps) : 1;
-  p.qchunk = (int)((qsteps + p.qsplit - 1) / p.qsplit);
-  if (p.qchunk < 1) p.qchunk = 1;
-  p.qsplit = (int)std::max<int64_t>(1, (qsteps + p.qchunk - 1) / p.qchunk);
+  // The other axis is split where a kernel's own blocks leave CUs without work. A tile's time: its four
+  // (dq: three) products at the 3 TFLOP/s that a CU reaches (fp32: 0.45), and a microsecond at least.
+  const double rate = dtype == LFAMD_F32 ? 0.45e6 : 3e6, f32 = sizeof(float);
+  const double ktile = std::max(1.0, 8.0 * 128 * qt * p.dc / rate), qtile = std::max(0.8, 6.0 * 128 * kt * p.dc / rate);
+  p.ksplit = kw && ksteps ? best_split(kw, ksteps, cus, ktile, 2.0, 2.0 * a.B * a.Hk * a.M * p.dc * f32) : 1;
+  p.qsplit = qw && qsteps ? best_split(qw, qsteps, cus, qtile, 2.0, 1.0 * a.B * a.H * a.N * p.dc * f32) : 1;
+  p.qchunk = (int)std::max<int64_t>(1, (qsteps + p.qsplit - 1) / p.qsplit);
   p.deltaBytes = up256((size_t)a.B * a.H * a.N * sizeof(float));
   if (dtype == LFAMD_F16)
     p.boundBytes = up256(((size_t)a.B * a.H * ((a.N + 63) / 64) * 2 + (size_t)a.B * a.Hk * ((a.M + 63) / 64)) * sizeof(float));
-  const size_t kp = p.ksplit > 1 ? (size_t)p.ksplit * 2 * a.B * a.Hk * a.M * p.dp * sizeof(float) : 0;
-  const size_t qp = p.qsplit > 1 ? (size_t)p.qsplit * a.B * a.H * a.N * p.dp * sizeof(float) : 0;
+  const size_t kp = p.ksplit > 1 ? (size_t)p.ksplit * 2 * a.B * a.Hk * a.M * p.dc * sizeof(float) : 0;
+  const size_t qp = p.qsplit > 1 ? (size_t)p.qsplit * a.B * a.H * a.N * p.dc * sizeof(float) : 0;
   p.partBytes = std::max(kp, qp);
   return p;
 }
@@ -511,55 +540,55 @@ int launch(const void* fn, int64_t grid, size_t lds, const AttnArgs& a, hipStrea
   return check_launch(what);
 }
 
-template <typename T, int DP, bool MASK> int bwd_launch(AttnArgs a, const BwdPlan& p, hipStream_t st) {
+template <typename T, int DC> int sum_launch(const SumOf& a, const SumOf& b, int D, hipStream_t st) {
+  constexpr int RPB = 256 / (DC == 96 ? 32 : DC / 4);
+  attn_sum_kernel<T, DC><<<dim3((unsigned)((a.rows + b.rows + RPB - 1) / RPB)), dim3(256), 0, st>>>(a, b, D);
+  return check_launch("softmax_attention backward (sums)");
+}
+
+template <typename T, int DC, bool MASK> int bwd_launch(AttnArgs a, const BwdPlan& p, hipStream_t st) {
   constexpr bool F16 = std::is_same<T, f16s>::value;
   const int qt = (a.N + 63) / 64, kt = (a.M + 63) / 64;
   int64_t grid = (int64_t)a.B * a.H * qt + (F16 ? (int64_t)a.B * a.Hk * kt : 0);
   if (grid)
     if (int e = launch((const void*)attn_delta_kernel<T, F16>, grid, 0, a, st)) return e;
-  constexpr int RPB = 256 / (DP / 4);
   if (a.dk) {
     a.nsplit = p.ksplit;
     a.tiles = p.ktiles;
-    const size_t lds = dkdv_lds<T, DP>();
-    if (int e = launch((const void*)attn_dkdv_kernel<T, DP, MASK>, (int64_t)a.B * a.Hk * p.ktiles * p.ksplit, lds, a, st))
+    if (int e = launch((const void*)attn_dkdv_kernel<T, DC, MASK>, (int64_t)a.B * a.Hk * p.ktiles * p.ksplit,
+                       dkdv_lds<T, DC>(), a, st))
       return e;
     if (p.ksplit > 1) {
       const int64_t rows = (int64_t)a.B * a.Hk * a.M;
-      for (int i = 0; i < 2; ++i) {
-        const int64_t* s = i ? a.dvs : a.dks;
-        attn_sum_kernel<T, DP><<<dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(256), 0, st>>>(
-            a.part + i * rows * DP, p.ksplit, 2 * rows * DP, (T*)(i ? a.dv : a.dk), s[0], s[1], s[2], a.Hk, a.M, rows, a.D,
-            i ? a.vecDv : a.vecDk);
-        if (int e = check_launch("softmax_attention backward (sums)")) return e;
-      }
+      const SumOf k{a.part, 2 * rows * DC, a.dks[0], a.dks[1], a.dks[2], rows, a.dk, p.ksplit, a.Hk, a.M};
+      const SumOf v{a.part + rows * DC, 2 * rows * DC, a.dvs[0], a.dvs[1], a.dvs[2], rows, a.dv, p.ksplit, a.Hk, a.M};
+      if (int e = sum_launch<T, DC>(k, v, a.D, st)) return e;
     }
   }
   if (a.dq) {
     a.nsplit = p.qsplit;
     a.tiles = p.qtiles;
     a.chunk = p.qchunk;
-    const size_t lds = dq_lds<T, DP>();
-    if (int e = launch((const void*)attn_dq_kernel<T, DP, MASK>, (int64_t)a.B * a.H * p.qtiles * p.qsplit, lds, a, st))
+    if (int e = launch((const void*)attn_dq_kernel<T, DC, MASK>, (int64_t)a.B * a.H * p.qtiles * p.qsplit, dq_lds<T, DC>(), a, st))
       return e;
     if (p.qsplit > 1) {
       const int64_t rows = (int64_t)a.B * a.H * a.N;
-      attn_sum_kernel<T, DP><<<dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(256), 0, st>>>(
-          a.part, p.qsplit, rows * DP, (T*)a.dq, a.dqs[0], a.dqs[1], a.dqs[2], a.H, a.N, rows, a.D, a.vecDq);
-      if (int e = check_launch("softmax_attention backward (sums)")) return e;
+      const SumOf q{a.part, rows * DC, a.dqs[0], a.dqs[1], a.dqs[2], rows, a.dq, p.qsplit, a.H, a.N};
+      if (int e = sum_launch<T, DC>(q, SumOf{}, a.D, st)) return e;
     }
   }
   return ok();
 }
 
-template <typename T, int DP> int bwd_mask(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
-  return a.maskKind ? bwd_launch<T, DP, true>(a, p, st) : bwd_launch<T, DP, false>(a, p, st);
+template <typename T, int DC> int bwd_mask(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
+  return a.maskKind ? bwd_launch<T, DC, true>(a, p, st) : bwd_launch<T, DC, false>(a, p, st);
 }
 
 template <typename T> int bwd_dim(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
-  switch (p.dp) {
+  switch (p.dc) {
     case 32: return bwd_mask<T, 32>(a, p, st);
     case 64: return bwd_mask<T, 64>(a, p, st);
+    case 96: return bwd_mask<T, 96>(a, p, st);
     default: return bwd_mask<T, 128>(a, p, st);
   }
 }

@@ -87,6 +87,10 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// Channels that a kernel computes with for heads of D, and elements from one LDS row to the next.
+inline int compute_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+__host__ __device__ constexpr int row_pitch(int dc) { return dc == 96 ? 128 : dc; }
+
 // A tile of rows of DP elements in LDS, in 16-byte chunks. A row's chunks are
 // exchanged (xor with f(row)) so that both ways it is read spread over the 64
 // banks: row_frag (32 rows, one chunk each) and col_frag (four rows x 32 bytes
@@ -168,8 +172,11 @@ __device__ __forceinline__ int launder(int x) {
   return x;
 }
 
-// Asks the scheduler to keep AHEAD fragment reads in flight in front of N matrix instructions that take
-// one each: left alone it reads, waits and multiplies in turn, to save registers that are free.
+// Keeps the order of what stands before and behind: left alone the scheduler puts every fragment's read
+// right in front of its product, and waits there, to save registers that are free.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// The weaker form for a row of N reads and products in one block: AHEAD reads in front, then one by one.
 template <int N, int AHEAD> __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
@@ -180,76 +187,119 @@ template <int N, int AHEAD> __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
 }
 
-// How a tensor's rows are read: to LDS directly, by 16-byte vectors, by elements.
-enum LoadMode { kElements = 0, kVector = 1, kAsync = 2 };
+// use(i, x) for i = 0 .. N - 1 on what read(i) gives, AHEAD reads in flight. ring: the first AHEAD reads,
+// which first_reads() has issued earlier (in front of other work that they then overlap).
+template <typename F, int AHEAD> struct Ring { F x[AHEAD + 1]; };
+template <int N, int AHEAD, typename F, typename R> __device__ __forceinline__ void first_reads(Ring<F, AHEAD>& ring, R&& read) {
+  unrolled<(AHEAD < N ? AHEAD : N)>([&](auto i) { ring.x[i] = read(i); });
+  fence();
+}
+template <int N, int AHEAD, typename F, typename R, typename U>
+__device__ __forceinline__ void read_and_use(Ring<F, AHEAD>& ring, R&& read, U&& use) {
+  unrolled<N>([&](auto i) {
+    if constexpr (i + AHEAD < N) ring.x[(i + AHEAD) % (AHEAD + 1)] = read(std::integral_constant<int, i + AHEAD>{});
+    fence();
+    use(i, ring.x[i % (AHEAD + 1)]);
+  });
+}
 
-// 16 bytes of a row from element c0 on, zero where row or column is outside.
-// vec: the row is 16-byte aligned and D a multiple of the chunk.
-template <typename T>
-__device__ __forceinline__ u32x4 load_chunk(const T* row, bool inside, int c0, int D, bool vec) {
+// How a tensor's rows are read: kAsync, to LDS directly by 16 bytes (rows 16-byte aligned, D a multiple of
+// 16 bytes); kAsync4, to LDS directly by 4 bytes (the same with 4); kPlain, through registers by 16 bytes at
+// any alignment. The first two keep a tile's offsets within 32 bits.
+enum LoadMode { kPlain = 0, kAsync4 = 1, kAsync = 2 };
+
+// 16 bytes of a row from element c0 on at any alignment, zero where row or column is outside.
+template <typename T> __device__ __forceinline__ u32x4 load_chunk(const T* row, bool inside, int c0, int D) {
   constexpr int CE = 16 / (int)sizeof(T);
   u32x4 r = {0, 0, 0, 0};
   if (!inside || c0 >= D) return r;
-  if (vec) return *(const u32x4*)(row + c0);
-  if constexpr (sizeof(T) == 2) {
-    const uint16_t* p = (const uint16_t*)(row + c0);
-#pragma unroll
-    for (int j = 0; j < CE; ++j)
-      if (c0 + j < D) r[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
-  } else {
-    const uint32_t* p = (const uint32_t*)(row + c0);
-#pragma unroll
-    for (int j = 0; j < CE; ++j)
-      if (c0 + j < D) r[j] = p[j];
+  if (c0 + CE <= D) {
+    __builtin_memcpy(&r, row + c0, 16);
+    return r;
   }
+#pragma unroll
+  for (int j = 0; j < CE - 1; ++j)
+    if (c0 + j < D) {
+      if constexpr (sizeof(T) == 2) r[j >> 1] |= (uint32_t)((const uint16_t*)(row + c0))[j] << (16 * (j & 1));
+      else r[j] = ((const uint32_t*)(row + c0))[j];
+    }
   return r;
 }
 
-// 16 bytes per lane from base + off (base uniform) to LDS at `lds` + 16 lane, without registers in between.
-// In asm because the compiler puts a wait for every such load in front of the next transposing LDS read,
-// whichever tile that reads; there is no output register that it could reuse early, and land() is the wait.
-// M0 takes the LDS address, one wait state in front of its use, and gets its value back (the compiler does not
-// take it as a clobber).
-__device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds) {
+// 16 (or 4) bytes per lane from base + off (base uniform) to LDS at lds + 16 (or 4) lane, without registers in
+// between. In asm because the compiler puts a wait for every such load in front of the next transposing LDS
+// read, whichever tile that reads; there is no output register that it could reuse early, and land() is the
+// wait. M0 takes the LDS address, one wait state in front of its use, and gets its value back (the compiler
+// does not take it as a clobber).
+template <int BYTES> __device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds) {
   uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-               : "=&s"(m0)
-               : "v"(off), "s"(base), "s"(lds)
-               : "memory");
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "v"(off), "s"(base), "s"(lds)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "v"(off), "s"(base), "s"(lds)
+                 : "memory");
 }
 
 // Rows of a matrix into an LDS tile by a workgroup of 256 threads. Thread t fills the
-// tile's t-th chunk of every 4 KiB, whose place in the row the tile's exchange gives:
-// the loads go to LDS without passing through registers, a wave's 64 chunks side by side.
-// Rows at or behind `limit`, columns behind D and rows whose bit in `live` is 0 are zero
-// and not read. fill() issues; land() waits for this wave's loads, before the barrier
-// behind which the tile may be read.
-template <typename T, int DP, int ROWS> struct Loader {
+// tile's t-th chunk of every 4 KiB (kAsync4: the t-th word of every 1 KiB), whose place in
+// the row the tile's exchange gives: a wave's loads land side by side. Rows at or behind
+// `limit`, columns from D to DC (what the kernel computes with) and rows whose bit in `live`
+// is 0 are zero and not read. fill() issues; land() waits for this wave's loads, before the
+// barrier behind which the tile may be read.
+template <typename T, int DP, int DC, int ROWS> struct Loader {
   using L = Tile<T, DP>;
   static constexpr int RPI = 256 / L::CPR, NIT = ROWS / RPI;
   static_assert(256 % L::CPR == 0 && ROWS % RPI == 0 && NIT <= 32, "tile shape");
 
   static __device__ __forceinline__ int row_of(int i) { return (int)threadIdx.x / L::CPR + i * RPI; }
 
-  // mode: kAsync, 16-byte aligned rows whose tile spans less than 2 GiB; kVector, 16-byte
-  // aligned; kElements, neither.
   static __device__ __forceinline__ void fill(char* tile, const T* base, int64_t stride, int row0, int limit, int D,
                                               int mode, uint32_t live = ~0u) {
     const int slot = threadIdx.x % L::CPR;
-    if (mode == kAsync) {
-      const char* from = (const char*)(base + (int64_t)row0 * stride);  // uniform
-      const uint32_t rowBytes = (uint32_t)stride * (uint32_t)sizeof(T);
-      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tile + uniform(threadIdx.x >> 6) * 1024;
-      const bool whole = row0 + ROWS <= limit && D == DP && live == ~0u;
+    const char* from = (const char*)(base + (int64_t)row0 * stride);  // uniform
+    const uint32_t rowBytes = (uint32_t)stride * (uint32_t)sizeof(T);
+    const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tile;
+    const int wave = uniform(threadIdx.x >> 6);
+    if (__builtin_expect(mode == kAsync && row0 + ROWS <= limit && live == ~0u, 1)) {
+      // A whole tile of rows, the loop's ordinary case: no branch between its loads at D = DP.
+      if (D == DP) {
 #pragma unroll
+        for (int i = 0; i < NIT; ++i) {
+          const int r = row_of(i), c = slot ^ L::swz(r);
+          load_to_lds<16>(from, (uint32_t)r * rowBytes + (uint32_t)c * 16, to + wave * 1024 + i * 4096);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NIT; ++i) {
+          const int r = row_of(i), c = slot ^ L::swz(r);
+          if (c * L::CE < D) load_to_lds<16>(from, (uint32_t)r * rowBytes + (uint32_t)c * 16, to + wave * 1024 + i * 4096);
+          else if (c * L::CE < DC) *(u32x4*)(tile + i * 4096 + threadIdx.x * 16) = (u32x4){0, 0, 0, 0};
+        }
+      }
+    } else if (mode == kAsync) {
+#pragma unroll 1
       for (int i = 0; i < NIT; ++i) {
         const int r = row_of(i), c = slot ^ L::swz(r);
-        const uint32_t off = (uint32_t)r * rowBytes + (uint32_t)c * 16;
-        if (whole || (row0 + r < limit && c * L::CE < D && (live >> i & 1))) {
-          load_to_lds(from, off, to + i * 4096);
-        } else {
+        if (row0 + r < limit && c * L::CE < D && (live >> i & 1))
+          load_to_lds<16>(from, (uint32_t)r * rowBytes + (uint32_t)c * 16, to + wave * 1024 + i * 4096);
+        else if (c * L::CE < DC)
           *(u32x4*)(tile + i * 4096 + threadIdx.x * 16) = (u32x4){0, 0, 0, 0};
-        }
+      }
+    } else if (mode == kAsync4) {
+      // `live` belongs to the rows of row_of: a call with a mask over keys takes kPlain instead.
+#pragma unroll 1
+      for (int i = 0; i < 4 * NIT; ++i) {
+        const int byte = i * 1024 + (int)threadIdx.x * 4, r = byte / L::ROW;
+        const int c = (byte % L::ROW / 16 ^ L::swz(r)) * L::CE + byte % 16 / (int)sizeof(T);
+        if (row0 + r < limit && c < D)
+          load_to_lds<4>(from, (uint32_t)r * rowBytes + (uint32_t)c * (uint32_t)sizeof(T), to + wave * 256 + i * 1024);
+        else if (c < DC)
+          *(uint32_t*)(tile + byte) = 0;
       }
     } else {
       // Not unrolled: few registers beside the kernel's accumulators.
@@ -257,7 +307,7 @@ template <typename T, int DP, int ROWS> struct Loader {
       for (int i = 0; i < NIT; ++i) {
         const int r = row_of(i), c = slot ^ L::swz(r);
         *(u32x4*)(tile + i * 4096 + threadIdx.x * 16) =
-            load_chunk<T>(base + (int64_t)(row0 + r) * stride, row0 + r < limit && (live >> i & 1), c * L::CE, D, mode == kVector);
+            load_chunk<T>(base + (int64_t)(row0 + r) * stride, row0 + r < limit && (live >> i & 1), c * L::CE, D);
       }
     }
   }
@@ -272,42 +322,41 @@ __device__ __forceinline__ void land() {
 
 // The eight elements 16 t + 8 h .. + 7 of a row in memory.
 template <typename T>
-__device__ __forceinline__ Frag<T> global_frag(const T* row, bool inside, int t, int h, int D, bool vec) {
+__device__ __forceinline__ Frag<T> global_frag(const T* row, bool inside, int t, int h, int D) {
   Frag<T> f;
   const int c0 = 16 * t + 8 * h;
   if constexpr (sizeof(T) == 2) {
-    f.v = load_chunk<T>(row, inside, c0, D, vec);
+    f.v = load_chunk<T>(row, inside, c0, D);
   } else {
-    const f32x4 a = __builtin_bit_cast(f32x4, load_chunk<T>(row, inside, c0, D, vec));
-    const f32x4 b = __builtin_bit_cast(f32x4, load_chunk<T>(row, inside, c0 + 4, D, vec));
+    const f32x4 a = __builtin_bit_cast(f32x4, load_chunk<T>(row, inside, c0, D));
+    const f32x4 b = __builtin_bit_cast(f32x4, load_chunk<T>(row, inside, c0 + 4, D));
     f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
   return f;
 }
 
-// Four consecutive elements of a row from c0 on, rounded from fp32.
+// Four consecutive elements of a row from c0 on, rounded from fp32, at any alignment.
 template <typename T>
-__device__ __forceinline__ void store4(T* row, int c0, int D, bool vec, float a, float b, float c, float d) {
+__device__ __forceinline__ void store4(T* row, int c0, int D, float a, float b, float c, float d) {
   if constexpr (sizeof(T) == 2) {
-    const uint32_t lo = pack2<T>(a, b), hi = pack2<T>(c, d);
-    if (vec) {
-      if (c0 < D) *(u32x2*)(row + c0) = (u32x2){lo, hi};
+    const u32x2 w = {pack2<T>(a, b), pack2<T>(c, d)};
+    if (c0 + 4 <= D) {
+      __builtin_memcpy(row + c0, &w, 8);
       return;
     }
     uint16_t* p = (uint16_t*)(row + c0);
-    if (c0 < D) p[0] = (uint16_t)lo;
-    if (c0 + 1 < D) p[1] = (uint16_t)(lo >> 16);
-    if (c0 + 2 < D) p[2] = (uint16_t)hi;
-    if (c0 + 3 < D) p[3] = (uint16_t)(hi >> 16);
+    if (c0 < D) p[0] = (uint16_t)w[0];
+    if (c0 + 1 < D) p[1] = (uint16_t)(w[0] >> 16);
+    if (c0 + 2 < D) p[2] = (uint16_t)w[1];
   } else {
-    if (vec) {
-      if (c0 < D) *(f32x4*)(row + c0) = (f32x4){a, b, c, d};
+    const f32x4 w = {a, b, c, d};
+    if (c0 + 4 <= D) {
+      __builtin_memcpy(row + c0, &w, 16);
       return;
     }
     if (c0 < D) row[c0] = a;
     if (c0 + 1 < D) row[c0 + 1] = b;
     if (c0 + 2 < D) row[c0 + 2] = c;
-    if (c0 + 3 < D) row[c0 + 3] = d;
   }
 }
 
@@ -340,8 +389,7 @@ struct AttnArgs {
   int64_t ms[4];                       // mask strides: batch, head, row, key (0 where broadcast)
   int B, H, Hk, G, N, M, D;
   int maskKind, causal, keyMask;       // keyMask: the mask is the same for every head and row
-  int modeQ, modeK, modeV, modeG;       // LoadMode of the streamed tensors
-  int vecO, vecDq, vecDk, vecDv;
+  int modeQ, modeK, modeV, modeG;      // LoadMode where the tensor streams through LDS
   int nsplit, tiles, chunk;            // work split along the other axis; tiles along the own one; steps per split
   float scale, c;                      // c = scale * log2(e)
   FastDiv divN;
@@ -449,6 +497,23 @@ template <typename LD> __device__ __forceinline__ uint32_t live_keys(const AttnA
     bits |= (uint32_t)(mask_bias(a, (int64_t)b * a.ms[0] + (int64_t)j * a.ms[3]) != kNegInf) << i;
   }
   return LD::NIT == 32 || bits != (1u << (LD::NIT & 31)) - 1 ? bits : ~0u;
+}
+
+// How many pieces to cut the streamed axis of `steps` tiles into, for `wgs` workgroups on `cus` CUs: the
+// least of what the busiest CU takes, at `tile` us per tile and `pro` us for a workgroup's start and end
+// (workgroups that share a CU overlap: each beyond the first adds 0.7), and of joining n pieces of `bytes`
+// fp32 each, written and read at 4 TB/s behind a launch of 4 us.
+inline int best_split(int64_t wgs, int64_t steps, int cus, double tile, double pro, double bytes) {
+  int best = 1;
+  double least = 0;
+  for (int64_t n = 1; n <= 64 && n <= steps; ++n) {
+    const int64_t chunk = (steps + n - 1) / n, share = (wgs * n + cus - 1) / cus;
+    if ((steps + chunk - 1) / chunk != n) continue;  // fewer pieces do the same
+    const double cost = (share <= 1 ? 1.0 : 0.7 * (double)share) * ((double)chunk * tile + pro) +
+                        (n > 1 ? 4.0 + (double)n * 2.0 * bytes / 4e6 : 0.0);
+    if (n == 1 || cost < least) best = (int)n, least = cost;
+  }
+  return best;
 }
 
 // The workgroup's place: consecutive places on one XCD (workgroups are dealt to

@@ -33,9 +33,9 @@ template <typename T, int DP, int KS> constexpr int num_buffers() {
 
 // QB: 32-query blocks per wave. KS: 1, the four waves take different queries; 4,
 // they take different keys of each tile and their results are joined at the end.
-template <typename T, int DP, int QB, int KS, bool MASK>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn_fwd_kernel(const AttnArgs a) {
-  constexpr int KT = key_tile<KS>(), NBUF = num_buffers<T, DP, KS>(), NT = DP / 16, ND = DP / 32;
+template <typename T, int DC, int QB, int KS, bool MASK>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_fwd_kernel(const AttnArgs a) {
+  constexpr int DP = row_pitch(DC), KT = key_tile<KS>(), NBUF = num_buffers<T, DP, KS>(), NT = DC / 16, ND = DC / 32;
   constexpr int KB = KS == 1 ? KT / 32 : 1;  // 32-key blocks per wave and tile
   constexpr int ROWS = KS == 1 ? 128 * QB : 32 * QB;
   using L = Tile<T, DP>;
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
 #pragma unroll
   for (int i = 0; i < QB; ++i)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) qf[i][t] = global_frag<T>((const T*)a.q + qoff[i], alive[i], t, h, a.D, a.modeQ != kElements);
+    for (int t = 0; t < NT; ++t) qf[i][t] = global_frag<T>((const T*)a.q + qoff[i], alive[i], t, h, a.D);
 
   f32x16 o[ND][QB];
   float m[QB], l[QB];
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
 
   const T* kbase = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1];
   const T* vbase = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1];
-  using LD = Loader<T, DP, KT>;
+  using LD = Loader<T, DP, DC, KT>;
   // Keys that a mask takes from every query are not read either: what they hold is nobody's.
   const bool byKey = MASK && a.keyMask;
   auto fill = [&](int buf, int key0, uint32_t live) {
@@ -141,16 +141,18 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
       }
       f32x16 s[KB][QB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < QB; ++i) s[kb][i] = f32x16{};
+      const char* tkw = tk + (KS == 1 ? 0 : 32 * wave) * L::ROW;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const Frag<T> kf = L::row_frag(tk + (KS == 1 ? 32 * kb : 32 * wave) * L::ROW, rl, t);
+          const Frag<T> kf = L::row_frag(tkw + 32 * kb * L::ROW, rl, t);
 #pragma unroll
           for (int i = 0; i < QB; ++i) s[kb][i] = mma<T>(kf, qf[i][t], s[kb][i]);
         }
-      }
       if constexpr (sizeof(T) == 2 && QB == 1) reads_ahead<KB * NT, (KB * NT < 4 ? KB * NT : 4)>();
       // The mask, and what lies behind the row's last key.
       if (MASK || wkey + 32 * KB > full) {
@@ -203,6 +205,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
           }
         l[i] += sum;
       }
+      const char* tvw = tv + (KS == 1 ? 0 : 32 * wave) * L::ROW;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -212,7 +215,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
           for (int i = 0; i < QB; ++i) pf[i] = acc_frag<T>(s[kb][i], st);
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
-            const Frag<T> vf = L::col_frag(tv + (KS == 1 ? 32 * kb : 32 * wave) * L::ROW, cl, st, d);
+            const Frag<T> vf = L::col_frag(tvw + 32 * kb * L::ROW, cl, st, d);
 #pragma unroll
             for (int i = 0; i < QB; ++i) o[d][i] = mma<T>(vf, pf[i], o[d][i]);
           }
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
   constexpr float kUnit = MASK ? kLog2e : 1.0f;
   if constexpr (KS == 4) {
     // Join the four waves' results through LDS (the loop's last barrier has passed).
-    constexpr int PS = DP + 4;  // floats per row: rows start four banks apart
+    constexpr int PS = DC + 4;  // floats per row: rows start four banks apart
     static_assert(QB == 1, "one query block where the waves share it");
     static_assert(4 * 32 * (PS + 2) * 4 <= 2 * NBUF * TB, "the tiles' LDS holds the partial results");
     float* po = (float*)smem;
@@ -275,14 +278,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
       x *= inv;
       if (!live) x = f32x4{0, 0, 0, 0};
       if (a.nsplit > 1) {
-        *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[0]) * DP + c0) = x;
+        *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[0]) * DC + c0) = x;
       } else {
-        store4<T>((T*)a.out + ooff[0], c0, a.D, a.vecO, x[0], x[1], x[2], x[3]);
+        store4<T>((T*)a.out + ooff[0], c0, a.D, x[0], x[1], x[2], x[3]);
       }
     }
     if (wave == 0 && h == 0) {
       if (a.nsplit > 1) {
-        float* ps = a.part + (int64_t)a.nsplit * a.B * a.Hk * R * DP + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[0]) * 2;
+        float* ps = a.part + (int64_t)a.nsplit * a.B * a.Hk * R * DC + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[0]) * 2;
         ps[0] = live ? mt : kNegInf;
         ps[1] = live ? lt : 0.0f;
       } else if (a.stat) {
@@ -310,14 +313,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
           x *= inv;
           if (none) x = f32x4{0, 0, 0, 0};
           if (a.nsplit > 1) {
-            *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[i]) * DP + c0) = x;
+            *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[i]) * DC + c0) = x;
           } else {
-            store4<T>((T*)a.out + ooff[i], c0, a.D, a.vecO, x[0], x[1], x[2], x[3]);
+            store4<T>((T*)a.out + ooff[i], c0, a.D, x[0], x[1], x[2], x[3]);
           }
         }
       if (h == 0) {
         if (a.nsplit > 1) {
-          float* ps = a.part + (int64_t)a.nsplit * a.B * a.Hk * R * DP +
+          float* ps = a.part + (int64_t)a.nsplit * a.B * a.Hk * R * DC +
                       (((int64_t)split * a.B * a.Hk + bh) * R + qrow[i]) * 2;
           ps[0] = none ? kNegInf : m[i];
           ps[1] = none ? 0.0f : l[i];
@@ -334,33 +337,62 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP >= 128 ? 1 : 2) attn
   }
 }
 
-// Joins the key splits' partial results: one row of DP columns per DP / 4 threads.
-template <typename T, int DP, bool MASK>
+// Joins the key splits' partial results. DC / 4 threads (32 for 96) take a row's columns, four
+// each; SHARE: a workgroup has one row, whose splits its groups of threads divide (few rows),
+// else each group has a row of its own.
+template <typename T, int DC, bool MASK, bool SHARE>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
-  constexpr int TPR = DP / 4, RPB = 256 / TPR;
+  constexpr int TPR = DC == 96 ? 32 : DC / 4, GROUPS = 256 / TPR;
   constexpr float kUnit = MASK ? kLog2e : 1.0f;
   const int64_t R = (int64_t)a.G * a.N, total = (int64_t)a.B * a.Hk * R;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  const int c0 = (threadIdx.x % TPR) * 4;
-  if (row >= total) return;
-  const float* ps = a.part + (int64_t)a.nsplit * total * DP;
+  const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR, c0 = t * 4, lane0 = (threadIdx.x & 63) - t;
+  const int64_t at = SHARE ? blockIdx.x : (int64_t)blockIdx.x * GROUPS + grp, row = at < total ? at : total - 1;
+  const float* ps = a.part + (int64_t)a.nsplit * total * DC;
+  const int first = SHARE ? grp : 0, step = SHARE ? GROUPS : 1;
+  const int mine = (a.nsplit - first + step - 1) / step;  // splits of this group: first + i step
   float m = kNegInf;
-  for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, ps[(s * total + row) * 2]);
+  for (int s = t; s < a.nsplit; s += TPR) m = fmaxf(m, ps[(s * total + row) * 2]);
+#pragma unroll
+  for (int i = 1; i < TPR; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
   const float ref = m == kNegInf ? 0.0f : m;
   float l = 0.0f;
   f32x4 x = {0, 0, 0, 0};
-  for (int s = 0; s < a.nsplit; ++s) {
-    const float f = exp2_fast((ps[(s * total + row) * 2] - ref) * kUnit);
-    l += f * ps[(s * total + row) * 2 + 1];
-    x += f * *(const f32x4*)(a.part + (s * total + row) * DP + c0);
+  for (int i0 = 0; i0 < mine; i0 += TPR) {
+    const int own = first + min(i0 + t, mine - 1) * step;
+    const f32x2 st = *(const f32x2*)(ps + (own * total + row) * 2);
+    const float f = i0 + t < mine ? exp2_fast((st[0] - ref) * kUnit) : 0.0f;
+    l += f * st[1];
+    const int n = min(TPR, mine - i0);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const f32x4 y = *(const f32x4*)(a.part + ((first + (i0 + i) * step) * total + row) * DC + min(c0, DC - 4));
+      x += __shfl(f, lane0 + i) * y;
+    }
   }
+#pragma unroll
+  for (int i = 1; i < TPR; i <<= 1) l += __shfl_xor(l, i);
+  if constexpr (SHARE) {
+    __shared__ float sx[256][4], sl[GROUPS];
+    *(f32x4*)sx[threadIdx.x] = x;
+    if (t == 0) sl[grp] = l;
+    __syncthreads();
+    if (grp) return;
+    l = 0.0f;
+    x = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      l += sl[g];
+      x += *(const f32x4*)sx[g * TPR + t];
+    }
+  }
+  if (at >= total || c0 >= DC) return;
   const bool none = l == 0.0f;
   x *= none ? 0.0f : 1.0f / l;
   if (none) x = f32x4{0, 0, 0, 0};
   const int bh = (int)(row / R), r = (int)(row % R), b = bh / a.Hk, hk = bh % a.Hk;
   const int g = a.divN.div(r), n = r - g * a.N, hq = hk * a.G + g;
   T* out = (T*)a.out + (int64_t)b * a.os[0] + (int64_t)hq * a.os[1] + (int64_t)n * a.os[2];
-  store4<T>(out, c0, a.D, a.vecO, x[0], x[1], x[2], x[3]);
+  store4<T>(out, c0, a.D, x[0], x[1], x[2], x[3]);
   if (a.stat && c0 == 0) {
     const int64_t so = ((int64_t)b * a.H + hq) * a.N + n;
     if (MASK) {
@@ -374,35 +406,34 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
 
 // How a call is laid over the chip.
 struct FwdPlan {
-  int ks, qb, rows, kt, tiles, nsplit, chunk, dp;
+  int ks, rows, kt, tiles, nsplit, chunk, dc;
 };
 
-FwdPlan fwd_plan(const AttnArgs& a, int cus) {
+FwdPlan fwd_plan(int dtype, const AttnArgs& a, int cus) {
   FwdPlan p;
   const int64_t R = (int64_t)a.G * a.N;
-  p.dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
+  p.dc = compute_dim(a.D);
   // Up to 32 rows per key head fill one wave's block: the four waves then share the
   // rows and divide each tile's keys.
   p.ks = R <= 32 ? 4 : 1;
-  p.qb = 1;
-  p.rows = p.ks == 4 ? 32 : 128 * p.qb;
+  p.rows = p.ks == 4 ? 32 : 128;
   p.kt = p.ks == 4 ? 128 : 64;
   p.tiles = (int)((R + p.rows - 1) / p.rows);
   const int64_t wgs = (int64_t)a.B * a.Hk * p.tiles;
   const int steps = (a.M + p.kt - 1) / p.kt;
-  // The keys are split where the rows alone leave CUs without work, into pieces of
-  // four tiles at least, so that the join stays small beside them.
-  int64_t ns = 1;
-  if (wgs < cus && steps >= 8) ns = std::min<int64_t>((2 * cus + wgs - 1) / wgs, steps / 4);
-  ns = std::max<int64_t>(1, std::min<int64_t>(ns, 64));
-  p.chunk = (int)((steps + ns - 1) / ns);
-  if (p.chunk < 1) p.chunk = 1;
+  // The keys are split where the rows alone leave CUs without work. A tile's time: its products at the
+  // 3.5 TFLOP/s that a CU reaches (fp32: 0.5), and a microsecond at least where one wave's latencies add up.
+  const double flops = 4.0 * (p.ks == 4 ? 128 : 128 * 64) * p.dc * (p.ks == 4 ? 32 : 1);
+  const double tile = std::max(p.ks == 4 ? 1.0 : 0.8, flops / (dtype == LFAMD_F32 ? 0.5e6 : 3.5e6));
+  const int ns = best_split(wgs, steps, cus, tile, 2.0, (double)a.B * a.Hk * R * p.dc * sizeof(float));
+  p.chunk = std::max(1, (steps + ns - 1) / ns);
   p.nsplit = std::max(1, (steps + p.chunk - 1) / p.chunk);
   return p;
 }
 
-template <typename T, int DP, bool MASK> int fwd_launch(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
-  const void* fn = p.ks == 4 ? (const void*)attn_fwd_kernel<T, DP, 1, 4, MASK> : (const void*)attn_fwd_kernel<T, DP, 1, 1, MASK>;
+template <typename T, int DC, bool MASK> int fwd_launch(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
+  constexpr int DP = row_pitch(DC);
+  const void* fn = p.ks == 4 ? (const void*)attn_fwd_kernel<T, DC, 1, 4, MASK> : (const void*)attn_fwd_kernel<T, DC, 1, 1, MASK>;
   const int nbuf = p.ks == 4 ? num_buffers<T, DP, 4>() : num_buffers<T, DP, 1>();
   const size_t lds = (size_t)2 * nbuf * p.kt * DP * sizeof(T);
   if (int e = set_dyn_lds(fn, lds, "softmax_attention")) return e;
@@ -415,35 +446,38 @@ template <typename T, int DP, bool MASK> int fwd_launch(const AttnArgs& a, const
   if (int e = check_launch("softmax_attention")) return e;
   if (p.nsplit > 1) {
     const int64_t rows = (int64_t)a.B * a.Hk * a.G * a.N;
-    constexpr int RPB = 256 / (DP / 4);
-    attn_join_kernel<T, DP, MASK><<<dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(256), 0, st>>>(a);
+    constexpr int RPB = 256 / (DC == 96 ? 32 : DC / 4);
+    // Up to eight workgroups per CU, a row each: what counts is the depth of the loop over the splits.
+    if (rows <= 8 * (int64_t)num_cus()) attn_join_kernel<T, DC, MASK, true><<<dim3((unsigned)rows), dim3(256), 0, st>>>(a);
+    else attn_join_kernel<T, DC, MASK, false><<<dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(256), 0, st>>>(a);
     return check_launch("softmax_attention (join)");
   }
   return ok();
 }
 
-template <typename T, int DP> int fwd_mask(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
-  return a.maskKind ? fwd_launch<T, DP, true>(a, p, st) : fwd_launch<T, DP, false>(a, p, st);
+template <typename T, int DC> int fwd_mask(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
+  return a.maskKind ? fwd_launch<T, DC, true>(a, p, st) : fwd_launch<T, DC, false>(a, p, st);
 }
 
 template <typename T> int fwd_dim(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
-  switch (p.dp) {
+  switch (p.dc) {
     case 32: return fwd_mask<T, 32>(a, p, st);
     case 64: return fwd_mask<T, 64>(a, p, st);
+    case 96: return fwd_mask<T, 96>(a, p, st);
     default: return fwd_mask<T, 128>(a, p, st);
   }
 }
 
 }  // namespace
 
-size_t attn_fwd_workspace(const AttnArgs& a) {
-  const FwdPlan p = fwd_plan(a, num_cus());
+size_t attn_fwd_workspace(int dtype, const AttnArgs& a) {
+  const FwdPlan p = fwd_plan(dtype, a, num_cus());
   if (p.nsplit <= 1) return 0;
-  return (size_t)p.nsplit * a.B * a.Hk * a.G * a.N * (p.dp + 2) * sizeof(float);
+  return (size_t)p.nsplit * a.B * a.Hk * a.G * a.N * (p.dc + 2) * sizeof(float);
 }
 
 int attn_fwd(int dtype, AttnArgs a, hipStream_t st) {
-  const FwdPlan p = fwd_plan(a, num_cus());
+  const FwdPlan p = fwd_plan(dtype, a, num_cus());
   a.nsplit = p.nsplit;
   a.tiles = p.tiles;
   a.chunk = p.chunk;

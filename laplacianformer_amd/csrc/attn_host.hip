@@ -11,14 +11,15 @@ namespace {
 
 constexpr int64_t kMostRows = (int64_t)1 << 30;
 
-bool vec_ok(const void* p, const int64_t* strides, int64_t d, int64_t ce) {
-  return ((uintptr_t)p & 15) == 0 && d % ce == 0 && strides[0] % ce == 0 && strides[1] % ce == 0 && strides[2] % ce == 0;
-}
-
-// The offsets inside a tile of at most 128 rows are 32-bit where loads go to LDS directly.
-int load_mode(const void* p, const int64_t* strides, int64_t d, int64_t ce) {
-  if (!vec_ok(p, strides, d, ce)) return kElements;
-  return strides[2] >= 0 && strides[2] < ((int64_t)1 << 22) ? kAsync : kVector;
+// How a streamed tensor is read (LoadMode): by the alignment of every row's start and end, for row
+// strides that keep a tile of at most 128 rows within 2^31 bytes.
+int load_mode(const void* p, const int64_t* strides, int64_t d, int64_t size, bool keyMask) {
+  auto all = [&](int64_t bytes) {
+    return (int64_t)((uintptr_t)p % bytes) == 0 && d * size % bytes == 0 && strides[0] * size % bytes == 0 &&
+           strides[1] * size % bytes == 0 && strides[2] * size % bytes == 0;
+  };
+  if (strides[2] < 0 || strides[2] >= ((int64_t)1 << 22)) return kPlain;
+  return all(16) ? kAsync : all(4) && !keyMask ? kAsync4 : kPlain;
 }
 
 // Sizes, types and what else needs no tensor pointer. *empty: there is no head.
@@ -61,8 +62,6 @@ AttnArgs make_args(const lfamd_attention* d) {
   return a;
 }
 
-int64_t chunk_elems(int dtype) { return dtype == LFAMD_F32 ? 4 : 8; }
-
 }  // namespace
 
 }  // namespace lfamd
@@ -74,7 +73,7 @@ extern "C" {
 size_t lfamd_softmax_attention_workspace_size(int dtype, const lfamd_attention* desc) {
   bool empty = false;
   if (check_desc("softmax_attention", dtype, desc, &empty) || empty || desc->q_len == 0) return 0;
-  return attn_fwd_workspace(make_args(desc));
+  return attn_fwd_workspace(dtype, make_args(desc));
 }
 
 int lfamd_softmax_attention(int dtype, const lfamd_attention* desc, const void* q, const void* k, const void* v, void* out,
@@ -86,13 +85,12 @@ int lfamd_softmax_attention(int dtype, const lfamd_attention* desc, const void* 
   if (!q || !out || (desc->k_len && (!k || !v)) || (desc->mask_kind && desc->k_len && !desc->mask))
     return fail(LFAMD_ERR_ARG, "%s: null pointer", who);
   AttnArgs a = make_args(desc);
-  const size_t need = attn_fwd_workspace(a);
+  const size_t need = attn_fwd_workspace(dtype, a);
   if (need && (!workspace || workspace_bytes < need)) return fail(LFAMD_ERR_ARG, "%s: workspace too small", who);
   if (need && ((uintptr_t)workspace & 15)) return fail(LFAMD_ERR_ARG, "%s: workspace must be 16-byte aligned", who);
-  const int64_t ce = chunk_elems(dtype);
+  const int64_t size = (int64_t)dtype_size(dtype);
   a.q = q, a.k = k, a.v = v, a.out = out, a.stat = stats, a.part = (float*)workspace;
-  a.modeQ = load_mode(q, a.qs, a.D, ce), a.modeK = load_mode(k, a.ks, a.D, ce), a.modeV = load_mode(v, a.vs, a.D, ce);
-  a.vecO = vec_ok(out, a.os, a.D, ce);
+  a.modeK = load_mode(k, a.ks, a.D, size, a.keyMask), a.modeV = load_mode(v, a.vs, a.D, size, a.keyMask);
   return attn_fwd(dtype, a, (hipStream_t)stream);
 }
 
@@ -124,12 +122,11 @@ int lfamd_softmax_attention_backward(int dtype, const lfamd_attention* desc, con
     a.gs[i] = grads->grad_out_strides[i], a.dqs[i] = grads->grad_q_strides[i];
     a.dks[i] = grads->grad_k_strides[i], a.dvs[i] = grads->grad_v_strides[i];
   }
-  const int64_t ce = chunk_elems(dtype);
+  const int64_t size = (int64_t)dtype_size(dtype);
   a.q = q, a.k = k, a.v = v, a.o = out, a.g = grads->grad_out, a.stat = (float*)stats;
   a.dq = a.N ? grads->grad_q : nullptr, a.dk = a.M ? grads->grad_k : nullptr, a.dv = a.M ? grads->grad_v : nullptr;
-  a.modeQ = load_mode(q, a.qs, a.D, ce), a.modeK = load_mode(k, a.ks, a.D, ce), a.modeV = load_mode(v, a.vs, a.D, ce);
-  a.vecO = vec_ok(out, a.os, a.D, ce), a.modeG = load_mode(a.g, a.gs, a.D, ce), a.vecDq = vec_ok(a.dq, a.dqs, a.D, ce);
-  a.vecDk = vec_ok(a.dk, a.dks, a.D, ce), a.vecDv = vec_ok(a.dv, a.dvs, a.D, ce);
+  a.modeQ = load_mode(q, a.qs, a.D, size, false), a.modeG = load_mode(a.g, a.gs, a.D, size, false);
+  a.modeK = load_mode(k, a.ks, a.D, size, a.keyMask), a.modeV = load_mode(v, a.vs, a.D, size, a.keyMask);
   return attn_bwd(dtype, a, workspace, (hipStream_t)stream);
 }
 

@@ -93,7 +93,7 @@ int mix_rows_trio(int dtype, const void* const* A, const float* const* B, void* 
 // softmax_attention on a filled-in call (attn_fwd.hip, attn_bwd.hip; the C entries
 // that check and fill it in are in attn_host.hip).
 struct AttnArgs;
-size_t attn_fwd_workspace(const AttnArgs& a);
+size_t attn_fwd_workspace(int dtype, const AttnArgs& a);
 int attn_fwd(int dtype, AttnArgs a, hipStream_t st);
 size_t attn_bwd_workspace(int dtype, const AttnArgs& a);
 int attn_bwd(int dtype, AttnArgs a, void* workspace, hipStream_t st);

@@ -3,8 +3,8 @@
 //
 // Memory-bound: every element is read and written once. A row stays in the registers
 // of the threads that own it (one wave, or a workgroup of 256 or 1024 threads, chosen
-// by the width so that a thread holds at most 4 vectors of 16 bytes or 16 single
-// elements) between the sum of squares and the scaling. The forward normalises the
+// by the width so that a thread holds at most 16 elements) between the sum of squares
+// and the scaling. Rows may begin and end anywhere: the 16-byte accesses need no alignment. The forward normalises the
 // fp32 sum, not its stored rounding. The backward's workgroups walk the rows with a
 // fixed stride, keep their share of dw in registers, and write one fp32 partial row
 // each; a second kernel adds those in their order, so the same call gives the same bits.
@@ -29,27 +29,48 @@ struct NormArgs {
   float eps;
 };
 
-// V consecutive elements of a row: one 16-byte access, or a single element.
-template <typename T, int V> struct Pack {
+// A thread's V = 16 / sizeof(T) adjacent elements from column c on: one 16-byte access at any
+// alignment, single elements at the row's end (zeros behind it).
+template <typename T> struct Pack {
+  static constexpr int V = 16 / (int)sizeof(T);
   T e[V];
-  __device__ __forceinline__ static Pack load(const T* p) {
-    Pack r;
-    if constexpr (V == 1) r.e[0] = *p;
-    else *(u32x4*)r.e = *(const u32x4*)p;
-    return r;
+  __device__ __forceinline__ static Pack load(const T* row, int c, int width) {
+    u32x4 v = {0, 0, 0, 0};  // one register block on both paths, so that the load stays whole
+    if (c + V <= width) {
+      __builtin_memcpy(&v, row + c, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V - 1; ++j)
+        if (c + j < width) {
+          if constexpr (V == 8) v[j >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, row[c + j]) << (16 * (j & 1));
+          else v[j] = __builtin_bit_cast(uint32_t, row[c + j]);
+        }
+    }
+    return __builtin_bit_cast(Pack, v);
   }
-  __device__ __forceinline__ void store(T* p) const {
-    if constexpr (V == 1) *p = e[0];
-    else *(u32x4*)p = *(const u32x4*)e;
+  __device__ __forceinline__ void store(T* row, int c, int width) const {
+    const u32x4 v = __builtin_bit_cast(u32x4, *this);
+    if (c + V <= width) {
+      __builtin_memcpy(row + c, &v, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V - 1; ++j)
+        if (c + j < width) row[c + j] = e[j];
+    }
   }
 };
 
-template <typename T, int V> __device__ __forceinline__ void load_weight(const NormArgs& a, int c, float* w) {
+template <typename T> __device__ __forceinline__ void load_weight(const NormArgs& a, int c, float* w) {
+  constexpr int V = Pack<T>::V;
   if (a.wf32) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) w[j] = ((const float*)a.w)[c + j];
+    for (int j = 0; j < V; j += 4) {
+      const Pack<float> p = Pack<float>::load((const float*)a.w, c + j, a.width);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[j + i] = p.e[i];
+    }
   } else {
-    const Pack<T, V> p = Pack<T, V>::load((const T*)a.w + c);
+    const Pack<T> p = Pack<T>::load((const T*)a.w, c, a.width);
 #pragma unroll
     for (int j = 0; j < V; ++j) w[j] = to_acc(p.e[j]);
   }
@@ -70,9 +91,9 @@ template <int TPR, bool MAX> __device__ __forceinline__ float row_reduce(float v
   return v;
 }
 
-template <typename T, int V, int TPR, int NV, bool F8>
+template <typename T, int TPR, int NV, bool F8>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(const NormArgs a) {
-  constexpr int THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR;
+  constexpr int THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR, V = Pack<T>::V;
   __shared__ float lds[16];
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
@@ -82,16 +103,16 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(con
   for (int i = 0; i < NV; ++i) {
     const int c = (t + i * TPR) * V;
     if (c < a.width) {
-      const Pack<T, V> px = Pack<T, V>::load((const T*)a.x + row * a.xs + c);
+      const Pack<T> px = Pack<T>::load((const T*)a.x + row * a.xs, c, a.width);
       if (a.res) {
-        const Pack<T, V> pr = Pack<T, V>::load((const T*)a.res + row * a.rs + c);
-        Pack<T, V> ps;
+        const Pack<T> pr = Pack<T>::load((const T*)a.res + row * a.rs, c, a.width);
+        Pack<T> ps;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           s[i][j] = to_acc(px.e[j]) + to_acc(pr.e[j]);
           ps.e[j] = from_acc<T>(s[i][j]);
         }
-        ps.store((T*)a.sum + row * a.width + c);
+        ps.store((T*)a.sum + row * a.width, c, a.width);
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) s[i][j] = to_acc(px.e[j]);
@@ -109,18 +130,15 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(con
     const int c = (t + i * TPR) * V;
     if (c < a.width) {
       float w[V];
-      load_weight<T, V>(a, c, w);
+      load_weight<T>(a, c, w);
+      Pack<T> py;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         s[i][j] = s[i][j] * r * w[j];
-        if (F8) top = fmaxf(top, fabsf(s[i][j]));
+        if constexpr (F8) top = fmaxf(top, fabsf(s[i][j]));
+        else py.e[j] = from_acc<T>(s[i][j]);
       }
-      if constexpr (!F8) {
-        Pack<T, V> py;
-#pragma unroll
-        for (int j = 0; j < V; ++j) py.e[j] = from_acc<T>(s[i][j]);
-        py.store((T*)a.y + row * a.width + c);
-      }
+      if constexpr (!F8) py.store((T*)a.y + row * a.width, c, a.width);
     }
   }
   if constexpr (F8) {
@@ -134,20 +152,24 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(con
       const int c = (t + i * TPR) * V;
       if (c < a.width) {
         // |y / scale| <= 448 (1 + 2^-23), which rounds to at most 448: nothing saturates.
-        float z[V];
+        uint32_t o[V / 4];
 #pragma unroll
-        for (int j = 0; j < V; ++j) z[j] = s[i][j] / scale;
-        if constexpr (V == 1) {
-          y[c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[0], 0, false);
-        } else {
-          uint32_t o[V / 4];
-#pragma unroll
-          for (int j = 0; j < V / 4; ++j) {
-            int p = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * j], z[4 * j + 1], 0, false);
-            o[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[4 * j + 2], z[4 * j + 3], p, true);
+        for (int j = 0; j < V / 4; ++j) {
+          const float* z = &s[i][4 * j];
+          const int p = __builtin_amdgcn_cvt_pk_fp8_f32(z[0] / scale, z[1] / scale, 0, false);
+          o[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2] / scale, z[3] / scale, p, true);
+        }
+        if (c + V <= a.width) {
+          if constexpr (V == 8) {
+            const uint64_t both = (uint64_t)o[1] << 32 | o[0];
+            __builtin_memcpy(y + c, &both, 8);
+          } else {
+            __builtin_memcpy(y + c, o, 4);
           }
-          if constexpr (V == 8) *(uint64_t*)(y + c) = (uint64_t)o[1] << 32 | o[0];
-          else *(uint32_t*)(y + c) = o[0];
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (c + j < a.width) y[c + j] = (uint8_t)(o[j >> 2] >> (8 * (j & 3)));
         }
       }
     }
@@ -155,9 +177,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(con
 }
 
 // a.sum: the stored sum (x itself without a residual). part: [gridDim.x][width].
-template <typename T, int V, int TPR, int NV>
+template <typename T, int TPR, int NV>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_bwd_kernel(const NormArgs a) {
-  constexpr int THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR;
+  constexpr int THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR, V = Pack<T>::V;
   __shared__ float lds[16];
   const int t = threadIdx.x % TPR;
   float w[NV][V], dw[NV][V];
@@ -166,49 +188,51 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_bwd_kernel
     const int c = (t + i * TPR) * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) w[i][j] = dw[i][j] = 0.0f;
-    if (c < a.width) load_weight<T, V>(a, c, w[i]);
+    if (c < a.width) load_weight<T>(a, c, w[i]);
   }
   // Without barriers in the loop (RPB > 1) the waves of a workgroup walk their rows alone.
   for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < a.rows; row += (int64_t)gridDim.x * RPB) {
-    const float r = a.rstd[row];
-    float n[NV][V], g[NV][V], dot = 0.0f;
+    Pack<T> ps[NV], py[NV], pg[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (t + i * TPR) * V;
       if (c < a.width) {
-        const Pack<T, V> ps = Pack<T, V>::load((const T*)a.sum + row * a.xs + c);
-        const Pack<T, V> pg = Pack<T, V>::load((const T*)a.gy + row * a.gys + c);
+        ps[i] = Pack<T>::load((const T*)a.sum + row * a.xs, c, a.width);
+        py[i] = Pack<T>::load((const T*)a.gy + row * a.gys, c, a.width);
+        if (a.gs) pg[i] = Pack<T>::load((const T*)a.gs + row * a.gss, c, a.width);
+      }
+    }
+    const float r = a.rstd[row];
+    float n[NV][V], g[NV][V], dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((t + i * TPR) * V < a.width)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          n[i][j] = to_acc(ps.e[j]) * r;
-          const float gy = to_acc(pg.e[j]);
+          n[i][j] = to_acc(ps[i].e[j]) * r;
+          const float gy = to_acc(py[i].e[j]);
           dw[i][j] = fmaf(gy, n[i][j], dw[i][j]);
           g[i][j] = gy * w[i][j];
           dot = fmaf(g[i][j], n[i][j], dot);
         }
-      }
-    }
     dot = row_reduce<TPR, false>(dot, lds) / (float)a.width;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (t + i * TPR) * V;
       if (c < a.width) {
-        Pack<T, V> pd;
-        float d[V];
+        Pack<T> pd;
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] = r * fmaf(-n[i][j], dot, g[i][j]);
-        if (a.gs) {
-          const Pack<T, V> pg = Pack<T, V>::load((const T*)a.gs + row * a.gss + c);
-#pragma unroll
-          for (int j = 0; j < V; ++j) d[j] += to_acc(pg.e[j]);
+        for (int j = 0; j < V; ++j) {
+          float d = r * fmaf(-n[i][j], dot, g[i][j]);
+          if (a.gs) d += to_acc(pg[i].e[j]);
+          pd.e[j] = from_acc<T>(d);
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j) pd.e[j] = from_acc<T>(d[j]);
-        pd.store((T*)a.dx + row * a.width + c);
+        pd.store((T*)a.dx + row * a.width, c, a.width);
       }
     }
   }
   if (!a.part) return;
+  float* part = a.part + (int64_t)blockIdx.x * a.width;
   if constexpr (RPB > 1) {
     // The four waves' shares, added in their order.
     extern __shared__ float share[];  // [width]
@@ -217,40 +241,45 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_bwd_kernel
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int c = (t + i * TPR) * V;
-          if (c < a.width)
 #pragma unroll
-            for (int j = 0; j < V; ++j) share[c + j] = k ? share[c + j] + dw[i][j] : dw[i][j];
+          for (int j = 0; j < V; ++j)
+            if (c + j < a.width) share[c + j] = k ? share[c + j] + dw[i][j] : dw[i][j];
         }
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < a.width; c += THREADS) a.part[(int64_t)blockIdx.x * a.width + c] = share[c];
+    for (int c = threadIdx.x; c < a.width; c += THREADS) part[c] = share[c];
   } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * TPR) * V;
-      if (c < a.width)
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) a.part[(int64_t)blockIdx.x * a.width + c + j] = dw[i][j];
-    }
+      for (int j = 0; j < V; j += 4) {
+        Pack<float> p;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p.e[k] = dw[i][j + k];
+        const int c = (t + i * TPR) * V + j;
+        if (c < a.width) p.store(part, c, a.width);
+      }
   }
 }
 
-// dw[c] = sum over the partial rows: 32 columns x 32 row groups per workgroup, then the
+// dw[c] = sum over the partial rows: 16 columns x 64 row groups per workgroup, then the
 // groups' sums in their order.
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_dw_kernel(const float* part, int n, int width, T* dw, int f32) {
-  __shared__ float s[32][33];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+  __shared__ float s[64][17];
+  const int c = blockIdx.x * 16 + (threadIdx.x & 15), k = threadIdx.x >> 4;
   float x = 0.0f;
-  if (c < width)
-    for (int i = k; i < n; i += 32) x += part[(int64_t)i * width + c];
-  s[k][threadIdx.x & 31] = x;
+  if (c < width) {
+#pragma unroll 8
+    for (int i = k; i < n; i += 64) x += part[(int64_t)i * width + c];
+  }
+  s[k][threadIdx.x & 15] = x;
   __syncthreads();
   if (k == 0 && c < width) {
     x = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) x += s[i][threadIdx.x];
+    for (int i = 0; i < 64; ++i) x += s[i][threadIdx.x];
     if (f32) ((float*)dw)[c] = x;
     else dw[c] = from_acc<T>(x);
   }
@@ -259,43 +288,41 @@ __global__ void __launch_bounds__(1024) norm_dw_kernel(const float* part, int n,
 constexpr int kNormMaxWidth = 16384;
 
 struct NormPlan {
-  bool vec;
   int tpr, nv;
 };
 
-// Threads per row and vectors per thread. One wave per row while a lane's share is at
-// most four vectors (16 single elements), as a wave reduces without barriers; then the
-// smallest workgroup that does.
-NormPlan norm_plan(int width, int V) {
-  NormPlan p{V > 1, 64, 1};
-  const int units = width / V, most = V > 1 ? 4 : 16;
-  for (int tpr : {64, 256, 1024}) {
-    p.tpr = tpr;
-    if (units <= tpr * most) break;
-  }
+// Threads per row and 16-byte vectors per thread, for at most 16 elements each (the backward
+// holds four values per element). One wave per row while that holds the row, as a wave
+// reduces without barriers; then the smallest workgroup that does.
+NormPlan norm_plan(int dtype, int width) {
+  const int V = dtype == LFAMD_F32 ? 4 : 8, most = 16 / V, units = (width + V - 1) / V;
+  NormPlan p{1024, 1};
+  for (int tpr : {64, 256, 1024})
+    if (units <= tpr * most) {
+      p.tpr = tpr;
+      break;
+    }
   const int need = (units + p.tpr - 1) / p.tpr;
-  p.nv = V > 1 ? (need <= 1 ? 1 : need <= 2 ? 2 : 4) : (need <= 4 ? 4 : 16);
+  p.nv = need <= 1 ? 1 : need <= 2 ? 2 : 4;
   return p;
 }
 
-// Calls f.template go<V, TPR, NV>() for a plan.
-template <int V, int TPR, typename F> int with_nv(const NormPlan& p, F&& f) {
-  if constexpr (V > 1) return p.nv == 1 ? f.template go<V, TPR, 1>() : p.nv == 2 ? f.template go<V, TPR, 2>() : f.template go<V, TPR, 4>();
-  else return p.nv == 4 ? f.template go<V, TPR, 4>() : f.template go<V, TPR, 16>();
-}
-template <int V, typename F> int with_tpr(const NormPlan& p, F&& f) {
-  return p.tpr == 64 ? with_nv<V, 64>(p, f) : p.tpr == 256 ? with_nv<V, 256>(p, f) : with_nv<V, 1024>(p, f);
+// Calls f.template go<TPR, NV>() for a plan. (fp32: wider workgroups begin at two vectors.)
+template <typename T, int TPR, typename F> int with_nv(const NormPlan& p, F&& f) {
+  if constexpr (sizeof(T) == 2) return p.nv == 1 ? f.template go<TPR, 1>() : f.template go<TPR, 2>();
+  else if constexpr (TPR == 64) return p.nv == 1 ? f.template go<TPR, 1>() : p.nv == 2 ? f.template go<TPR, 2>() : f.template go<TPR, 4>();
+  else return p.nv == 2 ? f.template go<TPR, 2>() : f.template go<TPR, 4>();
 }
 template <typename T, typename F> int with_plan(const NormPlan& p, F&& f) {
-  return p.vec ? with_tpr<16 / (int)sizeof(T)>(p, f) : with_tpr<1>(p, f);
+  return p.tpr == 64 ? with_nv<T, 64>(p, f) : p.tpr == 256 ? with_nv<T, 256>(p, f) : with_nv<T, 1024>(p, f);
 }
 
 template <typename T, bool F8> struct NormFwd {
   NormArgs a;
   hipStream_t st;
-  template <int V, int TPR, int NV> int go() {
+  template <int TPR, int NV> int go() {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
-    add_rms_norm_kernel<T, V, TPR, NV, F8>
+    add_rms_norm_kernel<T, TPR, NV, F8>
         <<<dim3((unsigned)((a.rows + RPB - 1) / RPB)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(a);
     return check_launch("add_rms_norm");
   }
@@ -303,7 +330,7 @@ template <typename T, bool F8> struct NormFwd {
 
 int bwd_grid(const NormPlan& p, int64_t rows) {
   const int rpb = p.tpr < 256 ? 256 / p.tpr : 1;
-  // Eight resident workgroups of 256 threads per CU, two of 1024.
+  // Four workgroups of 256 threads per CU, two of 1024.
   const int64_t most = (int64_t)num_cus() * (p.tpr > 256 ? 2 : 4);
   return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rpb - 1) / rpb, most));
 }
@@ -312,14 +339,12 @@ template <typename T> struct NormBwd {
   NormArgs a;
   hipStream_t st;
   int grid;
-  template <int V, int TPR, int NV> int go() {
+  template <int TPR, int NV> int go() {
     const size_t lds = TPR < 256 && a.part ? (size_t)a.width * sizeof(float) : 0;
-    add_rms_norm_bwd_kernel<T, V, TPR, NV><<<dim3(grid), dim3(TPR < 256 ? 256 : TPR), lds, st>>>(a);
+    add_rms_norm_bwd_kernel<T, TPR, NV><<<dim3(grid), dim3(TPR < 256 ? 256 : TPR), lds, st>>>(a);
     return check_launch("add_rms_norm backward");
   }
 };
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int check_sizes(const char* who, int dtype, int w_dtype, int64_t rows, int64_t width) {
   if (dtype != LFAMD_F32 && dtype != LFAMD_F16 && dtype != LFAMD_BF16)
@@ -334,10 +359,7 @@ int check_sizes(const char* who, int dtype, int w_dtype, int64_t rows, int64_t w
 }
 
 template <bool F8> int norm_forward(int dtype, const NormArgs& a, hipStream_t st) {
-  const int V = dtype == LFAMD_F32 ? 4 : 8;
-  const bool vec = a.width % V == 0 && a.xs % V == 0 && (!a.res || a.rs % V == 0) && aligned16(a.x) && aligned16(a.res) &&
-                   aligned16(a.y) && aligned16(a.sum) && aligned16(a.w);
-  const NormPlan p = norm_plan(a.width, vec ? V : 1);
+  const NormPlan p = norm_plan(dtype, a.width);
   switch (dtype) {
     case LFAMD_F32: return with_plan<float>(p, NormFwd<float, F8>{a, st});
     case LFAMD_F16: return with_plan<f16s>(p, NormFwd<f16s, F8>{a, st});
@@ -379,10 +401,7 @@ int lfamd_add_rms_norm_fp8(int dtype, const void* x, int64_t x_stride, const voi
 
 size_t lfamd_add_rms_norm_backward_workspace_size(int dtype, int64_t rows, int64_t width) {
   if (rows <= 0 || width < 1 || width > kNormMaxWidth || rows > INT32_MAX) return 0;
-  // Whichever of the two layouts the tensors' alignment selects.
-  const int V = dtype == LFAMD_F32 ? 4 : 8;
-  int grid = bwd_grid(norm_plan((int)width, 1), rows);
-  if (width % V == 0) grid = std::max(grid, bwd_grid(norm_plan((int)width, V), rows));
+  const int grid = bwd_grid(norm_plan(dtype, (int)width), rows);
   return (size_t)grid * width * sizeof(float);
 }
 
@@ -401,11 +420,7 @@ int lfamd_add_rms_norm_backward(int dtype, const void* grad_y, int64_t grad_y_st
   a.wf32 = w_dtype == LFAMD_F32;
   int grid = 0;
   if (rows > 0) {
-    const int V = dtype == LFAMD_F32 ? 4 : 8;
-    const bool vec = width % V == 0 && sum_stride % V == 0 && grad_y_stride % V == 0 &&
-                     (!grad_sum || grad_sum_stride % V == 0) && aligned16(sum) && aligned16(grad_y) && aligned16(grad_sum) &&
-                     aligned16(grad_x) && aligned16(weight);
-    const NormPlan p = norm_plan((int)width, vec ? V : 1);
+    const NormPlan p = norm_plan(dtype, (int)width);
     grid = bwd_grid(p, rows);
     if (grad_weight) {
       if (!workspace || workspace_bytes < lfamd_add_rms_norm_backward_workspace_size(dtype, rows, width))
@@ -422,7 +437,7 @@ int lfamd_add_rms_norm_backward(int dtype, const void* grad_y, int64_t grad_y_st
     if (e) return e;
   }
   if (grad_weight) {
-    const dim3 g((unsigned)((width + 31) / 32)), b(1024);
+    const dim3 g((unsigned)((width + 15) / 16)), b(1024);
     switch (w_dtype) {
       case LFAMD_F32: norm_dw_kernel<float><<<g, b, 0, st>>>(a.part, grid, (int)width, (float*)grad_weight, 1); break;
       case LFAMD_F16: norm_dw_kernel<f16s><<<g, b, 0, st>>>(a.part, grid, (int)width, (f16s*)grad_weight, 0); break;
