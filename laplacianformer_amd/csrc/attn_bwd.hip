@@ -34,9 +34,12 @@ template <typename T, int DC> constexpr int key_tile() { return sizeof(T) == 2 |
 // registers at two waves per SIMD (128 + 64 + 64 with the scores): V is read from LDS then.
 template <int DC> constexpr bool v_in_lds() { return DC >= 128; }
 
-template <typename T, int DC> constexpr size_t dkdv_lds() {
+// Bytes of a streamed query's statistics: lse, delta, 1 / sum and last key, or its bits of the 128 keys.
+template <int FORM> constexpr int row_stats() { return FORM == kBits ? 24 : 16; }
+
+template <typename T, int DC, int FORM> constexpr size_t dkdv_lds() {
   constexpr int DP = row_pitch(DC);
-  return (size_t)2 * query_tile<T, DC>() * (2 * DP * sizeof(T) + 16) + (v_in_lds<DC>() ? 128 * DP * sizeof(T) : 0);
+  return (size_t)2 * query_tile<T, DC>() * (2 * DP * sizeof(T) + row_stats<FORM>()) + (v_in_lds<DC>() ? 128 * DP * sizeof(T) : 0);
 }
 template <typename T, int DC> constexpr size_t dq_lds() { return (size_t)2 * key_tile<T, DC>() * 2 * row_pitch(DC) * sizeof(T); }
 
@@ -145,21 +148,22 @@ template <bool MASK> __device__ __forceinline__ float prob(float s, float c, flo
 }
 
 // Whether key j of sequence b takes part at all.
-template <bool MASK> __device__ __forceinline__ bool key_live(const AttnArgs& a, int b, int j, int klen) {
+template <int FORM> __device__ __forceinline__ bool key_live(const AttnArgs& a, int b, int j, int klen) {
   if (j >= klen) return false;
-  if (!MASK || !a.keyMask) return true;
+  if (FORM == kNoMask || !a.keyMask) return true;
   const int64_t off = (int64_t)b * a.ms[0] + (int64_t)j * a.ms[3];
   return mask_bias(a, off) != kNegInf;
 }
 
 // dk and dv of 128 keys, 32 per wave; queries stream through LDS in tiles of QT.
-template <typename T, int DC, bool MASK>
+template <typename T, int DC, int FORM>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
     __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DC >= 64 ? 1 : 2, 2))) attn_dkdv_kernel(const AttnArgs a) {
+  constexpr bool MASK = FORM == kAdd;
   constexpr int DP = row_pitch(DC), QT = query_tile<T, DC>(), NT = DC / 16, ND = DC / 32;
   constexpr bool F16 = std::is_same<T, f16s>::value;
   using L = Tile<T, DP>;
-  constexpr int TB = QT * L::ROW, SB = QT * 16;  // bytes of a tile, and of its rows' statistics
+  constexpr int TB = QT * L::ROW, SB = QT * row_stats<FORM>();  // bytes of a tile, and of its rows' statistics
   constexpr bool VL = v_in_lds<DC>();
   extern __shared__ __align__(16) char smem[];   // [2][q tile, g tile], [2][lse, delta, 1 / sum, last key], [v tile]
 
@@ -177,7 +181,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
   const int share = (total + a.nsplit - 1) / a.nsplit;
   const int beg = min(split * share, total), end = min(beg + share, total);
 
-  const bool live = key_live<MASK>(a, b, mykey, klen);
+  const bool live = key_live<FORM>(a, b, mykey, klen);
   Frag<T> kf[NT], vf[VL ? 1 : NT];
   const char* tv = smem + 4 * TB + 2 * SB + wave * 32 * L::ROW;
   {
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
     }
     if constexpr (VL) {
       using LV = Loader<T, DP, DC, 128>;
-      const uint32_t bits = MASK && a.keyMask && klen > 0 ? live_keys<LV>(a, b, key0) : ~0u;
+      const uint32_t bits = FORM != kNoMask && a.keyMask && klen > 0 ? live_keys<LV>(a, b, key0) : ~0u;
       LV::fill(smem + 4 * TB + 2 * SB, (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1], a.vs[2], key0, klen, a.D,
                a.modeV, bits);
     }
@@ -208,6 +212,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
   using LD = Loader<T, DP, DC, QT>;
   float st0 = 0.0f, st1 = 0.0f, st2 = 0.0f;
   int st3 = 0;
+  u32x4 st4 = {0, 0, 0, 0};
   auto fill = [&](int buf, int step) {
     const int g = step / perHead, row0 = (tb + step % perHead) * QT, hq = hk * a.G + g;
     LD::fill(smem + buf * 2 * TB, (const T*)a.q + (int64_t)b * a.qs[0] + (int64_t)hq * a.qs[1], a.qs[2], row0, qlen, a.D,
@@ -222,6 +227,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
       st1 = in ? a.delta[so] * fd : 0.0f;
       st2 = MASK && in ? a.stat[(int64_t)a.B * a.H * a.N + so] : 0.0f;
       st3 = !in ? 0 : a.causal ? min(klen, qstart + n + 1) : klen;
+      if constexpr (FORM == kBits) {
+        st4 = u32x4{0, 0, 0, 0};
+        if (in)
+          st4 = *(const u32x4*)(a.bits + (int64_t)b * a.bs[0] + (int64_t)hq * a.bs[1] + (int64_t)n * a.bs[2] + key0 / 32);
+      }
       if (F16) {
         if (MASK) st2 *= exp2f(kPShift);
         else st0 -= kPShift;
@@ -233,8 +243,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
       float* s = (float*)(smem + 4 * TB + buf * SB);
       s[threadIdx.x] = st0;
       s[QT + threadIdx.x] = st1;
-      s[2 * QT + threadIdx.x] = st2;
-      ((int*)s)[3 * QT + threadIdx.x] = st3;
+      if constexpr (FORM == kBits) {  // by 32 keys, one wave's: what the mask and the row's last key leave
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          ((uint32_t*)s)[(2 + w) * QT + threadIdx.x] = st4[w] & bits_below(st3, key0 + 32 * w);
+      } else {
+        s[2 * QT + threadIdx.x] = st2;
+        ((int*)s)[3 * QT + threadIdx.x] = st3;
+      }
     }
   };
 
@@ -276,18 +292,23 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
       }
       // Every row sees every key of the wave: nothing to leave out.
       const int wlast = key0 + wave * 32 + 31;
-      const bool check = MASK || wlast >= klen || row0 + qb + 32 > qlen || (a.causal && wlast > qstart + row0 + qb);
+      const bool check = FORM != kNoMask || wlast >= klen || row0 + qb + 32 > qlen || (a.causal && wlast > qstart + row0 + qb);
       // Pairs that are left out: score -inf, so that p = 0, and g.v = 0, so that dz = 0 (delta - 0).
       if (check) {
 #pragma unroll
-        for (int rq = 0; rq < 4; ++rq)
+        for (int rq = 0; rq < 4; ++rq) {
+          u32x4 w;
+          if constexpr (FORM == kBits) w = *(const u32x4*)(stats + (2 + wave) * QT + qb + 8 * rq + 4 * h);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = 4 * rq + i;
-            const bool in = mykey < ((const int*)stats)[3 * QT + qb + 8 * rq + 4 * h + i];
+            bool in;
+            if constexpr (FORM == kBits) in = (int)(w[i] << (31 - (lane & 31))) < 0;
+            else in = mykey < ((const int*)stats)[3 * QT + qb + 8 * rq + 4 * h + i];
             s[r] = !in ? kNegInf : MASK ? masked_score(a, s[r], bias[r]) : s[r];
             dp[r] = s[r] == kNegInf ? 0.0f : dp[r];
           }
+        }
       }
       // The first columns of g and q are read while the exponentials run.
       auto cread = [&](auto n) {
@@ -348,8 +369,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
 }
 
 // dq of 128 queries of one head, 32 per wave; keys stream through LDS in tiles of KT.
-template <typename T, int DC, bool MASK>
+template <typename T, int DC, int FORM>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_dq_kernel(const AttnArgs a) {
+  constexpr bool MASK = FORM == kAdd;
   constexpr int DP = row_pitch(DC), KT = key_tile<T, DC>(), NT = DC / 16, ND = DC / 32;
   constexpr bool F16 = std::is_same<T, f16s>::value;
   using L = Tile<T, DP>;
@@ -395,11 +417,21 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
   const T* kbase = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1];
   const T* vbase = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1];
   using LD = Loader<T, DP, DC, KT>;
-  const bool byKey = MASK && a.keyMask;
+  const bool byKey = FORM != kNoMask && a.keyMask;
   auto fill = [&](int buf, int k0, uint32_t live) {
     LD::fill(smem + buf * 2 * TB, kbase, a.ks[2], k0, kend, a.D, a.modeK, live);
     LD::fill(smem + buf * 2 * TB + TB, vbase, a.vs[2], k0, kend, a.D, a.modeV, live);
   };
+  // The row's bits of a tile's keys.
+  const int64_t boff = (int64_t)b * a.bs[0] + (int64_t)hq * a.bs[1] + (int64_t)nr * a.bs[2];
+  auto load_bits = [&](int k0) {
+    const uint32_t* p = a.bits + boff + k0 / 32;
+    if constexpr (KT == 32) return (uint64_t)*p;
+    else return *(const uint64_t*)p;
+  };
+  uint64_t bits = 0;
+  if constexpr (FORM == kBits)
+    if (kbeg < kend) bits = load_bits(kbeg);
   uint32_t live = ~0u;  // of the next tile to fill
   if (kbeg < kend) {
     if (byKey) live = live_keys<LD>(a, b, kbeg);
@@ -414,6 +446,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
     const bool more = key0 + KT < kend;
     if (more) fill(buf ^ 1, key0 + KT, live);
     if (byKey) live = live_keys<LD>(a, b, key0 + 2 * KT);
+    const uint64_t now = bits;
+    if constexpr (FORM == kBits)
+      if (more) bits = load_bits(key0 + KT);
     const char* tk = smem + buf * 2 * TB;
     const char* tv = tk + TB;
 #pragma unroll 1
@@ -431,12 +466,17 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
           else dp = mma<T>(x, gf[n - NT], dp);
         });
       }
-      const bool check = MASK || key0 + kb + 32 > full;
+      const bool check = FORM != kNoMask || key0 + kb + 32 > full;
       if (check) {
+        const uint32_t w = FORM == kBits ? ((uint32_t)(now >> kb) & bits_below(lim, key0 + kb)) >> (4 * h) : 0;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int j = key0 + kb + 8 * (r >> 2) + 4 * h + (r & 3);
-          s[r] = j >= lim ? kNegInf : MASK ? masked_score(a, s[r], bias[r]) : s[r];
+          if constexpr (FORM == kBits) {
+            s[r] = w & (1u << (8 * (r >> 2) + (r & 3))) ? s[r] : kNegInf;
+          } else {
+            const int j = key0 + kb + 8 * (r >> 2) + 4 * h + (r & 3);
+            s[r] = j >= lim ? kNegInf : MASK ? masked_score(a, s[r], bias[r]) : s[r];
+          }
           dp[r] = s[r] == kNegInf ? 0.0f : dp[r];
         }
       }
@@ -516,10 +556,10 @@ BwdPlan bwd_plan(int dtype, const AttnArgs& a, int cus) {
   const int64_t ksteps = (int64_t)a.G * ((a.N + qt - 1) / qt), qsteps = (a.M + kt - 1) / kt;
   // The other axis is split where a kernel's own blocks leave CUs without work. A tile's time: its four
   // (dq: three) products at the 3 TFLOP/s that a CU reaches (fp32: 0.45), and a microsecond at least.
-  const double rate = dtype == LFAMD_F32 ? 0.45e6 : 3e6, f32 = sizeof(float);
+  const double rate = dtype == LFAMD_F32 ? 0.45e6 : 3e6, f32 = sizeof(float), share = dtype == LFAMD_F32 ? 1.0 : 0.7;
   const double ktile = std::max(1.0, 8.0 * 128 * qt * p.dc / rate), qtile = std::max(0.8, 6.0 * 128 * kt * p.dc / rate);
-  p.ksplit = kw && ksteps ? best_split(kw, ksteps, cus, ktile, 2.0, 2.0 * a.B * a.Hk * a.M * p.dc * f32) : 1;
-  p.qsplit = qw && qsteps ? best_split(qw, qsteps, cus, qtile, 2.0, 1.0 * a.B * a.H * a.N * p.dc * f32) : 1;
+  p.ksplit = kw && ksteps ? best_split(kw, ksteps, cus, ktile, 4.0, share, 2.0 * a.B * a.Hk * a.M * p.dc * f32) : 1;
+  p.qsplit = qw && qsteps ? best_split(qw, qsteps, cus, qtile, 4.0, share, 1.0 * a.B * a.H * a.N * p.dc * f32) : 1;
   p.qchunk = (int)std::max<int64_t>(1, (qsteps + p.qsplit - 1) / p.qsplit);
   p.deltaBytes = up256((size_t)a.B * a.H * a.N * sizeof(float));
   if (dtype == LFAMD_F16)
@@ -546,7 +586,7 @@ template <typename T, int DC> int sum_launch(const SumOf& a, const SumOf& b, int
   return check_launch("softmax_attention backward (sums)");
 }
 
-template <typename T, int DC, bool MASK> int bwd_launch(AttnArgs a, const BwdPlan& p, hipStream_t st) {
+template <typename T, int DC, int FORM> int bwd_launch(AttnArgs a, const BwdPlan& p, hipStream_t st) {
   constexpr bool F16 = std::is_same<T, f16s>::value;
   const int qt = (a.N + 63) / 64, kt = (a.M + 63) / 64;
   int64_t grid = (int64_t)a.B * a.H * qt + (F16 ? (int64_t)a.B * a.Hk * kt : 0);
@@ -555,8 +595,8 @@ template <typename T, int DC, bool MASK> int bwd_launch(AttnArgs a, const BwdPla
   if (a.dk) {
     a.nsplit = p.ksplit;
     a.tiles = p.ktiles;
-    if (int e = launch((const void*)attn_dkdv_kernel<T, DC, MASK>, (int64_t)a.B * a.Hk * p.ktiles * p.ksplit,
-                       dkdv_lds<T, DC>(), a, st))
+    if (int e = launch((const void*)attn_dkdv_kernel<T, DC, FORM>, (int64_t)a.B * a.Hk * p.ktiles * p.ksplit,
+                       dkdv_lds<T, DC, FORM>(), a, st))
       return e;
     if (p.ksplit > 1) {
       const int64_t rows = (int64_t)a.B * a.Hk * a.M;
@@ -569,7 +609,7 @@ template <typename T, int DC, bool MASK> int bwd_launch(AttnArgs a, const BwdPla
     a.nsplit = p.qsplit;
     a.tiles = p.qtiles;
     a.chunk = p.qchunk;
-    if (int e = launch((const void*)attn_dq_kernel<T, DC, MASK>, (int64_t)a.B * a.H * p.qtiles * p.qsplit, dq_lds<T, DC>(), a, st))
+    if (int e = launch((const void*)attn_dq_kernel<T, DC, FORM>, (int64_t)a.B * a.H * p.qtiles * p.qsplit, dq_lds<T, DC>(), a, st))
       return e;
     if (p.qsplit > 1) {
       const int64_t rows = (int64_t)a.B * a.H * a.N;
@@ -581,7 +621,11 @@ template <typename T, int DC, bool MASK> int bwd_launch(AttnArgs a, const BwdPla
 }
 
 template <typename T, int DC> int bwd_mask(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
-  return a.maskKind ? bwd_launch<T, DC, true>(a, p, st) : bwd_launch<T, DC, false>(a, p, st);
+  switch (a.maskKind) {
+    case kMaskNone: return bwd_launch<T, DC, kNoMask>(a, p, st);
+    case kMaskBool: return bwd_launch<T, DC, kBits>(a, p, st);
+    default: return bwd_launch<T, DC, kAdd>(a, p, st);
+  }
 }
 
 template <typename T> int bwd_dim(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
@@ -597,17 +641,19 @@ template <typename T> int bwd_dim(const AttnArgs& a, const BwdPlan& p, hipStream
 
 size_t attn_bwd_workspace(int dtype, const AttnArgs& a) {
   const BwdPlan p = bwd_plan(dtype, a, num_cus());
-  return p.deltaBytes + p.boundBytes + p.partBytes;
+  return attn_bits_bytes(a) + p.deltaBytes + p.boundBytes + p.partBytes;
 }
 
 int attn_bwd(int dtype, AttnArgs a, void* workspace, hipStream_t st) {
   const BwdPlan p = bwd_plan(dtype, a, num_cus());
-  a.delta = (float*)workspace;
-  a.bounds = (float*)((char*)workspace + p.deltaBytes);
-  a.part = (float*)((char*)workspace + p.deltaBytes + p.boundBytes);
+  char* rest = (char*)workspace + attn_bits_bytes(a);
+  a.delta = (float*)rest;
+  a.bounds = (float*)(rest + p.deltaBytes);
+  a.part = (float*)(rest + p.deltaBytes + p.boundBytes);
   const int64_t most = std::max({(int64_t)a.B * a.Hk * p.ktiles * p.ksplit, (int64_t)a.B * a.H * p.qtiles * p.qsplit,
                                  (int64_t)a.B * a.H * ((a.N + 63) / 64) + (int64_t)a.B * a.Hk * ((a.M + 63) / 64)});
   if (most > INT32_MAX) return fail(LFAMD_ERR_UNSUPPORTED, "softmax_attention backward: too many workgroups");
+  if (int e = attn_pack_bits(a, workspace, st)) return e;
   switch (dtype) {
     case LFAMD_F32: return bwd_dim<float>(a, p, st);
     case LFAMD_F16: return bwd_dim<f16s>(a, p, st);

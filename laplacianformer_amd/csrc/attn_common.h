@@ -389,6 +389,8 @@ struct AttnArgs {
   int64_t ms[4];                       // mask strides: batch, head, row, key (0 where broadcast)
   int B, H, Hk, G, N, M, D;
   int maskKind, causal, keyMask;       // keyMask: the mask is the same for every head and row
+  uint32_t* bits;                      // a truth-value mask packed by attn_bits_kernel, strides bs in words
+  int64_t bs[3];
   int modeQ, modeK, modeV, modeG;      // LoadMode where the tensor streams through LDS
   int nsplit, tiles, chunk;            // work split along the other axis; tiles along the own one; steps per split
   float scale, c;                      // c = scale * log2(e)
@@ -407,7 +409,7 @@ __device__ __forceinline__ int query_start(const AttnArgs& a, int b) {
   return a.qstart ? min(max(a.qstart[b], -a.N), a.M) : a.M - a.N;
 }
 
-// An additive mask element in natural units.
+// A mask element as an additive term in natural units.
 __device__ __forceinline__ float mask_bias(const AttnArgs& a, int64_t off) {
   if (a.maskKind == kMaskBool) return ((const uint8_t*)a.mask)[off] ? 0.0f : kNegInf;
   if (a.maskKind == kMaskF32) return ((const float*)a.mask)[off];
@@ -415,19 +417,22 @@ __device__ __forceinline__ float mask_bias(const AttnArgs& a, int64_t off) {
   return to_acc(((const bf16s*)a.mask)[off]);
 }
 
-// The mask of a lane's 16 scores of one query: keys j0 + 8 (r / 4) + 4 h + r % 4. off: the
+// What a kernel does about a mask: nothing, an additive term per score, a bit per score.
+enum MaskForm { kNoMask = 0, kAdd = 1, kBits = 2 };
+
+// Bits of the keys in front of a row's last one: 32 keys from j0 on.
+__device__ __forceinline__ uint32_t bits_below(int lim, int j0) {
+  const int n = lim - j0;
+  return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
+}
+
+// The additive mask of a lane's 16 scores of one query: keys j0 + 8 (r / 4) + 4 h + r % 4. off: the
 // query's row. Keys at or behind M give -inf and are not read. Four adjacent keys are one
 // (unaligned) load where the mask's keys are adjacent.
 __device__ __forceinline__ void mask_of_keys(const AttnArgs& a, int64_t off, int j0, int h, f32x16& x) {
   if (a.ms[3] == 1 && j0 + 32 <= a.M) {
     const int64_t at = off + j0 + 4 * h;
-    if (a.maskKind == kMaskBool) {
-      uint32_t w[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) __builtin_memcpy(&w[q], (const uint8_t*)a.mask + at + 8 * q, 4);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = (w[r >> 2] >> (8 * (r & 3)) & 0xff) ? 0.0f : kNegInf;
-    } else if (a.maskKind == kMaskF32) {
+    if (a.maskKind == kMaskF32) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         f32x4 y;
@@ -458,13 +463,7 @@ __device__ __forceinline__ void mask_of_keys(const AttnArgs& a, int64_t off, int
 __device__ __forceinline__ void mask_of_queries(const AttnArgs& a, int64_t off, int n0, int h, f32x16& x) {
   const int64_t at = off + (int64_t)(n0 + 4 * h) * a.ms[2];
   if (n0 + 32 <= a.N) {
-    if (a.maskKind == kMaskBool) {
-      uint8_t w[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) w[r] = ((const uint8_t*)a.mask)[at + (8 * (r >> 2) + (r & 3)) * a.ms[2]];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = w[r] ? 0.0f : kNegInf;
-    } else if (a.maskKind == kMaskF32) {
+    if (a.maskKind == kMaskF32) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = ((const float*)a.mask)[at + (8 * (r >> 2) + (r & 3)) * a.ms[2]];
     } else {
@@ -501,15 +500,16 @@ template <typename LD> __device__ __forceinline__ uint32_t live_keys(const AttnA
 
 // How many pieces to cut the streamed axis of `steps` tiles into, for `wgs` workgroups on `cus` CUs: the
 // least of what the busiest CU takes, at `tile` us per tile and `pro` us for a workgroup's start and end
-// (workgroups that share a CU overlap: each beyond the first adds 0.7), and of joining n pieces of `bytes`
-// fp32 each, written and read at 4 TB/s behind a launch of 4 us.
-inline int best_split(int64_t wgs, int64_t steps, int cus, double tile, double pro, double bytes) {
+// (of workgroups that share a CU each adds `share` of its time: fp32 products fill the matrix cores alone,
+// 16-bit ones leave them waiting for the softmax), and of joining n pieces of `bytes` fp32 each, written
+// and read at 4 TB/s behind a launch of 4 us.
+inline int best_split(int64_t wgs, int64_t steps, int cus, double tile, double pro, double share, double bytes) {
   int best = 1;
   double least = 0;
   for (int64_t n = 1; n <= 64 && n <= steps; ++n) {
-    const int64_t chunk = (steps + n - 1) / n, share = (wgs * n + cus - 1) / cus;
+    const int64_t chunk = (steps + n - 1) / n, each = (wgs * n + cus - 1) / cus;
     if ((steps + chunk - 1) / chunk != n) continue;  // fewer pieces do the same
-    const double cost = (share <= 1 ? 1.0 : 0.7 * (double)share) * ((double)chunk * tile + pro) +
+    const double cost = (each <= 1 ? 1.0 : share * (double)each) * ((double)chunk * tile + pro) +
                         (n > 1 ? 4.0 + (double)n * 2.0 * bytes / 4e6 : 0.0);
     if (n == 1 || cost < least) best = (int)n, least = cost;
   }

@@ -7,15 +7,17 @@
 // softmax needs one exchange between lane halves per tile and P goes from the one
 // product's accumulators to the other's operand within the lane's registers.
 //
-// Units: without a mask the scores stay unscaled in the accumulators and the row
+// Units: without an additive mask the scores stay unscaled in the accumulators and the row
 // reference m is in log2 units, p = exp2(c S - m) with c = scale log2 e (one fma and
-// one exp2 per score). With a mask, x = scale S + mask in natural units, as an
-// additive mask may hold the type's lowest value, and p = exp2((x - m) log2 e).
+// one exp2 per score). With one, x = scale S + mask in natural units, as an
+// additive mask may hold the type's lowest value, and p = exp2((x - m) log2 e). A mask of truth
+// values is packed into bits first (attn_bits_kernel), whatever its strides: a lane then takes its
+// keys of a tile by one load, a tile ahead, and the scores stay in the units of no mask.
 // P is rounded to the element type for the product with V; its sum is of the
 // unrounded values.
 //
-// Row statistics for the backward pass, [B][H][N] planes: without a mask one plane,
-// m + log2(sum) (+inf for a row without keys: its p is then 0); with a mask two, m
+// Row statistics for the backward pass, [B][H][N] planes: without an additive mask one plane,
+// m + log2(sum) (+inf for a row without keys: its p is then 0); with one two, m
 // and 1 / sum, since m + log(sum) loses the sum where m is the type's lowest value.
 #include "attn_common.h"
 
@@ -33,8 +35,9 @@ template <typename T, int DP, int KS> constexpr int num_buffers() {
 
 // QB: 32-query blocks per wave. KS: 1, the four waves take different queries; 4,
 // they take different keys of each tile and their results are joined at the end.
-template <typename T, int DC, int QB, int KS, bool MASK>
+template <typename T, int DC, int QB, int KS, int FORM>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_fwd_kernel(const AttnArgs a) {
+  constexpr bool MASK = FORM == kAdd;
   constexpr int DP = row_pitch(DC), KT = key_tile<KS>(), NBUF = num_buffers<T, DP, KS>(), NT = DC / 16, ND = DC / 32;
   constexpr int KB = KS == 1 ? KT / 32 : 1;  // 32-key blocks per wave and tile
   constexpr int ROWS = KS == 1 ? 128 * QB : 32 * QB;
@@ -63,7 +66,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
 
   // This lane's queries.
   int qrow[QB], lim[QB], full = klen;
-  int64_t qoff[QB], ooff[QB], soff[QB], moff[QB];
+  int64_t qoff[QB], ooff[QB], soff[QB], moff[QB];  // moff: of the mask, or of the row of bits
   bool stored[QB], alive[QB];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
@@ -76,6 +79,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
     qoff[i] = (int64_t)b * a.qs[0] + (int64_t)hq * a.qs[1] + (int64_t)n * a.qs[2];
     ooff[i] = (int64_t)b * a.os[0] + (int64_t)hq * a.os[1] + (int64_t)n * a.os[2];
     soff[i] = ((int64_t)b * a.H + hq) * a.N + n;
+    if constexpr (FORM == kBits) moff[i] = (int64_t)b * a.bs[0] + (int64_t)hq * a.bs[1] + (int64_t)n * a.bs[2];
     if constexpr (MASK) moff[i] = (int64_t)b * a.ms[0] + (int64_t)hq * a.ms[1] + (int64_t)n * a.ms[2];
   }
   if (a.causal) {  // a row behind R or qlen needs no check: what it computes is not used
@@ -107,13 +111,24 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
   const T* vbase = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1];
   using LD = Loader<T, DP, DC, KT>;
   // Keys that a mask takes from every query are not read either: what they hold is nobody's.
-  const bool byKey = MASK && a.keyMask;
+  const bool byKey = FORM != kNoMask && a.keyMask;
   auto fill = [&](int buf, int key0, uint32_t live) {
     LD::fill(smem + buf * 2 * TB, kbase, a.ks[2], key0, kend, a.D, a.modeK, live);
     LD::fill(smem + buf * 2 * TB + TB, vbase, a.vs[2], key0, kend, a.D, a.modeV, live);
   };
 
+  // A row's bits of the wave's keys of one tile.
+  auto load_bits = [&](int i, int key0) {
+    const uint32_t* p = a.bits + moff[i] + key0 / 32;
+    if constexpr (KS == 4) return (uint64_t)p[wave];
+    else return *(const uint64_t*)p;
+  };
+  uint64_t bits[QB];
   uint32_t live = ~0u;  // of the next tile to fill
+  if constexpr (FORM == kBits)
+    if (kbeg < kend)
+#pragma unroll
+      for (int i = 0; i < QB; ++i) bits[i] = load_bits(i, kbeg);
   if (kbeg < kend) {
     if (byKey) live = live_keys<LD>(a, b, kbeg);
     fill(0, kbeg, live);
@@ -127,6 +142,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
     const bool more = key0 + KT < kend;
     if (NBUF == 2 && more) fill(buf ^ 1, key0 + KT, live);
     if (byKey) live = live_keys<LD>(a, b, key0 + (NBUF == 2 ? 2 : 1) * KT);
+    uint64_t now[QB];
+    if constexpr (FORM == kBits)
+#pragma unroll
+      for (int i = 0; i < QB; ++i) {
+        now[i] = bits[i];
+        if (more) bits[i] = load_bits(i, key0 + KT);
+      }
     const int rl = launder(rl0), cl = launder(cl0);
     const char* tk = smem + buf * 2 * TB;
     const char* tv = tk + TB;
@@ -155,7 +177,16 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
         }
       if constexpr (sizeof(T) == 2 && QB == 1) reads_ahead<KB * NT, (KB * NT < 4 ? KB * NT : 4)>();
       // The mask, and what lies behind the row's last key.
-      if (MASK || wkey + 32 * KB > full) {
+      if constexpr (FORM == kBits) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < QB; ++i) {
+            const uint32_t w = ((uint32_t)(now[i] >> (32 * kb)) & bits_below(lim[i], wkey + 32 * kb)) >> (4 * h);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[kb][i][r] = w & (1u << (8 * (r >> 2) + (r & 3))) ? s[kb][i][r] : kNegInf;
+          }
+      } else if (MASK || wkey + 32 * KB > full) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -404,6 +435,34 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
   }
 }
 
+// A mask of truth values as bits: one word of 32 keys per thread, rows of `words` words; bytes that are not
+// zero are ones, keys behind M zeros. The mask's own sizes (1 where it is broadcast): heads Hm, rows Nm.
+__global__ void __launch_bounds__(256) attn_bits_kernel(const uint8_t* mask, int64_t s0, int64_t s1, int64_t s2, int64_t s3,
+                                                        uint32_t* bits, int Hm, int Nm, int M, int words, int64_t total) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= total) return;
+  const int w = (int)(id % words);
+  const int64_t row = id / words, n = row % Nm, bh = row / Nm;
+  const uint8_t* p = mask + bh / Hm * s0 + bh % Hm * s1 + n * s2;
+  uint32_t out = 0;
+  if (s3 == 1 && 32 * w + 32 <= M) {
+    u32x4 x[2];
+    __builtin_memcpy(x, p + 32 * w, 32);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t y = x[i >> 2][i & 3];
+      const uint32_t t = ((((y & 0x7f7f7f7fu) + 0x7f7f7f7fu) | y) & 0x80808080u) >> 7;  // bits 0, 8, 16, 24
+      out |= ((t | t >> 7 | t >> 14 | t >> 21) & 15u) << (4 * i);
+    }
+  } else {
+    for (int i = 0; i < 32; ++i) {
+      const int j = 32 * w + i;
+      if (j < M) out |= (uint32_t)(p[j * s3] != 0) << i;
+    }
+  }
+  bits[id] = out;
+}
+
 // How a call is laid over the chip.
 struct FwdPlan {
   int ks, rows, kt, tiles, nsplit, chunk, dc;
@@ -425,15 +484,16 @@ FwdPlan fwd_plan(int dtype, const AttnArgs& a, int cus) {
   // 3.5 TFLOP/s that a CU reaches (fp32: 0.5), and a microsecond at least where one wave's latencies add up.
   const double flops = 4.0 * (p.ks == 4 ? 128 : 128 * 64) * p.dc * (p.ks == 4 ? 32 : 1);
   const double tile = std::max(p.ks == 4 ? 1.0 : 0.8, flops / (dtype == LFAMD_F32 ? 0.5e6 : 3.5e6));
-  const int ns = best_split(wgs, steps, cus, tile, 2.0, (double)a.B * a.Hk * R * p.dc * sizeof(float));
+  const int ns = best_split(wgs, steps, cus, tile, 4.0, dtype == LFAMD_F32 ? 1.0 : 0.7, (double)a.B * a.Hk * R * p.dc * sizeof(float));
   p.chunk = std::max(1, (steps + ns - 1) / ns);
   p.nsplit = std::max(1, (steps + p.chunk - 1) / p.chunk);
   return p;
 }
 
-template <typename T, int DC, bool MASK> int fwd_launch(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
+template <typename T, int DC, int FORM> int fwd_launch(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
   constexpr int DP = row_pitch(DC);
-  const void* fn = p.ks == 4 ? (const void*)attn_fwd_kernel<T, DC, 1, 4, MASK> : (const void*)attn_fwd_kernel<T, DC, 1, 1, MASK>;
+  constexpr bool MASK = FORM == kAdd;
+  const void* fn = p.ks == 4 ? (const void*)attn_fwd_kernel<T, DC, 1, 4, FORM> : (const void*)attn_fwd_kernel<T, DC, 1, 1, FORM>;
   const int nbuf = p.ks == 4 ? num_buffers<T, DP, 4>() : num_buffers<T, DP, 1>();
   const size_t lds = (size_t)2 * nbuf * p.kt * DP * sizeof(T);
   if (int e = set_dyn_lds(fn, lds, "softmax_attention")) return e;
@@ -456,7 +516,11 @@ template <typename T, int DC, bool MASK> int fwd_launch(const AttnArgs& a, const
 }
 
 template <typename T, int DC> int fwd_mask(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
-  return a.maskKind ? fwd_launch<T, DC, true>(a, p, st) : fwd_launch<T, DC, false>(a, p, st);
+  switch (a.maskKind) {
+    case kMaskNone: return fwd_launch<T, DC, kNoMask>(a, p, st);
+    case kMaskBool: return fwd_launch<T, DC, kBits>(a, p, st);
+    default: return fwd_launch<T, DC, kAdd>(a, p, st);
+  }
 }
 
 template <typename T> int fwd_dim(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
@@ -470,19 +534,53 @@ template <typename T> int fwd_dim(const AttnArgs& a, const FwdPlan& p, hipStream
 
 }  // namespace
 
-size_t attn_fwd_workspace(int dtype, const AttnArgs& a) {
-  const FwdPlan p = fwd_plan(dtype, a, num_cus());
-  if (p.nsplit <= 1) return 0;
-  return (size_t)p.nsplit * a.B * a.Hk * a.G * a.N * (p.dc + 2) * sizeof(float);
+namespace {
+
+// The mask's own sizes, its broadcast dimensions taken once.
+struct BitsShape {
+  int64_t B, H, N, words;
+};
+BitsShape bits_shape(const AttnArgs& a) {
+  return {a.ms[0] ? a.B : 1, a.ms[1] ? a.H : 1, a.ms[2] ? a.N : 1, (int64_t)(a.M + 127) / 128 * 4};
 }
 
-int attn_fwd(int dtype, AttnArgs a, hipStream_t st) {
+}  // namespace
+
+size_t attn_bits_bytes(const AttnArgs& a) {
+  if (a.maskKind != kMaskBool) return 0;
+  const BitsShape s = bits_shape(a);
+  return ((size_t)(s.B * s.H * s.N * s.words) * sizeof(uint32_t) + 255) / 256 * 256;
+}
+
+int attn_pack_bits(AttnArgs& a, void* workspace, hipStream_t st) {
+  if (a.maskKind != kMaskBool || a.M == 0 || a.N == 0) return LFAMD_OK;
+  const BitsShape s = bits_shape(a);
+  a.bits = (uint32_t*)workspace;
+  a.bs[0] = s.B > 1 ? s.H * s.N * s.words : 0;
+  a.bs[1] = s.H > 1 ? s.N * s.words : 0;
+  a.bs[2] = s.N > 1 ? s.words : 0;
+  const int64_t total = s.B * s.H * s.N * s.words;
+  if ((total + 255) / 256 > INT32_MAX) return fail(LFAMD_ERR_UNSUPPORTED, "softmax_attention: the mask is too large");
+  attn_bits_kernel<<<dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st>>>(
+      (const uint8_t*)a.mask, a.ms[0], a.ms[1], a.ms[2], a.ms[3], a.bits, (int)s.H, (int)s.N, a.M, (int)s.words, total);
+  return check_launch("softmax_attention (mask)");
+}
+
+size_t attn_fwd_workspace(int dtype, const AttnArgs& a) {
+  const FwdPlan p = fwd_plan(dtype, a, num_cus());
+  const size_t part = p.nsplit <= 1 ? 0 : (size_t)p.nsplit * a.B * a.Hk * a.G * a.N * (p.dc + 2) * sizeof(float);
+  return attn_bits_bytes(a) + part;
+}
+
+int attn_fwd(int dtype, AttnArgs a, void* workspace, hipStream_t st) {
   const FwdPlan p = fwd_plan(dtype, a, num_cus());
   a.nsplit = p.nsplit;
   a.tiles = p.tiles;
   a.chunk = p.chunk;
   if ((int64_t)a.B * a.Hk * p.tiles * p.nsplit > INT32_MAX)
     return fail(LFAMD_ERR_UNSUPPORTED, "softmax_attention: too many workgroups");
+  a.part = (float*)((char*)workspace + attn_bits_bytes(a));
+  if (int e = attn_pack_bits(a, workspace, st)) return e;
   switch (dtype) {
     case LFAMD_F32: return fwd_dim<float>(a, p, st);
     case LFAMD_F16: return fwd_dim<f16s>(a, p, st);

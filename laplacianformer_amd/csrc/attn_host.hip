@@ -89,9 +89,9 @@ int lfamd_softmax_attention(int dtype, const lfamd_attention* desc, const void* 
   if (need && (!workspace || workspace_bytes < need)) return fail(LFAMD_ERR_ARG, "%s: workspace too small", who);
   if (need && ((uintptr_t)workspace & 15)) return fail(LFAMD_ERR_ARG, "%s: workspace must be 16-byte aligned", who);
   const int64_t size = (int64_t)dtype_size(dtype);
-  a.q = q, a.k = k, a.v = v, a.out = out, a.stat = stats, a.part = (float*)workspace;
+  a.q = q, a.k = k, a.v = v, a.out = out, a.stat = stats;
   a.modeK = load_mode(k, a.ks, a.D, size, a.keyMask), a.modeV = load_mode(v, a.vs, a.D, size, a.keyMask);
-  return attn_fwd(dtype, a, (hipStream_t)stream);
+  return attn_fwd(dtype, a, workspace, (hipStream_t)stream);
 }
 
 size_t lfamd_softmax_attention_backward_workspace_size(int dtype, const lfamd_attention* desc) {

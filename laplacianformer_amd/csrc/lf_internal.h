@@ -94,7 +94,10 @@ int mix_rows_trio(int dtype, const void* const* A, const float* const* B, void* 
 // that check and fill it in are in attn_host.hip).
 struct AttnArgs;
 size_t attn_fwd_workspace(int dtype, const AttnArgs& a);
-int attn_fwd(int dtype, AttnArgs a, hipStream_t st);
+int attn_fwd(int dtype, AttnArgs a, void* workspace, hipStream_t st);
+// A truth-value mask as bits in the first attn_bits_bytes of a workspace (attn_fwd.hip); sets a.bits.
+size_t attn_bits_bytes(const AttnArgs& a);
+int attn_pack_bits(AttnArgs& a, void* workspace, hipStream_t st);
 size_t attn_bwd_workspace(int dtype, const AttnArgs& a);
 int attn_bwd(int dtype, AttnArgs a, void* workspace, hipStream_t st);
 
