@@ -18,8 +18,6 @@
 // dv. bf16 and fp32 have the exponents and take f = 1.
 #include "attn_common.h"
 
-#include <algorithm>
-
 namespace lfamd {
 
 namespace {
@@ -554,12 +552,14 @@ BwdPlan bwd_plan(int dtype, const AttnArgs& a, int cus) {
   const bool wide = dtype != LFAMD_F32 || p.dc == 32;
   const int qt = wide && p.dc < 96 ? 64 : 32, kt = wide ? 64 : 32;  // query_tile, key_tile
   const int64_t ksteps = (int64_t)a.G * ((a.N + qt - 1) / qt), qsteps = (a.M + kt - 1) / kt;
-  // The other axis is split where a kernel's own blocks leave CUs without work. A tile's time: its four
-  // (dq: three) products at the 3 TFLOP/s that a CU reaches (fp32: 0.45), and a microsecond at least.
-  const double rate = dtype == LFAMD_F32 ? 0.45e6 : 3e6, f32 = sizeof(float), share = dtype == LFAMD_F32 ? 1.0 : 0.7;
-  const double ktile = std::max(1.0, 8.0 * 128 * qt * p.dc / rate), qtile = std::max(0.8, 6.0 * 128 * kt * p.dc / rate);
-  p.ksplit = kw && ksteps ? best_split(kw, ksteps, cus, ktile, 4.0, share, 2.0 * a.B * a.Hk * a.M * p.dc * f32) : 1;
-  p.qsplit = qw && qsteps ? best_split(qw, qsteps, cus, qtile, 4.0, share, 1.0 * a.B * a.H * a.N * p.dc * f32) : 1;
+  // The other axis is split where a kernel's own blocks leave CUs without work. A tile's throughput: its
+  // four (dq: three) products at the 3 TFLOP/s that a CU reaches (fp32: 0.45); its latency as measured
+  // where a CU has one workgroup.
+  const double rate = dtype == LFAMD_F32 ? 0.45e6 : 3e6, f32 = sizeof(float), add = a.maskKind > kMaskBool ? 1.5 : 0.0;
+  const double kthr = 8.0 * 128 * qt * p.dc / rate, qthr = 6.0 * 128 * kt * p.dc / rate;
+  const double klat = std::max(kthr, qt == 64 ? 2.5 : 1.5) + add, qlat = std::max(qthr, kt == 64 ? 2.0 : 1.2) + add;
+  p.ksplit = kw && ksteps ? best_split(kw, ksteps, cus, klat, kthr + 0.3 * add, 2.0 * a.B * a.Hk * a.M * p.dc * f32) : 1;
+  p.qsplit = qw && qsteps ? best_split(qw, qsteps, cus, qlat, qthr + 0.3 * add, 1.0 * a.B * a.H * a.N * p.dc * f32) : 1;
   p.qchunk = (int)std::max<int64_t>(1, (qsteps + p.qsplit - 1) / p.qsplit);
   p.deltaBytes = up256((size_t)a.B * a.H * a.N * sizeof(float));
   if (dtype == LFAMD_F16)

@@ -14,6 +14,8 @@
 // which col_frag() reads the other operand by. No value crosses lanes.
 #pragma once
 
+#include <algorithm>
+
 #include "lf_common.h"
 #include "lf_internal.h"
 
@@ -292,7 +294,7 @@ template <typename T, int DP, int DC, int ROWS> struct Loader {
       }
     } else if (mode == kAsync4) {
       // `live` belongs to the rows of row_of: a call with a mask over keys takes kPlain instead.
-#pragma unroll 1
+#pragma unroll 4
       for (int i = 0; i < 4 * NIT; ++i) {
         const int byte = i * 1024 + (int)threadIdx.x * 4, r = byte / L::ROW;
         const int c = (byte % L::ROW / 16 ^ L::swz(r)) * L::CE + byte % 16 / (int)sizeof(T);
@@ -499,18 +501,18 @@ template <typename LD> __device__ __forceinline__ uint32_t live_keys(const AttnA
 }
 
 // How many pieces to cut the streamed axis of `steps` tiles into, for `wgs` workgroups on `cus` CUs: the
-// least of what the busiest CU takes, at `tile` us per tile and `pro` us for a workgroup's start and end
-// (of workgroups that share a CU each adds `share` of its time: fp32 products fill the matrix cores alone,
-// 16-bit ones leave them waiting for the softmax), and of joining n pieces of `bytes` fp32 each, written
-// and read at 4 TB/s behind a launch of 4 us.
-inline int best_split(int64_t wgs, int64_t steps, int cus, double tile, double pro, double share, double bytes) {
+// least of what the busiest CU takes and of joining. A workgroup alone takes `lat` us per tile (one wave
+// per SIMD waits for its own reads, products and exponentials in turn), workgroups that share a CU `thr`
+// each, and 4 us go to a start and an end; n pieces of `bytes` are written and read at 4 TB/s, behind a
+// launch of 6 us.
+inline int best_split(int64_t wgs, int64_t steps, int cus, double lat, double thr, double bytes) {
   int best = 1;
   double least = 0;
   for (int64_t n = 1; n <= 64 && n <= steps; ++n) {
     const int64_t chunk = (steps + n - 1) / n, each = (wgs * n + cus - 1) / cus;
     if ((steps + chunk - 1) / chunk != n) continue;  // fewer pieces do the same
-    const double cost = (each <= 1 ? 1.0 : share * (double)each) * ((double)chunk * tile + pro) +
-                        (n > 1 ? 4.0 + (double)n * 2.0 * bytes / 4e6 : 0.0);
+    const double cost = std::max(lat, thr * (double)each) * (double)chunk + 4.0 * (double)((each + 1) / 2) +
+                        (n > 1 ? 6.0 + (double)n * 2.0 * bytes / 4e6 : 0.0);
     if (n == 1 || cost < least) best = (int)n, least = cost;
   }
   return best;

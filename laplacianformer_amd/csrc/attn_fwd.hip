@@ -21,8 +21,6 @@
 // and 1 / sum, since m + log(sum) loses the sum where m is the type's lowest value.
 #include "attn_common.h"
 
-#include <algorithm>
-
 namespace lfamd {
 
 namespace {
@@ -480,11 +478,13 @@ FwdPlan fwd_plan(int dtype, const AttnArgs& a, int cus) {
   p.tiles = (int)((R + p.rows - 1) / p.rows);
   const int64_t wgs = (int64_t)a.B * a.Hk * p.tiles;
   const int steps = (a.M + p.kt - 1) / p.kt;
-  // The keys are split where the rows alone leave CUs without work. A tile's time: its products at the
-  // 3.5 TFLOP/s that a CU reaches (fp32: 0.5), and a microsecond at least where one wave's latencies add up.
-  const double flops = 4.0 * (p.ks == 4 ? 128 : 128 * 64) * p.dc * (p.ks == 4 ? 32 : 1);
-  const double tile = std::max(p.ks == 4 ? 1.0 : 0.8, flops / (dtype == LFAMD_F32 ? 0.5e6 : 3.5e6));
-  const int ns = best_split(wgs, steps, cus, tile, 4.0, dtype == LFAMD_F32 ? 1.0 : 0.7, (double)a.B * a.Hk * R * p.dc * sizeof(float));
+  // The keys are split where the rows alone leave CUs without work. A tile's throughput: its products at
+  // the 3.5 TFLOP/s that a CU reaches (fp32: 0.5), its 8192 exponentials at least. Its latency as measured
+  // where a CU has one workgroup; an additive mask's loads add to both.
+  const double thr = std::max(0.5, 4.0 * (p.ks == 4 ? 32 * 128 : 128 * 64) * p.dc / (dtype == LFAMD_F32 ? 0.5e6 : 3.5e6)) +
+                     (a.maskKind > kMaskBool ? 0.4 : 0.0);
+  const double lat = std::max((p.ks == 4 ? 1.0 : p.dc <= 64 ? 1.5 : 2.0) + (a.maskKind > kMaskBool ? 1.5 : 0.0), thr);
+  const int ns = best_split(wgs, steps, cus, lat, thr, (double)a.B * a.Hk * R * p.dc * sizeof(float));
   p.chunk = std::max(1, (steps + ns - 1) / ns);
   p.nsplit = std::max(1, (steps + p.chunk - 1) / p.chunk);
   return p;
