@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
     if constexpr (VL) {
       using LV = Loader<T, DP, DC, 128>;
       const uint32_t bits = FORM != kNoMask && a.keyMask && klen > 0 ? live_keys<LV>(a, b, key0) : ~0u;
-      LV::fill(smem + 4 * TB + 2 * SB, (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1], a.vs[2], key0, klen, a.D,
+      LV::fill(smem + 4 * TB + 2 * SB, (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1] + (int64_t)key0 * a.vs[2],
+               a.vs[2], key0, klen, a.D,
                a.modeV, bits);
     }
   }
@@ -211,12 +212,33 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
   float st0 = 0.0f, st1 = 0.0f, st2 = 0.0f;
   int st3 = 0;
   u32x4 st4 = {0, 0, 0, 0};
-  auto fill = [&](int buf, int step) {
-    const int g = step / perHead, row0 = (tb + step % perHead) * QT, hq = hk * a.G + g;
-    LD::fill(smem + buf * 2 * TB, (const T*)a.q + (int64_t)b * a.qs[0] + (int64_t)hq * a.qs[1], a.qs[2], row0, qlen, a.D,
-             a.modeQ);
-    LD::fill(smem + buf * 2 * TB + TB, (const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)hq * a.gs[1], a.gs[2], row0, qlen,
-             a.D, a.modeG);
+  // The next tile to fill: its head, rows, and where they begin. Counted on, as a division per tile is
+  // forty scalar instructions of each wave.
+  int nextG = perHead ? beg / perHead : 0, nextT = perHead ? beg % perHead : 0, nextH = hk * a.G + nextG;
+  int nextRow = (tb + nextT) * QT;
+  const T *qnext, *gnext;
+  auto settle = [&]() {
+    nextH = hk * a.G + nextG;
+    nextRow = (tb + nextT) * QT;
+    qnext = (const T*)a.q + (int64_t)b * a.qs[0] + (int64_t)nextH * a.qs[1] + (int64_t)nextRow * a.qs[2];
+    gnext = (const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)nextH * a.gs[1] + (int64_t)nextRow * a.gs[2];
+  };
+  settle();
+  auto advance = [&]() {
+    if (++nextT == perHead) {
+      nextT = 0;
+      ++nextG;
+      settle();
+    } else {
+      nextRow += QT;
+      qnext += QT * a.qs[2];
+      gnext += QT * a.gs[2];
+    }
+  };
+  auto fill = [&](int buf) {
+    const int row0 = nextRow, hq = nextH;
+    LD::fill(smem + buf * 2 * TB, qnext, a.qs[2], row0, qlen, a.D, a.modeQ);
+    LD::fill(smem + buf * 2 * TB + TB, gnext, a.gs[2], row0, qlen, a.D, a.modeG);
     if (threadIdx.x < QT) {
       const int n = row0 + threadIdx.x;
       const bool in = n < qlen;
@@ -253,7 +275,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
   };
 
   if (beg < end) {
-    fill(0, beg);
+    fill(0);
     store(0);
   }
   land();
@@ -262,11 +284,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
   int buf = 0;
   for (int step = beg; step < end; ++step) {
     const bool more = step + 1 < end;
-    if (more) fill(buf ^ 1, step + 1);
+    const int row0 = nextRow, hq = nextH;
+    if (more) {
+      advance();
+      fill(buf ^ 1);
+    }
     const char* tq = smem + buf * 2 * TB;
     const char* tg = tq + TB;
     const float* stats = (const float*)(smem + 4 * TB + buf * SB);
-    const int g = step / perHead, row0 = (tb + step % perHead) * QT, hq = hk * a.G + g;
 #pragma unroll 1
     for (int qb = 0; qb < QT; qb += 32) {
       const int rl = launder(rl0), cl = launder(cl0);
@@ -280,7 +305,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 64 ? 1 : 2)
           if constexpr (VL && n >= NT) p.b = L::row_frag(tv, rl, n % NT);
           return p;
         };
-        Ring<Pair, VL ? 2 : 4> ring;
+        Ring<Pair, (sizeof(T) == 4 ? 1 : VL ? 2 : 4)> ring;
         first_reads<2 * NT>(ring, read);
         read_and_use<2 * NT>(ring, read, [&](auto n, const Pair& p) {
           if constexpr (n < NT) s = mma<T>(p.a, kf[n], s);
@@ -412,13 +437,16 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
 #pragma unroll
   for (int d = 0; d < ND; ++d) dq[d] = f32x16{};
 
-  const T* kbase = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1];
-  const T* vbase = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1];
+  // The next tile to fill.
+  const T* knext = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1] + (int64_t)kbeg * a.ks[2];
+  const T* vnext = (const T*)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1] + (int64_t)kbeg * a.vs[2];
   using LD = Loader<T, DP, DC, KT>;
   const bool byKey = FORM != kNoMask && a.keyMask;
   auto fill = [&](int buf, int k0, uint32_t live) {
-    LD::fill(smem + buf * 2 * TB, kbase, a.ks[2], k0, kend, a.D, a.modeK, live);
-    LD::fill(smem + buf * 2 * TB + TB, vbase, a.vs[2], k0, kend, a.D, a.modeV, live);
+    LD::fill(smem + buf * 2 * TB, knext, a.ks[2], k0, kend, a.D, a.modeK, live);
+    LD::fill(smem + buf * 2 * TB + TB, vnext, a.vs[2], k0, kend, a.D, a.modeV, live);
+    knext += KT * a.ks[2];
+    vnext += KT * a.vs[2];
   };
   // The row's bits of a tile's keys.
   const int64_t boff = (int64_t)b * a.bs[0] + (int64_t)hq * a.bs[1] + (int64_t)nr * a.bs[2];
@@ -457,7 +485,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
       if constexpr (MASK) mask_of_keys(a, moff, key0 + kb, h, bias);
       {
         auto read = [&](auto n) { return L::row_frag((n < NT ? tk : tv) + kb * L::ROW, rl, n % NT); };
-        Ring<Frag<T>, 4> ring;
+        Ring<Frag<T>, (sizeof(T) == 4 ? 1 : 4)> ring;
         first_reads<2 * NT>(ring, read);
         read_and_use<2 * NT>(ring, read, [&](auto n, const Frag<T>& x) {
           if constexpr (n < NT) s = mma<T>(x, qf[n], s);
@@ -480,7 +508,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
       }
       // The first columns of k are read while the exponentials run.
       auto cread = [&](auto n) { return L::col_frag(tk + kb * L::ROW, cl, n / ND, n % ND); };
-      Ring<Frag<T>, (sizeof(T) == 2 && DC <= 64 ? 4 : 2)> cring;
+      Ring<Frag<T>, (sizeof(T) == 4 ? 1 : DC <= 64 ? 4 : 2)> cring;
       first_reads<2 * ND>(cring, cread);
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = prob<MASK>(s[r], a.c, x0, x1) * (F16 ? fmaf(dp[r], f, -de) : dp[r] - de);

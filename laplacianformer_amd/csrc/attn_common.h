@@ -260,10 +260,11 @@ template <typename T, int DP, int DC, int ROWS> struct Loader {
 
   static __device__ __forceinline__ int row_of(int i) { return (int)threadIdx.x / L::CPR + i * RPI; }
 
-  static __device__ __forceinline__ void fill(char* tile, const T* base, int64_t stride, int row0, int limit, int D,
+  // first: row row0 (uniform).
+  static __device__ __forceinline__ void fill(char* tile, const T* first, int64_t stride, int row0, int limit, int D,
                                               int mode, uint32_t live = ~0u) {
     const int slot = threadIdx.x % L::CPR;
-    const char* from = (const char*)(base + (int64_t)row0 * stride);  // uniform
+    const char* from = (const char*)first;
     const uint32_t rowBytes = (uint32_t)stride * (uint32_t)sizeof(T);
     const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tile;
     const int wave = uniform(threadIdx.x >> 6);
@@ -309,7 +310,7 @@ template <typename T, int DP, int DC, int ROWS> struct Loader {
       for (int i = 0; i < NIT; ++i) {
         const int r = row_of(i), c = slot ^ L::swz(r);
         *(u32x4*)(tile + i * 4096 + threadIdx.x * 16) =
-            load_chunk<T>(base + (int64_t)(row0 + r) * stride, row0 + r < limit && (live >> i & 1), c * L::CE, D);
+            load_chunk<T>(first + (int64_t)r * stride, row0 + r < limit && (live >> i & 1), c * L::CE, D);
       }
     }
   }
