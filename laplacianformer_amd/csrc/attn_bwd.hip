@@ -680,7 +680,7 @@ int attn_bwd(int dtype, AttnArgs a, void* workspace, hipStream_t st) {
   a.part = (float*)(rest + p.deltaBytes + p.boundBytes);
   const int64_t most = std::max({(int64_t)a.B * a.Hk * p.ktiles * p.ksplit, (int64_t)a.B * a.H * p.qtiles * p.qsplit,
                                  (int64_t)a.B * a.H * ((a.N + 63) / 64) + (int64_t)a.B * a.Hk * ((a.M + 63) / 64)});
-  if (most > INT32_MAX) return fail(LFAMD_ERR_UNSUPPORTED, "softmax_attention backward: too many workgroups");
+  if (most > kMostWorkgroups) return fail(LFAMD_ERR_UNSUPPORTED, "softmax_attention backward: too many workgroups");
   if (int e = attn_pack_bits(a, workspace, st)) return e;
   switch (dtype) {
     case LFAMD_F32: return bwd_dim<float>(a, p, st);

@@ -86,6 +86,8 @@ __device__ __forceinline__ float half_sum(float x) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+constexpr int64_t kMostWorkgroups = (1 << 24) - 1;  // of 256 threads: a grid has below 2^32
+
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f;
 

@@ -569,7 +569,7 @@ int attn_pack_bits(AttnArgs& a, void* workspace, hipStream_t st) {
   a.bs[1] = s.H > 1 ? s.N * s.words : 0;
   a.bs[2] = s.N > 1 ? s.words : 0;
   const int64_t total = s.B * s.H * s.N * s.words;
-  if ((total + 255) / 256 > INT32_MAX) return fail(LFAMD_ERR_UNSUPPORTED, "softmax_attention: the mask is too large");
+  if ((total + 255) / 256 > kMostWorkgroups) return fail(LFAMD_ERR_UNSUPPORTED, "softmax_attention: the mask is too large");
   attn_bits_kernel<<<dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st>>>(
       (const uint8_t*)a.mask, a.ms[0], a.ms[1], a.ms[2], a.ms[3], a.bits, (int)s.H, (int)s.N, a.M, (int)s.words, total);
   return check_launch("softmax_attention (mask)");
@@ -586,7 +586,7 @@ int attn_fwd(int dtype, AttnArgs a, void* workspace, hipStream_t st) {
   a.nsplit = p.nsplit;
   a.tiles = p.tiles;
   a.chunk = p.chunk;
-  if ((int64_t)a.B * a.Hk * p.tiles * p.nsplit > INT32_MAX)
+  if ((int64_t)a.B * a.Hk * p.tiles * p.nsplit > kMostWorkgroups)
     return fail(LFAMD_ERR_UNSUPPORTED, "softmax_attention: too many workgroups");
   a.part = (float*)((char*)workspace + attn_bits_bytes(a));
   if (int e = attn_pack_bits(a, workspace, st)) return e;

@@ -161,8 +161,8 @@ extern "C" int lfamd_rotary(int dtype, const void* q, const int64_t* q_strides, 
   if ((q_heads && (!q || !q_out || !q_strides || !q_out_strides)) || (k_heads && (!k || !k_out || !k_strides || !k_out_strides)) ||
       !positions || !position_strides)
     return fail(LFAMD_ERR_ARG, "rotary: null pointer");
-  if (batch > 65535 || tokens > INT32_MAX / 2 || heads > 65535 || head_dim > 1024)
-    return fail(LFAMD_ERR_UNSUPPORTED, "rotary: batch, heads <= 65535, tokens <= 2^30 and head size <= 1024 are taken");
+  if (batch > 65535 || tokens > (1 << 27) || heads > 65535 || head_dim > 1024)
+    return fail(LFAMD_ERR_UNSUPPORTED, "rotary: batch, heads <= 65535, tokens <= 2^27 and head size <= 1024 are taken");
   const int V = dtype == LFAMD_F32 ? 4 : 8;
   bool vec = head_dim % V == 0 && (interleaved ? 2 * pairs : pairs) % V == 0;
   const void* in[2] = {q, k};

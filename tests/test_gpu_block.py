@@ -105,6 +105,18 @@ def test_norm_fp8(gpu, dtype, width):
     assert y8b.shape == x.shape
 
 
+def test_norm_many_rows(gpu):
+    """More rows than a grid has workgroups: each sign of a two-element row comes out."""
+    import laplacianformer_amd as lf
+
+    rows = 9_000_001
+    x = torch.ones(rows, 2, dtype=torch.bfloat16, device=gpu)
+    x[::3, 0] = -4.0
+    x[::3, 1] = 4.0
+    y = lf.add_rms_norm(x, torch.ones(2, dtype=torch.bfloat16, device=gpu))
+    assert torch.equal(y, x.sign())  # rstd = 1 / |x| (eps rounds away)
+
+
 def test_norm_gradients_against_differences(gpu):
     import laplacianformer_amd as lf
 

@@ -144,12 +144,13 @@ def test_tokens_over_a_cache(gpu, dtype, N):
     assert bool((got["out"][1] == 0).all()) and bool((got["dq"][1] == 0).all())
 
 
+@pytest.mark.parametrize("d", [48, 50, 97])
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-def test_what_is_masked_may_hold_anything(gpu, dtype):
+def test_what_is_masked_may_hold_anything(gpu, dtype, d):
     """NaN and infinities in keys that a length or a mask over keys takes out, and in queries behind
     q_lengths, reach nothing; those keys' and queries' gradients are 0."""
-    print(f"softmax attention non-finite {dtype}", flush=True)
-    B, H, Hk, N, M, d = 2, 4, 2, 70, 150, 48
+    print(f"softmax attention non-finite {dtype} {d}", flush=True)
+    B, H, Hk, N, M = 2, 4, 2, 70, 150
     q, k, v, g, _ = make((B, H, Hk, N, M, d), "plain", dtype, 60)
     for kind in ("bool", "bias"):
         keep = torch.rand(B, 1, 1, M, generator=torch.Generator().manual_seed(61)) > 0.4
@@ -322,6 +323,35 @@ def test_repeats_streams_and_graphs(gpu):
             for t, n in zip(s.grads, ("dq", "dk", "dv")):
                 assert torch.equal(t, w[n]), (rep, n)
             call(gpu, *p)  # eager work between replays
+
+
+def test_mask_broadcasts(gpu):
+    """Masks of fewer dimensions, broadcast along every axis, transposed, and expanded."""
+    import laplacianformer_amd as lf
+
+    B, H, N, M, d = 2, 4, 37, 150, 32
+    q, k, v, _, _ = make((B, H, 2, N, M, d), "plain", "f32", 160)
+    r = torch.Generator().manual_seed(161)
+    masks = [torch.rand(N, M, generator=r) > 0.3, torch.rand(M, generator=r) > 0.3, torch.rand(B, 1, N, 1, generator=r) > 0.3,
+             torch.rand(H, 1, M, generator=r) > 0.3, (torch.rand(M, N, generator=r) > 0.3).t(),
+             (torch.rand(1, 1, 1, M, generator=r) > 0.3).expand(B, H, N, M), torch.tensor(True), torch.tensor(False),
+             torch.randn(H, N, 1, generator=r), torch.randn(M, N, generator=r).t(), torch.randn(B, 1, 1, M, generator=r)]
+    for i, m in enumerate(masks):
+        print("mask", i, tuple(m.shape), flush=True)
+        out = lf.softmax_attention(q.to(gpu), k.to(gpu), v.to(gpu), mask=m.to(gpu))
+        ref = reference(q, k, v, None, {"mask": torch.broadcast_to(m, (B, H, N, M))})
+        bc.assert_within(out, *ref["out"], i)
+
+
+def test_no_second_derivative(gpu):
+    import laplacianformer_amd as lf
+
+    q = torch.randn(1, 2, 4, 8, device=gpu, requires_grad=True)
+    w = torch.ones(8, device=gpu)
+    pos = torch.zeros(1, 4, dtype=torch.int32, device=gpu)
+    for out in (lf.softmax_attention(q, q, q), lf.add_rms_norm(q, w), lf.rotary(q, None, pos, [4])[0]):
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            torch.autograd.grad(out.sum(), q, create_graph=True)
 
 
 def test_refusals(gpu):
