@@ -96,82 +96,80 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(con
   constexpr int THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR, V = Pack<T>::V;
   __shared__ float lds[16];
   const int t = threadIdx.x % TPR;
-  // One row each but for calls of more rows than a grid has. No barrier where a workgroup's waves have rows
-  // of their own (RPB > 1).
-  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < a.rows; row += (int64_t)gridDim.x * RPB) {
-    float s[NV][V], sq = 0.0f;
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * RPB + threadIdx.x / TPR;
+  if (row >= a.rows) return;  // whole waves, and whole workgroups where they meet at barriers (RPB = 1)
+  float s[NV][V], sq = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * TPR) * V;
-      if (c < a.width) {
-        const Pack<T> px = Pack<T>::load((const T*)a.x + row * a.xs, c, a.width);
-        if (a.res) {
-          const Pack<T> pr = Pack<T>::load((const T*)a.res + row * a.rs, c, a.width);
-          Pack<T> ps;
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            s[i][j] = to_acc(px.e[j]) + to_acc(pr.e[j]);
-            ps.e[j] = from_acc<T>(s[i][j]);
-          }
-          ps.store((T*)a.sum + row * a.width, c, a.width);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) s[i][j] = to_acc(px.e[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) sq = fmaf(s[i][j], s[i][j], sq);
-      }
-    }
-    sq = row_reduce<TPR, false>(sq, lds);
-    const float r = 1.0f / sqrtf(sq / (float)a.width + a.eps);
-    if (t == 0 && a.rstd) a.rstd[row] = r;
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * TPR) * V;
-      if (c < a.width) {
-        float w[V];
-        load_weight<T>(a, c, w);
-        Pack<T> py;
+  for (int i = 0; i < NV; ++i) {
+    const int c = (t + i * TPR) * V;
+    if (c < a.width) {
+      const Pack<T> px = Pack<T>::load((const T*)a.x + row * a.xs, c, a.width);
+      if (a.res) {
+        const Pack<T> pr = Pack<T>::load((const T*)a.res + row * a.rs, c, a.width);
+        Pack<T> ps;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          s[i][j] = s[i][j] * r * w[j];
-          if constexpr (F8) top = fmaxf(top, fabsf(s[i][j]));
-          else py.e[j] = from_acc<T>(s[i][j]);
+          s[i][j] = to_acc(px.e[j]) + to_acc(pr.e[j]);
+          ps.e[j] = from_acc<T>(s[i][j]);
         }
-        if constexpr (!F8) py.store((T*)a.y + row * a.width, c, a.width);
+        ps.store((T*)a.sum + row * a.width, c, a.width);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[i][j] = to_acc(px.e[j]);
       }
+#pragma unroll
+      for (int j = 0; j < V; ++j) sq = fmaf(s[i][j], s[i][j], sq);
     }
-    if constexpr (F8) {
-      top = row_reduce<TPR, true>(top, lds);
-      // An all-zero row keeps scale 1: its zeros need none.
-      const float scale = top == 0.0f ? 1.0f : top / 448.0f;
-      if (t == 0) a.scale[row] = scale;
-      uint8_t* y = (uint8_t*)a.y + row * a.width;
+  }
+  sq = row_reduce<TPR, false>(sq, lds);
+  const float r = 1.0f / sqrtf(sq / (float)a.width + a.eps);
+  if (t == 0 && a.rstd) a.rstd[row] = r;
+  float top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * TPR) * V;
-        if (c < a.width) {
-          // |y / scale| <= 448 (1 + 2^-23), which rounds to at most 448: nothing saturates.
-          uint32_t o[V / 4];
+  for (int i = 0; i < NV; ++i) {
+    const int c = (t + i * TPR) * V;
+    if (c < a.width) {
+      float w[V];
+      load_weight<T>(a, c, w);
+      Pack<T> py;
 #pragma unroll
-          for (int j = 0; j < V / 4; ++j) {
-            const float* z = &s[i][4 * j];
-            const int p = __builtin_amdgcn_cvt_pk_fp8_f32(z[0] / scale, z[1] / scale, 0, false);
-            o[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2] / scale, z[3] / scale, p, true);
-          }
-          if (c + V <= a.width) {
-            if constexpr (V == 8) {
-              const uint64_t both = (uint64_t)o[1] << 32 | o[0];
-              __builtin_memcpy(y + c, &both, 8);
-            } else {
-              __builtin_memcpy(y + c, o, 4);
-            }
+      for (int j = 0; j < V; ++j) {
+        s[i][j] = s[i][j] * r * w[j];
+        if constexpr (F8) top = fmaxf(top, fabsf(s[i][j]));
+        else py.e[j] = from_acc<T>(s[i][j]);
+      }
+      if constexpr (!F8) py.store((T*)a.y + row * a.width, c, a.width);
+    }
+  }
+  if constexpr (F8) {
+    top = row_reduce<TPR, true>(top, lds);
+    // An all-zero row keeps scale 1: its zeros need none.
+    const float scale = top == 0.0f ? 1.0f : top / 448.0f;
+    if (t == 0) a.scale[row] = scale;
+    uint8_t* y = (uint8_t*)a.y + row * a.width;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (t + i * TPR) * V;
+      if (c < a.width) {
+        // |y / scale| <= 448 (1 + 2^-23), which rounds to at most 448: nothing saturates.
+        uint32_t o[V / 4];
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) {
+          const float* z = &s[i][4 * j];
+          const int p = __builtin_amdgcn_cvt_pk_fp8_f32(z[0] / scale, z[1] / scale, 0, false);
+          o[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2] / scale, z[3] / scale, p, true);
+        }
+        if (c + V <= a.width) {
+          if constexpr (V == 8) {
+            const uint64_t both = (uint64_t)o[1] << 32 | o[0];
+            __builtin_memcpy(y + c, &both, 8);
           } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-              if (c + j < a.width) y[c + j] = (uint8_t)(o[j >> 2] >> (8 * (j & 3)));
+            __builtin_memcpy(y + c, o, 4);
           }
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (c + j < a.width) y[c + j] = (uint8_t)(o[j >> 2] >> (8 * (j & 3)));
         }
       }
     }
@@ -324,8 +322,10 @@ template <typename T, bool F8> struct NormFwd {
   hipStream_t st;
   template <int TPR, int NV> int go() {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
-    const int64_t grid = std::min<int64_t>((a.rows + RPB - 1) / RPB, 1 << 21);  // a grid has below 2^32 threads
-    add_rms_norm_kernel<T, TPR, NV, F8><<<dim3((unsigned)grid), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(a);
+    // A grid's axis has below 2^32 threads: the workgroups beyond 2^21 go along the second.
+    const int64_t n = (a.rows + RPB - 1) / RPB, x = std::min<int64_t>(n, 1 << 21);
+    add_rms_norm_kernel<T, TPR, NV, F8>
+        <<<dim3((unsigned)x, (unsigned)((n + x - 1) / x)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(a);
     return check_launch("add_rms_norm");
   }
 };
