@@ -86,8 +86,9 @@ def softmax_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: t
     (positive) defaults to ``1 / sqrt(d)``.
 
     A query that nothing is left for gives 0. Keys that ``k_lengths``, or a mask that is the
-    same for every head and query, takes out may hold anything; elsewhere a masked key or value has to be
-    finite, as its probability of 0 is multiplied by it. 16-bit types round the
+    same for every head and query, takes out may hold anything, as may queries from ``q_lengths[b]`` on;
+    elsewhere masked keys and values (and queries and output gradients) have to be finite, as a probability of
+    0 is multiplied by them. 16-bit types round the
     probabilities to that type in front of the product with v. With autograd.
     """
     if scale is None:

@@ -16,6 +16,11 @@
 // two f per key head, with |dz| <= |g_i| |v_j| + |delta_i| <= bound and f bound <= 2^14,
 // which the result is divided by; p <= 1 likewise carries 2^15 into the product for
 // dv. bf16 and fp32 have the exponents and take f = 1.
+//
+// What bounds it (one MI355X, bf16, 4096 x 4096 at 64 channels and 64 heads): dk/dv 663 us for four products, 0.83
+// PFLOP/s, matrix cores busy 41 % and VALU 43 % of the cycles at 1.84 GHz, two waves per SIMD (accumulators 64,
+// operands 32, scores 32 and reads in flight make 204 registers); dq 431 us for three, 0.96 PFLOP/s, three waves.
+// Both run at the power limit, where a large library product reaches 1.18.
 #include "attn_common.h"
 
 namespace lfamd {

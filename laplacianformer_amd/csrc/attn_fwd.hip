@@ -19,6 +19,14 @@
 // Row statistics for the backward pass, [B][H][N] planes: without an additive mask one plane,
 // m + log2(sum) (+inf for a row without keys: its p is then 0); with one two, m
 // and 1 / sum, since m + log(sum) loses the sum where m is the type's lowest value.
+//
+// What bounds it (one MI355X, bf16): 8192 x 8192 causal at 128 channels and 32 heads runs 544 us, 1.01 PFLOP/s at
+// the power-limited 1.6 GHz with the matrix cores busy half the cycles and the VALU (an fma, an exp2, an add,
+// half a maximum and half a rounding per score) the other half, 85 % of a large library product's rate;
+// 4096 x 4096 at 64 channels and 64 heads 326 us, VALU issue 75 %. 128 rows per workgroup (32 per wave) keep two
+// (64 channels: three) waves per SIMD, whose products and softmaxes overlap; a 64-key tile is what four waves load
+// while they compute on the other. One token over 8192 keys (16 sequences, 8 key heads, 128 channels): 81 us
+// for 403 MB, 4.97 TB/s, the rate of a large copy.
 #include "attn_common.h"
 
 namespace lfamd {
