@@ -315,7 +315,8 @@ int lfamd_add_rms_norm(int dtype, const void* x, int64_t x_stride, const void* r
                        float eps, void* stream);
 
 /* The same with y in e4m3 (OCP, largest value 448) and one fp32 scale per row:
- * scale = max|y| / 448 (1 for a row of zeros), y8 = e4m3(y / scale), to nearest even. */
+ * scale = max|y| / 448 (1 for a row whose max|y| is below 2^-117, which becomes zeros), y8 = e4m3(y /
+ * scale), to nearest even. */
 int lfamd_add_rms_norm_fp8(int dtype, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                            int w_dtype, const void* weight, void* y, float* scale, void* sum, int64_t rows,
                            int64_t width, float eps, void* stream);
@@ -357,7 +358,7 @@ int lfamd_rotary(int dtype, const void* q, const int64_t* q_strides, void* q_out
 /* One softmax attention: query [batch][heads][q_len][head_dim], key and value
  * [batch][kv_heads][k_len][head_dim], heads a multiple of kv_heads (query head i reads key
  * head i / (heads / kv_heads)). Strides in elements for batch, head and row; channels are
- * adjacent. head_dim <= 128, q_len * heads / kv_heads and k_len <= 2^30.
+ * adjacent. head_dim <= 128, q_len * heads / kv_heads and k_len <= 2^29.
  *   k_lengths  [batch] or NULL: keys at or behind it do not take part and are not read
  *   q_lengths  [batch] or NULL: queries at or behind it are not read, their output is 0
  *   causal     query n sees keys j <= start + n, start = q_starts[b], or k_len - q_len if NULL

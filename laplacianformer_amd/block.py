@@ -35,7 +35,7 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
 
     Returns ``(y8, scale)`` or ``(y8, scale, sum)``: y8 is float8_e4m3fn, scale float32
     ``[..., 1]`` with ``y = y8 * scale`` and ``scale = max|y| / 448`` over each row (1 for a
-    row of zeros).
+    row of zeros or of values below 2^-117, which become zeros).
     """
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("add_rms_norm_fp8 has no gradient: call it under torch.no_grad()")

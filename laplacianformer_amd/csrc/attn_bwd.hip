@@ -552,14 +552,14 @@ struct SumOf {
   int nsplit, heads, len;
 };
 
-// Adds the splits' partial gradients in their order: DC / 4 threads per row, up to two gradients.
+// Adds the splits' partial gradients in their order: DC / 4 threads per row, up to three gradients.
 template <typename T, int DC>
-__global__ void __launch_bounds__(256) attn_sum_kernel(const SumOf a0, const SumOf a1, int D) {
+__global__ void __launch_bounds__(256) attn_sum_kernel(const SumOf a0, const SumOf a1, const SumOf a2, int D) {
   constexpr int TPR = DC == 96 ? 32 : DC / 4, RPB = 256 / TPR;
   int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  const bool second = row >= a0.rows;
-  const SumOf& a = second ? a1 : a0;
-  if (second) row -= a0.rows;
+  const int which = row < a0.rows ? 0 : row < a0.rows + a1.rows ? 1 : 2;
+  const SumOf& a = which == 0 ? a0 : which == 1 ? a1 : a2;
+  if (which) row -= which == 1 ? a0.rows : a0.rows + a1.rows;
   const int c0 = (threadIdx.x % TPR) * 4;
   if (row >= a.rows || c0 >= DC) return;
   f32x4 x = {0, 0, 0, 0};
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(256) attn_sum_kernel(const SumOf a0, const Sum
 
 struct BwdPlan {
   int dc, ktiles, ksplit, qtiles, qsplit, qchunk;
-  size_t deltaBytes, boundBytes, partBytes;
+  size_t deltaBytes, boundBytes, kpartBytes, partBytes;
 };
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -597,9 +597,11 @@ BwdPlan bwd_plan(int dtype, const AttnArgs& a, int cus) {
   p.deltaBytes = up256((size_t)a.B * a.H * a.N * sizeof(float));
   if (dtype == LFAMD_F16)
     p.boundBytes = up256(((size_t)a.B * a.H * ((a.N + 63) / 64) * 2 + (size_t)a.B * a.Hk * ((a.M + 63) / 64)) * sizeof(float));
+  // Both kernels' partial results at once: one launch adds them all.
   const size_t kp = p.ksplit > 1 ? (size_t)p.ksplit * 2 * a.B * a.Hk * a.M * p.dc * sizeof(float) : 0;
   const size_t qp = p.qsplit > 1 ? (size_t)p.qsplit * a.B * a.H * a.N * p.dc * sizeof(float) : 0;
-  p.partBytes = std::max(kp, qp);
+  p.kpartBytes = up256(kp);
+  p.partBytes = p.kpartBytes + qp;
   return p;
 }
 
@@ -613,18 +615,14 @@ int launch(const void* fn, int64_t grid, size_t lds, const AttnArgs& a, hipStrea
   return check_launch(what);
 }
 
-template <typename T, int DC> int sum_launch(const SumOf& a, const SumOf& b, int D, hipStream_t st) {
-  constexpr int RPB = 256 / (DC == 96 ? 32 : DC / 4);
-  attn_sum_kernel<T, DC><<<dim3((unsigned)((a.rows + b.rows + RPB - 1) / RPB)), dim3(256), 0, st>>>(a, b, D);
-  return check_launch("softmax_attention backward (sums)");
-}
-
 template <typename T, int DC, int FORM> int bwd_launch(AttnArgs a, const BwdPlan& p, hipStream_t st) {
   constexpr bool F16 = std::is_same<T, f16s>::value;
   const int qt = (a.N + 63) / 64, kt = (a.M + 63) / 64;
   int64_t grid = (int64_t)a.B * a.H * qt + (F16 ? (int64_t)a.B * a.Hk * kt : 0);
   if (grid)
     if (int e = launch((const void*)attn_delta_kernel<T, F16>, grid, 0, a, st)) return e;
+  float* const part = a.part;
+  SumOf sums[3] = {};
   if (a.dk) {
     a.nsplit = p.ksplit;
     a.tiles = p.ktiles;
@@ -633,24 +631,27 @@ template <typename T, int DC, int FORM> int bwd_launch(AttnArgs a, const BwdPlan
       return e;
     if (p.ksplit > 1) {
       const int64_t rows = (int64_t)a.B * a.Hk * a.M;
-      const SumOf k{a.part, 2 * rows * DC, a.dks[0], a.dks[1], a.dks[2], rows, a.dk, p.ksplit, a.Hk, a.M};
-      const SumOf v{a.part + rows * DC, 2 * rows * DC, a.dvs[0], a.dvs[1], a.dvs[2], rows, a.dv, p.ksplit, a.Hk, a.M};
-      if (int e = sum_launch<T, DC>(k, v, a.D, st)) return e;
+      sums[0] = SumOf{part, 2 * rows * DC, a.dks[0], a.dks[1], a.dks[2], rows, a.dk, p.ksplit, a.Hk, a.M};
+      sums[1] = SumOf{part + rows * DC, 2 * rows * DC, a.dvs[0], a.dvs[1], a.dvs[2], rows, a.dv, p.ksplit, a.Hk, a.M};
     }
   }
   if (a.dq) {
     a.nsplit = p.qsplit;
     a.tiles = p.qtiles;
     a.chunk = p.qchunk;
+    a.part = (float*)((char*)part + p.kpartBytes);
     if (int e = launch((const void*)attn_dq_kernel<T, DC, FORM>, (int64_t)a.B * a.H * p.qtiles * p.qsplit, dq_lds<T, DC>(), a, st))
       return e;
     if (p.qsplit > 1) {
       const int64_t rows = (int64_t)a.B * a.H * a.N;
-      const SumOf q{a.part, rows * DC, a.dqs[0], a.dqs[1], a.dqs[2], rows, a.dq, p.qsplit, a.H, a.N};
-      if (int e = sum_launch<T, DC>(q, SumOf{}, a.D, st)) return e;
+      sums[2] = SumOf{a.part, rows * DC, a.dqs[0], a.dqs[1], a.dqs[2], rows, a.dq, p.qsplit, a.H, a.N};
     }
   }
-  return ok();
+  const int64_t rows = sums[0].rows + sums[1].rows + sums[2].rows;
+  if (!rows) return ok();
+  constexpr int RPB = 256 / (DC == 96 ? 32 : DC / 4);
+  attn_sum_kernel<T, DC><<<dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(256), 0, st>>>(sums[0], sums[1], sums[2], a.D);
+  return check_launch("softmax_attention backward (sums)");
 }
 
 template <typename T, int DC> int bwd_mask(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {

@@ -9,7 +9,7 @@ namespace lfamd {
 
 namespace {
 
-constexpr int64_t kMostRows = (int64_t)1 << 30;
+constexpr int64_t kMostRows = (int64_t)1 << 29;  // sums of a query's and a key's position stay 32-bit
 
 // How a streamed tensor is read (LoadMode): by the alignment of every row's start and end, for row
 // strides that keep a tile of at most 128 rows within 2^31 bytes.
@@ -39,7 +39,7 @@ int check_desc(const char* who, int dtype, const lfamd_attention* d, bool* empty
     return fail(LFAMD_ERR_ARG, "%s: unknown mask kind %d", who, d->mask_kind);
   const int64_t g = d->kv_heads ? d->heads / d->kv_heads : 0;
   if (d->q_len > kMostRows || d->k_len > kMostRows || (g && d->q_len > kMostRows / g))
-    return fail(LFAMD_ERR_UNSUPPORTED, "%s: at most 2^30 keys, and queries per key head, are taken", who);
+    return fail(LFAMD_ERR_UNSUPPORTED, "%s: at most 2^29 keys, and queries per key head, are taken", who);
   if (d->batch > INT32_MAX || d->heads > INT32_MAX || (d->heads && d->batch > INT32_MAX / d->heads))
     return fail(LFAMD_ERR_UNSUPPORTED, "%s: batch * heads must be below 2^31", who);
   *empty = d->batch == 0 || d->heads == 0;

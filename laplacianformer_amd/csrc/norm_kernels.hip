@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(con
   }
   if constexpr (F8) {
     top = row_reduce<TPR, true>(top, lds);
-    // An all-zero row keeps scale 1: its zeros need none.
-    const float scale = top == 0.0f ? 1.0f : top / 448.0f;
+    // Below 2^-117 the scale would be subnormal: such a row, all zeros among them, keeps 1 and becomes zeros.
+    const float scale = top < 6.0185310762101e-36f ? 1.0f : top / 448.0f;
     if (t == 0) a.scale[row] = scale;
     uint8_t* y = (uint8_t*)a.y + row * a.width;
 #pragma unroll

@@ -103,6 +103,10 @@ def test_norm_fp8(gpu, dtype, width):
         lf.add_rms_norm_fp8(x.to(gpu).requires_grad_(), w.to(gpu))
     y8b, _ = lf.add_rms_norm_fp8(total, w.to(gpu))
     assert y8b.shape == x.shape
+    # a row far below eps: its scale would be subnormal, it becomes zeros
+    if dtype != "f16":
+        y8c, sc = lf.add_rms_norm_fp8(torch.full((2, width), 1e-38, dtype=TORCH_DT[dtype], device=gpu), w.to(gpu), eps=1.0)
+        assert bool((y8c.float() == 0).all()) and bool((sc == 1).all())
 
 
 def test_norm_many_rows(gpu):
