@@ -378,10 +378,11 @@ typedef struct {
   float scale;
 } lfamd_attention;
 
-/* out[b,h,n,:] = sum_j softmax_j(scale * q.k_j + mask) v_j. stats (fp32, may be NULL): what
- * the backward reads of each row, batch * heads * q_len values, twice as many with an additive
- * mask. The workspace (16-byte aligned; 0 bytes without a truth-value mask where the rows alone
- * fill the chip) holds the mask's bits and fp32 results of key ranges. Deterministic. */
+/* out[b,h,n,:] = sum_j softmax_j(scale * q.k_j + mask) v_j. stats (4-byte aligned, may be NULL): what
+ * the backward reads of each row, lfamd_softmax_attention_stats_size bytes. The workspace (16-byte
+ * aligned; 0 bytes without a truth-value mask where the rows alone fill the chip) holds the mask's
+ * bits and fp32 results of key ranges. Deterministic. */
+size_t lfamd_softmax_attention_stats_size(int dtype, const lfamd_attention* desc);
 size_t lfamd_softmax_attention_workspace_size(int dtype, const lfamd_attention* desc);
 int lfamd_softmax_attention(int dtype, const lfamd_attention* desc, const void* q, const void* k, const void* v, void* out,
                             float* stats, void* workspace, size_t workspace_bytes, void* stream);

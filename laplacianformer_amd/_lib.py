@@ -63,6 +63,7 @@ CAPI_PROTOTYPES = [
     ("lfamd_rotary", _I, [_I, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I, _P, _I, _P,
                           ctypes.c_double, _I, _I, _P]),
     ("lfamd_softmax_attention_workspace_size", _SZ, [_I, _P]),
+    ("lfamd_softmax_attention_stats_size", _SZ, [_I, _P]),
     ("lfamd_softmax_attention", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     ("lfamd_softmax_attention_backward_workspace_size", _SZ, [_I, _P]),
     ("lfamd_softmax_attention_backward", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),

@@ -1,5 +1,5 @@
 // softmax_attention, backward. With p_ij recomputed from the forward's row statistics,
-//   delta_i = g_i . o_i
+//   delta_i = g_i . o_i   (o_i in fp32: the stored output and what its rounding took off)
 //   dv_j = sum_i p_ij g_i
 //   dz_ij = p_ij (g_i . v_j - delta_i)
 //   dk_j = scale sum_i dz_ij q_i,   dq_i = scale sum_j dz_ij k_j.
@@ -82,9 +82,13 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
     const T* pg = (const T*)a.g + (int64_t)b * a.gs[0] + (int64_t)hd * a.gs[1] + (int64_t)row * a.gs[2];
     for (int c = part * CE; c < a.D; c += 4 * CE) {
       const u32x4 x = load_chunk<T>(po, in, c, a.D), y = load_chunk<T>(pg, in, c, a.D);
+      u32x4 z;
+      if constexpr (sizeof(T) == 2) z = load_chunk<T>(rest_row<T>(a, bh * a.N + row), in, c, a.D);
 #pragma unroll
       for (int j = 0; j < CE; ++j) {
-        const float u = to_acc(((const T*)&x)[j]), v = to_acc(((const T*)&y)[j]);
+        float u = to_acc(((const T*)&x)[j]);
+        if constexpr (sizeof(T) == 2) u += to_acc(((const T*)&z)[j]);
+        const float v = to_acc(((const T*)&y)[j]);
         dot = fmaf(u, v, dot);
         if (BOUND) sq = fmaf(v, v, sq);
       }

@@ -365,6 +365,16 @@ __device__ __forceinline__ void store4(T* row, int c0, int D, float a, float b, 
   }
 }
 
+// What store4 rounds off its four values, rounded itself (16-bit types).
+template <typename T>
+__device__ __forceinline__ void store4_rest(T* row, int c0, int D, float a, float b, float c, float d) {
+  const float x[4] = {a, b, c, d};
+  float r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = x[i] - to_acc(from_acc<T>(x[i]));
+  store4<T>(row, c0, D, r[0], r[1], r[2], r[3]);
+}
+
 // n / d for 0 <= n < 2^31 by a multiplication (d >= 1).
 struct FastDiv {
   uint32_t mul = 0, shift = 0, d = 1;
@@ -401,6 +411,15 @@ struct AttnArgs {
   float scale, c;                      // c = scale * log2(e)
   FastDiv divN;
 };
+
+// Row statistics: planes of [B][H][N] fp32 (two with an additive mask), then for the 16-bit types what the
+// output's rounding took off, [B][H][N][D].
+__host__ __device__ inline int64_t stat_planes(const AttnArgs& a) {
+  return (a.maskKind > kMaskBool ? 2 : 1) * (int64_t)a.B * a.H * a.N;
+}
+template <typename T> __device__ __forceinline__ T* rest_row(const AttnArgs& a, int64_t row) {
+  return (T*)(a.stat + stat_planes(a)) + row * a.D;
+}
 
 // Keys of sequence b that exist, and queries.
 __device__ __forceinline__ int key_count(const AttnArgs& a, int b) {

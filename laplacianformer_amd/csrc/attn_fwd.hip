@@ -18,7 +18,10 @@
 //
 // Row statistics for the backward pass, [B][H][N] planes: without an additive mask one plane,
 // m + log2(sum) (+inf for a row without keys: its p is then 0); with one two, m
-// and 1 / sum, since m + log(sum) loses the sum where m is the type's lowest value.
+// and 1 / sum, since m + log(sum) loses the sum where m is the type's lowest value. For the
+// 16-bit types what the output's rounding took off follows, so that the backward's
+// delta = rowsum(g o) is of the fp32 output: where few keys weigh in, o is of the size of v, and
+// its half step in delta was the third that the gradients of q and k carried (2.8e-3 against 2.4e-3 in bf16).
 //
 // What bounds it (one MI355X, bf16): 8192 x 8192 causal at 128 channels and 32 heads runs 544 us, 1.01 PFLOP/s at
 // the power-limited 1.6 GHz with the matrix cores busy half the cycles and the VALU (an fma, an exp2, an add,
@@ -327,6 +330,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
         *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[0]) * DC + c0) = x;
       } else {
         store4<T>((T*)a.out + ooff[0], c0, a.D, x[0], x[1], x[2], x[3]);
+        if constexpr (sizeof(T) == 2)
+          if (a.stat) store4_rest<T>(rest_row<T>(a, soff[0]), c0, a.D, x[0], x[1], x[2], x[3]);
       }
     }
     if (wave == 0 && h == 0) {
@@ -362,6 +367,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
             *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[i]) * DC + c0) = x;
           } else {
             store4<T>((T*)a.out + ooff[i], c0, a.D, x[0], x[1], x[2], x[3]);
+            if constexpr (sizeof(T) == 2)
+              if (a.stat) store4_rest<T>(rest_row<T>(a, soff[i]), c0, a.D, x[0], x[1], x[2], x[3]);
           }
         }
       if (h == 0) {
@@ -439,8 +446,10 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
   const int g = a.divN.div(r), n = r - g * a.N, hq = hk * a.G + g;
   T* out = (T*)a.out + (int64_t)b * a.os[0] + (int64_t)hq * a.os[1] + (int64_t)n * a.os[2];
   store4<T>(out, c0, a.D, x[0], x[1], x[2], x[3]);
+  const int64_t so = ((int64_t)b * a.H + hq) * a.N + n;
+  if constexpr (sizeof(T) == 2)
+    if (a.stat) store4_rest<T>(rest_row<T>(a, so), c0, a.D, x[0], x[1], x[2], x[3]);
   if (a.stat && c0 == 0) {
-    const int64_t so = ((int64_t)b * a.H + hq) * a.N + n;
     if (MASK) {
       a.stat[so] = none ? 0.0f : m;
       a.stat[(int64_t)a.B * a.H * a.N + so] = none ? 0.0f : 1.0f / l;

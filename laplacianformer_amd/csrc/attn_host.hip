@@ -76,6 +76,14 @@ size_t lfamd_softmax_attention_workspace_size(int dtype, const lfamd_attention* 
   return attn_fwd_workspace(dtype, make_args(desc));
 }
 
+size_t lfamd_softmax_attention_stats_size(int dtype, const lfamd_attention* desc) {
+  bool empty = false;
+  if (check_desc("softmax_attention", dtype, desc, &empty) || empty) return 0;
+  const AttnArgs a = make_args(desc);
+  const size_t rest = dtype == LFAMD_F32 ? 0 : (size_t)a.B * a.H * a.N * a.D * dtype_size(dtype);
+  return (size_t)stat_planes(a) * sizeof(float) + (rest + 3) / 4 * 4;
+}
+
 int lfamd_softmax_attention(int dtype, const lfamd_attention* desc, const void* q, const void* k, const void* v, void* out,
                             float* stats, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "softmax_attention";

@@ -243,7 +243,7 @@ std::vector<Tensor> SoftmaxAttention_forward(const Tensor q, const Tensor k, con
   Tensor out = at::empty_like(in.q), stats, ws;
   set_strides(in.d.out_strides, out);
   if (need_stats)
-    stats = at::empty({in.d.mask_kind > LFAMD_MASK_BOOL ? 2 : 1, in.d.batch, in.d.heads, in.d.q_len}, q.options().dtype(at::kFloat));
+    stats = at::empty({(int64_t)lfamd_softmax_attention_stats_size(in.dt, &in.d) / 4}, q.options().dtype(at::kFloat));
   const size_t wsb = lfamd_softmax_attention_workspace_size(in.dt, &in.d);
   if (wsb) ws = at::empty({(int64_t)wsb}, q.options().dtype(at::kByte));
   detail::check_status(lfamd_softmax_attention(in.dt, &in.d, ptr(in.q), ptr(in.k), ptr(in.v), ptr(out),
@@ -261,7 +261,7 @@ std::vector<Tensor> SoftmaxAttention_backward(const Tensor grad_out, const Tenso
   detail::same_type(q, grad_out, "grad_out");
   detail::same_type(q, out, "out");
   TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.device() == q.device() &&
-                  stats.numel() == (in.d.mask_kind > LFAMD_MASK_BOOL ? 2 : 1) * in.d.batch * in.d.heads * in.d.q_len,
+                  stats.numel() * 4 == (int64_t)lfamd_softmax_attention_stats_size(in.dt, &in.d),
               op, ": stats must be the forward's");
   at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   const Tensor o = unit_last(out), g = unit_last(grad_out);

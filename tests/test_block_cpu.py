@@ -78,6 +78,10 @@ def test_attention_refusals(lib):
     assert size(3, ctypes.byref(desc())) == 0 and size(0, ctypes.byref(desc(head_dim=200))) == 0
     fsize = lib.lfamd_softmax_attention_workspace_size
     assert fsize(2, ctypes.byref(desc())) == 0 and fsize(2, ctypes.byref(desc(q_len=1, k_len=100000))) > 0
+    stats = lib.lfamd_softmax_attention_stats_size
+    assert stats(0, ctypes.byref(desc())) == 4 * 8 * 4 and stats(2, ctypes.byref(desc())) == 4 * 8 * (4 + 2 * 16)
+    assert stats(1, ctypes.byref(desc(mask_kind=2, head_dim=1, q_len=7))) == 4 * 7 * (8 + 2)
+    assert stats(3, ctypes.byref(desc())) == 0
     long = desc(q_len=1, k_len=100000)
     assert f(long, 2) == 1 and b"workspace" in lib.lfamd_last_error()
 
