@@ -42,14 +42,14 @@ template <typename T, int DP, int KS> constexpr int num_buffers() {
   return 4 * key_tile<KS>() * DP * (int)sizeof(T) <= 128 * 1024 ? 2 : 1;
 }
 
-// QB: 32-query blocks per wave. KS: 1, the four waves take different queries; 4,
+// 32 queries per wave. KS: 1, the four waves take different queries; 4,
 // they take different keys of each tile and their results are joined at the end.
-template <typename T, int DC, int QB, int KS, int FORM>
+template <typename T, int DC, int KS, int FORM>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_fwd_kernel(const AttnArgs a) {
   constexpr bool MASK = FORM == kAdd;
   constexpr int DP = row_pitch(DC), KT = key_tile<KS>(), NBUF = num_buffers<T, DP, KS>(), NT = DC / 16, ND = DC / 32;
   constexpr int KB = KS == 1 ? KT / 32 : 1;  // 32-key blocks per wave and tile
-  constexpr int ROWS = KS == 1 ? 128 * QB : 32 * QB;
+  constexpr int ROWS = KS == 1 ? 128 : 32;
   using L = Tile<T, DP>;
   constexpr int TB = KT * L::ROW;  // bytes of one tile
   extern __shared__ __align__(16) char smem[];
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
   const int split = place % a.nsplit, t0 = place / a.nsplit;
   const int bh = t0 / a.tiles, tile = a.tiles - 1 - t0 % a.tiles;  // the longest rows of a causal mask first
   const int b = bh / a.Hk, hk = bh % a.Hk;
-  const int R = a.G * a.N, row0 = tile * ROWS + (KS == 1 ? wave * 32 * QB : 0);
+  const int R = a.G * a.N, row0 = tile * ROWS + (KS == 1 ? wave * 32 : 0);
   const int klen = key_count(a, b), qlen = query_count(a, b), qstart = query_start(a, b);
 
   // Bounds of the keys that any row of the workgroup, or every row of the wave, sees.
@@ -71,50 +71,35 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
   };
   const int kendAll = max(last_key(tile * ROWS, ROWS), 0);
   const int kbeg = split * a.chunk * KT, kend = min(kendAll, kbeg + a.chunk * KT);
-  const int wend = row0 < R ? min(kend, last_key(row0, 32 * QB)) : 0;
+  const int wend = row0 < R ? min(kend, last_key(row0, 32)) : 0;
 
   // This lane's queries.
-  int qrow[QB], lim[QB], full = klen;
-  int64_t qoff[QB], ooff[QB], soff[QB], moff[QB];  // moff: of the mask, or of the row of bits
-  bool stored[QB], alive[QB];
+  const bool stored = row0 + (lane & 31) < R;
+  const int qrow = stored ? row0 + (lane & 31) : 0;
+  const int g = a.divN.div(qrow), n = qrow - g * a.N, hq = hk * a.G + g;
+  const bool alive = stored && n < qlen;
+  const int lim = !alive ? 0 : a.causal ? min(klen, qstart + n + 1) : klen;
+  const int64_t qoff = (int64_t)b * a.qs[0] + (int64_t)hq * a.qs[1] + (int64_t)n * a.qs[2];
+  const int64_t ooff = (int64_t)b * a.os[0] + (int64_t)hq * a.os[1] + (int64_t)n * a.os[2];
+  const int64_t soff = ((int64_t)b * a.H + hq) * a.N + n;
+  const int64_t moff = FORM == kBits ? (int64_t)b * a.bs[0] + (int64_t)hq * a.bs[1] + (int64_t)n * a.bs[2]
+                                     : (int64_t)b * a.ms[0] + (int64_t)hq * a.ms[1] + (int64_t)n * a.ms[2];
+  int full = klen;  // every row of the wave sees the keys in front of it
+  if (a.causal) {   // a row behind R or qlen needs no check: what it computes is not used
+    int f = alive ? lim : klen;
 #pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    const int r = row0 + 32 * i + (lane & 31);
-    stored[i] = r < R;
-    qrow[i] = stored[i] ? r : 0;
-    const int g = a.divN.div(qrow[i]), n = qrow[i] - g * a.N, hq = hk * a.G + g;
-    alive[i] = stored[i] && n < qlen;
-    lim[i] = !alive[i] ? 0 : a.causal ? min(klen, qstart + n + 1) : klen;
-    qoff[i] = (int64_t)b * a.qs[0] + (int64_t)hq * a.qs[1] + (int64_t)n * a.qs[2];
-    ooff[i] = (int64_t)b * a.os[0] + (int64_t)hq * a.os[1] + (int64_t)n * a.os[2];
-    soff[i] = ((int64_t)b * a.H + hq) * a.N + n;
-    if constexpr (FORM == kBits) moff[i] = (int64_t)b * a.bs[0] + (int64_t)hq * a.bs[1] + (int64_t)n * a.bs[2];
-    if constexpr (MASK) moff[i] = (int64_t)b * a.ms[0] + (int64_t)hq * a.ms[1] + (int64_t)n * a.ms[2];
-  }
-  if (a.causal) {  // a row behind R or qlen needs no check: what it computes is not used
-    int m = klen;
-#pragma unroll
-    for (int i = 0; i < QB; ++i) m = min(m, alive[i] ? lim[i] : klen);
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) m = min(m, __shfl_xor(m, s));
-    full = uniform(m);
+    for (int s = 1; s < 64; s <<= 1) f = min(f, __shfl_xor(f, s));
+    full = uniform(f);
   }
 
-  Frag<T> qf[QB][NT];
+  Frag<T> qf[NT];
 #pragma unroll
-  for (int i = 0; i < QB; ++i)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) qf[i][t] = global_frag<T>((const T*)a.q + qoff[i], alive[i], t, h, a.D);
+  for (int t = 0; t < NT; ++t) qf[t] = global_frag<T>((const T*)a.q + qoff, alive, t, h, a.D);
 
-  f32x16 o[ND][QB];
-  float m[QB], l[QB];
+  f32x16 o[ND];
+  float m = kNegInf, l = 0.0f;
 #pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    m[i] = kNegInf;
-    l[i] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) o[d][i] = f32x16{};
-  }
+  for (int d = 0; d < ND; ++d) o[d] = f32x16{};
 
   // The next tile to fill.
   const T* knext = (const T*)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1] + (int64_t)kbeg * a.ks[2];
@@ -130,18 +115,15 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
   };
 
   // A row's bits of the wave's keys of one tile.
-  auto load_bits = [&](int i, int key0) {
-    const uint32_t* p = a.bits + moff[i] + key0 / 32;
+  auto load_bits = [&](int key0) {
+    const uint32_t* p = a.bits + moff + key0 / 32;
     if constexpr (KS == 4) return (uint64_t)p[wave];
     else return *(const uint64_t*)p;
   };
-  uint64_t bits[QB];
+  uint64_t bits = 0;
   uint32_t live = ~0u;  // of the next tile to fill
-  if constexpr (FORM == kBits)
-    if (kbeg < kend)
-#pragma unroll
-      for (int i = 0; i < QB; ++i) bits[i] = load_bits(i, kbeg);
   if (kbeg < kend) {
+    if constexpr (FORM == kBits) bits = load_bits(kbeg);
     if (byKey) live = live_keys<LD>(a, b, kbeg);
     fill(0, kbeg, live);
     if (NBUF == 2 && byKey) live = live_keys<LD>(a, b, kbeg + KT);
@@ -154,30 +136,22 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
     const bool more = key0 + KT < kend;
     if (NBUF == 2 && more) fill(buf ^ 1, key0 + KT, live);
     if (byKey) live = live_keys<LD>(a, b, key0 + (NBUF == 2 ? 2 : 1) * KT);
-    uint64_t now[QB];
+    const uint64_t now = bits;
     if constexpr (FORM == kBits)
-#pragma unroll
-      for (int i = 0; i < QB; ++i) {
-        now[i] = bits[i];
-        if (more) bits[i] = load_bits(i, key0 + KT);
-      }
+      if (more) bits = load_bits(key0 + KT);
     const int rl = launder(rl0), cl = launder(cl0);
     const char* tk = smem + buf * 2 * TB;
     const char* tv = tk + TB;
     const int wkey = key0 + (KS == 1 ? 0 : 32 * wave);
     if (wkey < wend) {
-      f32x16 bias[MASK ? KB : 1][QB];
+      f32x16 bias[MASK ? KB : 1];
       if constexpr (MASK) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int i = 0; i < QB; ++i) mask_of_keys(a, moff[i], wkey + 32 * kb, h, bias[kb][i]);
+        for (int kb = 0; kb < KB; ++kb) mask_of_keys(a, moff, wkey + 32 * kb, h, bias[kb]);
       }
-      f32x16 s[KB][QB];
+      f32x16 s[KB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < QB; ++i) s[kb][i] = f32x16{};
+      for (int kb = 0; kb < KB; ++kb) s[kb] = f32x16{};
       // At two waves per SIMD (DC >= 96) the one in its products goes first: 8192 causal keys at 128 channels
       // 658 -> 646 us, but 332 -> 352 us for 4096 x 4096 at 64, where three waves share a SIMD.
       if constexpr (DC >= 96) __builtin_amdgcn_s_setprio(1);
@@ -187,85 +161,74 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const Frag<T> kf = L::row_frag(tkw + 32 * kb * L::ROW, rl, t);
-#pragma unroll
-          for (int i = 0; i < QB; ++i) s[kb][i] = mma<T>(kf, qf[i][t], s[kb][i]);
+          s[kb] = mma<T>(kf, qf[t], s[kb]);
         }
-      if constexpr (sizeof(T) == 2 && QB == 1) reads_ahead<KB * NT, (KB * NT < 4 ? KB * NT : 4)>();
+      if constexpr (sizeof(T) == 2) reads_ahead<KB * NT, (KB * NT < 4 ? KB * NT : 4)>();
       if constexpr (DC >= 96) __builtin_amdgcn_s_setprio(0);
       // The mask, and what lies behind the row's last key.
       if constexpr (FORM == kBits) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+        for (int kb = 0; kb < KB; ++kb) {
+          const uint32_t w = ((uint32_t)(now >> (32 * kb)) & bits_below(lim, wkey + 32 * kb)) >> (4 * h);
 #pragma unroll
-          for (int i = 0; i < QB; ++i) {
-            const uint32_t w = ((uint32_t)(now[i] >> (32 * kb)) & bits_below(lim[i], wkey + 32 * kb)) >> (4 * h);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[kb][i][r] = w & (1u << (8 * (r >> 2) + (r & 3))) ? s[kb][i][r] : kNegInf;
-          }
+          for (int r = 0; r < 16; ++r) s[kb][r] = w & (1u << (8 * (r >> 2) + (r & 3))) ? s[kb][r] : kNegInf;
+        }
       } else if (MASK || wkey + 32 * KB > full) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int i = 0; i < QB; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int j = wkey + 32 * kb + 8 * (r >> 2) + 4 * h + (r & 3);
-              if constexpr (MASK) {
-                s[kb][i][r] = j < lim[i] ? masked_score(a, s[kb][i][r], bias[kb][i][r]) : kNegInf;
-              } else {
-                s[kb][i][r] = j < lim[i] ? s[kb][i][r] : kNegInf;
-              }
-            }
-      }
-#pragma unroll
-      for (int i = 0; i < QB; ++i) {
-        float mx = s[0][i][0];
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][i][r]);
-        mx = half_max(mx);
-        if (!MASK) mx *= a.c;
-        // The reference follows the maximum only when that has grown by 2^8: p stays
-        // below 2^8, which every element type holds at full precision, and the
-        // accumulators are rescaled in few tiles.
-        const float slack = MASK ? 8.0f / kLog2e : 8.0f;
-        if (__any(mx > m[i] + slack)) {
-          const float mn = fmaxf(m[i], mx), ms = mn == kNegInf ? 0.0f : mn;
-          const float alpha = exp2_fast(MASK ? (m[i] - ms) * kLog2e : m[i] - ms);
-          m[i] = mn;
-          l[i] *= alpha;
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][i][r] *= alpha;
-        }
-        const float ref = m[i] == kNegInf ? 0.0f : m[i];
-        float sum = 0.0f;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float p = exp2_fast(MASK ? (s[kb][i][r] - ref) * kLog2e : fmaf(s[kb][i][r], a.c, -ref));
-            s[kb][i][r] = p;
-            sum += p;
+            const int j = wkey + 32 * kb + 8 * (r >> 2) + 4 * h + (r & 3);
+            if constexpr (MASK) {
+              s[kb][r] = j < lim ? masked_score(a, s[kb][r], bias[kb][r]) : kNegInf;
+            } else {
+              s[kb][r] = j < lim ? s[kb][r] : kNegInf;
+            }
           }
-        l[i] += sum;
       }
+      float mx = s[0][0];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+      mx = half_max(mx);
+      if (!MASK) mx *= a.c;
+      // The reference follows the maximum only when that has grown by 2^8: p stays
+      // below 2^8, which every element type holds at full precision, and the
+      // accumulators are rescaled in few tiles.
+      const float slack = MASK ? 8.0f / kLog2e : 8.0f;
+      if (__any(mx > m + slack)) {
+        const float mn = fmaxf(m, mx), ms = mn == kNegInf ? 0.0f : mn;
+        const float alpha = exp2_fast(MASK ? (m - ms) * kLog2e : m - ms);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+      }
+      const float ref = m == kNegInf ? 0.0f : m;
+      float sum = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float p = exp2_fast(MASK ? (s[kb][r] - ref) * kLog2e : fmaf(s[kb][r], a.c, -ref));
+          s[kb][r] = p;
+          sum += p;
+        }
+      l += sum;
       if constexpr (DC >= 96) __builtin_amdgcn_s_setprio(1);
       const char* tvw = tv + (KS == 1 ? 0 : 32 * wave) * L::ROW;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-          Frag<T> pf[QB];
-#pragma unroll
-          for (int i = 0; i < QB; ++i) pf[i] = acc_frag<T>(s[kb][i], st);
+          const Frag<T> pf = acc_frag<T>(s[kb], st);
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
             const Frag<T> vf = L::col_frag(tvw + 32 * kb * L::ROW, cl, st, d);
-#pragma unroll
-            for (int i = 0; i < QB; ++i) o[d][i] = mma<T>(vf, pf[i], o[d][i]);
+            o[d] = mma<T>(vf, pf, o[d]);
           }
         }
       if constexpr (DC >= 96) __builtin_amdgcn_s_setprio(0);
@@ -280,14 +243,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
     __syncthreads();
   }
 
-#pragma unroll
-  for (int i = 0; i < QB; ++i) l[i] = half_sum(l[i]);
+  l = half_sum(l);
 
   constexpr float kUnit = MASK ? kLog2e : 1.0f;
   if constexpr (KS == 4) {
     // Join the four waves' results through LDS (the loop's last barrier has passed).
     constexpr int PS = DC + 4;  // floats per row: rows start four banks apart
-    static_assert(QB == 1, "one query block where the waves share it");
     static_assert(4 * 32 * (PS + 2) * 4 <= 2 * NBUF * TB, "the tiles' LDS holds the partial results");
     float* po = (float*)smem;
     float* pm = po + 4 * 32 * PS;
@@ -298,10 +259,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
 #pragma unroll
       for (int gq = 0; gq < 4; ++gq)
         *(f32x4*)(po + (wave * 32 + q) * PS + 32 * d + 8 * gq + 4 * h) =
-            (f32x4){o[d][0][4 * gq], o[d][0][4 * gq + 1], o[d][0][4 * gq + 2], o[d][0][4 * gq + 3]};
+            (f32x4){o[d][4 * gq], o[d][4 * gq + 1], o[d][4 * gq + 2], o[d][4 * gq + 3]};
     if (h == 0) {
-      pm[wave * 32 + q] = m[0];
-      pl[wave * 32 + q] = l[0];
+      pm[wave * 32 + q] = m;
+      pl[wave * 32 + q] = l;
     }
     __syncthreads();
     // Wave w takes columns 8 w + 4 h of every 32.
@@ -315,9 +276,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
       f[w] = exp2_fast((pm[w * 32 + q] - ref) * kUnit);
       lt += f[w] * pl[w * 32 + q];
     }
-    if (!stored[0]) return;
+    if (!stored) return;
     const float inv = a.nsplit > 1 ? 1.0f : lt == 0.0f ? 0.0f : 1.0f / lt;
-    const bool live = alive[0];
+    const bool live = alive;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       const int c0 = 32 * d + 8 * wave + 4 * h;
@@ -327,63 +288,60 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DC >= 96 ? 1 : 2) attn_
       x *= inv;
       if (!live) x = f32x4{0, 0, 0, 0};
       if (a.nsplit > 1) {
-        *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[0]) * DC + c0) = x;
+        *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow) * DC + c0) = x;
       } else {
-        store4<T>((T*)a.out + ooff[0], c0, a.D, x[0], x[1], x[2], x[3]);
+        store4<T>((T*)a.out + ooff, c0, a.D, x[0], x[1], x[2], x[3]);
         if constexpr (sizeof(T) == 2)
-          if (a.stat) store4_rest<T>(rest_row<T>(a, soff[0]), c0, a.D, x[0], x[1], x[2], x[3]);
+          if (a.stat) store4_rest<T>(rest_row<T>(a, soff), c0, a.D, x[0], x[1], x[2], x[3]);
       }
     }
     if (wave == 0 && h == 0) {
       if (a.nsplit > 1) {
-        float* ps = a.part + (int64_t)a.nsplit * a.B * a.Hk * R * DC + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[0]) * 2;
+        float* ps = a.part + (int64_t)a.nsplit * a.B * a.Hk * R * DC + (((int64_t)split * a.B * a.Hk + bh) * R + qrow) * 2;
         ps[0] = live ? mt : kNegInf;
         ps[1] = live ? lt : 0.0f;
       } else if (a.stat) {
         const bool none = !live || lt == 0.0f;
         if (MASK) {
-          a.stat[soff[0]] = none ? 0.0f : mt;
-          a.stat[(int64_t)a.B * a.H * a.N + soff[0]] = none ? 0.0f : 1.0f / lt;
+          a.stat[soff] = none ? 0.0f : mt;
+          a.stat[(int64_t)a.B * a.H * a.N + soff] = none ? 0.0f : 1.0f / lt;
         } else {
-          a.stat[soff[0]] = none ? __builtin_inff() : mt + log2f(lt);
+          a.stat[soff] = none ? __builtin_inff() : mt + log2f(lt);
         }
       }
     }
   } else {
+    if (!stored) return;
+    const bool none = !alive || l == 0.0f;
+    const float inv = a.nsplit > 1 ? 1.0f : none ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int i = 0; i < QB; ++i) {
-      if (!stored[i]) continue;
-      const bool none = !alive[i] || l[i] == 0.0f;
-      const float inv = a.nsplit > 1 ? 1.0f : none ? 0.0f : 1.0f / l[i];
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int gq = 0; gq < 4; ++gq) {
-          const int c0 = 32 * d + 8 * gq + 4 * h;
-          f32x4 x = {o[d][i][4 * gq], o[d][i][4 * gq + 1], o[d][i][4 * gq + 2], o[d][i][4 * gq + 3]};
-          x *= inv;
-          if (none) x = f32x4{0, 0, 0, 0};
-          if (a.nsplit > 1) {
-            *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow[i]) * DC + c0) = x;
-          } else {
-            store4<T>((T*)a.out + ooff[i], c0, a.D, x[0], x[1], x[2], x[3]);
-            if constexpr (sizeof(T) == 2)
-              if (a.stat) store4_rest<T>(rest_row<T>(a, soff[i]), c0, a.D, x[0], x[1], x[2], x[3]);
-          }
-        }
-      if (h == 0) {
+      for (int gq = 0; gq < 4; ++gq) {
+        const int c0 = 32 * d + 8 * gq + 4 * h;
+        f32x4 x = {o[d][4 * gq], o[d][4 * gq + 1], o[d][4 * gq + 2], o[d][4 * gq + 3]};
+        x *= inv;
+        if (none) x = f32x4{0, 0, 0, 0};
         if (a.nsplit > 1) {
-          float* ps = a.part + (int64_t)a.nsplit * a.B * a.Hk * R * DC +
-                      (((int64_t)split * a.B * a.Hk + bh) * R + qrow[i]) * 2;
-          ps[0] = none ? kNegInf : m[i];
-          ps[1] = none ? 0.0f : l[i];
-        } else if (a.stat) {
-          if (MASK) {
-            a.stat[soff[i]] = none ? 0.0f : m[i];
-            a.stat[(int64_t)a.B * a.H * a.N + soff[i]] = none ? 0.0f : 1.0f / l[i];
-          } else {
-            a.stat[soff[i]] = none ? __builtin_inff() : m[i] + log2f(l[i]);
-          }
+          *(f32x4*)(a.part + (((int64_t)split * a.B * a.Hk + bh) * R + qrow) * DC + c0) = x;
+        } else {
+          store4<T>((T*)a.out + ooff, c0, a.D, x[0], x[1], x[2], x[3]);
+          if constexpr (sizeof(T) == 2)
+            if (a.stat) store4_rest<T>(rest_row<T>(a, soff), c0, a.D, x[0], x[1], x[2], x[3]);
+        }
+      }
+    if (h == 0) {
+      if (a.nsplit > 1) {
+        float* ps = a.part + (int64_t)a.nsplit * a.B * a.Hk * R * DC +
+                    (((int64_t)split * a.B * a.Hk + bh) * R + qrow) * 2;
+        ps[0] = none ? kNegInf : m;
+        ps[1] = none ? 0.0f : l;
+      } else if (a.stat) {
+        if (MASK) {
+          a.stat[soff] = none ? 0.0f : m;
+          a.stat[(int64_t)a.B * a.H * a.N + soff] = none ? 0.0f : 1.0f / l;
+        } else {
+          a.stat[soff] = none ? __builtin_inff() : m + log2f(l);
         }
       }
     }
@@ -519,7 +477,7 @@ FwdPlan fwd_plan(int dtype, const AttnArgs& a, int cus) {
 template <typename T, int DC, int FORM> int fwd_launch(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
   constexpr int DP = row_pitch(DC);
   constexpr bool MASK = FORM == kAdd;
-  const void* fn = p.ks == 4 ? (const void*)attn_fwd_kernel<T, DC, 1, 4, FORM> : (const void*)attn_fwd_kernel<T, DC, 1, 1, FORM>;
+  const void* fn = p.ks == 4 ? (const void*)attn_fwd_kernel<T, DC, 4, FORM> : (const void*)attn_fwd_kernel<T, DC, 1, FORM>;
   const int nbuf = p.ks == 4 ? num_buffers<T, DP, 4>() : num_buffers<T, DP, 1>();
   const size_t lds = (size_t)2 * nbuf * p.kt * DP * sizeof(T);
   if (int e = set_dyn_lds(fn, lds, "softmax_attention")) return e;
