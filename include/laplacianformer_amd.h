@@ -324,13 +324,15 @@ int lfamd_add_rms_norm_fp8(int dtype, const void* x, int64_t x_stride, const voi
 /* Gradients of lfamd_add_rms_norm: with gn = grad_y * weight and n = sum * rstd,
  * grad_x = grad_sum + rstd * (gn - n * mean(gn * n)) (the gradient of both addends;
  * grad_sum NULL: taken as zero), grad_weight = sum over the rows of grad_y * n (type
- * w_dtype, or NULL to skip it). `sum` is the stored sum, rows sum_stride apart; grad_x is
+ * w_dtype, or NULL to skip it). sum is x + residual in fp32, as in the forward pass; with
+ * residual NULL, x is the sum (the stored one will do, at the price of its rounding). grad_x is
  * contiguous. The workspace (4-byte aligned) is needed for grad_weight only. Deterministic. */
 size_t lfamd_add_rms_norm_backward_workspace_size(int dtype, int64_t rows, int64_t width);
 int lfamd_add_rms_norm_backward(int dtype, const void* grad_y, int64_t grad_y_stride, const void* grad_sum,
-                                int64_t grad_sum_stride, const void* sum, int64_t sum_stride, int w_dtype,
-                                const void* weight, const float* rstd, void* grad_x, void* grad_weight, int64_t rows,
-                                int64_t width, void* workspace, size_t workspace_bytes, void* stream);
+                                int64_t grad_sum_stride, const void* x, int64_t x_stride, const void* residual,
+                                int64_t residual_stride, int w_dtype, const void* weight, const float* rstd,
+                                void* grad_x, void* grad_weight, int64_t rows, int64_t width, void* workspace,
+                                size_t workspace_bytes, void* stream);
 
 /* Rotary positions of q [batch][q_heads][tokens][head_dim] and k (k_heads; either may have
  * no heads) over num_axes <= 8 axes: sections[a] channel pairs belong to axis a, in order;

@@ -58,8 +58,8 @@ CAPI_PROTOTYPES = [
     ("lfamd_add_rms_norm", _I, [_I, _P, _I64, _P, _I64, _I, _P, _P, _P, _P, _I64, _I64, ctypes.c_float, _P]),
     ("lfamd_add_rms_norm_fp8", _I, [_I, _P, _I64, _P, _I64, _I, _P, _P, _P, _P, _I64, _I64, ctypes.c_float, _P]),
     ("lfamd_add_rms_norm_backward_workspace_size", _SZ, [_I, _I64, _I64]),
-    ("lfamd_add_rms_norm_backward", _I, [_I, _P, _I64, _P, _I64, _P, _I64, _I, _P, _P, _P, _P, _I64, _I64, _P, _SZ,
-                                         _P]),
+    ("lfamd_add_rms_norm_backward", _I, [_I, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _P, _P, _P, _P, _I64, _I64,
+                                         _P, _SZ, _P]),
     ("lfamd_rotary", _I, [_I, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I, _P, _I, _P,
                           ctypes.c_double, _I, _I, _P]),
     ("lfamd_softmax_attention_workspace_size", _SZ, [_I, _P]),

@@ -5,9 +5,12 @@
 // of the threads that own it (one wave, or a workgroup of 256 or 1024 threads, chosen
 // by the width so that a thread holds at most 16 elements) between the sum of squares
 // and the scaling. Rows may begin and end anywhere: the 16-byte accesses need no alignment. The forward normalises the
-// fp32 sum, not its stored rounding; the backward reads the stored one (one tensor
-// instead of the two addends: a seventh of its traffic), whose half step enters n and
-// dw once beside their own rounding. The backward's workgroups walk the rows with a
+// fp32 sum, not its stored rounding, and so does the backward where the two addends are
+// given (16-bit types: a quarter more to move, and gradients 1.4 times as exact, as the stored
+// sum's half step would enter n beside the gradients' own rounding: dw of 2048 x 16000 bf16
+// 93 us and 1.6e-3 off, from the stored sum 72 us and 2.4e-3; equal times at 4096 x 4096).
+// gn is formed twice rather than held, which keeps 8192 columns and more in 128 registers
+// (104 -> 93 us, fp32 159 -> 145). The backward's workgroups walk the rows with a
 // fixed stride, keep their share of dw in registers, and write one fp32 partial row
 // each; a second kernel adds those in their order, so the same call gives the same bits.
 // Measured on one MI355X: 16384 x 4096 bf16 to 8 bits 88 us (470 MB, 5.3 TB/s, the rate of a large copy); 12544 x 333
@@ -180,8 +183,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(con
   }
 }
 
-// a.sum: the stored sum (x itself without a residual). part: [gridDim.x][width].
-template <typename T, int TPR, int NV>
+// ADD: a.x and a.res are the addends; otherwise a.x is their sum. part: [gridDim.x][width].
+template <typename T, int TPR, int NV, bool ADD>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_bwd_kernel(const NormArgs a) {
   constexpr int THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR, V = Pack<T>::V;
   __shared__ float lds[16];
@@ -196,28 +199,30 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_bwd_kernel
   }
   // Without barriers in the loop (RPB > 1) the waves of a workgroup walk their rows alone.
   for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < a.rows; row += (int64_t)gridDim.x * RPB) {
-    Pack<T> ps[NV], py[NV], pg[NV];
+    Pack<T> ps[NV], pr[ADD ? NV : 1], py[NV], pg[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (t + i * TPR) * V;
       if (c < a.width) {
-        ps[i] = Pack<T>::load((const T*)a.sum + row * a.xs, c, a.width);
+        ps[i] = Pack<T>::load((const T*)a.x + row * a.xs, c, a.width);
+        if constexpr (ADD) pr[i] = Pack<T>::load((const T*)a.res + row * a.rs, c, a.width);
         py[i] = Pack<T>::load((const T*)a.gy + row * a.gys, c, a.width);
         if (a.gs) pg[i] = Pack<T>::load((const T*)a.gs + row * a.gss, c, a.width);
       }
     }
     const float r = a.rstd[row];
-    float n[NV][V], g[NV][V], dot = 0.0f;
+    float n[NV][V], dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((t + i * TPR) * V < a.width)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          n[i][j] = to_acc(ps[i].e[j]) * r;
+          float s = to_acc(ps[i].e[j]);
+          if constexpr (ADD) s += to_acc(pr[i].e[j]);
+          n[i][j] = s * r;
           const float gy = to_acc(py[i].e[j]);
           dw[i][j] = fmaf(gy, n[i][j], dw[i][j]);
-          g[i][j] = gy * w[i][j];
-          dot = fmaf(g[i][j], n[i][j], dot);
+          dot = fmaf(gy * w[i][j], n[i][j], dot);
         }
     dot = row_reduce<TPR, false>(dot, lds) / (float)a.width;
 #pragma unroll
@@ -227,7 +232,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_bwd_kernel
         Pack<T> pd;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          float d = r * fmaf(-n[i][j], dot, g[i][j]);
+          float d = r * fmaf(-n[i][j], dot, to_acc(py[i].e[j]) * w[i][j]);
           if (a.gs) d += to_acc(pg[i].e[j]);
           pd.e[j] = from_acc<T>(d);
         }
@@ -347,7 +352,9 @@ template <typename T> struct NormBwd {
   int grid;
   template <int TPR, int NV> int go() {
     const size_t lds = TPR < 256 && a.part ? (size_t)a.width * sizeof(float) : 0;
-    add_rms_norm_bwd_kernel<T, TPR, NV><<<dim3(grid), dim3(TPR < 256 ? 256 : TPR), lds, st>>>(a);
+    const dim3 g(grid), b(TPR < 256 ? 256 : TPR);
+    if (a.res) add_rms_norm_bwd_kernel<T, TPR, NV, true><<<g, b, lds, st>>>(a);
+    else add_rms_norm_bwd_kernel<T, TPR, NV, false><<<g, b, lds, st>>>(a);
     return check_launch("add_rms_norm backward");
   }
 };
@@ -412,17 +419,19 @@ size_t lfamd_add_rms_norm_backward_workspace_size(int dtype, int64_t rows, int64
 }
 
 int lfamd_add_rms_norm_backward(int dtype, const void* grad_y, int64_t grad_y_stride, const void* grad_sum,
-                                int64_t grad_sum_stride, const void* sum, int64_t sum_stride, int w_dtype,
-                                const void* weight, const float* rstd, void* grad_x, void* grad_weight, int64_t rows,
-                                int64_t width, void* workspace, size_t workspace_bytes, void* stream) {
+                                int64_t grad_sum_stride, const void* x, int64_t x_stride, const void* residual,
+                                int64_t residual_stride, int w_dtype, const void* weight, const float* rstd,
+                                void* grad_x, void* grad_weight, int64_t rows, int64_t width, void* workspace,
+                                size_t workspace_bytes, void* stream) {
   const char* who = "add_rms_norm backward";
   if (int e = check_sizes(who, dtype, w_dtype, rows, width)) return e;
   hipStream_t st = (hipStream_t)stream;
-  if (rows > 0 && (!grad_y || !sum || !weight || !rstd || !grad_x)) return fail(LFAMD_ERR_ARG, "%s: null pointer", who);
+  if (rows > 0 && (!grad_y || !x || !weight || !rstd || !grad_x)) return fail(LFAMD_ERR_ARG, "%s: null pointer", who);
   if (rows == 0 && !grad_weight) return ok();
   NormArgs a{};
-  a.gy = grad_y, a.gs = grad_sum, a.sum = (void*)sum, a.w = weight, a.rstd = (float*)rstd, a.dx = grad_x;
-  a.gys = grad_y_stride, a.gss = grad_sum_stride, a.xs = sum_stride, a.rows = rows, a.width = (int)width;
+  a.gy = grad_y, a.gs = grad_sum, a.x = x, a.res = residual, a.w = weight, a.rstd = (float*)rstd, a.dx = grad_x;
+  a.gys = grad_y_stride, a.gss = grad_sum_stride, a.xs = x_stride, a.rs = residual_stride;
+  a.rows = rows, a.width = (int)width;
   a.wf32 = w_dtype == LFAMD_F32;
   int grid = 0;
   if (rows > 0) {

@@ -95,35 +95,35 @@ std::vector<Tensor> AddRmsNorm_forward_fp8(const Tensor x, const Tensor weight, 
   return {y, scale, sum.defined() ? sum : x};
 }
 
-std::vector<Tensor> AddRmsNorm_backward(const Tensor grad_y, const OptTensor grad_sum, const Tensor sum,
-                                        const Tensor weight, const Tensor rstd, bool need_weight) {
+std::vector<Tensor> AddRmsNorm_backward(const Tensor grad_y, const OptTensor grad_sum, const Tensor x,
+                                        const Tensor weight, const OptTensor residual, const Tensor rstd, bool need_weight) {
   const char* op = "add_rms_norm backward";
   const Tensor w = weight.contiguous();
-  NormIn n = norm_in(op, sum, weight, std::nullopt);
-  TORCH_CHECK(grad_y.sizes() == sum.sizes(), op, ": grad_y and the sum must have the same shape");
-  detail::same_type(sum, grad_y, "grad_y");
-  TORCH_CHECK(rstd.scalar_type() == at::kFloat && rstd.numel() == n.rows && rstd.is_contiguous() && rstd.device() == sum.device(),
+  NormIn n = norm_in(op, x, weight, residual);
+  TORCH_CHECK(grad_y.sizes() == x.sizes(), op, ": grad_y and x must have the same shape");
+  detail::same_type(x, grad_y, "grad_y");
+  TORCH_CHECK(rstd.scalar_type() == at::kFloat && rstd.numel() == n.rows && rstd.is_contiguous() && rstd.device() == x.device(),
               op, ": rstd must be the forward's");
   Tensor gy = grad_y, gs;
   const int64_t gys = row_view(gy);
   int64_t gss = 0;
   if (given(grad_sum)) {
-    TORCH_CHECK(grad_sum->sizes() == sum.sizes(), op, ": grad_sum and the sum must have the same shape");
-    detail::same_type(sum, *grad_sum, "grad_sum");
+    TORCH_CHECK(grad_sum->sizes() == x.sizes(), op, ": grad_sum and x must have the same shape");
+    detail::same_type(x, *grad_sum, "grad_sum");
     gs = *grad_sum;
     gss = row_view(gs);
   }
-  at::hip::HIPGuardMasqueradingAsCUDA guard(sum.device());
-  Tensor dx = at::empty(sum.sizes(), sum.options()), dw, ws;
+  at::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  Tensor dx = at::empty(x.sizes(), x.options()), dw, ws;
   size_t wsb = 0;
   if (need_weight) {
     dw = at::empty_like(w);
     wsb = lfamd_add_rms_norm_backward_workspace_size(n.dt, n.rows, n.width);
-    ws = at::empty({(int64_t)wsb}, sum.options().dtype(at::kByte));
+    ws = at::empty({(int64_t)wsb}, x.options().dtype(at::kByte));
   }
-  detail::check_status(lfamd_add_rms_norm_backward(n.dt, ptr(gy), gys, ptr(gs), gss, ptr(n.x), n.xs, n.wt, ptr(w),
-                                                   rstd.data_ptr<float>(), ptr(dx), ptr(dw), n.rows, n.width, ptr(ws), wsb,
-                                                   detail::stream_of(sum)));
+  detail::check_status(lfamd_add_rms_norm_backward(n.dt, ptr(gy), gys, ptr(gs), gss, ptr(n.x), n.xs, ptr(n.res), n.rs,
+                                                   n.wt, ptr(w), rstd.data_ptr<float>(), ptr(dx), ptr(dw), n.rows,
+                                                   n.width, ptr(ws), wsb, detail::stream_of(x)));
   return {dx, need_weight ? dw : Tensor()};
 }
 
@@ -300,7 +300,9 @@ struct AddRmsNormNode : torch::autograd::Function<AddRmsNormNode> {
                                double eps) {
     ctx->set_materialize_grads(false);
     const auto r = AddRmsNorm_forward(x, weight, residual, eps, true);
-    ctx->save_for_backward({r[1], weight, r[2]});
+    // In 16-bit types the addends, whose sum has not been rounded; in fp32 the sum, one tensor less.
+    const bool addends = given(residual) && x.element_size() == 2;
+    ctx->save_for_backward({addends ? x : r[1], weight, r[2], addends ? *residual : Tensor()});
     if (given(residual)) return {r[0], r[1]};
     return {r[0]};
   }
@@ -310,7 +312,8 @@ struct AddRmsNormNode : torch::autograd::Function<AddRmsNormNode> {
     const Tensor gs = g.size() > 1 ? g[1] : Tensor();
     if (!g[0].defined() && !gs.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const Tensor gy = g[0].defined() ? g[0] : at::zeros_like(saved[0]);
-    const auto d = AddRmsNorm_backward(gy, gs.defined() ? OptTensor(gs) : std::nullopt, saved[0], saved[1], saved[2],
+    const auto d = AddRmsNorm_backward(gy, gs.defined() ? OptTensor(gs) : std::nullopt, saved[0], saved[1],
+                                       saved[3].defined() ? OptTensor(saved[3]) : std::nullopt, saved[2],
                                        ctx->needs_input_grad(1));
     return {d[0], d[1], g.size() > 1 ? d[0] : Tensor(), Tensor()};
   }

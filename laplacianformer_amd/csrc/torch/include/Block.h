@@ -13,7 +13,8 @@ std::vector<at::Tensor> AddRmsNorm_forward(const at::Tensor x, const at::Tensor 
 std::vector<at::Tensor> AddRmsNorm_forward_fp8(const at::Tensor x, const at::Tensor weight,
                                                const std::optional<at::Tensor> residual, double eps);
 std::vector<at::Tensor> AddRmsNorm_backward(const at::Tensor grad_y, const std::optional<at::Tensor> grad_sum,
-                                            const at::Tensor sum, const at::Tensor weight, const at::Tensor rstd,
+                                            const at::Tensor x, const at::Tensor weight,
+                                            const std::optional<at::Tensor> residual, const at::Tensor rstd,
                                             bool need_weight);
 std::vector<at::Tensor> Rotary(const at::Tensor q, const std::optional<at::Tensor> k, const at::Tensor positions,
                                const std::vector<int64_t> sections, double base, bool interleaved, bool inverse);

@@ -131,7 +131,7 @@ def rms_norm(x, weight, residual, eps, gy=None, gs=None):
     if gy is None:
         return res
     g = gy.double()
-    us = u if residual is not None else 0.0  # the backward reads the stored sum
+    us = U32 if residual is not None else 0.0  # the fp32 sum, or in fp32 the stored one
     gn = g * w
     dot = (gn * n).mean(-1, keepdim=True)
     err_n = (us + c) * n.abs()

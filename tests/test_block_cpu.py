@@ -96,7 +96,7 @@ def test_norm_refusals(lib):
     f8 = lambda scale: lib.lfamd_add_rms_norm_fp8(0, DUMMY, 8, NULL, 8, 0, DUMMY, DUMMY, scale, NULL, 4, 8, 1e-6, NULL)
     assert f8(NULL) == 1
     b = lambda ws=NULL, n=0, dw=DUMMY, gy=DUMMY: lib.lfamd_add_rms_norm_backward(
-        0, gy, 8, NULL, 8, DUMMY, 8, 0, DUMMY, DUMMY, DUMMY, dw, 4, 8, ws, n, NULL)
+        0, gy, 8, NULL, 8, DUMMY, 8, NULL, 8, 0, DUMMY, DUMMY, DUMMY, dw, 4, 8, ws, n, NULL)
     assert b() == 1 and b"workspace" in lib.lfamd_last_error()
     assert b(ctypes.c_void_p(18), 1 << 20) == 1 and b"aligned" in lib.lfamd_last_error()
     assert b(gy=NULL) == 1
