@@ -6,7 +6,7 @@ addition, rotary positions on the token grid, exact softmax attention, and
 All run on hand-written HIP kernels in float32, float16 and bfloat16 (float64 and CPU
 tensors are refused), take strided inputs where the last dimension's elements are
 adjacent, and record into a HIP graph. Results do not depend on the launch: the same
-call gives the same bits. Gradients are of first order (no create_graph).
+call gives the same bits. Gradients are of first order (no create_graph); forward-mode tangents are refused.
 """
 from __future__ import annotations
 

@@ -66,6 +66,14 @@ NormIn norm_in(const char* op, const Tensor& x, const Tensor& weight, const OptT
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+const Tensor* if_given(const OptTensor& t) { return given(t) ? &*t : nullptr; }
+
+// The kernels carry no tangents: a dual tensor's would be dropped, which says that the derivative is zero.
+void no_tangent(const char* op, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), op, " has no forward-mode derivative");
+}
+
 }  // namespace
 
 std::vector<Tensor> AddRmsNorm_forward(const Tensor x, const Tensor weight, const OptTensor residual, double eps,
@@ -82,6 +90,7 @@ std::vector<Tensor> AddRmsNorm_forward(const Tensor x, const Tensor weight, cons
 }
 
 std::vector<Tensor> AddRmsNorm_forward_fp8(const Tensor x, const Tensor weight, const OptTensor residual, double eps) {
+  no_tangent("add_rms_norm_fp8", {&x, &weight, if_given(residual)});
   const Tensor w = weight.contiguous();
   NormIn n = norm_in("add_rms_norm_fp8", x, weight, residual);
   at::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
@@ -291,8 +300,9 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 // The backward passes are kernels without a derivative of their own.
-void once(const char* op) {
+void once(const char* op, const variable_list& grads) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, " has no second derivative: call backward without create_graph");
+  for (const Tensor& g : grads) no_tangent(op, {&g});
 }
 
 struct AddRmsNormNode : torch::autograd::Function<AddRmsNormNode> {
@@ -307,7 +317,7 @@ struct AddRmsNormNode : torch::autograd::Function<AddRmsNormNode> {
     return {r[0]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once("add_rms_norm");
+    once("add_rms_norm", g);
     const auto saved = ctx->get_saved_variables();
     const Tensor gs = g.size() > 1 ? g[1] : Tensor();
     if (!g[0].defined() && !gs.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
@@ -332,7 +342,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
     return r;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once("rotary");
+    once("rotary", g);
     const Tensor positions = ctx->get_saved_variables()[0];
     const auto sections = ctx->saved_data["sections"].toIntVector();
     const double base = ctx->saved_data["base"].toDouble();
@@ -361,7 +371,7 @@ struct SoftmaxAttentionNode : torch::autograd::Function<SoftmaxAttentionNode> {
     return r[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once("softmax_attention");
+    once("softmax_attention", g);
     const auto s = ctx->get_saved_variables();
     auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
     const bool need_k = ctx->needs_input_grad(1), need_v = ctx->needs_input_grad(2);
@@ -386,7 +396,8 @@ bool records(std::initializer_list<const Tensor*> ts) {
 }  // namespace
 
 std::vector<Tensor> AddRmsNorm(const Tensor x, const Tensor weight, const OptTensor residual, double eps) {
-  if (records({&x, &weight, given(residual) ? &*residual : nullptr})) return AddRmsNormNode::apply(x, weight, residual, eps);
+  no_tangent("add_rms_norm", {&x, &weight, if_given(residual)});
+  if (records({&x, &weight, if_given(residual)})) return AddRmsNormNode::apply(x, weight, residual, eps);
   auto r = AddRmsNorm_forward(x, weight, residual, eps, false);
   r.resize(given(residual) ? 2 : 1);
   return r;
@@ -394,7 +405,8 @@ std::vector<Tensor> AddRmsNorm(const Tensor x, const Tensor weight, const OptTen
 
 std::vector<Tensor> RotaryPositions(const Tensor q, const OptTensor k, const Tensor positions,
                                     const std::vector<int64_t> sections, double base, bool interleaved) {
-  if (records({&q, given(k) ? &*k : nullptr})) {
+  no_tangent("rotary", {&q, if_given(k)});
+  if (records({&q, if_given(k)})) {
     auto r = RotaryNode::apply(q, k, positions, sections, base, interleaved);
     r.resize(2);
     return r;
@@ -405,6 +417,7 @@ std::vector<Tensor> RotaryPositions(const Tensor q, const OptTensor k, const Ten
 Tensor SoftmaxAttention(const Tensor q, const Tensor k, const Tensor v, const OptTensor mask, bool causal,
                         const OptTensor k_lengths, const OptTensor q_lengths, const OptTensor q_starts, double scale) {
   TORCH_CHECK(!given(mask) || !mask->requires_grad(), "softmax_attention: the mask has no gradient");
+  no_tangent("softmax_attention", {&q, &k, &v, if_given(mask)});
   if (records({&q, &k, &v}))
     return SoftmaxAttentionNode::apply(q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale);
   return SoftmaxAttention_forward(q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale, false)[0];

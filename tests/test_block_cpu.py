@@ -142,3 +142,24 @@ def test_host_helpers():
     assert lf.rotary_sections(64, 2) == [16, 16] and lf.rotary_sections(128, 3) == [22, 21, 21]
     with pytest.raises(ValueError):
         lf.AttentionBlock(30, 4)
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor without requires_grad takes no autograd node: its tangent must not be dropped silently."""
+    import laplacianformer_amd as lf
+    from torch.autograd import forward_ad
+
+    r = lambda *s: torch.randn(*s)
+    x, w, q, pos = r(2, 8), r(8), r(1, 2, 4, 8), lf.grid_positions((2, 2))
+    mask = r(4, 4)
+    with forward_ad.dual_level():
+        d = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for fn in (lambda: lf.add_rms_norm(d(x), w), lambda: lf.add_rms_norm(x, d(w)), lambda: lf.add_rms_norm(x, w, d(x)),
+                   lambda: lf.add_rms_norm_fp8(d(x), w), lambda: lf.add_rms_norm_fp8(x, w, d(x)),
+                   lambda: lf.rotary(d(q), None, pos, [2, 2]), lambda: lf.rotary(q, d(q), pos, [2, 2]),
+                   lambda: lf.softmax_attention(d(q), q, q), lambda: lf.softmax_attention(q, d(q), q),
+                   lambda: lf.softmax_attention(q, q, d(q)), lambda: lf.softmax_attention(q, q, q, mask=d(mask))):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                fn()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                fn()

@@ -385,3 +385,23 @@ def test_norm_and_rotary_streams_and_graphs(gpu):
         eager()
     for o, d in got:
         assert torch.equal(o, want[0]) and torch.equal(d, want[1])
+
+
+def test_forward_mode_is_refused(gpu):
+    """A tangent of an input, or of an output gradient, raises: none is dropped."""
+    import laplacianformer_amd as lf
+    from torch.autograd import forward_ad
+
+    q = torch.randn(1, 2, 4, 8, device=gpu)
+    w, pos = torch.ones(8, device=gpu), lf.grid_positions((2, 2), gpu)
+    fns = (lambda t: lf.add_rms_norm(t, w), lambda t: lf.rotary(t, None, pos, [2, 2])[0],
+           lambda t: lf.softmax_attention(t, q, q))
+    with forward_ad.dual_level():
+        for fn in fns:
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                fn(forward_ad.make_dual(q, q))
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                fn(forward_ad.make_dual(q.clone().requires_grad_(), q))
+            x = q.clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                torch.autograd.grad(fn(x), x, forward_ad.make_dual(q, q))
