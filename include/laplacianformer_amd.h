@@ -341,8 +341,8 @@ int lfamd_add_rms_norm_backward(int dtype, const void* grad_y, int64_t grad_y_st
  * (2p, 2p + 1) if interleaved. inverse != 0: by the negative angle (the backward pass).
  * Strides (elements): batch, head, token, channels adjacent; output may be the input.
  * positions: int32, or int64 if positions_64, element strides {axis, batch, token}; the
- * angle is reduced exactly for any position. At most 128 pairs, head_dim <= 1024, batch and
- * heads <= 65535, tokens <= 2^27. */
+ * angle has fp32 accuracy at any position (base >= 1; below, where |position| / base <= 2^78). At most
+ * 128 pairs, head_dim <= 1024, batch and heads <= 65535, tokens <= 2^27. */
 int lfamd_rotary(int dtype, const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
                  int64_t q_heads, const void* k, const int64_t* k_strides, void* k_out, const int64_t* k_out_strides,
                  int64_t k_heads, int64_t batch, int64_t tokens, int64_t head_dim, const void* positions,

@@ -63,7 +63,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, sec
 
     ``positions`` is int32 or int64, ``[axes, N]`` or ``[axes, B, N]``; ``sections[a]`` channel
     pairs belong to axis a, in order, and pair j of axis a turns by ``position_a * base **
-    (-j / sections[a])``, exact for any position. Pair p is channels ``(p, p + pairs)``, or
+    (-j / sections[a])``, with the angle in fp32 accuracy at any position (base >= 1; below, where
+    ``|position| / base`` is at most 2^78). Pair p is channels ``(p, p + pairs)``, or
     ``(2 p, 2 p + 1)`` if ``interleaved``; channels behind the pairs are copied. At most 128
     pairs. Returns ``(q', k')``. With autograd.
     """

@@ -3,9 +3,9 @@
 //   angle = position_a * base^(-j / n_a).
 // Channels behind the pairs pass through. The backward pass is the rotation by -angle.
 //
-// The angle is reduced exactly: base^(-j / n) / (2 pi) is held as a 64-bit fraction of a
-// turn, and position * fraction modulo 2^64, an integer product, is the turn's fractional
-// part for positions of any size. Its upper 32 bits go through sincospi in fp32.
+// The angle is reduced in integers: base^(-j / n) / (2 pi) is held as a 96-bit fraction of a
+// turn (rotary_turns.h), and position * fraction modulo 2^96 is the turn's fractional part: a position of
+// 63 bits moves it by 2^-33 turns at most. Its upper 32 bits go through sincospi in fp32.
 //
 // Memory-bound. A workgroup takes 16 tokens of a sequence: it computes their cosines
 // and sines into LDS once, then walks the heads of q and of k with 16-byte accesses
@@ -16,6 +16,7 @@
 
 #include "lf_common.h"
 #include "lf_internal.h"
+#include "rotary_turns.h"
 
 namespace lfamd {
 
@@ -34,7 +35,8 @@ struct RotaryArgs {
   int64_t ps[3];               // axis, batch, token
   int pos64, N, D, pairs, headsPerBlock;
   float sign;                  // -1: the inverse rotation
-  uint64_t turn[kMaxPairs];
+  uint64_t turn[kMaxPairs];    // the fraction's upper 64 bits
+  uint32_t low[kMaxPairs];     // its next 32
   uint8_t axis[kMaxPairs];
 };
 
@@ -47,7 +49,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     const int t = i / P, p = i - t * P;
     const int64_t off = a.axis[p] * a.ps[0] + b * a.ps[1] + (int64_t)(tok0 + t) * a.ps[2];
     const int64_t pos = a.pos64 ? ((const int64_t*)a.pos)[off] : (int64_t)((const int32_t*)a.pos)[off];
-    const int32_t f = (int32_t)(((uint64_t)pos * a.turn[p]) >> 32);  // of a turn, times 2^32
+    // Bits 32 .. 95 of the signed position times the fraction.
+    const uint64_t up = (uint64_t)pos * a.turn[p] + ((uint64_t)(uint32_t)pos * a.low[p] >> 32) + (uint64_t)((pos >> 32) * (int64_t)a.low[p]);
+    const int32_t f = (int32_t)(up >> 32);                           // of a turn, times 2^32
     float s, c;
     sincospif((float)f * 4.656612873077393e-10f, &s, &c);            // 2^-31: half turns
     cs[i] = make_float2(c, s * a.sign);
@@ -147,10 +151,10 @@ extern "C" int lfamd_rotary(int dtype, const void* q, const int64_t* q_strides, 
   int64_t pairs = 0;
   for (int i = 0; i < num_axes; ++i) {
     if (sections[i] < 0 || sections[i] > kMaxPairs) return fail(LFAMD_ERR_ARG, "rotary: section %d has %lld pairs", i, (long long)sections[i]);
+    turn128 turns[kMaxPairs];
+    rotary_turns(base, (int)sections[i], turns);
     for (int64_t j = 0; j < sections[i] && pairs + j < kMaxPairs; ++j) {
-      // A fraction of a turn, modulo whole turns (a base below 1 gives frequencies above 1).
-      const double turn = pow(base, -(double)j / (double)sections[i]) / (2.0 * M_PI), part = turn - floor(turn);
-      a.turn[pairs + j] = (uint64_t)(part * 9007199254740992.0) << 11;  // 53 bits
+      a.turn[pairs + j] = (uint64_t)(turns[j] >> 64), a.low[pairs + j] = (uint32_t)(turns[j] >> 32);
       a.axis[pairs + j] = (uint8_t)i;
     }
     pairs += sections[i];
