@@ -92,8 +92,11 @@ def laplacian_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, grid:
     """LaplacianFormer attention of q, k, v [B,H,N,d] (autograd through the HIP ops).
 
     ``grid`` is the token grid (default square); landmarks are ``pool x pool`` averages of k.
-    Returns [B,H,N,d] in the input type.
+    Returns [B,H,N,d] in the input type. Autocast does not reach the layer's own fp32 products.
     """
+    if torch.is_autocast_enabled("cuda"):
+        with torch.autocast("cuda", enabled=False):
+            return laplacian_attention(q, k, v, grid, pool, iters)
     in_dtype = q.dtype
     B, H, N, d = q.shape
     if grid is None:

@@ -12,6 +12,7 @@
 //   K_xy = exp(-s L1(x, y)), s = 1 / sqrt(d), fp32
 //   out = K_qm . W,  W = NewtonInverse(K_mm) . (K_km^T V)
 #include <ATen/ATen.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <torch/types.h>
 
 #include <cmath>
@@ -170,6 +171,7 @@ void check_layer(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, 
 std::vector<at::Tensor> LaplacianAttention_forward(at::Tensor q, at::Tensor k, at::Tensor v, int64_t gh, int64_t gw,
                                                    int64_t pool, int64_t iters) {
   check_layer(q, k, v, gh, gw, pool);
+  const c10::impl::ExcludeDispatchKeyGuard fp32(c10::DispatchKey::AutocastCUDA);  // the M x M products stay fp32
   const at::ScalarType in = q.scalar_type();
   q = q.contiguous();
   k = k.contiguous();
@@ -203,6 +205,7 @@ std::vector<at::Tensor> LaplacianAttention_backward(at::Tensor g, std::vector<at
   const at::Tensor &k_qm = saved[5], &k_mm = saved[6], &k_km = saved[7], &inv = saved[8], &kv = saved[9];
   const at::Tensor& w = saved[10];
   check_layer(q, k, v, gh, gw, pool);
+  const c10::impl::ExcludeDispatchKeyGuard fp32(c10::DispatchKey::AutocastCUDA);
   TORCH_CHECK(g.sizes() == q.sizes(), "laplacian attention backward: grad_output must be [B,H,N,d]");
   TORCH_CHECK(g.device() == q.device(), "laplacian attention backward: grad_output must be on the inputs' GPU");
   for (const at::Tensor& t : saved)

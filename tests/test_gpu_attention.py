@@ -190,3 +190,27 @@ def test_attention_host_entry_rejects(gpu):
         L.LaplacianAttention_backward(out.cpu(), [q, q, q] + saved, 8, 8, 4)
     with pytest.raises(RuntimeError, match="saved tensors"):
         L.LaplacianAttention_backward(out, [q, q, q] + saved[:-1] + [saved[-1].cpu()], 8, 8, 4)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("grid,d,pool", [((8, 8), 32, 2), ((28, 28), 64, 4), ((8, 8), 80, 2)])
+def test_attention_under_autocast(gpu, grid, d, pool, dtype):
+    """The layer on tensors of one type gives the same bits with autocast on as without: its own products between
+    the kernels (M x M, in fp32) are no autocast products, forward or, in the one-node layer (d <= 64), backward."""
+    import laplacianformer_amd as lf
+
+    print(f"attention autocast {dtype} {grid} {d}", flush=True)
+    shape = (2, 2, grid[0] * grid[1], d)
+    x = [gen(shape, 200 + i, dtype).to(gpu).requires_grad_() for i in range(3)]
+    g = gen(shape, 203, dtype).to(gpu)
+    out = lf.laplacian_attention(*x, grid=grid, pool=pool)
+    grads = torch.autograd.grad(out, x, g)
+    for amp in (torch.bfloat16, torch.float16):
+        with torch.autocast("cuda", amp):
+            got = lf.laplacian_attention(*x, grid=grid, pool=pool)
+            inside = torch.autograd.grad(got, x, g, retain_graph=True) if d <= 64 else None
+        outside = torch.autograd.grad(got, x, g)
+        assert got.dtype == out.dtype and torch.equal(got, out)
+        for some in (inside, outside):
+            for a, b in zip(some or grads, grads):
+                assert torch.equal(a, b)
