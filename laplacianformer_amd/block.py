@@ -23,7 +23,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     """Root-mean-square norm over the last dimension, with the residual's addition.
 
     ``sum = x + residual``, ``y = sum / sqrt(mean(sum^2) + eps) * weight`` (statistics of the
-    float32 sum). Returns ``(y, sum)`` in x's type, or ``y`` alone without a residual.
+    float32 sum). Returns ``(y, sum)`` in x's type, which is the residual's too, or ``y`` alone without a residual.
     ``weight`` has x's type or float32; the last dimension is at most 16384. With autograd.
     """
     out = ext().AddRmsNorm(x, weight, residual, eps)
@@ -102,7 +102,8 @@ class AttentionBlock(torch.nn.Module):
 
     ``forward(x, residual)`` adds and norms (add_rms_norm), projects to q, k and v, turns q
     and k by their tokens' grid positions (rotary), attends, and projects back. It returns
-    ``(out, sum)``: the next block's ``(x, residual)``. ``attention`` is "softmax"
+    ``(out, sum)``: the next block's ``(x, residual)``, also under autocast, where out is of 16 bits and the
+    sum stays float32 (x and residual of different types are widened to the wider one). ``attention`` is "softmax"
     (softmax_attention, ``kv_heads`` key heads shared by ``heads`` query heads) or
     "laplacian" (laplacian_attention with ``pool`` and ``iters``, one key head per query head).
     """
@@ -141,6 +142,9 @@ class AttentionBlock(torch.nn.Module):
         if residual is None:
             y, total = add_rms_norm(x, self.weight, eps=self.eps), x
         else:
+            if x.dtype != residual.dtype:  # under autocast: a 16-bit projection beside the fp32 stream, which stays fp32
+                wide = torch.promote_types(x.dtype, residual.dtype)
+                x, residual = x.to(wide), residual.to(wide)
             y, total = add_rms_norm(x, self.weight, residual, eps=self.eps)
         qkv = self.qkv(y).view(B, N, self.heads + 2 * self.kv_heads, d).transpose(1, 2)
         q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1)

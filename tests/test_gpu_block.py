@@ -405,3 +405,36 @@ def test_forward_mode_is_refused(gpu):
             x = q.clone().requires_grad_()
             with pytest.raises(RuntimeError, match="no forward-mode derivative"):
                 torch.autograd.grad(fn(x), x, forward_ad.make_dual(q, q))
+
+
+@pytest.mark.parametrize("attention", ["softmax", "laplacian"])
+@pytest.mark.parametrize("amp", ["bf16", "f16"])
+def test_attention_blocks_under_autocast(gpu, amp, attention):
+    """Three blocks in a row under autocast, as a pyramid's stage trains: each projection's 16-bit output meets the fp32
+    residual stream. The sums stay fp32, and every gradient arrives in its leaf's type. Against the same blocks in
+    fp32: per block and direction nine roundings of the type in a row (as in test_attention_block), each of at
+    most u, through three blocks and back; a condition of 4 for the attention: 6 * 36 u of the norm."""
+    import laplacianformer_amd as lf
+
+    print(f"attention blocks autocast {amp} {attention}", flush=True)
+    torch.manual_seed(7)
+    blocks = torch.nn.ModuleList([lf.AttentionBlock(64, 2, attention=attention, pool=2) for _ in range(3)]).to(gpu)
+    x = gen((2, 64, 64), 90, "f32").to(gpu).requires_grad_()
+    g, gs = gen((2, 64, 64), 91, "f32").to(gpu), gen((2, 64, 64), 92, "f32").to(gpu)
+
+    def step():
+        y, s = x, None
+        for b in blocks:
+            y, s = b(y, s, grid=(8, 8))
+        leaves = [x, *blocks.parameters()]
+        return y, s, torch.autograd.grad((y, s), leaves, (g.to(y.dtype), gs), allow_unused=False)
+
+    want = step()
+    with torch.autocast("cuda", TORCH_DT[amp]):
+        got = step()
+    assert got[0].dtype == TORCH_DT[amp] and got[1].dtype == torch.float32
+    tol = 6 * 36 * bc.unit(TORCH_DT[amp])
+    for i, (a, w) in enumerate(zip([got[0], got[1], *got[2]], [want[0], want[1], *want[2]])):
+        assert i == 0 or a.dtype == torch.float32
+        err = (a.double() - w.double()).norm() / w.double().norm()
+        assert err <= tol, (i, err.item(), tol)
