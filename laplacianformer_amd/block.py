@@ -129,15 +129,21 @@ class AttentionBlock(torch.nn.Module):
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, grid: Sequence[int] | None = None,
                 positions: torch.Tensor | None = None, mask: torch.Tensor | None = None,
                 lengths: torch.Tensor | None = None):
-        """x, residual [B, N, dim]. ``grid``: the token grid (default: a square), ``positions``
-        [axes, N] or [axes, B, N] in its place; ``mask`` and ``lengths`` (int32 [B], the tokens that
-        each sequence has) go to softmax_attention."""
+        """x, residual [B, N, dim]. ``grid``: the token grid, ``positions`` [axes, N] or [axes, B, N] in its
+        place. With neither, the tokens of a causal block, or of a batch with ``lengths``, are sequences: one axis,
+        whatever N is, so that a prefix has the same positions; else N has to be a square's.
+        ``mask`` and ``lengths`` (int32 [B], the tokens that each sequence has) go to softmax_attention."""
         B, N, C = x.shape
         d = C // self.heads
-        if grid is None:
+        if grid is None and (self.attention == "laplacian" or self.positions and positions is None):
             side = math.isqrt(N)
-            grid = (side, side) if side * side == N else (N,)
-        if math.prod(grid) != N:
+            if self.causal or lengths is not None:
+                grid = (N,)
+            elif side * side == N:
+                grid = (side, side)
+            else:
+                raise ValueError(f"N={N} tokens are no square: their grid or positions are needed")
+        if grid is not None and math.prod(grid) != N:
             raise ValueError(f"token grid {tuple(grid)} does not match N={N}")
         if residual is None:
             y, total = add_rms_norm(x, self.weight, eps=self.eps), x

@@ -163,3 +163,21 @@ def test_forward_mode_is_refused():
                 fn()
             with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
                 fn()
+
+
+def test_block_infers_no_axes_from_a_token_count():
+    """Tokens that are no square's and have neither grid nor positions raise, before any kernel; a causal block
+    and a batch with lengths take one axis at any count, and a block without positions needs no grid."""
+    import laplacianformer_amd as lf
+
+    for n in (10, 63, 65):
+        with pytest.raises(ValueError, match="no square"):
+            lf.AttentionBlock(8, 2)(torch.randn(1, n, 8))
+        with pytest.raises(ValueError, match="no square"):
+            lf.AttentionBlock(8, 2, attention="laplacian", positions=False)(torch.randn(1, n, 8))
+        x, k = torch.randn(1, n, 8), torch.ones(1, dtype=torch.int32)
+        for fn in (lambda: lf.AttentionBlock(8, 2, causal=True)(x), lambda: lf.AttentionBlock(8, 2)(x, lengths=k),
+                   lambda: lf.AttentionBlock(8, 2, positions=False)(x), lambda: lf.AttentionBlock(8, 2)(x, grid=(1, n)),
+                   lambda: lf.AttentionBlock(8, 2)(x, positions=torch.zeros(1, n, dtype=torch.int32))):
+            with pytest.raises(RuntimeError, match="must be on GPU"):
+                fn()

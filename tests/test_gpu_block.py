@@ -438,3 +438,28 @@ def test_attention_blocks_under_autocast(gpu, amp, attention):
         assert i == 0 or a.dtype == torch.float32
         err = (a.double() - w.double()).norm() / w.double().norm()
         assert err <= tol, (i, err.item(), tol)
+
+
+def test_block_prefixes_across_square_counts(gpu):
+    """Without a grid a causal block gives a prefix the outputs that it has in the longer sequence, and a padded batch
+    those of any padding, whether or not a token count is a square's. Sums in another order only: fp32, and the
+    products' bound of test_attention_block."""
+    import laplacianformer_amd as lf
+
+    torch.manual_seed(8)
+    x = gen((2, 65, 48), 95, "f32").to(gpu)
+    tol = 400 * bc.U32
+    causal = lf.AttentionBlock(48, 3, causal=True).to(gpu)
+    plain = lf.AttentionBlock(48, 3).to(gpu)
+    lengths = torch.tensor([48, 31], dtype=torch.int32, device=gpu)
+    with torch.no_grad():
+        want, padded = causal(x)[0], plain(x, lengths=lengths)[0]
+        for n in (48, 49, 50, 63, 64):
+            print("prefix", n, flush=True)
+            got = causal(x[:, :n])[0]
+            assert (got - want[:, :n]).norm() <= tol * want[:, :n].norm(), n
+            got = plain(x[:, :n], lengths=lengths)[0]
+            for b, m in enumerate(lengths.tolist()):
+                assert (got[b, :m] - padded[b, :m]).norm() <= tol * padded[b, :m].norm(), (n, b)
+        square = plain(x[:, :64])[0]
+        assert torch.equal(square, plain(x[:, :64], grid=(8, 8))[0])
