@@ -135,6 +135,8 @@ class AttentionBlock(torch.nn.Module):
         ``mask`` and ``lengths`` (int32 [B], the tokens that each sequence has) go to softmax_attention."""
         B, N, C = x.shape
         d = C // self.heads
+        if self.attention == "laplacian" and (mask is not None or lengths is not None):
+            raise ValueError("laplacian attention takes neither mask nor lengths")
         if grid is None and (self.attention == "laplacian" or self.positions and positions is None):
             side = math.isqrt(N)
             if self.causal or lengths is not None:
@@ -142,9 +144,11 @@ class AttentionBlock(torch.nn.Module):
             elif side * side == N:
                 grid = (side, side)
             else:
-                raise ValueError(f"N={N} tokens are no square: their grid or positions are needed")
+                raise ValueError(f"N={N} tokens are no square: their grid is missing")
         if grid is not None and math.prod(grid) != N:
             raise ValueError(f"token grid {tuple(grid)} does not match N={N}")
+        if self.attention == "laplacian" and (len(grid) != 2 or any(n % self.pool for n in grid)):
+            raise ValueError(f"laplacian attention pools a grid of two axes by {self.pool}, not {tuple(grid)}")
         if residual is None:
             y, total = add_rms_norm(x, self.weight, eps=self.eps), x
         else:
@@ -161,8 +165,6 @@ class AttentionBlock(torch.nn.Module):
         if self.attention == "softmax":
             o = softmax_attention(q, k, v, mask=mask, causal=self.causal, k_lengths=lengths, q_lengths=lengths)
         else:
-            if mask is not None or lengths is not None:
-                raise ValueError("laplacian attention takes neither mask nor lengths")
             o = laplacian_attention(q.contiguous(), k.contiguous(), v.contiguous(), grid=tuple(grid), pool=self.pool,
                                     iters=self.iters)
         return self.proj(o.transpose(1, 2).reshape(B, N, C)), total

@@ -181,3 +181,20 @@ def test_block_infers_no_axes_from_a_token_count():
                    lambda: lf.AttentionBlock(8, 2)(x, positions=torch.zeros(1, n, dtype=torch.int32))):
             with pytest.raises(RuntimeError, match="must be on GPU"):
                 fn()
+
+
+def test_laplacian_block_refuses_grids_before_any_kernel():
+    """The Laplacian attention pools two axes: other grids, and masks or lengths, raise by name."""
+    import laplacianformer_amd as lf
+
+    block = lf.AttentionBlock(8, 2, attention="laplacian", pool=2)
+    x = torch.randn(1, 64, 8)
+    for grid in ((64,), (4, 4, 4), (1, 64), (64, 1)):
+        with pytest.raises(ValueError, match="two axes"):
+            block(x, grid=grid)
+    for kw in ({"mask": torch.ones(64, 64, dtype=torch.bool)}, {"lengths": torch.ones(1, dtype=torch.int32)}):
+        with pytest.raises(ValueError, match="neither mask"):
+            block(x, **kw)
+    for kw in ({}, {"grid": (4, 16)}):
+        with pytest.raises(RuntimeError, match="must be on GPU"):
+            block(x, **kw)
