@@ -141,6 +141,13 @@ namespace {
 // [B, heads, tokens, channels] with adjacent channels.
 Tensor unit_last(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
+// An output in t's order of dimensions, its channels adjacent: empty_like alone takes the channels of windows
+// into one row (tokens and channels both one element apart, fewer tokens than channels) for the outer dimension.
+Tensor output_like(const Tensor& t) {
+  const Tensor out = at::empty_like(t);
+  return out.size(-1) <= 1 || out.stride(-1) == 1 ? out : at::empty(t.sizes(), t.options());
+}
+
 }  // namespace
 
 std::vector<Tensor> Rotary(const Tensor q, const OptTensor k, const Tensor positions, const std::vector<int64_t> sections,
@@ -167,7 +174,7 @@ std::vector<Tensor> Rotary(const Tensor q, const OptTensor k, const Tensor posit
   const int64_t ps[3] = {positions.stride(0), positions.dim() == 3 ? positions.stride(1) : 0, positions.stride(-1)};
   at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   const Tensor qi = unit_last(q), ki = has_k ? unit_last(*k) : Tensor();
-  Tensor qo = at::empty_like(qi), ko = has_k ? at::empty_like(ki) : Tensor();
+  Tensor qo = output_like(qi), ko = has_k ? output_like(ki) : Tensor();
   detail::check_status(lfamd_rotary(dt, ptr(qi), qi.strides().data(), ptr(qo), qo.strides().data(), q.size(1), ptr(ki),
                                     has_k ? ki.strides().data() : nullptr, ptr(ko), has_k ? ko.strides().data() : nullptr,
                                     has_k ? k->size(1) : 0, B, N, D, ptr(positions), positions.scalar_type() == at::kLong,
@@ -249,7 +256,7 @@ std::vector<Tensor> SoftmaxAttention_forward(const Tensor q, const Tensor k, con
                                              const OptTensor q_starts, double scale, bool need_stats) {
   AttnIn in = attn_in("softmax_attention", q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale);
   at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
-  Tensor out = at::empty_like(in.q), stats, ws;
+  Tensor out = output_like(in.q), stats, ws;
   set_strides(in.d.out_strides, out);
   if (need_stats)
     stats = at::empty({(int64_t)lfamd_softmax_attention_stats_size(in.dt, &in.d) / 4}, q.options().dtype(at::kFloat));
@@ -277,8 +284,8 @@ std::vector<Tensor> SoftmaxAttention_backward(const Tensor grad_out, const Tenso
   set_strides(in.d.out_strides, o);
   Tensor dq, dk, dv;
   lfamd_attention_grads gr{};
-  if (need_q) dq = at::empty_like(in.q);
-  if (need_kv) dk = at::empty_like(in.k), dv = at::empty_like(in.v);
+  if (need_q) dq = output_like(in.q);
+  if (need_kv) dk = output_like(in.k), dv = output_like(in.v);
   gr.grad_out = ptr(g);
   set_strides(gr.grad_out_strides, g);
   if (need_q) gr.grad_q = ptr(dq), set_strides(gr.grad_q_strides, dq);

@@ -385,3 +385,26 @@ def test_refusals(gpu):
     for kw, msg in bad:
         with pytest.raises(RuntimeError, match=msg):
             lf.softmax_attention(**kw)
+
+
+@pytest.mark.parametrize("d", [20, 64])
+def test_windows_into_one_row(gpu, d):
+    """Tokens that are windows one element apart into a row, fewer than channels: tokens and channels have the same
+    stride. Outputs and gradients have places of their own, and the bits of a copy's."""
+    import laplacianformer_amd as lf
+
+    print(f"softmax attention windows {d}", flush=True)
+    N = d // 2 + 1
+    rows = [gen((2, 3, N + d - 1), 170 + i, "bf16").to(gpu) for i in range(4)]
+    q, k, v, g = (r.unfold(-1, d, 1) for r in rows)
+    assert q.shape == (2, 3, N, d) and q.stride()[2:] == (1, 1) and torch.empty_like(q).stride(3) != 1
+    pos = torch.arange(N, dtype=torch.int32, device=gpu)[None]
+
+    def step(q, k, v, g):
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        a, b = lf.rotary(q, k, pos, [d // 2])
+        out = lf.softmax_attention(q, k, v, causal=True)
+        return [a, b, out, *torch.autograd.grad(out, (q, k, v), g), *torch.autograd.grad((a, b), (q, k), (g, g))]
+
+    for x, y in zip(step(q, k, v, g), step(*(t.contiguous() for t in (q, k, v, g)))):
+        assert x.stride(3) == 1 and torch.equal(x, y)
