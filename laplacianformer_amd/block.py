@@ -52,6 +52,8 @@ def rotary_sections(head_dim: int, axes: int) -> list[int]:
 def grid_positions(grid: Sequence[int], device=None, start: Sequence[int] | None = None) -> torch.Tensor:
     """int32 ``[axes, tokens]``: the coordinates of a row-major token grid (height x width,
     time x height x width, ...), axis a counted from ``start[a]`` (default 0)."""
+    if start is not None and len(start) != len(grid):
+        raise ValueError(f"a grid of {len(grid)} axes takes as many starts, not {len(start)}")
     axes = [torch.arange(s, s + n, dtype=torch.int32, device=device)
             for n, s in zip(grid, start if start is not None else [0] * len(grid))]
     return torch.stack([a.reshape(-1) for a in torch.meshgrid(*axes, indexing="ij")])

@@ -198,3 +198,13 @@ def test_laplacian_block_refuses_grids_before_any_kernel():
     for kw in ({}, {"grid": (4, 16)}):
         with pytest.raises(RuntimeError, match="must be on GPU"):
             block(x, **kw)
+
+
+def test_grid_positions_refuse_missing_starts():
+    """A start per axis: with fewer, the axes behind them were dropped, and with them their tokens."""
+    import laplacianformer_amd as lf
+
+    for start in ((5,), (1, 2, 3), ()):
+        with pytest.raises(ValueError, match="as many starts"):
+            lf.grid_positions((2, 3), start=start)
+    assert lf.grid_positions((2, 3), start=[0, 7])[1].tolist() == [7, 8, 9, 7, 8, 9]
