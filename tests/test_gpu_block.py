@@ -463,3 +463,30 @@ def test_block_prefixes_across_square_counts(gpu):
                 assert (got[b, :m] - padded[b, :m]).norm() <= tol * padded[b, :m].norm(), (n, b)
         square = plain(x[:, :64])[0]
         assert torch.equal(square, plain(x[:, :64], grid=(8, 8))[0])
+
+
+@pytest.mark.parametrize("width", [5, 64, 333, 1024, 2056, 4096, 8192, 16381, 16384])
+def test_norm_backward_of_fp32_addends(gpu, width):
+    """The C entry's fp32 backward from both addends, which the autograd node leaves to the stored sum."""
+    import ctypes
+
+    import laplacianformer_amd as lf
+
+    print(f"norm backward fp32 addends {width}", flush=True)
+    lib, rows = lf.capi(), 37
+    x, res, gy, gs = (gen((rows, width), 100 + i, "f32") for i in range(4))
+    w = 1 + 0.2 * gen((width,), 104, "f32")
+    ref = bc.rms_norm(x, w, res, 1e-5, gy, gs)
+    t = [a.to(gpu) for a in (x, res, gy, gs, w)]
+    y, total, dx, dw = (torch.empty_like(a) for a in (t[0], t[0], t[0], t[4]))
+    rstd = torch.empty(rows, device=gpu)
+    p = lambda a: ctypes.c_void_p(a.data_ptr())
+    st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    lf.check(lib.lfamd_add_rms_norm(0, p(t[0]), width, p(t[1]), width, 0, p(t[4]), p(y), p(total), p(rstd), rows, width, 1e-5, st))
+    n = lib.lfamd_add_rms_norm_backward_workspace_size(0, rows, width)
+    ws = torch.empty(n, dtype=torch.uint8, device=gpu)
+    lf.check(lib.lfamd_add_rms_norm_backward(0, p(t[2]), width, p(t[3]), width, p(t[0]), width, p(t[1]), width, 0, p(t[4]), p(rstd),
+                                             p(dx), p(dw), rows, width, p(ws), n, st))
+    torch.cuda.synchronize()
+    for name, got in (("y", y), ("sum", total), ("dx", dx), ("dw", dw)):
+        bc.assert_within(got, *ref[name], (width, name))

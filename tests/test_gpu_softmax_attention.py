@@ -408,3 +408,36 @@ def test_windows_into_one_row(gpu, d):
 
     for x, y in zip(step(q, k, v, g), step(*(t.contiguous() for t in (q, k, v, g)))):
         assert x.stride(3) == 1 and torch.equal(x, y)
+
+
+def _splits_keys(q, k, kw):
+    """Whether the forward of this call splits its keys: its workspace holds more than a mask's bits."""
+    import ctypes
+
+    import laplacianformer_amd as lf
+    import laplacianformer_amd._lib as L
+
+    assert "mask" not in kw or kw["mask"].dtype != torch.bool
+    kind = {None: 0, torch.float32: 2, torch.float16: 3, torch.bfloat16: 4}[kw["mask"].dtype if "mask" in kw else None]
+    B, H, N, d = q.shape
+    desc = L.Attention(batch=B, heads=H, kv_heads=k.shape[1], q_len=N, k_len=k.shape[2], head_dim=d, scale=1.0, mask_kind=kind)
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[q.dtype]
+    return lf.capi().lfamd_softmax_attention_workspace_size(code, ctypes.byref(desc)) > 0
+
+
+@pytest.mark.parametrize("mode", ["plain", "bias", "lengths", "causal_lengths"])
+@pytest.mark.parametrize("d", [24, 64, 80, 128])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_split_keys_of_many_rows(gpu, dtype, d, mode):
+    """More rows than eight workgroups per CU join, each with a few of a workgroup's threads, over keys that are split;
+    lengths leave some splits, and a whole sequence, without keys."""
+    print(f"softmax attention split rows {dtype} {d} {mode}", flush=True)
+    shape = (4, 4, 4, 160, 1000, d)
+    q, k, v, g, kw = make(shape, mode, dtype, 180)
+    if "lengths" in mode:
+        kw["k_lengths"] = torch.tensor([1000, 37, 0, 500], dtype=torch.int32)
+        kw["q_lengths"] = torch.tensor([160, 160, 160, 90], dtype=torch.int32)
+        if mode == "causal_lengths":
+            kw["q_starts"] = kw["k_lengths"] - 160
+    assert 4 * 4 * 160 > 8 * torch.cuda.get_device_properties(gpu).multi_processor_count and _splits_keys(q, k, kw)
+    check(call(gpu, q, k, v, g, kw), reference(q, k, v, g, kw), (dtype, d, mode))
