@@ -34,7 +34,9 @@ template <typename T, int DC> constexpr int query_tile() { return DC < 96 && (si
 template <typename T, int DC> constexpr int key_tile() { return sizeof(T) == 2 || DC == 32 ? 64 : 32; }
 
 // At 128 channels the accumulators of dk and dv and both owned operands are more than a lane's
-// registers at two waves per SIMD (128 + 64 + 64 with the scores): V is read from LDS then.
+// registers at two waves per SIMD (128 + 64 + 64 with the scores): V is read from LDS then. That leaves the 16-bit
+// forms still above the 256: 48 to 84 bytes a lane in scratch, part of them written and read in the loop (140 to 152
+// with an additive mask, whose 16 values are held across the products, and 28 to 36 with one at 96 channels).
 template <int DC> constexpr bool v_in_lds() { return DC >= 128; }
 
 // Bytes of a streamed query's statistics: lse, delta, 1 / sum and last key, or its bits of the 128 keys.

@@ -9,8 +9,9 @@
 // given (16-bit types: a quarter more to move, and gradients 1.4 times as exact, as the stored
 // sum's half step would enter n beside the gradients' own rounding: dw of 2048 x 16000 bf16
 // 93 us and 1.6e-3 off, from the stored sum 72 us and 2.4e-3; equal times at 4096 x 4096).
-// gn is formed twice rather than held, which keeps 8192 columns and more in 128 registers
-// (104 -> 93 us, fp32 159 -> 145). The backward's workgroups walk the rows with a
+// gn is formed twice rather than held: beyond 8192 columns, where 1024 threads have 128 registers each, fewer
+// values go through scratch (104 -> 93 us, fp32 159 -> 145; fp32 still keeps 60 bytes a thread there, 128 from
+// addends, and fp16 and bf16 from addends 44 and 12). The backward's workgroups walk the rows with a
 // fixed stride, keep their share of dw in registers, and write one fp32 partial row
 // each; a second kernel adds those in their order, so the same call gives the same bits.
 // Measured on one MI355X: 16384 x 4096 bf16 to 8 bits 88 us (470 MB, 5.3 TB/s, the rate of a large copy); 12544 x 333
@@ -301,7 +302,7 @@ struct NormPlan {
 };
 
 // Threads per row and 16-byte vectors per thread, for at most 16 elements each (the backward
-// holds four values per element). One wave per row while that holds the row, as a wave
+// holds the weight, dw and n of each in fp32, and its inputs packed). One wave per row while that holds the row, as a wave
 // reduces without barriers; then the smallest workgroup that does.
 NormPlan norm_plan(int dtype, int width) {
   const int V = dtype == LFAMD_F32 ? 4 : 8, most = 16 / V, units = (width + V - 1) / V;

@@ -136,3 +136,34 @@ def test_fit_rule_on_the_probe_shape(tmp_path):
     r = subprocess.run(base + ["-Werror=inline-asm", "-o", str(tmp_path / "probe2.o")], capture_output=True,
                        text=True)
     assert r.returncode != 0 and "reserved registers" in r.stderr
+
+
+# Scratch bytes per lane of the transformer-block kernels that do not fit their registers: 1024 threads
+# have 128 each, two workgroups of 256 per CU 256. (kernel, type, its integer arguments): the most that it may take.
+SCRATCH = {
+    ("add_rms_norm_bwd_kernel", "f", (1024, 4, 0)): 60, ("add_rms_norm_bwd_kernel", "f", (1024, 4, 1)): 128,
+    ("add_rms_norm_bwd_kernel", "f16s", (1024, 2, 1)): 44, ("add_rms_norm_bwd_kernel", "bf16s", (1024, 2, 1)): 12,
+    ("attn_fwd_kernel", "f", (64, 1, 1)): 20,
+    ("attn_fwd_kernel", "f16s", (128, 1, 1)): 12, ("attn_fwd_kernel", "bf16s", (128, 1, 1)): 12,
+    ("attn_dkdv_kernel", "f16s", (96, 1)): 36, ("attn_dkdv_kernel", "bf16s", (96, 1)): 28,
+    ("attn_dkdv_kernel", "f16s", (128, 0)): 48, ("attn_dkdv_kernel", "bf16s", (128, 0)): 60,
+    ("attn_dkdv_kernel", "f16s", (128, 2)): 84, ("attn_dkdv_kernel", "bf16s", (128, 2)): 76,
+    ("attn_dkdv_kernel", "f16s", (128, 1)): 152, ("attn_dkdv_kernel", "bf16s", (128, 1)): 140,
+    ("attn_dq_kernel", "f16s", (128, 1)): 20, ("attn_dq_kernel", "bf16s", (128, 1)): 20,
+}
+
+
+def test_block_kernels_scratch(tmp_path):
+    """Every other kernel of the transformer-block operators keeps to its registers, and these to their scratch."""
+    seen, over = set(), []
+    for k in _kernels(tmp_path):
+        m = re.search(r"\d(attn_[a-z]+_kernel|add_rms_norm(?:_bwd)?_kernel|rotary_kernel|norm_dw_kernel)(?:I(f|NS_\d+(b?f16s)E)((?:L[ib]\d+E)*)E)?",
+                      k["name"])
+        if not m:
+            continue
+        key = (m[1], m[3] or m[2], tuple(int(x) for x in re.findall(r"L[ib](\d+)E", m[4] or "")))
+        seen.add(key)
+        if int(k.get("private_segment_fixed_size", 0)) > SCRATCH.get(key, 0):
+            over.append((key, k["private_segment_fixed_size"]))
+    assert not over, over
+    assert len(seen) >= 250 and set(SCRATCH) <= seen
