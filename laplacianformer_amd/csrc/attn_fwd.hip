@@ -537,7 +537,7 @@ size_t attn_bits_bytes(const AttnArgs& a) {
 }
 
 int attn_pack_bits(AttnArgs& a, void* workspace, hipStream_t st) {
-  if (a.maskKind != kMaskBool || a.M == 0 || a.N == 0) return LFAMD_OK;
+  if (a.maskKind != kMaskBool) return LFAMD_OK;
   const BitsShape s = bits_shape(a);
   a.bits = (uint32_t*)workspace;
   a.bs[0] = s.B > 1 ? s.H * s.N * s.words : 0;

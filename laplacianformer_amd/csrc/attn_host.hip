@@ -54,9 +54,11 @@ AttnArgs make_args(const lfamd_attention* d) {
     a.qs[i] = d->q_strides[i], a.ks[i] = d->k_strides[i], a.vs[i] = d->v_strides[i], a.os[i] = d->out_strides[i];
   }
   a.klen = d->k_lengths, a.qlen = d->q_lengths, a.qstart = d->q_starts;
-  a.mask = d->mask, a.maskKind = d->mask_kind, a.causal = d->causal != 0;
+  // Without a query or a key no mask is read, not even for which keys take part: its pointer may be null.
+  const int kind = a.N && a.M ? d->mask_kind : LFAMD_MASK_NONE;
+  a.mask = d->mask, a.maskKind = kind, a.causal = d->causal != 0;
   for (int i = 0; i < 4; ++i) a.ms[i] = d->mask_strides[i];
-  a.keyMask = d->mask_kind && d->mask_strides[1] == 0 && d->mask_strides[2] == 0;
+  a.keyMask = kind && d->mask_strides[1] == 0 && d->mask_strides[2] == 0;
   a.scale = d->scale, a.c = d->scale * kLog2e;
   a.divN = FastDiv((uint32_t)std::max(a.N, 1));
   return a;

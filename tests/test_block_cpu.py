@@ -208,3 +208,15 @@ def test_grid_positions_refuse_missing_starts():
         with pytest.raises(ValueError, match="as many starts"):
             lf.grid_positions((2, 3), start=start)
     assert lf.grid_positions((2, 3), start=[0, 7])[1].tolist() == [7, 8, 9, 7, 8, 9]
+
+
+def test_no_mask_is_planned_without_queries_or_keys(lib):
+    """A call without queries, or without keys, may come with an empty mask, whose pointer is null, and strides of 0,
+    which say that the mask is the same for every query: it is taken as a call without a mask throughout."""
+    fwd, bwd, stats = (lib.lfamd_softmax_attention_workspace_size, lib.lfamd_softmax_attention_backward_workspace_size,
+                       lib.lfamd_softmax_attention_stats_size)
+    for sizes in ({"q_len": 0}, {"k_len": 0}, {"q_len": 0, "k_len": 0}):
+        for kind in (1, 2, 3, 4):
+            for dt in (0, 1, 2):
+                for f in (fwd, bwd, stats):
+                    assert f(dt, ctypes.byref(desc(mask_kind=kind, **sizes))) == f(dt, ctypes.byref(desc(**sizes)))

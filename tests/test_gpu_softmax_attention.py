@@ -441,3 +441,24 @@ def test_split_keys_of_many_rows(gpu, dtype, d, mode):
             kw["q_starts"] = kw["k_lengths"] - 160
     assert 4 * 4 * 160 > 8 * torch.cuda.get_device_properties(gpu).multi_processor_count and _splits_keys(q, k, kw)
     check(call(gpu, q, k, v, g, kw), reference(q, k, v, g, kw), (dtype, d, mode))
+
+
+@pytest.mark.parametrize("d", [16, 128])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_empty_masks(gpu, dtype, d):
+    """No queries or no keys, with masks expanded to that: empty tensors of strides 0. The others' gradients are 0."""
+    import laplacianformer_amd as lf
+
+    print(f"softmax attention empty masks {dtype} {d}", flush=True)
+    t = TORCH_DT[dtype]
+    for N, M in ((0, 150), (5, 0), (0, 0)):
+        ones = torch.ones(2, 1, 1, min(M, 1) * M, device=gpu)
+        for mask in (ones.bool(), ones, ones.to(t)):
+            mask = mask.expand(2, 4, N, M)
+            assert mask.numel() == 0
+            q = torch.randn(2, 4, N, d, dtype=t, device=gpu, requires_grad=True)
+            k, v = (torch.randn(2, 2, M, d, dtype=t, device=gpu, requires_grad=True) for _ in range(2))
+            out = lf.softmax_attention(q, k, v, mask=mask, k_lengths=torch.tensor([M, 3], dtype=torch.int32, device=gpu))
+            grads = torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+            torch.cuda.synchronize()
+            assert bool((out == 0).all()) and all(bool((x == 0).all()) for x in grads)
