@@ -24,7 +24,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
 
     ``sum = x + residual``, ``y = sum / sqrt(mean(sum^2) + eps) * weight`` (statistics of the
     float32 sum). Returns ``(y, sum)`` in x's type, which is the residual's too, or ``y`` alone without a residual.
-    ``weight`` has x's type or float32; the last dimension is at most 16384. With autograd.
+    ``weight`` has x's type or float32; the last dimension is at most 16384. With autograd, which keeps x (and
+    in 16-bit types the residual, for the unrounded sum; in float32 the sum in their place) for the backward.
     """
     out = ext().AddRmsNorm(x, weight, residual, eps)
     return out[0] if residual is None else tuple(out)
@@ -88,11 +89,13 @@ def softmax_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: t
     tokens over a cache filled to uneven lengths, ``q_starts = k_lengths - N``. ``scale``
     (positive) defaults to ``1 / sqrt(d)``.
 
-    A query that nothing is left for gives 0. Keys that ``k_lengths``, or a mask that is the
-    same for every head and query, takes out may hold anything, as may queries from ``q_lengths[b]`` on;
+    A query that nothing is left for gives 0. Keys that ``k_lengths``, or a mask that is broadcast
+    over heads and queries, takes out may hold anything, as may queries from ``q_lengths[b]`` on;
     elsewhere masked keys and values (and queries and output gradients) have to be finite, as a probability of
     0 is multiplied by them. 16-bit types round the
-    probabilities to that type in front of the product with v. With autograd.
+    probabilities to that type in front of the product with v. With autograd, which keeps, beside the
+    inputs, the output and a number per row (two with an additive mask), in 16-bit types what the
+    output's rounding took off: a second tensor of its size.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.shape[-1] else 1.0
@@ -107,7 +110,8 @@ class AttentionBlock(torch.nn.Module):
     ``(out, sum)``: the next block's ``(x, residual)``, also under autocast, where out is of 16 bits and the
     sum stays float32 (x and residual of different types are widened to the wider one). ``attention`` is "softmax"
     (softmax_attention, ``kv_heads`` key heads shared by ``heads`` query heads) or
-    "laplacian" (laplacian_attention with ``pool`` and ``iters``, one key head per query head).
+    "laplacian" (laplacian_attention with ``pool`` and ``iters``, one key head per query head, a grid of two
+    axes). Caches of keys and the 8-bit norm are for callers of the functions: the block takes neither.
     """
 
     def __init__(self, dim: int, heads: int, kv_heads: int | None = None, attention: str = "softmax",

@@ -526,8 +526,8 @@ template <typename LD> __device__ __forceinline__ uint32_t live_keys(const AttnA
 // least of what the busiest CU takes and of joining. A workgroup alone takes `lat` us per tile (one wave
 // per SIMD waits for its own reads, products and exponentials in turn), workgroups that share a CU `thr`
 // each, and 4 us go to a start and an end; n pieces of `bytes` are written and read at 4 TB/s, behind a
-// launch of 6 us. At most 64 pieces: that bounds the workspace, and leaves a call of one or two workgroups per
-// piece with as many CUs. `steps` are the buffer's: lengths are known to the device alone, and the pieces behind
+// launch of 6 us. At most 64 pieces, which bounds the workspace; a call of one workgroup then uses 64 CUs
+// (one token over 131072 keys of 128 channels: 31 us). `steps` are the buffer's: lengths are known to the device alone, and the pieces behind
 // a short sequence's end are written and joined empty.
 inline int best_split(int64_t wgs, int64_t steps, int cus, double lat, double thr, double bytes) {
   int best = 1;

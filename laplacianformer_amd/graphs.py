@@ -20,7 +20,9 @@ class GraphedStep:
     After construction ``out`` is the captured forward result and ``grads`` the
     inputs' gradients; ``replay()`` re-runs the step on whatever the static
     ``inputs`` and ``grad_out`` tensors hold at that time and overwrites ``out``
-    and ``grads`` in place (gradients are not accumulated across replays).
+    and ``grads`` in place (gradients are not accumulated across replays). While it is captured no eager
+    result that leads back to the same leaves, inputs or parameters, may be alive: their accumulation
+    would belong to another stream, which a capture must not join.
     """
 
     def __init__(self, fn: Callable[..., torch.Tensor], inputs: Sequence[torch.Tensor], grad_out: torch.Tensor,
