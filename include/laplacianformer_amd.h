@@ -404,6 +404,54 @@ int lfamd_softmax_attention_backward(int dtype, const lfamd_attention* desc, con
                                      const void* out, const float* stats, const lfamd_attention_grads* grads,
                                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* Causal linear attention with a decay for each head, and its state: with a = exp(log_decay[h]),
+ *   S_t = a S_(t-1) + k_t v_t^T (S_(-1) = state),  out_t = scale S_t^T q_t.
+ * query [batch][heads][tokens][key_dim], key [batch][kv_heads][tokens][key_dim], value and out
+ * [batch][kv_heads or heads][tokens][value_dim], heads a multiple of kv_heads (query head i reads key
+ * head i / (heads / kv_heads)); strides in elements for batch, head and token, channels adjacent.
+ * States are fp32, contiguous [batch][heads][key_dim][value_dim]. Both sizes of a head at most 128,
+ * tokens <= 2^29, batch * heads <= 4194303.
+ *   log_decay  [heads] fp32, at most 0 (-inf: a token sees itself alone); not read by the host
+ *   lengths    [batch] or NULL: tokens at or behind it are not read, their output is 0 and the state
+ *              does not see them. Clamped to the buffer.
+ *   scale      positive and finite */
+typedef struct {
+  int64_t batch, heads, kv_heads, tokens, key_dim, value_dim;
+  int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];
+  const float* log_decay;
+  const int32_t* lengths;
+  float scale;
+} lfamd_decay;
+
+/* state may be NULL (zero), and so may last_state, which takes the state behind the last token and may be
+ * state itself. The workspace (16-byte aligned; 0 bytes where the heads alone fill the chip) holds the
+ * states of the segments that long sequences are cut into. Deterministic. */
+size_t lfamd_decay_attention_workspace_size(int dtype, const lfamd_decay* desc);
+int lfamd_decay_attention(int dtype, const lfamd_decay* desc, const void* q, const void* k, const void* v, const float* state,
+                          void* out, float* last_state, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients from the forward's inputs; nothing else is kept. grad_last_state NULL: zero. grad_q, grad_k and
+ * grad_v together, and grad_state (with the two; fp32, like the states) may be NULL. Deterministic,
+ * without atomics; heads that share a key head are added in fp32. log_decay has no gradient. */
+typedef struct {
+  const void* grad_out;
+  const float* grad_last_state;
+  void* grad_q;
+  void* grad_k;
+  void* grad_v;
+  float* grad_state;
+  int64_t grad_out_strides[3], grad_q_strides[3], grad_k_strides[3], grad_v_strides[3];
+} lfamd_decay_grads;
+size_t lfamd_decay_attention_backward_workspace_size(int dtype, const lfamd_decay* desc);
+int lfamd_decay_attention_backward(int dtype, const lfamd_decay* desc, const void* q, const void* k, const void* v,
+                                   const float* state, const lfamd_decay_grads* grads, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* One new token (tokens = 1; lengths is not read): the state is updated in place. Its strides of batch and
+ * head are in elements, [key_dim][value_dim] contiguous; no two states may overlap. */
+int lfamd_decay_attention_step(int dtype, const lfamd_decay* desc, const void* q, const void* k, const void* v, void* out,
+                               float* state, const int64_t* state_strides, void* stream);
+
 /* ---- Runtime ------------------------------------------------------------ */
 
 /* HIP runtime version as major*100 + minor (e.g. 700 for 7.0), the convention

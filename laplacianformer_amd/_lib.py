@@ -67,6 +67,11 @@ CAPI_PROTOTYPES = [
     ("lfamd_softmax_attention", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     ("lfamd_softmax_attention_backward_workspace_size", _SZ, [_I, _P]),
     ("lfamd_softmax_attention_backward", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    ("lfamd_decay_attention_workspace_size", _SZ, [_I, _P]),
+    ("lfamd_decay_attention", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    ("lfamd_decay_attention_backward_workspace_size", _SZ, [_I, _P]),
+    ("lfamd_decay_attention_backward", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    ("lfamd_decay_attention_step", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _P]),
     ("lfamd_runtime_version", _I, []),
     ("lfamd_status_string", ctypes.c_char_p, [_I]),
     ("lfamd_last_error", ctypes.c_char_p, []),
@@ -87,6 +92,21 @@ class AttentionGrads(ctypes.Structure):
     """lfamd_attention_grads of include/laplacianformer_amd.h."""
 
     _fields_ = [(n, _P) for n in ("grad_out", "grad_q", "grad_k", "grad_v")] + \
+        [(n, _I64 * 3) for n in ("grad_out_strides", "grad_q_strides", "grad_k_strides", "grad_v_strides")]
+
+
+class Decay(ctypes.Structure):
+    """lfamd_decay of include/laplacianformer_amd.h."""
+
+    _fields_ = [(n, _I64) for n in ("batch", "heads", "kv_heads", "tokens", "key_dim", "value_dim")] + \
+        [(n, _I64 * 3) for n in ("q_strides", "k_strides", "v_strides", "out_strides")] + \
+        [("log_decay", _P), ("lengths", _P), ("scale", ctypes.c_float)]
+
+
+class DecayGrads(ctypes.Structure):
+    """lfamd_decay_grads of include/laplacianformer_amd.h."""
+
+    _fields_ = [(n, _P) for n in ("grad_out", "grad_last_state", "grad_q", "grad_k", "grad_v", "grad_state")] + \
         [(n, _I64 * 3) for n in ("grad_out_strides", "grad_q_strides", "grad_k_strides", "grad_v_strides")]
 
 

@@ -102,6 +102,42 @@ def softmax_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: t
     return ext().SoftmaxAttention(q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale)
 
 
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                    state: torch.Tensor | None = None, lengths: torch.Tensor | None = None, scale: float | None = None,
+                    return_state: bool = False):
+    """Causal linear attention whose memory decays, q ``[B, H, N, d]`` over k ``[B, Hk, N, d]``, v ``[B, Hk, N, e]`` ->
+    ``[B, H, N, e]``: with ``a = exp(log_decay[h])``, ``S_t = a S_(t-1) + k_t v_t^T``, ``out_t = scale S_t^T q_t``.
+
+    H is a multiple of Hk: query head ``h`` reads key head ``h // (H // Hk)``. d and e are at most 128.
+    ``log_decay`` is float32 ``[H]``, at most 0 (-inf: a token sees itself alone), without a gradient; nothing checks
+    its values. ``state`` is the S in front of the first token, float32 ``[B, H, d, e]`` (default: zero);
+    with ``return_state`` the result is ``(out, state behind the last token)``, from which the next
+    tokens go on, here or in decay_attention_step. ``lengths`` is int32 ``[B]``: tokens from ``lengths[b]`` on are not
+    read, give 0, and the state does not see them. ``scale`` (positive) defaults to ``1 / sqrt(d)``.
+
+    What is rounded between the products is carried in pieces: results are those of float32 arithmetic, rounded
+    once. Values in front of a length have to be finite: tiles of 32 tokens multiply zeros by
+    them. With autograd (q, k, v and state, through both results), which keeps the inputs alone.
+    """
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1]) if q.shape[-1] else 1.0
+    out = ext().DecayAttention(q, k, v, log_decay, state, lengths, scale, return_state)
+    return tuple(out) if return_state else out[0]
+
+
+def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor,
+                         scale: float | None = None) -> torch.Tensor:
+    """decay_attention for one new token (N = 1) without gradients: ``state`` is updated in place.
+
+    Each head's state has to be contiguous; sequences and heads may be apart (a part of a larger buffer).
+    """
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+        raise RuntimeError("decay_attention_step has no gradient: call it under torch.no_grad(), or decay_attention")
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1]) if q.shape[-1] else 1.0
+    return ext().DecayAttentionStep(q, k, v, log_decay, state, scale)
+
+
 class AttentionBlock(torch.nn.Module):
     """The attention half of a pre-norm transformer block on a token grid.
 

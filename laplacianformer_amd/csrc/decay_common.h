@@ -1,0 +1,444 @@
+// decay_attention: causal linear attention with a decay for each head,
+//   S_t = a S_(t-1) + k_t v_t^T,   out_t = scale S_t^T q_t,   a = exp(log_decay).
+//
+// Tiles of 32 tokens. With S the state in front of a tile and i, j its tokens,
+//   out_i = scale (a^(i+1) S^T q_i + sum over j <= i of a^(i-j) (q_i . k_j) v_j),
+//   S'    = a^32 S + sum over j of a^(31-j) k_j v_j^T.
+// A wave owns 32 value columns: their part of S stays in its accumulators from one tile to the
+// next (rows: key channels), and every product is on matrix cores:
+//   scores   P^T = K Q^T          rows j, columns i; every wave forms them, one 32 x 32 block
+//   memory   O^T = S^T Q^T        S goes from accumulators to operand within the lane
+//   inside   O^T += V^T P^T       likewise P
+//   state    S  += K^T (a^(31-j) V)   V's operand of the product above, scaled
+// so that nothing crosses lanes or waves, and the only barriers are those of the tiles' loads.
+//
+// Operands are of 16 bits where the inputs are, and whatever is rounded in front of a product (P, S,
+// the scaled V) is carried in two pieces x = hi + lo (V in bf16 in three), whose products the
+// accumulators add: results have the accuracy of 32-bit arithmetic, the state among them, which is
+// fp32. In fp16 the pieces are scaled by powers of two that keep both ends of the type's range away: P
+// for each query, S and V for each wave and tile.
+//
+// The gradients are the same operator on other operands: with g the gradient of out and S^T for S,
+//   dq = run(g, v, k) forwards;   dk = run(v, g, q),  dv = run(k, q, g) backwards in time,
+// the latter two from the gradient of the last state. Backwards, R stands behind a tile of c tokens,
+//   out_i = a^(c-1-i) R^T q_i + sum over j >= i of a^(j-i) scale (q_i . k_j) v_j,
+//   R'    = a^c R + scale sum over j of a^(j+1) k_j v_j^T.
+//
+// Where heads are few, a sequence is cut into segments: their own states first (decay_state kernel), those
+// joined in order (decay_join_kernel), then every segment from the state in front of it.
+#pragma once
+
+#include "attn_common.h"
+
+namespace lfamd {
+
+constexpr int kDecayTile = 32;
+constexpr int kDecayJobs = 3;
+
+// One run of the operator over every sequence and head.
+struct DecayJob {
+  const void *q, *k, *v;              // in their roles in this run
+  const float* first;                 // state in front (behind, if reverse), or null: zero
+  void* out;
+  float* last;                        // the state that it ends with, or null
+  float* seg;                         // [B H][nseg][dk][dv], see decay_join_kernel
+  int64_t qs[3], ks[3], vs[3], os[3]; // element strides of batch, head, token
+  int qg, kg, vg;                     // query heads per head of q, k, v
+  int dk, dv;
+  int reverse, outF32, firstT;        // firstT: first is [dv][dk]
+  int modeQ, modeK, modeV;            // LoadMode, kPlain or kAsync
+  float sp, so, sk;                   // scales of the scores, of the state's part and of what is added to the state
+};
+
+struct DecayArgs {
+  DecayJob job[kDecayJobs];
+  const float* logDecay;
+  const int32_t* lengths;
+  int B, H, N, jobs, nseg, segTiles;
+};
+
+// Pieces that a value is carried in.
+template <typename T> struct DecayPieces { static constexpr int P = 2, S = 2, V = 2; };
+template <> struct DecayPieces<bf16s> { static constexpr int P = 2, S = 2, V = 3; };
+template <> struct DecayPieces<float> { static constexpr int P = 1, S = 1, V = 1; };
+
+__device__ __forceinline__ int decay_length(const DecayArgs& a, int b) {
+  return a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
+}
+// exp(lg n) for whole n >= 0, of a log_decay of -inf too.
+__device__ __forceinline__ float decay_pow(float lg, int n) { return n == 0 ? 1.0f : expf(lg * (float)n); }
+// The same in 64 bits: the factor of a whole tile or segment, which powers are taken of.
+__device__ __forceinline__ float decay_pow64(float lg, int n) { return n == 0 ? 1.0f : (float)exp((double)lg * (double)n); }
+
+template <typename T> __device__ __forceinline__ float low_half(uint32_t w);
+template <typename T> __device__ __forceinline__ float high_half(uint32_t w);
+template <> __device__ __forceinline__ float low_half<bf16s>(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+template <> __device__ __forceinline__ float high_half<bf16s>(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+template <> __device__ __forceinline__ float low_half<f16s>(uint32_t w) { return to_acc(f16s{(uint16_t)w}); }
+template <> __device__ __forceinline__ float high_half<f16s>(uint32_t w) { return to_acc(f16s{(uint16_t)(w >> 16)}); }
+
+// Eight values as NP pieces of an operand.
+template <typename T, int NP> __device__ __forceinline__ void split_pieces(f32x8 x, Frag<T> (&f)[NP]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0].v = x;
+  } else {
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w = pack2<T>(x[2 * j], x[2 * j + 1]);
+        f[p].v[j] = w;
+        x[2 * j] -= low_half<T>(w);
+        x[2 * j + 1] -= high_half<T>(w);
+      }
+  }
+}
+
+template <typename T> __device__ __forceinline__ f32x8 frag_values(const Frag<T>& f) {
+  f32x8 x;
+  if constexpr (sizeof(T) == 4) {
+    x = f.v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[2 * j] = low_half<T>(f.v[j]), x[2 * j + 1] = high_half<T>(f.v[j]);
+  }
+  return x;
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) x = fmaxf(x, __shfl_xor(x, s));
+  return half_max(x);
+}
+
+// The tile of tokens t0 .. into LDS: Tile<T, DP>'s layout by THREADS threads, whole waves at a time.
+template <typename T, int DC, int THREADS> struct DecayLoader {
+  static constexpr int DP = row_pitch(DC);
+  using L = Tile<T, DP>;
+  static constexpr int CHUNKS = kDecayTile * L::CPR, NIT = (CHUNKS + THREADS - 1) / THREADS;
+  static_assert(CHUNKS % 64 == 0, "whole waves");
+
+  // first: the tile's first row (uniform); rows: how many of it exist.
+  static __device__ __forceinline__ void fill(char* tile, const T* first, int64_t stride, int rows, int D, int mode) {
+    const uint32_t rowBytes = (uint32_t)stride * (uint32_t)sizeof(T);
+    const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tile;
+    const int wave = uniform(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+      const int s = i * THREADS + (int)threadIdx.x;
+      if (CHUNKS % THREADS != 0 && i * THREADS + wave * 64 >= CHUNKS) break;
+      const int r = s / L::CPR, c = (s % L::CPR) ^ L::swz(r);
+      if (mode == kAsync) {
+        if (r < rows && c * L::CE < D)
+          load_to_lds<16>(first, (uint32_t)r * rowBytes + (uint32_t)c * 16, to + (i * THREADS + wave * 64) * 16);
+        else if (c * L::CE < DC)
+          *(u32x4*)(tile + s * 16) = (u32x4){0, 0, 0, 0};
+      } else {
+        *(u32x4*)(tile + s * 16) = load_chunk<T>(first + (int64_t)r * stride, r < rows, c * L::CE, D);
+      }
+    }
+  }
+};
+
+// Row lane % 32 of a tile, the channels of step t as acc_frag deals them.
+template <typename T, int DP> struct DealtRow {
+  using L = Tile<T, DP>;
+  static __device__ __forceinline__ int lane_offset(int lane) {
+    const int r = lane & 31, h = lane >> 5;
+    if constexpr (sizeof(T) == 2) return r * L::ROW + (L::swz(r) << 4) + 8 * h;
+    else return r * L::ROW + ((h ^ L::swz(r)) << 4);
+  }
+  static __device__ __forceinline__ Frag<T> read(const char* tile, int dl, int t) {
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const u32x2 y = *(const u32x2*)(tile + (dl ^ ((2 * t + u) << 4)));
+        f.v[2 * u] = y[0];
+        f.v[2 * u + 1] = y[1];
+      }
+    } else {
+      const f32x4 a = *(const f32x4*)(tile + (dl ^ ((4 * t) << 4)));
+      const f32x4 b = *(const f32x4*)(tile + (dl ^ ((4 * t + 2) << 4)));
+      f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    return f;
+  }
+};
+
+// Bytes of LDS: two buffers of the three tiles (of two, for the states alone).
+template <typename T, int DK, int DV, bool OUT> constexpr size_t decay_lds() {
+  return (size_t)2 * kDecayTile * ((OUT ? 2 : 1) * row_pitch(DK) + row_pitch(DV)) * sizeof(T);
+}
+
+// Grid: jobs x B H x segments. OUT: the outputs; otherwise the segments' own states only. DK, DV: channels
+// computed with; a wave for every 32 of DV.
+template <typename T, int DK, int DV, bool OUT>
+__global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) decay_kernel(const DecayArgs a) {
+  constexpr int THREADS = DV * 2, NT = DK / 16, ND = DK / 32, TILE = kDecayTile;
+  constexpr int NPP = DecayPieces<T>::P, NPS = DecayPieces<T>::S, NPV = DecayPieces<T>::V;
+  constexpr bool F16 = std::is_same<T, f16s>::value;
+  using LK = DecayLoader<T, DK, THREADS>;
+  using LV = DecayLoader<T, DV, THREADS>;
+  using TK = typename LK::L;
+  using TV = typename LV::L;
+  using DR = DealtRow<T, LK::DP>;
+  constexpr int BK = TILE * TK::ROW, BV = TILE * TV::ROW, BUF = (OUT ? 2 : 1) * BK + BV;
+  extern __shared__ __align__(16) char smem[];
+
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, i = lane & 31;
+  const uint32_t place = xcd_place(blockIdx.x, gridDim.x);
+  const int seg = uniform(place % a.nseg), rest = uniform(place / a.nseg), bh = uniform(rest % (a.B * a.H));
+  const DecayJob& jb = a.job[uniform(rest / (a.B * a.H))];
+  const int b = uniform(bh / a.H), hq = bh - b * a.H;
+  const bool rev = jb.reverse;
+  const float lg = a.logDecay[hq];
+  const int len = uniform(decay_length(a, b));
+  const int t0 = seg * a.segTiles * TILE, t1 = (int)min((int64_t)len, (int64_t)t0 + (int64_t)a.segTiles * TILE);  // its tokens
+  const int tiles = t1 > t0 ? (t1 - t0 + TILE - 1) / TILE : 0;
+  const int dk = jb.dk, dv = jb.dv;
+  const int c = 32 * wave + i;  // this lane's value column
+
+  const T* kp = uniform_ptr((const T*)jb.k + (int64_t)b * jb.ks[0] + (int64_t)uniform(hq / jb.kg) * jb.ks[1]);
+  const T* vp = uniform_ptr((const T*)jb.v + (int64_t)b * jb.vs[0] + (int64_t)uniform(hq / jb.vg) * jb.vs[1]);
+  const T* qp = OUT ? uniform_ptr((const T*)jb.q + (int64_t)b * jb.qs[0] + (int64_t)uniform(hq / jb.qg) * jb.qs[1]) : nullptr;
+  const int64_t ooff = (int64_t)b * jb.os[0] + (int64_t)hq * jb.os[1];
+
+  auto fill = [&](int buf, int n) {
+    const int at = t0 + (rev ? tiles - 1 - n : n) * TILE, rows = min(TILE, t1 - at);
+    char* to = smem + buf * BUF;
+    LK::fill(to, kp + (int64_t)at * jb.ks[2], jb.ks[2], rows, dk, jb.modeK);
+    LV::fill(to + BK, vp + (int64_t)at * jb.vs[2], jb.vs[2], rows, dv, jb.modeV);
+    if constexpr (OUT) LK::fill(to + BK + BV, qp + (int64_t)at * jb.qs[2], jb.qs[2], rows, dk, jb.modeQ);
+  };
+  if (tiles) fill(0, 0);
+
+  // The state's rows 32 m + 8 (r / 4) + 4 h + r % 4 of column c.
+  f32x16 st[ND];
+#pragma unroll
+  for (int m = 0; m < ND; ++m) st[m] = f32x16{};
+  const float* from = !OUT ? nullptr : a.nseg > 1 ? jb.seg + ((int64_t)bh * a.nseg + seg) * dk * dv
+                                     : jb.first ? jb.first + (int64_t)bh * dk * dv : nullptr;
+  if (from && c < dv) {
+    const bool tr = a.nseg == 1 && jb.firstT;
+#pragma unroll
+    for (int m = 0; m < ND; ++m)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = 32 * m + 8 * (r >> 2) + 4 * h + (r & 3);
+        if (d < dk) st[m][r] = from[tr ? c * dk + d : d * dv + c];
+      }
+  }
+
+  // Powers of the decay: of a score's distance (0 outside the triangle), of a token's to the state that it goes
+  // into, of the query's from the state in front, and of a whole tile.
+  f32x16 pw, gam;
+  float lam = 0.0f, whole = 1.0f;
+  auto row_of = [&](int r) { return 8 * (r >> 2) + 4 * h + (r & 3); };
+  auto tables = [&](int rows) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int j = row_of(r);
+      gam[r] = jb.sk * decay_pow(lg, rev ? j + 1 : max(rows - 1 - j, 0));
+    }
+    lam = jb.so * decay_pow(lg, rev ? max(rows - 1 - i, 0) : i + 1);
+    whole = decay_pow64(lg, rows);
+  };
+  tables(TILE);
+  if constexpr (OUT) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int n = rev ? row_of(r) - i : i - row_of(r);
+      pw[r] = n < 0 ? 0.0f : jb.sp * decay_pow(lg, n);
+    }
+  }
+
+  const int krl = TK::row_lane(lane), kcl = TK::col_lane(lane), vcl = TV::col_lane(lane), qdl = DR::lane_offset(lane);
+  int unit = 0;  // fp16: st holds the state times 2^unit
+  land();
+  __syncthreads();
+  for (int n = 0; n < tiles; ++n) {
+    const int buf = n & 1, at = t0 + (rev ? tiles - 1 - n : n) * TILE, rows = min(TILE, t1 - at);
+    if (n + 1 < tiles) fill(buf ^ 1, n + 1);
+    if (rows < TILE) tables(rows);  // the sequence's last tile
+    else if (rev && n == 1) tables(TILE);  // and the ones in front of it
+    const char* tk = smem + buf * BUF;
+    const char* tv = tk + BK;
+    const char* tq = tv + BV;
+    Frag<T> vf[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) vf[s] = TV::col_frag(tv, vcl, s, wave);
+
+    f32x16 o = f32x16{};
+    float back = 1.0f;  // fp16: what takes the output out of its unit
+    if constexpr (OUT) {
+      f32x16 p = f32x16{};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) p = mma<T>(TK::row_frag(tk, krl, t), TK::row_frag(tq, krl, t), p);
+      float mul = 1.0f, front = lam;
+      if constexpr (F16) {
+        float top = 0.0f;
+#pragma unroll
+        for (int m = 0; m < ND; ++m)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(st[m][r]));
+        const int e = 15 - min(max(__builtin_amdgcn_frexp_expf(wave_max(top)), -45), 120);
+        mul = __builtin_amdgcn_ldexpf(1.0f, e);
+        front = __builtin_amdgcn_ldexpf(lam, -e - unit);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x8 x;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = st[t >> 1][8 * (t & 1) + j] * (F16 ? mul : 1.0f);
+        Frag<T> sf[NPS];
+        split_pieces<T, NPS>(x, sf);
+        const Frag<T> qf = DR::read(tq, qdl, t);
+#pragma unroll
+        for (int z = NPS - 1; z >= 0; --z) o = mma<T>(sf[z], qf, o);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[r] *= pw[r];
+      if constexpr (F16) {
+        float top = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(p[r]));
+        const int e = 15 - min(max(__builtin_amdgcn_frexp_expf(half_max(top)), -25), 60);
+        const float f = __builtin_amdgcn_ldexpf(1.0f, e);
+        back = __builtin_amdgcn_ldexpf(1.0f, -e);
+        front *= f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] *= f;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[r] *= front;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        Frag<T> pf[NPP];
+        split_pieces<T, NPP>(s ? __builtin_shufflevector(p, p, 8, 9, 10, 11, 12, 13, 14, 15)
+                               : __builtin_shufflevector(p, p, 0, 1, 2, 3, 4, 5, 6, 7), pf);
+#pragma unroll
+        for (int z = NPP - 1; z >= 0; --z) o = mma<T>(vf[s], pf[z], o);
+      }
+    }
+
+    // The state behind the tile.
+    f32x8 x[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      x[s] = frag_values<T>(vf[s]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[s][j] *= gam[8 * s + j];
+    }
+    float keep = whole;
+    if constexpr (F16) {
+      float top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[s][j]));
+      const int next = 15 - min(max(__builtin_amdgcn_frexp_expf(wave_max(top)), -45), 60);
+      const float f = __builtin_amdgcn_ldexpf(1.0f, next);
+      keep = __builtin_amdgcn_ldexpf(whole, next - unit);
+      unit = next;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[s][j] *= f;
+    }
+#pragma unroll
+    for (int m = 0; m < ND; ++m)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[m][r] *= keep;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      Frag<T> xf[NPV];
+      split_pieces<T, NPV>(x[s], xf);
+#pragma unroll
+      for (int m = 0; m < ND; ++m) {
+        const Frag<T> kf = TK::col_frag(tk, kcl, s, m);
+#pragma unroll
+        for (int z = NPV - 1; z >= 0; --z) st[m] = mma<T>(kf, xf[z], st[m]);
+      }
+    }
+
+    land();  // the next tile; in front of the stores, so that they are not waited for
+    if constexpr (OUT) {
+      if (i < rows) {
+        const int64_t off = ooff + (int64_t)(at + i) * jb.os[2];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int c0 = 32 * wave + 8 * u + 4 * h;
+          if (jb.outF32) store4<float>((float*)jb.out + off, c0, dv, o[4 * u] * back, o[4 * u + 1] * back, o[4 * u + 2] * back, o[4 * u + 3] * back);
+          else store4<T>((T*)jb.out + off, c0, dv, o[4 * u] * back, o[4 * u + 1] * back, o[4 * u + 2] * back, o[4 * u + 3] * back);
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  float* to = nullptr;
+  if constexpr (OUT) {
+    if (jb.last && seg == (rev || len == 0 ? 0 : (len - 1) / (a.segTiles * TILE))) to = jb.last + (int64_t)bh * dk * dv;
+  } else {
+    to = jb.seg + ((int64_t)bh * a.nseg + seg) * dk * dv;
+  }
+  if (to && c < dv) {
+    const float f = F16 ? __builtin_amdgcn_ldexpf(1.0f, -unit) : 1.0f;
+#pragma unroll
+    for (int m = 0; m < ND; ++m)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = 32 * m + row_of(r);
+        if (d < dk) to[d * dv + c] = st[m][r] * f;
+      }
+  }
+  if constexpr (OUT) {
+    // Tokens behind the sequence's length are zero.
+    const int end = (int)min((int64_t)a.N, (int64_t)t0 + (int64_t)a.segTiles * TILE);
+    for (int t = max(len, t0) + (int)threadIdx.x / 32; t < end; t += THREADS / 32) {
+      const int64_t off = ooff + (int64_t)t * jb.os[2];
+      for (int x = threadIdx.x & 31; x < dv; x += 32) {
+        if (jb.outF32) ((float*)jb.out)[off + x] = 0.0f;
+        else ((T*)jb.out)[off + x] = T{};
+      }
+    }
+  }
+}
+
+template <typename T, int DK, int DV, bool OUT> int decay_launch(const DecayArgs& a, hipStream_t st) {
+  constexpr size_t lds = decay_lds<T, DK, DV, OUT>();
+  const void* fn = (const void*)decay_kernel<T, DK, DV, OUT>;
+  if (int e = set_dyn_lds(fn, lds, "decay_attention")) return e;
+  const int64_t n = (int64_t)a.jobs * a.B * a.H * a.nseg;
+  decay_kernel<T, DK, DV, OUT><<<dim3((unsigned)n), dim3(DV * 2), lds, st>>>(a);
+  return check_launch("decay_attention");
+}
+
+// Channels computed with for `d`: of keys, of values.
+inline int decay_key_dim(int d) { return compute_dim(d); }
+inline int decay_value_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+template <typename T, bool OUT> int decay_dispatch(const DecayArgs& a, hipStream_t st) {
+  auto values = [&](auto dk) {
+    constexpr int DK = decltype(dk)::value;
+    switch (decay_value_dim(a.job[0].dv)) {
+      case 32: return decay_launch<T, DK, 32, OUT>(a, st);
+      case 64: return decay_launch<T, DK, 64, OUT>(a, st);
+      default: return decay_launch<T, DK, 128, OUT>(a, st);
+    }
+  };
+  switch (decay_key_dim(a.job[0].dk)) {
+    case 32: return values(std::integral_constant<int, 32>{});
+    case 64: return values(std::integral_constant<int, 64>{});
+    case 96: return values(std::integral_constant<int, 96>{});
+    default: return values(std::integral_constant<int, 128>{});
+  }
+}
+
+// Jobs whose channels computed with agree, on a filled-in call: the segments' own states (out == 0) or the outputs.
+int decay_run_f32(const DecayArgs& a, int out, hipStream_t st);
+int decay_run_f16(const DecayArgs& a, int out, hipStream_t st);
+int decay_run_bf16(const DecayArgs& a, int out, hipStream_t st);
+
+}  // namespace lfamd

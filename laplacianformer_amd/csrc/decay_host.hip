@@ -1,0 +1,392 @@
+// C entries of decay_attention and decay_attention_step: argument checks, the plan of a call's segments, and
+// the kernels around the tiles' (decay_common.h): the segments' states joined, gradients of shared heads
+// added, and the single token.
+#include <math.h>
+
+#include <algorithm>
+
+#include "decay_common.h"
+
+namespace lfamd {
+
+namespace {
+
+// The segments' own states become the states in front of them (behind them, if reverse), in place and in
+// order: S(s + 1) = a^tokens(s) S(s) + own(s). One thread per element, its loads eight segments ahead.
+__global__ void __launch_bounds__(256) decay_join_kernel(const DecayArgs a) {
+  const DecayJob& jb = a.job[blockIdx.z];
+  const int size = jb.dk * jb.dv, e = blockIdx.y * 256 + threadIdx.x, bh = blockIdx.x;
+  if (e >= size) return;
+  const int b = bh / a.H, len = decay_length(a, b), span = a.segTiles * kDecayTile;
+  const float lg = a.logDecay[bh % a.H], full = decay_pow64(lg, span);
+  float* p = jb.seg + (int64_t)bh * a.nseg * size + e;
+  float s = 0.0f;
+  if (jb.first) {
+    const int d = e / jb.dv, c = e - d * jb.dv;
+    s = jb.first[(int64_t)bh * size + (jb.firstT ? c * jb.dk + d : e)];
+  }
+  for (int n0 = 0; n0 < a.nseg; n0 += 8) {
+    float own[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int n = min(n0 + u, a.nseg - 1);
+      own[u] = p[(int64_t)(jb.reverse ? a.nseg - 1 - n : n) * size];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int n = n0 + u, at = jb.reverse ? a.nseg - 1 - n : n;
+      if (n >= a.nseg) break;
+      const int64_t left = (int64_t)len - (int64_t)at * span;
+      p[(int64_t)at * size] = s;
+      s = fmaf(left >= span ? full : left > 0 ? decay_pow64(lg, (int)left) : 1.0f, s, own[u]);
+    }
+  }
+}
+
+// out[b][hk][n] = sum over the heads that share hk, in order, of part[b][h][n] (fp32), rounded once.
+template <typename T>
+__global__ void __launch_bounds__(256) decay_share_kernel(const float* part, T* out, int64_t s0, int64_t s1, int64_t s2, int B,
+                                                         int Hk, int G, int N, int D) {
+  const int packs = (D + 3) / 4;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= (int64_t)B * Hk * N * packs) return;
+  const int64_t row = at / packs;
+  const int c = (int)(at - row * packs) * 4;
+  const int64_t bh = row / N, n = row - bh * N;
+  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int g = 0; g < G; ++g) {
+    const float* p = part + ((bh * G + g) * N + n) * D + c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < D) x[j] += p[j];
+  }
+  store4<T>(out + (bh / Hk) * s0 + (bh % Hk) * s1 + n * s2, c, D, x[0], x[1], x[2], x[3]);
+}
+
+struct StepArgs {
+  const void *q, *k, *v;
+  void* out;
+  float* state;
+  const float* logDecay;
+  int64_t qs[2], ks[2], vs[2], os[2], ss[2];  // strides of batch and head
+  int B, H, G, dk, dv, blocks;
+  float scale;
+};
+
+// One token: S <- a S + k v^T in place, out = scale S^T q. Memory-bound by the state, read and written once:
+// a workgroup takes 32 value columns of a head's state, a thread four of them (16 bytes) in every 32nd row,
+// all of its rows in flight at once; the rows' shares of out are added in a fixed order.
+template <typename T> __global__ void __launch_bounds__(256) decay_step_kernel(const StepArgs a) {
+  __shared__ float share[4][32];
+  const int block = blockIdx.x % a.blocks, bh = blockIdx.x / a.blocks, b = bh / a.H, hq = bh % a.H;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c0 = 32 * block + 4 * (threadIdx.x & 7), row0 = threadIdx.x >> 3;
+  const float lg = a.logDecay[hq], keep = expf(lg);
+  const T* q = (const T*)a.q + b * a.qs[0] + hq * a.qs[1];
+  const T* k = (const T*)a.k + b * a.ks[0] + (hq / a.G) * a.ks[1];
+  const T* v = (const T*)a.v + b * a.vs[0] + (hq / a.G) * a.vs[1];
+  float* s = a.state + b * a.ss[0] + hq * a.ss[1];
+  f32x4 x[4];
+  float kr[4], qr[4], vc[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int r = row0 + 32 * u;
+    x[u] = __builtin_bit_cast(f32x4, load_chunk<float>(s + (int64_t)r * a.dv, r < a.dk, c0, a.dv));
+    kr[u] = r < a.dk ? to_acc(k[r]) : 0.0f;
+    qr[u] = r < a.dk ? to_acc(q[r]) : 0.0f;
+    vc[u] = c0 + u < a.dv ? to_acc(v[c0 + u]) : 0.0f;
+  }
+  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int r = row0 + 32 * u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[u][j] = fmaf(x[u][j], keep, kr[u] * vc[j]);
+      o[j] = fmaf(qr[u], x[u][j], o[j]);
+    }
+    if (r < a.dk) store4<float>(s + (int64_t)r * a.dv, c0, a.dv, x[u][0], x[u][1], x[u][2], x[u][3]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int d = 8; d < 64; d <<= 1) o[j] += __shfl_xor(o[j], d);
+    if (lane < 8) share[wave][4 * lane + j] = o[j];
+  }
+  __syncthreads();
+  const int c = 32 * block + (int)threadIdx.x;
+  if (threadIdx.x < 32 && c < a.dv) {
+    const float y = share[0][threadIdx.x] + share[1][threadIdx.x] + share[2][threadIdx.x] + share[3][threadIdx.x];
+    ((T*)a.out)[b * a.os[0] + hq * a.os[1] + c] = from_acc<T>(y * a.scale);
+  }
+}
+
+constexpr int64_t kMostTokens = (int64_t)1 << 29, kMostHeads = kMostWorkgroups / 4;
+
+int check_desc(const char* who, int dtype, const lfamd_decay* d, bool* empty) {
+  if (dtype != LFAMD_F32 && dtype != LFAMD_F16 && dtype != LFAMD_BF16)
+    return fail(LFAMD_ERR_DTYPE, "%s: unsupported dtype %d", who, dtype);
+  if (!d) return fail(LFAMD_ERR_ARG, "%s: null description", who);
+  if (d->batch < 0 || d->heads < 0 || d->kv_heads < 0 || d->tokens < 0 || d->key_dim < 0 || d->value_dim < 0)
+    return fail(LFAMD_ERR_ARG, "%s: negative size", who);
+  if (d->key_dim < 1 || d->key_dim > 128 || d->value_dim < 1 || d->value_dim > 128)
+    return fail(LFAMD_ERR_UNSUPPORTED, "%s: head sizes %lld and %lld are outside 1 .. 128", who, (long long)d->key_dim,
+                (long long)d->value_dim);
+  if (d->heads ? !d->kv_heads || d->heads % d->kv_heads : d->kv_heads)
+    return fail(LFAMD_ERR_ARG, "%s: %lld query heads do not share %lld key heads evenly", who, (long long)d->heads,
+                (long long)d->kv_heads);
+  if (!(d->scale > 0.0f) || !isfinite(d->scale)) return fail(LFAMD_ERR_ARG, "%s: scale must be positive and finite", who);
+  if (d->tokens > kMostTokens) return fail(LFAMD_ERR_UNSUPPORTED, "%s: at most 2^29 tokens are taken", who);
+  *empty = d->batch == 0 || d->heads == 0;
+  if (!*empty && (d->batch > kMostHeads || d->heads > kMostHeads || d->batch > kMostHeads / d->heads))
+    return fail(LFAMD_ERR_UNSUPPORTED, "%s: batch * heads is above %lld", who, (long long)kMostHeads);
+  if (!*empty && !d->log_decay) return fail(LFAMD_ERR_ARG, "%s: null log_decay", who);
+  return LFAMD_OK;
+}
+
+int load_mode(const void* p, const int64_t* strides, int64_t d, int64_t size) {
+  auto whole = [](int64_t bytes) { return bytes % 16 == 0; };
+  return (uintptr_t)p % 16 == 0 && whole(d * size) && whole(strides[0] * size) && whole(strides[1] * size) &&
+                 whole(strides[2] * size) && strides[2] >= 0 && strides[2] < ((int64_t)1 << 22)
+             ? kAsync
+             : kPlain;
+}
+
+// How many segments to cut the sequences of `runs` (runs of the operator times sequences times heads) into.
+void plan_segments(DecayArgs& a, int64_t runs, int dv) {
+  const int64_t tiles = ((int64_t)a.N + kDecayTile - 1) / kDecayTile;
+  const int64_t want = (int64_t)num_cus() * (decay_value_dim(dv) == 128 ? 2 : decay_value_dim(dv) == 64 ? 4 : 8);
+  int64_t n = std::max<int64_t>(1, std::min<int64_t>({want / std::max<int64_t>(runs, 1), tiles / 4, 64}));
+  a.segTiles = (int)std::max<int64_t>(1, (tiles + n - 1) / n);
+  a.nseg = (int)std::max<int64_t>(1, (tiles + a.segTiles - 1) / a.segTiles);
+}
+
+DecayArgs base_args(const lfamd_decay* d) {
+  DecayArgs a{};
+  a.logDecay = d->log_decay, a.lengths = d->lengths;
+  a.B = (int)d->batch, a.H = (int)d->heads, a.N = (int)d->tokens;
+  return a;
+}
+
+int run_tiles(int dtype, const DecayArgs& a, int out, hipStream_t st) {
+  return dtype == LFAMD_F32 ? decay_run_f32(a, out, st) : dtype == LFAMD_F16 ? decay_run_f16(a, out, st) : decay_run_bf16(a, out, st);
+}
+
+// The jobs of `a`, whose channels computed with agree, through their segments.
+int run_jobs(int dtype, const DecayArgs& a, hipStream_t st) {
+  if (a.nseg > 1) {
+    if (int e = run_tiles(dtype, a, 0, st)) return e;
+    int most = 0;
+    for (int j = 0; j < a.jobs; ++j) most = std::max(most, a.job[j].dk * a.job[j].dv);
+    decay_join_kernel<<<dim3(a.B * a.H, (most + 255) / 256, a.jobs), dim3(256), 0, st>>>(a);
+    if (int e = check_launch("decay_attention")) return e;
+  }
+  return run_tiles(dtype, a, 1, st);
+}
+
+void set3(int64_t* to, const int64_t* from) {
+  for (int i = 0; i < 3; ++i) to[i] = from[i];
+}
+
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+// The three runs of a backward pass, in one launch where their channels computed with agree.
+struct BackwardPlan {
+  DecayArgs both, own;  // dq and dk (keys as wide as the values); dv by itself, if the widths differ
+  bool split, shared;
+  size_t segs[3], part[2], total;  // bytes of each run's segments (dq, dk, dv), of the shared heads' parts of dk and dv
+};
+
+BackwardPlan plan_backward(const lfamd_decay* d) {
+  BackwardPlan p{};
+  p.split = decay_key_dim((int)d->key_dim) != decay_key_dim((int)d->value_dim) ||
+            decay_value_dim((int)d->key_dim) != decay_value_dim((int)d->value_dim);
+  p.shared = d->kv_heads != d->heads;
+  p.both = p.own = base_args(d);
+  const int64_t bh = d->batch * d->heads;
+  plan_segments(p.both, bh * (p.split ? 2 : 3), (int)d->key_dim);
+  plan_segments(p.own, bh, (int)d->value_dim);
+  if (!p.split) p.own.nseg = p.both.nseg, p.own.segTiles = p.both.segTiles;
+  const size_t state = (size_t)bh * d->key_dim * d->value_dim * sizeof(float);
+  for (int j = 0; j < 3; ++j) {
+    const int n = j == 2 ? p.own.nseg : p.both.nseg;
+    p.segs[j] = n > 1 ? round16(state * n) : 0;
+    p.total += p.segs[j];
+  }
+  const size_t rows = (size_t)bh * d->tokens * sizeof(float);
+  p.part[0] = p.shared ? round16(rows * d->key_dim) : 0;
+  p.part[1] = p.shared ? round16(rows * d->value_dim) : 0;
+  p.total += p.part[0] + p.part[1];
+  return p;
+}
+
+int check_workspace(const char* who, const void* ws, size_t have, size_t need) {
+  if (need && (!ws || have < need)) return fail(LFAMD_ERR_ARG, "%s: workspace too small", who);
+  if (need && ((uintptr_t)ws & 15)) return fail(LFAMD_ERR_ARG, "%s: workspace must be 16-byte aligned", who);
+  return LFAMD_OK;
+}
+
+template <typename T>
+int share_heads(const float* part, void* out, const int64_t* s, const lfamd_decay* d, int64_t D, hipStream_t st) {
+  const int64_t n = d->batch * d->kv_heads * d->tokens * ((D + 3) / 4);
+  decay_share_kernel<T><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(
+      part, (T*)out, s[0], s[1], s[2], (int)d->batch, (int)d->kv_heads, (int)(d->heads / d->kv_heads), (int)d->tokens, (int)D);
+  return check_launch("decay_attention backward");
+}
+
+}  // namespace
+
+}  // namespace lfamd
+
+using namespace lfamd;
+
+extern "C" {
+
+size_t lfamd_decay_attention_workspace_size(int dtype, const lfamd_decay* desc) {
+  bool empty = false;
+  if (check_desc("decay_attention", dtype, desc, &empty) || empty) return 0;
+  DecayArgs a = base_args(desc);
+  plan_segments(a, desc->batch * desc->heads, (int)desc->value_dim);
+  return a.nseg > 1 ? (size_t)desc->batch * desc->heads * a.nseg * desc->key_dim * desc->value_dim * sizeof(float) : 0;
+}
+
+int lfamd_decay_attention(int dtype, const lfamd_decay* desc, const void* q, const void* k, const void* v, const float* state,
+                          void* out, float* last_state, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "decay_attention";
+  bool empty = false;
+  if (int e = check_desc(who, dtype, desc, &empty)) return e;
+  if (empty || (desc->tokens == 0 && !last_state)) return ok();
+  if (desc->tokens && (!q || !k || !v || !out)) return fail(LFAMD_ERR_ARG, "%s: null pointer", who);
+  if (int e = check_workspace(who, workspace, workspace_bytes, lfamd_decay_attention_workspace_size(dtype, desc))) return e;
+  DecayArgs a = base_args(desc);
+  plan_segments(a, desc->batch * desc->heads, (int)desc->value_dim);
+  const int64_t size = (int64_t)dtype_size(dtype);
+  DecayJob& j = a.job[0];
+  a.jobs = 1;
+  j.q = q, j.k = k, j.v = v, j.first = state, j.out = out, j.last = last_state, j.seg = (float*)workspace;
+  set3(j.qs, desc->q_strides), set3(j.ks, desc->k_strides), set3(j.vs, desc->v_strides), set3(j.os, desc->out_strides);
+  j.qg = 1, j.kg = j.vg = (int)(desc->heads / desc->kv_heads);
+  j.dk = (int)desc->key_dim, j.dv = (int)desc->value_dim;
+  j.modeQ = load_mode(q, j.qs, j.dk, size), j.modeK = load_mode(k, j.ks, j.dk, size), j.modeV = load_mode(v, j.vs, j.dv, size);
+  j.sp = j.so = desc->scale, j.sk = 1.0f;
+  return run_jobs(dtype, a, (hipStream_t)stream);
+}
+
+size_t lfamd_decay_attention_backward_workspace_size(int dtype, const lfamd_decay* desc) {
+  bool empty = false;
+  if (check_desc("decay_attention backward", dtype, desc, &empty) || empty) return 0;
+  return plan_backward(desc).total;
+}
+
+int lfamd_decay_attention_backward(int dtype, const lfamd_decay* desc, const void* q, const void* k, const void* v,
+                                   const float* state, const lfamd_decay_grads* grads, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  const char* who = "decay_attention backward";
+  bool empty = false;
+  if (int e = check_desc(who, dtype, desc, &empty)) return e;
+  if (!grads) return fail(LFAMD_ERR_ARG, "%s: null gradients", who);
+  const bool kv = grads->grad_k != nullptr;
+  if (kv != (grads->grad_v != nullptr)) return fail(LFAMD_ERR_ARG, "%s: grad_k and grad_v come together", who);
+  if (desc->tokens && grads->grad_state && !kv) return fail(LFAMD_ERR_ARG, "%s: grad_state comes with grad_k and grad_v", who);
+  if (empty || (!kv && !grads->grad_q && !grads->grad_state)) return ok();
+  if (desc->tokens == 0 && !grads->grad_state) return ok();
+  if (desc->tokens && (!q || !k || !v || !grads->grad_out)) return fail(LFAMD_ERR_ARG, "%s: null pointer", who);
+  BackwardPlan p = plan_backward(desc);
+  if (int e = check_workspace(who, workspace, workspace_bytes, p.total)) return e;
+  char* ws = (char*)workspace;
+  auto take = [&](size_t n) {
+    char* x = ws;
+    ws += n;
+    return (float*)x;
+  };
+  float* segs[3];
+  for (int j = 0; j < 3; ++j) segs[j] = take(p.segs[j]);
+  float* part[2] = {take(p.part[0]), take(p.part[1])};
+  const int64_t size = (int64_t)dtype_size(dtype);
+  const int G = (int)(desc->heads / desc->kv_heads);
+  const int dk = (int)desc->key_dim, dv = (int)desc->value_dim;
+  struct Role {
+    const void* p;
+    const int64_t* s;
+    int g, d;
+  };
+  const Role Q{q, desc->q_strides, 1, dk}, K{k, desc->k_strides, G, dk}, V{v, desc->v_strides, G, dv},
+      O{grads->grad_out, grads->grad_out_strides, 1, dv};
+  auto job = [&](const Role& x, const Role& y, const Role& z, void* out, const int64_t* os, float* seg) {
+    DecayJob j{};
+    j.q = x.p, j.k = y.p, j.v = z.p, j.out = out, j.seg = seg;
+    set3(j.qs, x.s), set3(j.ks, y.s), set3(j.vs, z.s), set3(j.os, os);
+    j.qg = x.g, j.kg = y.g, j.vg = z.g, j.dk = x.d, j.dv = z.d;
+    j.modeQ = load_mode(x.p, x.s, x.d, size), j.modeK = load_mode(y.p, y.s, y.d, size), j.modeV = load_mode(z.p, z.s, z.d, size);
+    j.sp = desc->scale;
+    return j;
+  };
+  DecayArgs& a = p.both;
+  DecayArgs& o = p.split ? p.own : p.both;
+  if (grads->grad_q && desc->tokens) {
+    DecayJob j = job(O, V, K, grads->grad_q, grads->grad_q_strides, segs[0]);
+    j.first = state, j.firstT = 1, j.so = desc->scale, j.sk = 1.0f;
+    a.job[a.jobs++] = j;
+  }
+  const int64_t rows[2][3] = {{desc->heads * desc->tokens * dk, desc->tokens * dk, dk},
+                              {desc->heads * desc->tokens * dv, desc->tokens * dv, dv}};
+  if (kv && desc->tokens) {
+    DecayJob j = job(V, O, Q, p.shared ? part[0] : grads->grad_k, p.shared ? rows[0] : grads->grad_k_strides, segs[1]);
+    j.first = grads->grad_last_state, j.firstT = 1, j.reverse = 1, j.outF32 = p.shared, j.so = 1.0f, j.sk = desc->scale;
+    a.job[a.jobs++] = j;
+  }
+  if (kv || grads->grad_state) {
+    DecayJob j = job(K, Q, O, p.shared ? part[1] : grads->grad_v, p.shared ? rows[1] : grads->grad_v_strides, segs[2]);
+    j.first = grads->grad_last_state, j.reverse = 1, j.outF32 = p.shared, j.so = 1.0f, j.sk = desc->scale;
+    j.last = grads->grad_state;
+    o.job[o.jobs++] = j;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (a.jobs)
+    if (int e = run_jobs(dtype, a, st)) return e;
+  if (p.split && o.jobs)
+    if (int e = run_jobs(dtype, o, st)) return e;
+  if (p.shared && kv && desc->tokens) {
+    const struct {
+      const float* part;
+      void* out;
+      const int64_t* s;
+      int64_t D;
+    } each[2] = {{part[0], grads->grad_k, grads->grad_k_strides, dk}, {part[1], grads->grad_v, grads->grad_v_strides, dv}};
+    for (const auto& x : each) {
+      const int e = dtype == LFAMD_F32   ? share_heads<float>(x.part, x.out, x.s, desc, x.D, st)
+                    : dtype == LFAMD_F16 ? share_heads<f16s>(x.part, x.out, x.s, desc, x.D, st)
+                                         : share_heads<bf16s>(x.part, x.out, x.s, desc, x.D, st);
+      if (e) return e;
+    }
+  }
+  return ok();
+}
+
+int lfamd_decay_attention_step(int dtype, const lfamd_decay* desc, const void* q, const void* k, const void* v, void* out,
+                               float* state, const int64_t* state_strides, void* stream) {
+  const char* who = "decay_attention_step";
+  bool empty = false;
+  if (int e = check_desc(who, dtype, desc, &empty)) return e;
+  if (desc->tokens != 1) return fail(LFAMD_ERR_ARG, "%s: takes one token, not %lld", who, (long long)desc->tokens);
+  if (empty) return ok();
+  if (!q || !k || !v || !out || !state || !state_strides) return fail(LFAMD_ERR_ARG, "%s: null pointer", who);
+  StepArgs a{};
+  a.q = q, a.k = k, a.v = v, a.out = out, a.state = state, a.logDecay = desc->log_decay, a.scale = desc->scale;
+  for (int i = 0; i < 2; ++i) {
+    a.qs[i] = desc->q_strides[i], a.ks[i] = desc->k_strides[i], a.vs[i] = desc->v_strides[i], a.os[i] = desc->out_strides[i];
+    a.ss[i] = state_strides[i];
+  }
+  a.B = (int)desc->batch, a.H = (int)desc->heads, a.G = (int)(desc->heads / desc->kv_heads);
+  a.dk = (int)desc->key_dim, a.dv = (int)desc->value_dim, a.blocks = (a.dv + 31) / 32;
+  const dim3 g((unsigned)((int64_t)a.B * a.H * a.blocks)), t(256);
+  hipStream_t st = (hipStream_t)stream;
+  switch (dtype) {
+    case LFAMD_F32: decay_step_kernel<float><<<g, t, 0, st>>>(a); break;
+    case LFAMD_F16: decay_step_kernel<f16s><<<g, t, 0, st>>>(a); break;
+    default: decay_step_kernel<bf16s><<<g, t, 0, st>>>(a); break;
+  }
+  return check_launch(who);
+}
+
+}  // extern "C"

@@ -303,6 +303,150 @@ std::vector<Tensor> SoftmaxAttention_backward(const Tensor grad_out, const Tenso
 
 namespace {
 
+struct DecayIn {
+  Tensor q, k, v, state;
+  lfamd_decay d{};
+  int dt = 0;
+};
+
+void check_state(const char* op, const Tensor& q, const Tensor& t, const lfamd_decay& d, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == q.device(), op, ": ", name, " must be on the same GPU as q");
+  TORCH_CHECK(t.scalar_type() == at::kFloat, op, ": ", name, " must be float32");
+  TORCH_CHECK(t.dim() == 4 && t.size(0) == d.batch && t.size(1) == d.heads && t.size(2) == d.key_dim && t.size(3) == d.value_dim,
+              op, ": ", name, " must be [", d.batch, ", ", d.heads, ", ", d.key_dim, ", ", d.value_dim, "], got ", t.sizes());
+}
+
+DecayIn decay_in(const char* op, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
+                 const OptTensor& state, const OptTensor& lengths, double scale) {
+  TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda(), op, ": tensors must be on GPU");
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, op, ": q, k and v must be [batch, heads, tokens, channels]");
+  DecayIn in;
+  in.dt = detail::abi_dtype(q, op);
+  detail::same_type(q, k, "k");
+  detail::same_type(q, v, "v");
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3), op, ": q ", q.sizes(), " and k ",
+              k.sizes(), " may differ in their heads only");
+  TORCH_CHECK(v.size(0) == k.size(0) && v.size(1) == k.size(1) && v.size(2) == k.size(2), op, ": k ", k.sizes(), " and v ",
+              v.sizes(), " may differ in their channels only");
+  TORCH_CHECK(log_decay.scalar_type() == at::kFloat && log_decay.dim() == 1 && log_decay.size(0) == q.size(1) &&
+                  log_decay.is_contiguous(),
+              op, ": log_decay must be a contiguous float32 tensor of one value per query head");
+  TORCH_CHECK(log_decay.is_cuda() && log_decay.device() == q.device(), op, ": log_decay must be on the same GPU as q");
+  in.q = unit_last(q), in.k = unit_last(k), in.v = unit_last(v);
+  lfamd_decay& d = in.d;
+  d.batch = q.size(0), d.heads = q.size(1), d.kv_heads = k.size(1), d.tokens = q.size(2), d.key_dim = q.size(3);
+  d.value_dim = v.size(3);
+  set_strides(d.q_strides, in.q);
+  set_strides(d.k_strides, in.k);
+  set_strides(d.v_strides, in.v);
+  d.log_decay = log_decay.data_ptr<float>();
+  d.lengths = per_batch(op, q, lengths, "lengths");
+  d.scale = (float)scale;
+  if (given(state)) {
+    check_state(op, q, *state, d, "state");
+    in.state = state->contiguous();
+  }
+  return in;
+}
+
+// The values' channels in q's order of dimensions.
+Tensor decay_output(const DecayIn& in) {
+  if (in.d.key_dim == in.d.value_dim) return output_like(in.q);
+  const bool tokens_first = in.q.dim() == 4 && in.q.stride(1) < in.q.stride(2);
+  const auto o = in.q.options();
+  return tokens_first ? at::empty({in.d.batch, in.d.tokens, in.d.heads, in.d.value_dim}, o).transpose(1, 2)
+                      : at::empty({in.d.batch, in.d.heads, in.d.tokens, in.d.value_dim}, o);
+}
+
+}  // namespace
+
+std::vector<Tensor> DecayAttention_forward(const Tensor q, const Tensor k, const Tensor v, const Tensor log_decay,
+                                           const OptTensor state, const OptTensor lengths, double scale, bool need_last) {
+  DecayIn in = decay_in("decay_attention", q, k, v, log_decay, state, lengths, scale);
+  at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  Tensor out = decay_output(in), last, ws;
+  set_strides(in.d.out_strides, out);
+  if (need_last) last = at::empty({in.d.batch, in.d.heads, in.d.key_dim, in.d.value_dim}, q.options().dtype(at::kFloat));
+  const size_t wsb = lfamd_decay_attention_workspace_size(in.dt, &in.d);
+  if (wsb) ws = at::empty({(int64_t)wsb}, q.options().dtype(at::kByte));
+  detail::check_status(lfamd_decay_attention(in.dt, &in.d, ptr(in.q), ptr(in.k), ptr(in.v), (const float*)ptr(in.state), ptr(out),
+                                             (float*)ptr(last), ptr(ws), wsb, detail::stream_of(q)));
+  return {out, last};
+}
+
+std::vector<Tensor> DecayAttention_backward(const OptTensor grad_out, const OptTensor grad_last, const Tensor q, const Tensor k,
+                                            const Tensor v, const Tensor log_decay, const OptTensor state,
+                                            const OptTensor lengths, double scale, bool need_q, bool need_kv, bool need_state) {
+  const char* op = "decay_attention backward";
+  DecayIn in = decay_in(op, q, k, v, log_decay, state, lengths, scale);
+  const lfamd_decay& d = in.d;
+  at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  Tensor g, gl;
+  if (given(grad_out)) {
+    TORCH_CHECK(grad_out->dim() == 4 && grad_out->size(0) == d.batch && grad_out->size(1) == d.heads &&
+                    grad_out->size(2) == d.tokens && grad_out->size(3) == d.value_dim,
+                op, ": grad_out must have the output's shape");
+    detail::same_type(q, *grad_out, "grad_out");
+    g = unit_last(*grad_out);
+  } else {
+    g = at::zeros({d.batch, d.heads, d.tokens, d.value_dim}, q.options());
+  }
+  if (given(grad_last)) {
+    check_state(op, q, *grad_last, d, "the last state's gradient");
+    gl = grad_last->contiguous();
+  }
+  need_kv = need_kv || need_state;
+  Tensor dq, dk, dv, ds;
+  lfamd_decay_grads gr{};
+  gr.grad_out = ptr(g), gr.grad_last_state = (const float*)ptr(gl);
+  set_strides(gr.grad_out_strides, g);
+  if (need_q) {
+    dq = output_like(in.q);
+    gr.grad_q = ptr(dq), set_strides(gr.grad_q_strides, dq);
+  }
+  if (need_kv) {
+    dk = output_like(in.k), dv = output_like(in.v);
+    gr.grad_k = ptr(dk), gr.grad_v = ptr(dv);
+    set_strides(gr.grad_k_strides, dk);
+    set_strides(gr.grad_v_strides, dv);
+  }
+  if (need_state) {
+    ds = at::empty({d.batch, d.heads, d.key_dim, d.value_dim}, q.options().dtype(at::kFloat));
+    gr.grad_state = (float*)ptr(ds);
+  }
+  const size_t wsb = lfamd_decay_attention_backward_workspace_size(in.dt, &in.d);
+  const Tensor ws = at::empty({(int64_t)wsb}, q.options().dtype(at::kByte));
+  detail::check_status(lfamd_decay_attention_backward(in.dt, &in.d, ptr(in.q), ptr(in.k), ptr(in.v), (const float*)ptr(in.state),
+                                                      &gr, ptr(ws), wsb, detail::stream_of(q)));
+  return {dq, dk, dv, ds};
+}
+
+Tensor DecayAttentionStep(const Tensor q, const Tensor k, const Tensor v, const Tensor log_decay, const Tensor state,
+                          double scale) {
+  const char* op = "decay_attention_step";
+  no_tangent(op, {&q, &k, &v, &log_decay, &state});
+  DecayIn in = decay_in(op, q, k, v, log_decay, std::nullopt, std::nullopt, scale);
+  const lfamd_decay& d = in.d;
+  TORCH_CHECK(d.tokens == 1, op, ": takes one token, not ", d.tokens);
+  check_state(op, q, state, d, "state");
+  const int64_t size = d.key_dim * d.value_dim, sb = state.stride(0), sh = state.stride(1);
+  TORCH_CHECK(state.numel() == 0 || ((d.value_dim == 1 || state.stride(3) == 1) && (d.key_dim == 1 || state.stride(2) == d.value_dim)),
+              op, ": each head's state must be contiguous");
+  TORCH_CHECK((d.heads <= 1 || sh >= size) && (d.batch <= 1 || sb >= size) &&
+                  (d.heads <= 1 || d.batch <= 1 || sb >= d.heads * sh || sh >= d.batch * sb),
+              op, ": the states of sequences or heads overlap");
+  at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  Tensor out = decay_output(in);
+  set_strides(in.d.out_strides, out);
+  const int64_t ss[2] = {sb, sh};
+  state.unsafeGetTensorImpl()->bump_version();
+  detail::check_status(lfamd_decay_attention_step(in.dt, &in.d, ptr(in.q), ptr(in.k), ptr(in.v), ptr(out), (float*)ptr(state), ss,
+                                                  detail::stream_of(q)));
+  return out;
+}
+
+namespace {
+
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -393,6 +537,36 @@ struct SoftmaxAttentionNode : torch::autograd::Function<SoftmaxAttentionNode> {
   }
 };
 
+struct DecayAttentionNode : torch::autograd::Function<DecayAttentionNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
+                               const OptTensor& state, const OptTensor& lengths, double scale, bool return_state) {
+    ctx->set_materialize_grads(false);
+    auto r = DecayAttention_forward(q, k, v, log_decay, state, lengths, scale, return_state);
+    auto or_none = [](const OptTensor& t) { return given(t) ? *t : Tensor(); };
+    ctx->save_for_backward({q, k, v, log_decay, or_none(state), or_none(lengths)});
+    ctx->saved_data["scale"] = scale;
+    if (!return_state) r.pop_back();
+    return r;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("decay_attention", g);
+    const auto s = ctx->get_saved_variables();
+    auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+    variable_list out(8);
+    const Tensor gl = g.size() > 1 ? g[1] : Tensor();
+    if (!g[0].defined() && !gl.defined()) return out;
+    const bool need_k = ctx->needs_input_grad(1), need_v = ctx->needs_input_grad(2);
+    const bool need_s = s[4].defined() && ctx->needs_input_grad(4);
+    const auto d = DecayAttention_backward(opt(g[0]), opt(gl), s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]),
+                                           ctx->saved_data["scale"].toDouble(), ctx->needs_input_grad(0), need_k || need_v, need_s);
+    out[0] = d[0];
+    if (need_k) out[1] = d[1];
+    if (need_v) out[2] = d[2];
+    out[4] = d[3];
+    return out;
+  }
+};
+
 bool records(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -428,6 +602,17 @@ Tensor SoftmaxAttention(const Tensor q, const Tensor k, const Tensor v, const Op
   if (records({&q, &k, &v}))
     return SoftmaxAttentionNode::apply(q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale);
   return SoftmaxAttention_forward(q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale, false)[0];
+}
+
+std::vector<Tensor> DecayAttention(const Tensor q, const Tensor k, const Tensor v, const Tensor log_decay, const OptTensor state,
+                                   const OptTensor lengths, double scale, bool return_state) {
+  TORCH_CHECK(!log_decay.requires_grad(), "decay_attention: log_decay has no gradient");
+  no_tangent("decay_attention", {&q, &k, &v, &log_decay, if_given(state)});
+  if (records({&q, &k, &v, if_given(state)}))
+    return DecayAttentionNode::apply(q, k, v, log_decay, state, lengths, scale, return_state);
+  auto r = DecayAttention_forward(q, k, v, log_decay, state, lengths, scale, return_state);
+  if (!return_state) r.pop_back();
+  return r;
 }
 
 }  // namespace laplace

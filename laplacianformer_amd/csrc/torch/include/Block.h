@@ -32,7 +32,20 @@ std::vector<at::Tensor> SoftmaxAttention_backward(const at::Tensor grad_out, con
                                                   const std::optional<at::Tensor> q_starts, double scale, bool need_q,
                                                   bool need_kv);
 
-// The three with autograd: [y] or [y, sum]; [q', k' or undefined]; out.
+// state, last and their gradients: fp32 [batch, heads, key channels, value channels]; undefined where not asked for.
+std::vector<at::Tensor> DecayAttention_forward(const at::Tensor q, const at::Tensor k, const at::Tensor v,
+                                               const at::Tensor log_decay, const std::optional<at::Tensor> state,
+                                               const std::optional<at::Tensor> lengths, double scale, bool need_last);
+std::vector<at::Tensor> DecayAttention_backward(const std::optional<at::Tensor> grad_out,
+                                                const std::optional<at::Tensor> grad_last, const at::Tensor q,
+                                                const at::Tensor k, const at::Tensor v, const at::Tensor log_decay,
+                                                const std::optional<at::Tensor> state,
+                                                const std::optional<at::Tensor> lengths, double scale, bool need_q,
+                                                bool need_kv, bool need_state);
+at::Tensor DecayAttentionStep(const at::Tensor q, const at::Tensor k, const at::Tensor v, const at::Tensor log_decay,
+                              const at::Tensor state, double scale);
+
+// Those with autograd: [y] or [y, sum]; [q', k' or undefined]; out.
 std::vector<at::Tensor> AddRmsNorm(const at::Tensor x, const at::Tensor weight, const std::optional<at::Tensor> residual,
                                    double eps);
 std::vector<at::Tensor> RotaryPositions(const at::Tensor q, const std::optional<at::Tensor> k, const at::Tensor positions,
@@ -41,5 +54,9 @@ at::Tensor SoftmaxAttention(const at::Tensor q, const at::Tensor k, const at::Te
                             bool causal, const std::optional<at::Tensor> k_lengths,
                             const std::optional<at::Tensor> q_lengths, const std::optional<at::Tensor> q_starts,
                             double scale);
+// [out] or [out, last].
+std::vector<at::Tensor> DecayAttention(const at::Tensor q, const at::Tensor k, const at::Tensor v, const at::Tensor log_decay,
+                                       const std::optional<at::Tensor> state, const std::optional<at::Tensor> lengths,
+                                       double scale, bool return_state);
 
 }  // namespace laplace
