@@ -404,6 +404,34 @@ int lfamd_softmax_attention_backward(int dtype, const lfamd_attention* desc, con
                                      const void* out, const float* stats, const lfamd_attention_grads* grads,
                                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* A block's output through its own norm, a gate and a scale onto the residual, and the norm of that sum:
+ *   m = x * rx, rx = 1 / sqrt(mean(x^2) + eps) (post_weight NULL: m = x), z = m * post_weight,
+ *   sum = residual + scale * gate * z (gate NULL: 1), rs = 1 / sqrt(mean(sum^2) + eps), y = sum * rs * weight,
+ * statistics of fp32 values, of the unrounded sum. x and residual [rows][width] with rows x_stride /
+ * residual_stride elements apart, y and sum contiguous, the weights [width] and the gate [rows / gate_rows][width]
+ * (gate_rows 0: one gate row for all) with rows gate_stride apart; each of them of its own type, dtype or F32.
+ * rstd and post_rstd [rows] fp32 (rs and rx) or NULL: the backward reads them. 1 <= width <= 8192
+ * (LFAMD_ERR_UNSUPPORTED beyond), rows below 2^30; scale finite. */
+typedef struct {
+  int64_t rows, width, x_stride, residual_stride, gate_rows, gate_stride;
+  int weight_dtype, post_weight_dtype, gate_dtype;
+  float scale, eps;
+} lfamd_gated_norm;
+int lfamd_gated_add_rms_norm(int dtype, const lfamd_gated_norm* desc, const void* x, const void* residual, const void* weight,
+                             const void* post_weight, const void* gate, void* y, void* sum, float* rstd, float* post_rstd,
+                             void* stream);
+
+/* Gradients from the forward's inputs and statistics (grad_sum NULL: taken as zero). grad_x, grad_residual
+ * and grad_gate are contiguous; those of the weights and the gate have their types and may be NULL. The
+ * workspace is 4-byte aligned. Deterministic, without atomics. */
+size_t lfamd_gated_add_rms_norm_backward_workspace_size(int dtype, const lfamd_gated_norm* desc);
+int lfamd_gated_add_rms_norm_backward(int dtype, const lfamd_gated_norm* desc, const void* grad_y, int64_t grad_y_stride,
+                                      const void* grad_sum, int64_t grad_sum_stride, const void* x, const void* residual,
+                                      const void* weight, const void* post_weight, const void* gate, const float* rstd,
+                                      const float* post_rstd, void* grad_x, void* grad_residual, void* grad_weight,
+                                      void* grad_post_weight, void* grad_gate, void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
 /* Causal linear attention with a decay for each head, and its state: with a = exp(log_decay[h]),
  *   S_t = a S_(t-1) + k_t v_t^T (S_(-1) = state),  out_t = scale S_t^T q_t.
  * query [batch][heads][tokens][key_dim], key [batch][kv_heads][tokens][key_dim], value and out

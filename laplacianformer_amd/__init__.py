@@ -9,7 +9,7 @@ transformer block around it (norm, rotary positions, softmax attention).
 from ._lib import EXT_PATH, LIB_PATH, capi, check, dtype_code, ext
 from .attention import LaplacianAttention, laplacian_attention
 from .block import (AttentionBlock, add_rms_norm, add_rms_norm_fp8, decay_attention, decay_attention_step,
-                    grid_positions, rotary, rotary_sections, softmax_attention)
+                    gated_add_rms_norm, grid_positions, rotary, rotary_sections, softmax_attention)
 from .graphs import GraphedStep
 from .functional import (LaplaceKernelFunction, LaplaceSubtractionFunction, NewtonInverseFunction,
                          TallMixFunction, TallProductFunction, laplace_kernel, laplace_subtraction, mix_rows,
@@ -21,5 +21,5 @@ __all__ = [
     "laplace_subtraction", "laplacian_attention", "newton_inverse", "TallMixFunction", "TallProductFunction",
     "mix_rows", "tall_mix", "tall_product", "tall_t", "GraphedStep",
     "AttentionBlock", "add_rms_norm", "add_rms_norm_fp8", "grid_positions", "rotary", "rotary_sections",
-    "softmax_attention", "decay_attention", "decay_attention_step",
+    "softmax_attention", "decay_attention", "decay_attention_step", "gated_add_rms_norm",
 ]

@@ -67,6 +67,9 @@ CAPI_PROTOTYPES = [
     ("lfamd_softmax_attention", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     ("lfamd_softmax_attention_backward_workspace_size", _SZ, [_I, _P]),
     ("lfamd_softmax_attention_backward", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    ("lfamd_gated_add_rms_norm", _I, [_I] + [_P] * 11),
+    ("lfamd_gated_add_rms_norm_backward_workspace_size", _SZ, [_I, _P]),
+    ("lfamd_gated_add_rms_norm_backward", _I, [_I, _P, _P, _I64, _P, _I64] + [_P] * 13 + [_SZ, _P]),
     ("lfamd_decay_attention_workspace_size", _SZ, [_I, _P]),
     ("lfamd_decay_attention", _I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     ("lfamd_decay_attention_backward_workspace_size", _SZ, [_I, _P]),
@@ -93,6 +96,14 @@ class AttentionGrads(ctypes.Structure):
 
     _fields_ = [(n, _P) for n in ("grad_out", "grad_q", "grad_k", "grad_v")] + \
         [(n, _I64 * 3) for n in ("grad_out_strides", "grad_q_strides", "grad_k_strides", "grad_v_strides")]
+
+
+class GatedNorm(ctypes.Structure):
+    """lfamd_gated_norm of include/laplacianformer_amd.h."""
+
+    _fields_ = [(n, _I64) for n in ("rows", "width", "x_stride", "residual_stride", "gate_rows", "gate_stride")] + \
+        [(n, _I) for n in ("weight_dtype", "post_weight_dtype", "gate_dtype")] + \
+        [("scale", ctypes.c_float), ("eps", ctypes.c_float)]
 
 
 class Decay(ctypes.Structure):

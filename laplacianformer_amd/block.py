@@ -44,6 +44,20 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     return (y, scale) if residual is None else (y, scale, total)
 
 
+def gated_add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor | None = None,
+                       gate: torch.Tensor | None = None, scale: float = 1.0, eps: float = 1e-6):
+    """The norms behind one block and in front of the next, with the first one's gate and residual scale.
+
+    ``sum = residual + scale * gate * norm(x) * post_weight``, ``y = norm(sum) * weight``, where
+    ``norm(t) = t / sqrt(mean(t^2) + eps)`` over the last dimension (statistics of float32 values, of the unrounded
+    sum); without ``post_weight`` x itself takes the place of its norm. Returns ``(y, sum)`` in x's type, which is
+    the residual's too. ``gate`` is ``[width]``, or has x's dimensions with ones behind some of the leading ones
+    (``[B, 1, width]``: one for each sequence). Each weight and the gate has x's type or float32; the last
+    dimension is at most 8192. With autograd, for all five, which keeps them.
+    """
+    return tuple(ext().GatedAddRmsNorm(x, weight, residual, post_weight, gate, scale, eps))
+
+
 def rotary_sections(head_dim: int, axes: int) -> list[int]:
     """head_dim // 2 channel pairs dealt evenly to the axes; the first takes the remainder."""
     n = head_dim // 2 // axes

@@ -138,6 +138,105 @@ std::vector<Tensor> AddRmsNorm_backward(const Tensor grad_y, const OptTensor gra
 
 namespace {
 
+struct GatedIn {
+  NormIn n;
+  Tensor w, wp, gate;
+  lfamd_gated_norm d{};
+};
+
+GatedIn gated_in(const char* op, const Tensor& x, const Tensor& weight, const Tensor& residual, const OptTensor& post_weight,
+                 const OptTensor& gate, double scale, double eps) {
+  GatedIn in;
+  in.w = weight.contiguous();
+  in.n = norm_in(op, x, weight, residual);
+  lfamd_gated_norm& d = in.d;
+  d.rows = in.n.rows, d.width = in.n.width, d.x_stride = in.n.xs, d.residual_stride = in.n.rs;
+  d.weight_dtype = in.n.wt, d.post_weight_dtype = d.gate_dtype = in.n.dt;
+  d.scale = (float)scale, d.eps = (float)eps;
+  if (given(post_weight)) {
+    TORCH_CHECK(post_weight->is_cuda() && post_weight->device() == x.device(), op, ": post_weight must be on the same GPU as x");
+    TORCH_CHECK(post_weight->dim() == 1 && post_weight->size(0) == x.size(-1), op, ": post_weight must have x's last size, ",
+                x.size(-1));
+    d.post_weight_dtype = detail::abi_dtype(*post_weight, op);
+    in.wp = post_weight->contiguous();
+  }
+  if (given(gate)) {
+    TORCH_CHECK(gate->is_cuda() && gate->device() == x.device(), op, ": gate must be on the same GPU as x");
+    const int64_t nd = x.dim();
+    int64_t same = 0;  // leading dimensions that the gate has in full; behind them it has ones
+    bool fits = (gate->dim() == 1 || gate->dim() == nd) && gate->size(-1) == x.size(-1);
+    if (fits && gate->dim() == nd) {
+      while (same < nd - 1 && gate->size(same) == x.size(same)) ++same;
+      for (int64_t i = same; i < nd - 1; ++i) fits = fits && gate->size(i) == 1;
+    }
+    TORCH_CHECK(fits, op, ": gate must be [", x.size(-1), "], or of x's dimensions with ones behind some of the leading ones, got ",
+                gate->sizes(), " for x ", x.sizes());
+    d.gate_dtype = detail::abi_dtype(*gate, op);
+    in.gate = *gate;
+    d.gate_stride = row_view(in.gate);
+    if (same) {
+      d.gate_rows = 1;
+      for (int64_t i = same; i < nd - 1; ++i) d.gate_rows *= x.size(i);
+    }
+  }
+  return in;
+}
+
+}  // namespace
+
+std::vector<Tensor> GatedAddRmsNorm_forward(const Tensor x, const Tensor weight, const Tensor residual,
+                                            const OptTensor post_weight, const OptTensor gate, double scale, double eps,
+                                            bool need_rstd) {
+  GatedIn in = gated_in("gated_add_rms_norm", x, weight, residual, post_weight, gate, scale, eps);
+  at::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  Tensor y = at::empty(x.sizes(), x.options()), sum = at::empty(x.sizes(), x.options()), rstd, post;
+  if (need_rstd) {
+    rstd = at::empty({in.n.rows}, x.options().dtype(at::kFloat));
+    if (in.wp.defined()) post = at::empty({in.n.rows}, x.options().dtype(at::kFloat));
+  }
+  detail::check_status(lfamd_gated_add_rms_norm(in.n.dt, &in.d, ptr(in.n.x), ptr(in.n.res), ptr(in.w), ptr(in.wp), ptr(in.gate),
+                                                ptr(y), ptr(sum), (float*)ptr(rstd), (float*)ptr(post), detail::stream_of(x)));
+  return {y, sum, rstd, post};
+}
+
+std::vector<Tensor> GatedAddRmsNorm_backward(const Tensor grad_y, const OptTensor grad_sum, const Tensor x, const Tensor weight,
+                                             const Tensor residual, const OptTensor post_weight, const OptTensor gate,
+                                             const Tensor rstd, const OptTensor post_rstd, double scale, double eps,
+                                             bool need_weight, bool need_post_weight, bool need_gate) {
+  const char* op = "gated_add_rms_norm backward";
+  GatedIn in = gated_in(op, x, weight, residual, post_weight, gate, scale, eps);
+  TORCH_CHECK(grad_y.sizes() == x.sizes(), op, ": grad_y and x must have the same shape");
+  detail::same_type(x, grad_y, "grad_y");
+  for (const Tensor* t : {&rstd, if_given(post_rstd)})
+    TORCH_CHECK(t ? t->scalar_type() == at::kFloat && t->numel() == in.n.rows && t->is_contiguous() && t->device() == x.device()
+                  : !in.wp.defined(),
+                op, ": the statistics must be the forward's");
+  Tensor gy = grad_y, gs;
+  const int64_t gys = row_view(gy);
+  int64_t gss = 0;
+  if (given(grad_sum)) {
+    TORCH_CHECK(grad_sum->sizes() == x.sizes(), op, ": grad_sum and x must have the same shape");
+    detail::same_type(x, *grad_sum, "grad_sum");
+    gs = *grad_sum;
+    gss = row_view(gs);
+  }
+  at::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  Tensor dx = at::empty(x.sizes(), x.options()), dr = at::empty(x.sizes(), x.options()), dw, dwp, dg;
+  if (need_weight) dw = at::empty(in.w.sizes(), in.w.options());
+  if (need_post_weight) dwp = at::empty(in.wp.sizes(), in.wp.options());
+  if (need_gate) dg = in.n.rows ? at::empty(gate->sizes(), gate->options()) : at::zeros(gate->sizes(), gate->options());
+  const size_t wsb = lfamd_gated_add_rms_norm_backward_workspace_size(in.n.dt, &in.d);
+  const Tensor ws = at::empty({(int64_t)wsb}, x.options().dtype(at::kByte));
+  detail::check_status(lfamd_gated_add_rms_norm_backward(in.n.dt, &in.d, ptr(gy), gys, ptr(gs), gss, ptr(in.n.x), ptr(in.n.res),
+                                                         ptr(in.w), ptr(in.wp), ptr(in.gate), rstd.data_ptr<float>(),
+                                                         given(post_rstd) ? post_rstd->data_ptr<float>() : nullptr, ptr(dx), ptr(dr),
+                                                         ptr(dw), ptr(dwp), in.n.rows ? ptr(dg) : nullptr, ptr(ws), wsb,
+                                                         detail::stream_of(x)));
+  return {dx, dr, dw, dwp, dg};
+}
+
+namespace {
+
 // [B, heads, tokens, channels] with adjacent channels.
 Tensor unit_last(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
@@ -480,6 +579,34 @@ struct AddRmsNormNode : torch::autograd::Function<AddRmsNormNode> {
   }
 };
 
+struct GatedAddRmsNormNode : torch::autograd::Function<GatedAddRmsNormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& residual,
+                               const OptTensor& post_weight, const OptTensor& gate, double scale, double eps) {
+    ctx->set_materialize_grads(false);
+    const auto r = GatedAddRmsNorm_forward(x, weight, residual, post_weight, gate, scale, eps, true);
+    auto or_none = [](const OptTensor& t) { return given(t) ? *t : Tensor(); };
+    ctx->save_for_backward({x, weight, residual, or_none(post_weight), or_none(gate), r[2], r[3]});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["eps"] = eps;
+    return {r[0], r[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("gated_add_rms_norm", g);
+    variable_list out(7);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+    const Tensor gy = g[0].defined() ? g[0] : at::zeros_like(s[0]);
+    const size_t gate_at = s[3].defined() ? 4 : 3;  // needs_input_grad counts the tensors that are given
+    const auto d = GatedAddRmsNorm_backward(gy, opt(g[1]), s[0], s[1], s[2], opt(s[3]), opt(s[4]), s[5], opt(s[6]),
+                                            ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(),
+                                            ctx->needs_input_grad(1), s[3].defined() && ctx->needs_input_grad(3),
+                                            s[4].defined() && ctx->needs_input_grad(gate_at));
+    out[0] = d[0], out[1] = d[2], out[2] = d[1], out[3] = d[3], out[4] = d[4];
+    return out;
+  }
+};
+
 struct RotaryNode : torch::autograd::Function<RotaryNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k, const Tensor& positions,
                                std::vector<int64_t> sections, double base, bool interleaved) {
@@ -581,6 +708,16 @@ std::vector<Tensor> AddRmsNorm(const Tensor x, const Tensor weight, const OptTen
   if (records({&x, &weight, if_given(residual)})) return AddRmsNormNode::apply(x, weight, residual, eps);
   auto r = AddRmsNorm_forward(x, weight, residual, eps, false);
   r.resize(given(residual) ? 2 : 1);
+  return r;
+}
+
+std::vector<Tensor> GatedAddRmsNorm(const Tensor x, const Tensor weight, const Tensor residual, const OptTensor post_weight,
+                                    const OptTensor gate, double scale, double eps) {
+  no_tangent("gated_add_rms_norm", {&x, &weight, &residual, if_given(post_weight), if_given(gate)});
+  if (records({&x, &weight, &residual, if_given(post_weight), if_given(gate)}))
+    return GatedAddRmsNormNode::apply(x, weight, residual, post_weight, gate, scale, eps);
+  auto r = GatedAddRmsNorm_forward(x, weight, residual, post_weight, gate, scale, eps, false);
+  r.resize(2);
   return r;
 }
 

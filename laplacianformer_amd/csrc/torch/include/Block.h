@@ -32,6 +32,16 @@ std::vector<at::Tensor> SoftmaxAttention_backward(const at::Tensor grad_out, con
                                                   const std::optional<at::Tensor> q_starts, double scale, bool need_q,
                                                   bool need_kv);
 
+// [y, sum, rstd, post_rstd]; [dx, dresidual, dweight, dpost_weight, dgate], undefined where not asked for.
+std::vector<at::Tensor> GatedAddRmsNorm_forward(const at::Tensor x, const at::Tensor weight, const at::Tensor residual,
+                                                const std::optional<at::Tensor> post_weight,
+                                                const std::optional<at::Tensor> gate, double scale, double eps, bool need_rstd);
+std::vector<at::Tensor> GatedAddRmsNorm_backward(const at::Tensor grad_y, const std::optional<at::Tensor> grad_sum,
+                                                 const at::Tensor x, const at::Tensor weight, const at::Tensor residual,
+                                                 const std::optional<at::Tensor> post_weight,
+                                                 const std::optional<at::Tensor> gate, const at::Tensor rstd,
+                                                 const std::optional<at::Tensor> post_rstd, double scale, double eps,
+                                                 bool need_weight, bool need_post_weight, bool need_gate);
 // state, last and their gradients: fp32 [batch, heads, key channels, value channels]; undefined where not asked for.
 std::vector<at::Tensor> DecayAttention_forward(const at::Tensor q, const at::Tensor k, const at::Tensor v,
                                                const at::Tensor log_decay, const std::optional<at::Tensor> state,
@@ -54,6 +64,9 @@ at::Tensor SoftmaxAttention(const at::Tensor q, const at::Tensor k, const at::Te
                             bool causal, const std::optional<at::Tensor> k_lengths,
                             const std::optional<at::Tensor> q_lengths, const std::optional<at::Tensor> q_starts,
                             double scale);
+std::vector<at::Tensor> GatedAddRmsNorm(const at::Tensor x, const at::Tensor weight, const at::Tensor residual,
+                                        const std::optional<at::Tensor> post_weight, const std::optional<at::Tensor> gate,
+                                        double scale, double eps);
 // [out] or [out, last].
 std::vector<at::Tensor> DecayAttention(const at::Tensor q, const at::Tensor k, const at::Tensor v, const at::Tensor log_decay,
                                        const std::optional<at::Tensor> state, const std::optional<at::Tensor> lengths,

@@ -84,6 +84,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Rotary (q, k or None, positions, sections, base, interleaved) -> [q', k'], with autograd");
   m.def("SoftmaxAttention", &SoftmaxAttention,
         "SoftmaxAttention (q, k, v, mask, causal, k_lengths, q_lengths, q_starts, scale) -> out, with autograd");
+  m.def("GatedAddRmsNorm", &GatedAddRmsNorm,
+        "GatedAddRmsNorm (x, weight, residual, post_weight or None, gate or None, scale, eps) -> [y, sum], with autograd");
   m.def("DecayAttention", &DecayAttention,
         "DecayAttention (q, k, v, log_decay, state or None, lengths or None, scale, return_state) -> [out] or [out, state], "
         "with autograd");

@@ -91,3 +91,73 @@ def decay(q, k, v, log_decay, scale, state=None, lengths=None, g=None, g_last=No
     ds = whole * R + scale * T(Q * ahead) @ g
     res["dstate"] = rounded(ds, whole * R.abs() + scale * T(Q.abs() * ahead) @ g.abs(), 0.0, U32)
     return res
+
+
+def gated_norm(x, weight, residual, post_weight, gate, scale, eps, gy=None, gs=None):
+    """{name: (reference, bound)}: y, sum and, if gy is given, dx, dres, dw, dwp and dgate.
+
+    First-order error propagation through the formula: a mean over a row is off by c = 96 U32 of its terms'
+    magnitudes (at most 64 terms in a thread and a tree of ten, and the root's), a product by U32."""
+    u, W = unit(x.dtype), x.shape[-1]
+    c = 96 * U32
+    mean = lambda t: t.mean(-1, keepdim=True)  # noqa: E731
+    X, r, w = x.double(), residual.double(), weight.double()
+    if post_weight is not None:
+        rx = 1.0 / (mean(X.square()) + eps).sqrt()
+        m, wp = X * rx, post_weight.double()
+        err_m = c * m.abs()
+    else:
+        rx, m, wp, err_m = torch.ones(()).double(), X, torch.ones(W).double(), 0.0 * X
+    g = gate.double() if gate is not None else torch.ones(W).double()
+    z = m * wp
+    err_z = err_m * wp.abs() + U32 * z.abs()
+    s = r + scale * g * z
+    err_s = abs(scale) * g.abs() * (err_z + 3 * U32 * z.abs()) + U32 * s.abs()
+    ms = mean(s.square()) + eps
+    rs = 1.0 / ms.sqrt()
+    rel = mean(s.abs() * err_s) / ms + c
+    n = s * rs
+    err_n = rs * err_s + (rel + U32) * n.abs()
+    y = n * w
+    err_y = err_n * w.abs() + U32 * y.abs()
+    res = {"y": (y, err_y + u * (y.abs() + err_y)), "sum": (s, err_s + u * (s.abs() + err_s))}
+    if gy is None:
+        return res
+    G = gy.double()
+    gn = G * w
+    dot = mean(gn * n)
+    err_dot = mean(gn.abs() * err_n) + (c + 2 * U32) * mean((gn * n).abs())
+    core = rs * (gn - n * dot)
+    err_ds = rs * (err_n * dot.abs() + n.abs() * err_dot) + (rel + 4 * U32) * rs * (gn.abs() + (n * dot).abs())
+    ds = core + (gs.double() if gs is not None else 0.0)
+    err_ds = err_ds + U32 * ds.abs()
+    rows = max(1, x.numel() // W)
+    flat = lambda t: t.expand_as(X).reshape(-1, W)  # noqa: E731
+
+    def summed(terms, err, like):
+        """Over the dimensions that `like` has once."""
+        if like.dim() == 1:
+            total, e, size = flat(terms).sum(0), flat(err).sum(0), flat(terms.abs()).sum(0)
+        else:
+            dims = [i for i in range(like.dim()) if like.shape[i] == 1 and terms.shape[i] != 1]
+            pick = lambda t: t.sum(dims, keepdim=True) if dims else t  # noqa: E731
+            total, e, size = pick(terms), pick(err), pick(terms.abs())
+        e = e + (rows + 8) * U32 * size
+        return total, e + unit(like.dtype) * (total.abs() + e)
+
+    dm = scale * g * wp * ds
+    err_dm = (scale * g * wp).abs() * err_ds + 4 * U32 * dm.abs()
+    if post_weight is not None:
+        back = mean(dm * m)
+        err_back = mean(err_dm * m.abs() + dm.abs() * err_m) + (c + 2 * U32) * mean((dm * m).abs())
+        dx = rx * (dm - m * back)
+        err_x = rx * (err_dm + err_m * back.abs() + m.abs() * err_back) + (c + 4 * U32) * rx * (dm.abs() + (m * back).abs())
+        res["dwp"] = summed(scale * g * ds * m, abs(scale) * g.abs() * (err_ds * m.abs() + ds.abs() * err_m), post_weight)
+    else:
+        dx, err_x = dm, err_dm
+    res["dx"] = (dx, err_x + u * (dx.abs() + err_x))
+    res["dres"] = (ds, err_ds + u * (ds.abs() + err_ds))
+    res["dw"] = summed(G * n, G.abs() * err_n, weight)
+    if gate is not None:
+        res["dgate"] = summed(scale * ds * z, abs(scale) * (err_ds * z.abs() + ds.abs() * err_z), gate)
+    return res
