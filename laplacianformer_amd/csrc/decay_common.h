@@ -24,7 +24,10 @@
 //   out_i = a^(c-1-i) R^T q_i + sum over j >= i of a^(j-i) scale (q_i . k_j) v_j,
 //   R'    = a^c R + scale sum over j of a^(j+1) k_j v_j^T.
 //
-// Where heads are few, a sequence is cut into segments: their own states first (decay_state kernel), those
+// A run's first tile may be short, the others are whole: forwards the tiles end where the sequence does,
+// backwards they begin where it does. Only a (c) and the query's power a^(c-1-i) or a^(i+1) know of it.
+//
+// Where heads are few, a sequence is cut into segments: their own states first (the kernel without OUT), those
 // joined in order (decay_join_kernel), then every segment from the state in front of it.
 #pragma once
 
@@ -70,6 +73,14 @@ __device__ __forceinline__ float decay_pow(float lg, int n) { return n == 0 ? 1.
 // The same in 64 bits: the factor of a whole tile or segment, which powers are taken of.
 __device__ __forceinline__ float decay_pow64(float lg, int n) { return n == 0 ? 1.0f : (float)exp((double)lg * (double)n); }
 
+// The tokens of a segment of a sequence of len: cut from its end if it is run forwards, from its start if backwards.
+__device__ __forceinline__ void decay_segment(const DecayArgs& a, int len, int seg, bool rev, int* begin, int* end) {
+  const int64_t span = (int64_t)a.segTiles * kDecayTile;
+  const int64_t at = rev ? seg * span : len - (a.nseg - seg) * span;
+  *begin = (int)min(max(at, (int64_t)0), (int64_t)len);
+  *end = (int)min(max(at + span, (int64_t)0), (int64_t)len);
+}
+
 template <typename T> __device__ __forceinline__ float low_half(uint32_t w);
 template <typename T> __device__ __forceinline__ float high_half(uint32_t w);
 template <> __device__ __forceinline__ float low_half<bf16s>(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
@@ -77,20 +88,19 @@ template <> __device__ __forceinline__ float high_half<bf16s>(uint32_t w) { retu
 template <> __device__ __forceinline__ float low_half<f16s>(uint32_t w) { return to_acc(f16s{(uint16_t)w}); }
 template <> __device__ __forceinline__ float high_half<f16s>(uint32_t w) { return to_acc(f16s{(uint16_t)(w >> 16)}); }
 
-// Eight values as NP pieces of an operand.
+// Eight values as NP pieces of an operand. (Without loops, as all of a step is: the compiler moves the products
+// behind every block boundary that a step has, and all of their operands then wait in registers.)
 template <typename T, int NP> __device__ __forceinline__ void split_pieces(f32x8 x, Frag<T> (&f)[NP]) {
   if constexpr (sizeof(T) == 4) {
     f[0].v = x;
   } else {
-#pragma unroll
-    for (int p = 0; p < NP; ++p)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w = pack2<T>(x[2 * j], x[2 * j + 1]);
-        f[p].v[j] = w;
-        x[2 * j] -= low_half<T>(w);
-        x[2 * j + 1] -= high_half<T>(w);
-      }
+    unrolled<4 * NP>([&](auto y) {
+      constexpr int p = y / 4, j = y % 4;
+      const uint32_t w = pack2<T>(x[2 * j], x[2 * j + 1]);
+      f[p].v[j] = w;
+      x[2 * j] -= low_half<T>(w);
+      x[2 * j + 1] -= high_half<T>(w);
+    });
   }
 }
 
@@ -118,23 +128,34 @@ template <typename T, int DC, int THREADS> struct DecayLoader {
   static constexpr int CHUNKS = kDecayTile * L::CPR, NIT = (CHUNKS + THREADS - 1) / THREADS;
   static_assert(CHUNKS % 64 == 0, "whole waves");
 
-  // first: the tile's first row (uniform); rows: how many of it exist.
-  static __device__ __forceinline__ void fill(char* tile, const T* first, int64_t stride, int rows, int D, int mode) {
+  // first: the tile's row 0 (uniform); rows from lo on and below hi exist.
+  static __device__ __forceinline__ void fill(char* tile, const T* first, int64_t stride, int lo, int hi, int D, int mode) {
     const uint32_t rowBytes = (uint32_t)stride * (uint32_t)sizeof(T);
     const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tile;
     const int wave = uniform(threadIdx.x >> 6);
+    if (__builtin_expect(mode == kAsync && hi - lo == kDecayTile && D == DP, 1)) {
+      // The loop's ordinary case: no branch between its loads.
 #pragma unroll
+      for (int i = 0; i < NIT; ++i) {
+        const int s = i * THREADS + (int)threadIdx.x;
+        if (CHUNKS % THREADS != 0 && i * THREADS + wave * 64 >= CHUNKS) break;
+        const int r = s / L::CPR, c = (s % L::CPR) ^ L::swz(r);
+        load_to_lds<16>(first, (uint32_t)r * rowBytes + (uint32_t)c * 16, to + (i * THREADS + wave * 64) * 16);
+      }
+      return;
+    }
+#pragma unroll 1
     for (int i = 0; i < NIT; ++i) {
       const int s = i * THREADS + (int)threadIdx.x;
       if (CHUNKS % THREADS != 0 && i * THREADS + wave * 64 >= CHUNKS) break;
       const int r = s / L::CPR, c = (s % L::CPR) ^ L::swz(r);
       if (mode == kAsync) {
-        if (r < rows && c * L::CE < D)
+        if (r >= lo && r < hi && c * L::CE < D)
           load_to_lds<16>(first, (uint32_t)r * rowBytes + (uint32_t)c * 16, to + (i * THREADS + wave * 64) * 16);
         else if (c * L::CE < DC)
           *(u32x4*)(tile + s * 16) = (u32x4){0, 0, 0, 0};
       } else {
-        *(u32x4*)(tile + s * 16) = load_chunk<T>(first + (int64_t)r * stride, r < rows, c * L::CE, D);
+        *(u32x4*)(tile + s * 16) = load_chunk<T>(first + (int64_t)r * stride, r >= lo && r < hi, c * L::CE, D);
       }
     }
   }
@@ -151,12 +172,9 @@ template <typename T, int DP> struct DealtRow {
   static __device__ __forceinline__ Frag<T> read(const char* tile, int dl, int t) {
     Frag<T> f;
     if constexpr (sizeof(T) == 2) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const u32x2 y = *(const u32x2*)(tile + (dl ^ ((2 * t + u) << 4)));
-        f.v[2 * u] = y[0];
-        f.v[2 * u + 1] = y[1];
-      }
+      const u32x2 a = *(const u32x2*)(tile + (dl ^ ((2 * t) << 4)));
+      const u32x2 b = *(const u32x2*)(tile + (dl ^ ((2 * t + 1) << 4)));
+      f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3);
     } else {
       const f32x4 a = *(const f32x4*)(tile + (dl ^ ((4 * t) << 4)));
       const f32x4 b = *(const f32x4*)(tile + (dl ^ ((4 * t + 2) << 4)));
@@ -178,6 +196,7 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
   constexpr int THREADS = DV * 2, NT = DK / 16, ND = DK / 32, TILE = kDecayTile;
   constexpr int NPP = DecayPieces<T>::P, NPS = DecayPieces<T>::S, NPV = DecayPieces<T>::V;
   constexpr bool F16 = std::is_same<T, f16s>::value;
+  constexpr int AHEAD = sizeof(T) == 2 ? 3 : 1;  // fragment reads in flight in front of their products
   using LK = DecayLoader<T, DK, THREADS>;
   using LV = DecayLoader<T, DV, THREADS>;
   using TK = typename LK::L;
@@ -194,8 +213,10 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
   const bool rev = jb.reverse;
   const float lg = a.logDecay[hq];
   const int len = uniform(decay_length(a, b));
-  const int t0 = seg * a.segTiles * TILE, t1 = (int)min((int64_t)len, (int64_t)t0 + (int64_t)a.segTiles * TILE);  // its tokens
-  const int tiles = t1 > t0 ? (t1 - t0 + TILE - 1) / TILE : 0;
+  int begin, end;
+  decay_segment(a, len, seg, rev, &begin, &end);
+  const int tiles = (end - begin + TILE - 1) / TILE;
+  const int short_ = end - begin - (tiles - 1) * TILE;  // tokens of the tile that is run first
   const int dk = jb.dk, dv = jb.dv;
   const int c = 32 * wave + i;  // this lane's value column
 
@@ -204,12 +225,14 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
   const T* qp = OUT ? uniform_ptr((const T*)jb.q + (int64_t)b * jb.qs[0] + (int64_t)uniform(hq / jb.qg) * jb.qs[1]) : nullptr;
   const int64_t ooff = (int64_t)b * jb.os[0] + (int64_t)hq * jb.os[1];
 
+  // Row 0 of the n-th tile that is run; the first may lack rows in front (forwards) or behind.
+  auto tile_at = [&](int n) { return rev ? begin + (tiles - 1 - n) * TILE : end - (tiles - n) * TILE; };
   auto fill = [&](int buf, int n) {
-    const int at = t0 + (rev ? tiles - 1 - n : n) * TILE, rows = min(TILE, t1 - at);
+    const int at = tile_at(n), lo = n || rev ? 0 : TILE - short_, hi = n || !rev ? TILE : short_;
     char* to = smem + buf * BUF;
-    LK::fill(to, kp + (int64_t)at * jb.ks[2], jb.ks[2], rows, dk, jb.modeK);
-    LV::fill(to + BK, vp + (int64_t)at * jb.vs[2], jb.vs[2], rows, dv, jb.modeV);
-    if constexpr (OUT) LK::fill(to + BK + BV, qp + (int64_t)at * jb.qs[2], jb.qs[2], rows, dk, jb.modeQ);
+    LK::fill(to, kp + (int64_t)at * jb.ks[2], jb.ks[2], lo, hi, dk, jb.modeK);
+    LV::fill(to + BK, vp + (int64_t)at * jb.vs[2], jb.vs[2], lo, hi, dv, jb.modeV);
+    if constexpr (OUT) LK::fill(to + BK + BV, qp + (int64_t)at * jb.qs[2], jb.qs[2], lo, hi, dk, jb.modeQ);
   };
   if (tiles) fill(0, 0);
 
@@ -232,49 +255,54 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
 
   // Powers of the decay: of a score's distance (0 outside the triangle), of a token's to the state that it goes
   // into, of the query's from the state in front, and of a whole tile.
-  f32x16 pw, gam;
-  float lam = 0.0f, whole = 1.0f;
   auto row_of = [&](int r) { return 8 * (r >> 2) + 4 * h + (r & 3); };
-  auto tables = [&](int rows) {
+  f32x16 pw, gam;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int j = row_of(r);
-      gam[r] = jb.sk * decay_pow(lg, rev ? j + 1 : max(rows - 1 - j, 0));
-    }
-    lam = jb.so * decay_pow(lg, rev ? max(rows - 1 - i, 0) : i + 1);
-    whole = decay_pow64(lg, rows);
-  };
-  tables(TILE);
-  if constexpr (OUT) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int n = rev ? row_of(r) - i : i - row_of(r);
-      pw[r] = n < 0 ? 0.0f : jb.sp * decay_pow(lg, n);
-    }
+  for (int r = 0; r < 16; ++r) {
+    const int j = row_of(r), n = rev ? j - i : i - j;
+    gam[r] = jb.sk * decay_pow(lg, rev ? j + 1 : TILE - 1 - j);
+    if constexpr (OUT) pw[r] = n < 0 ? 0.0f : jb.sp * decay_pow(lg, n);
   }
+  const int ahead = TILE - short_;  // rows that the first tile lacks
+  float lam = jb.so * decay_pow(lg, max(rev ? short_ - 1 - i : i + 1 - ahead, 0));
+  const float lams = jb.so * decay_pow(lg, rev ? TILE - 1 - i : i + 1);
+  float whole = decay_pow64(lg, max(short_, 0));
+  const float wholes = decay_pow64(lg, TILE);
 
-  const int krl = TK::row_lane(lane), kcl = TK::col_lane(lane), vcl = TV::col_lane(lane), qdl = DR::lane_offset(lane);
+  const int kcl0 = TK::col_lane(lane), vcl = TV::col_lane(lane), dl0 = DR::lane_offset(lane);
+  struct KQ {
+    Frag<T> k, q;
+  };
+  // The lane's four output columns of every eight, and where they go.
+  const bool wide = 32 * wave + 32 <= dv;
+  const int64_t step = (rev ? -TILE : TILE) * jb.os[2];
+  int64_t off = ooff + (int64_t)(tile_at(0) + i) * jb.os[2] + 32 * wave + 4 * h;
   int unit = 0;  // fp16: st holds the state times 2^unit
   land();
   __syncthreads();
   for (int n = 0; n < tiles; ++n) {
-    const int buf = n & 1, at = t0 + (rev ? tiles - 1 - n : n) * TILE, rows = min(TILE, t1 - at);
+    const int buf = n & 1;
     if (n + 1 < tiles) fill(buf ^ 1, n + 1);
-    if (rows < TILE) tables(rows);  // the sequence's last tile
-    else if (rev && n == 1) tables(TILE);  // and the ones in front of it
     const char* tk = smem + buf * BUF;
     const char* tv = tk + BK;
     const char* tq = tv + BV;
+    // Two addresses of one offset: reads of both tiles from one would be merged, and their halves copied apart.
+    const int dlk = launder(dl0), dlq = launder(dl0), kcl = launder(kcl0);
     Frag<T> vf[2];
+    auto read_v = [&] {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) vf[s] = TV::col_frag(tv, vcl, s, wave);
+      for (int s = 0; s < 2; ++s) vf[s] = TV::col_frag(tv, vcl, s, wave);
+    };
+    auto read_k = [&](auto x) { return TK::col_frag(tk, kcl, x & 1, x >> 1); };
+    Ring<Frag<T>, AHEAD> kring;
 
     f32x16 o = f32x16{};
     float back = 1.0f;  // fp16: what takes the output out of its unit
     if constexpr (OUT) {
+      Ring<KQ, AHEAD> ring;
+      auto read_kq = [&](auto t) { return KQ{DR::read(tk, dlk, t), DR::read(tq, dlq, t)}; };
+      first_reads<NT, AHEAD>(ring, read_kq);
       f32x16 p = f32x16{};
-#pragma unroll
-      for (int t = 0; t < NT; ++t) p = mma<T>(TK::row_frag(tk, krl, t), TK::row_frag(tq, krl, t), p);
       float mul = 1.0f, front = lam;
       if constexpr (F16) {
         float top = 0.0f;
@@ -286,17 +314,19 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
         mul = __builtin_amdgcn_ldexpf(1.0f, e);
         front = __builtin_amdgcn_ldexpf(lam, -e - unit);
       }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        f32x8 x;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = st[t >> 1][8 * (t & 1) + j] * (F16 ? mul : 1.0f);
+      // Scores and memory by 16 channels: the pieces of one step's state are made while the products of the
+      // step before it run.
+      read_and_use<NT, AHEAD>(ring, read_kq, [&](auto t, const KQ& f) {
+        constexpr int m = t >> 1, e = 8 * (t & 1);
+        f32x8 x = __builtin_shufflevector(st[m], st[m], e, e + 1, e + 2, e + 3, e + 4, e + 5, e + 6, e + 7);
+        if constexpr (F16) x *= mul;
         Frag<T> sf[NPS];
         split_pieces<T, NPS>(x, sf);
-        const Frag<T> qf = DR::read(tq, qdl, t);
-#pragma unroll
-        for (int z = NPS - 1; z >= 0; --z) o = mma<T>(sf[z], qf, o);
-      }
+        p = mma<T>(f.k, f.q, p);
+        unrolled<NPS>([&](auto z) { o = mma<T>(sf[NPS - 1 - z], f.q, o); });
+      });
+      read_v();
+      first_reads<2 * ND, AHEAD>(kring, read_k);
 #pragma unroll
       for (int r = 0; r < 16; ++r) p[r] *= pw[r];
       if constexpr (F16) {
@@ -320,6 +350,9 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
 #pragma unroll
         for (int z = NPP - 1; z >= 0; --z) o = mma<T>(vf[s], pf[z], o);
       }
+    } else {
+      read_v();
+      first_reads<2 * ND, AHEAD>(kring, read_k);
     }
 
     // The state behind the tile.
@@ -346,40 +379,40 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[s][j] *= f;
     }
+    Frag<T> xf[2][NPV];
 #pragma unroll
-    for (int m = 0; m < ND; ++m)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) st[m][r] *= keep;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      Frag<T> xf[NPV];
-      split_pieces<T, NPV>(x[s], xf);
-#pragma unroll
-      for (int m = 0; m < ND; ++m) {
-        const Frag<T> kf = TK::col_frag(tk, kcl, s, m);
-#pragma unroll
-        for (int z = NPV - 1; z >= 0; --z) st[m] = mma<T>(kf, xf[z], st[m]);
-      }
-    }
+    for (int s = 0; s < 2; ++s) split_pieces<T, NPV>(x[s], xf[s]);
+    read_and_use<2 * ND, AHEAD>(kring, read_k, [&](auto y, const Frag<T>& kf) {
+      constexpr int m = y >> 1, s = y & 1;
+      if constexpr (s == 0) st[m] *= keep;
+      unrolled<NPV>([&](auto z) { st[m] = mma<T>(kf, xf[s][NPV - 1 - z], st[m]); });
+    });
 
     land();  // the next tile; in front of the stores, so that they are not waited for
     if constexpr (OUT) {
-      if (i < rows) {
-        const int64_t off = ooff + (int64_t)(at + i) * jb.os[2];
+      if (n || (rev ? i < short_ : i >= ahead)) {
+        if (wide && !jb.outF32) {
+          T* to = (T*)jb.out + off;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int c0 = 32 * wave + 8 * u + 4 * h;
-          if (jb.outF32) store4<float>((float*)jb.out + off, c0, dv, o[4 * u] * back, o[4 * u + 1] * back, o[4 * u + 2] * back, o[4 * u + 3] * back);
-          else store4<T>((T*)jb.out + off, c0, dv, o[4 * u] * back, o[4 * u + 1] * back, o[4 * u + 2] * back, o[4 * u + 3] * back);
+          for (int u = 0; u < 4; ++u) store4<T>(to + 8 * u, 0, 4, o[4 * u] * back, o[4 * u + 1] * back, o[4 * u + 2] * back, o[4 * u + 3] * back);
+        } else {
+          const int left = dv - 32 * wave - 4 * h;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (jb.outF32) store4<float>((float*)jb.out + off, 8 * u, left, o[4 * u] * back, o[4 * u + 1] * back, o[4 * u + 2] * back, o[4 * u + 3] * back);
+            else store4<T>((T*)jb.out + off, 8 * u, left, o[4 * u] * back, o[4 * u + 1] * back, o[4 * u + 2] * back, o[4 * u + 3] * back);
+          }
         }
       }
+      off += step;
     }
+    lam = lams, whole = wholes;
     __syncthreads();
   }
 
   float* to = nullptr;
   if constexpr (OUT) {
-    if (jb.last && seg == (rev || len == 0 ? 0 : (len - 1) / (a.segTiles * TILE))) to = jb.last + (int64_t)bh * dk * dv;
+    if (jb.last && seg == (rev ? 0 : a.nseg - 1)) to = jb.last + (int64_t)bh * dk * dv;
   } else {
     to = jb.seg + ((int64_t)bh * a.nseg + seg) * dk * dv;
   }
@@ -395,12 +428,12 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
   }
   if constexpr (OUT) {
     // Tokens behind the sequence's length are zero.
-    const int end = (int)min((int64_t)a.N, (int64_t)t0 + (int64_t)a.segTiles * TILE);
-    for (int t = max(len, t0) + (int)threadIdx.x / 32; t < end; t += THREADS / 32) {
-      const int64_t off = ooff + (int64_t)t * jb.os[2];
-      for (int x = threadIdx.x & 31; x < dv; x += 32) {
-        if (jb.outF32) ((float*)jb.out)[off + x] = 0.0f;
-        else ((T*)jb.out)[off + x] = T{};
+    constexpr int RPP = THREADS / 32;
+    for (int64_t t = (int64_t)len + seg * RPP + (int)threadIdx.x / 32; t < a.N; t += a.nseg * RPP) {
+      const int64_t row = ooff + t * jb.os[2];
+      for (int y = threadIdx.x & 31; y < dv; y += 32) {
+        if (jb.outF32) ((float*)jb.out)[row + y] = 0.0f;
+        else ((T*)jb.out)[row + y] = T{};
       }
     }
   }

@@ -36,9 +36,10 @@ __global__ void __launch_bounds__(256) decay_join_kernel(const DecayArgs a) {
     for (int u = 0; u < 8; ++u) {
       const int n = n0 + u, at = jb.reverse ? a.nseg - 1 - n : n;
       if (n >= a.nseg) break;
-      const int64_t left = (int64_t)len - (int64_t)at * span;
+      int begin, end;
+      decay_segment(a, len, at, jb.reverse, &begin, &end);
       p[(int64_t)at * size] = s;
-      s = fmaf(left >= span ? full : left > 0 ? decay_pow64(lg, (int)left) : 1.0f, s, own[u]);
+      s = fmaf(end - begin == span ? full : decay_pow64(lg, end - begin), s, own[u]);
     }
   }
 }
