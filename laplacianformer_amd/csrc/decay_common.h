@@ -88,8 +88,11 @@ template <> __device__ __forceinline__ float high_half<bf16s>(uint32_t w) { retu
 template <> __device__ __forceinline__ float low_half<f16s>(uint32_t w) { return to_acc(f16s{(uint16_t)w}); }
 template <> __device__ __forceinline__ float high_half<f16s>(uint32_t w) { return to_acc(f16s{(uint16_t)(w >> 16)}); }
 
-// Eight values as NP pieces of an operand. (Without loops, as all of a step is: the compiler moves the products
-// behind every block boundary that a step has, and all of their operands then wait in registers.)
+// Keeps what computes x in front: products of which nothing in a step is read are moved behind all steps
+// otherwise, and their operands wait in registers. There is no instruction in it that could read x early.
+__device__ __forceinline__ void hold(f32x16& x) { asm volatile("" : "+v"(x)); }
+
+// Eight values as NP pieces of an operand.
 template <typename T, int NP> __device__ __forceinline__ void split_pieces(f32x8 x, Frag<T> (&f)[NP]) {
   if constexpr (sizeof(T) == 4) {
     f[0].v = x;
@@ -161,6 +164,12 @@ template <typename T, int DC, int THREADS> struct DecayLoader {
   }
 };
 
+// LDS addresses as numbers: a pointer to the workgroup's memory, whose place the compiler does not know, costs an
+// addition for every read.
+template <typename X> __device__ __forceinline__ __attribute__((address_space(3))) X* lds(int at) {
+  return (__attribute__((address_space(3))) X*)(uint32_t)at;
+}
+
 // Row lane % 32 of a tile, the channels of step t as acc_frag deals them.
 template <typename T, int DP> struct DealtRow {
   using L = Tile<T, DP>;
@@ -169,20 +178,35 @@ template <typename T, int DP> struct DealtRow {
     if constexpr (sizeof(T) == 2) return r * L::ROW + (L::swz(r) << 4) + 8 * h;
     else return r * L::ROW + ((h ^ L::swz(r)) << 4);
   }
-  static __device__ __forceinline__ Frag<T> read(const char* tile, int dl, int t) {
+  // dl: the lane's offset with the tile's LDS address.
+  static __device__ __forceinline__ Frag<T> read(int dl, int t) {
     Frag<T> f;
     if constexpr (sizeof(T) == 2) {
-      const u32x2 a = *(const u32x2*)(tile + (dl ^ ((2 * t) << 4)));
-      const u32x2 b = *(const u32x2*)(tile + (dl ^ ((2 * t + 1) << 4)));
+      const u32x2 a = *lds<u32x2>(dl ^ ((2 * t) << 4));
+      const u32x2 b = *lds<u32x2>(dl ^ ((2 * t + 1) << 4));
       f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3);
     } else {
-      const f32x4 a = *(const f32x4*)(tile + (dl ^ ((4 * t) << 4)));
-      const f32x4 b = *(const f32x4*)(tile + (dl ^ ((4 * t + 2) << 4)));
+      const f32x4 a = *lds<f32x4>(dl ^ ((4 * t) << 4));
+      const f32x4 b = *lds<f32x4>(dl ^ ((4 * t + 2) << 4));
       f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     return f;
   }
 };
+
+// Column 32 db + lane % 32 of contraction step s of a tile (Tile::col_frag). cl: col_lane with the tile's LDS address; at: that alone.
+template <typename T, int DP> __device__ __forceinline__ Frag<T> dealt_column(int at, int cl, int lane, int s, int db) {
+  using L = Tile<T, DP>;
+  if constexpr (sizeof(T) == 2) {
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<s16x4>((cl ^ (db << 6)) + 16 * s * L::ROW));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<s16x4>((cl ^ (db << 6) ^ 32) + (16 * s + 8) * L::ROW));
+    Frag<T> f;
+    f.v = __builtin_shufflevector(__builtin_bit_cast(u32x2, a), __builtin_bit_cast(u32x2, b), 0, 1, 2, 3);
+    return f;
+  } else {
+    return L::col_frag((const char*)lds<char>(at), lane, s, db);
+  }
+}
 
 // Bytes of LDS: two buffers of the three tiles (of two, for the states alone).
 template <typename T, int DK, int DV, bool OUT> constexpr size_t decay_lds() {
@@ -203,12 +227,14 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
   using TV = typename LV::L;
   using DR = DealtRow<T, LK::DP>;
   constexpr int BK = TILE * TK::ROW, BV = TILE * TV::ROW, BUF = (OUT ? 2 : 1) * BK + BV;
-  extern __shared__ __align__(16) char smem[];
+  extern __shared__ __align__(256) char smem[];
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, i = lane & 31;
-  const uint32_t place = xcd_place(blockIdx.x, gridDim.x);
-  const int seg = uniform(place % a.nseg), rest = uniform(place / a.nseg), bh = uniform(rest % (a.B * a.H));
-  const DecayJob& jb = a.job[uniform(rest / (a.B * a.H))];
+  // A segment's jobs side by side, on one XCD; the outputs from the last segment on, whose keys and values the
+  // states' launch has read last.
+  const uint32_t ahead_ = xcd_place(blockIdx.x, gridDim.x), place = OUT ? gridDim.x - 1 - ahead_ : ahead_;
+  const int rest = uniform(place / a.jobs), seg = uniform(rest % a.nseg), bh = uniform(rest / a.nseg);
+  const DecayJob& jb = a.job[uniform(place - rest * a.jobs)];
   const int b = uniform(bh / a.H), hq = bh - b * a.H;
   const bool rev = jb.reverse;
   const float lg = a.logDecay[hq];
@@ -269,41 +295,54 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
   float whole = decay_pow64(lg, max(short_, 0));
   const float wholes = decay_pow64(lg, TILE);
 
-  const int kcl0 = TK::col_lane(lane), vcl = TV::col_lane(lane), dl0 = DR::lane_offset(lane);
+  const int kcl0 = TK::col_lane(lane), vcl0 = TV::col_lane(lane), dl0 = DR::lane_offset(lane);
   struct KQ {
     Frag<T> k, q;
   };
+  const int base = (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
   // The lane's four output columns of every eight, and where they go.
   const bool wide = 32 * wave + 32 <= dv;
   const int64_t step = (rev ? -TILE : TILE) * jb.os[2];
   int64_t off = ooff + (int64_t)(tile_at(0) + i) * jb.os[2] + 32 * wave + 4 * h;
-  int unit = 0;  // fp16: st holds the state times 2^unit
+  float due = 1.0f;
+  int unit = 0;  // fp16: st holds the state times 2^unit as well
   land();
   __syncthreads();
   for (int n = 0; n < tiles; ++n) {
     const int buf = n & 1;
     if (n + 1 < tiles) fill(buf ^ 1, n + 1);
-    const char* tk = smem + buf * BUF;
-    const char* tv = tk + BK;
-    const char* tq = tv + BV;
-    // Two addresses of one offset: reads of both tiles from one would be merged, and their halves copied apart.
-    const int dlk = launder(dl0), dlq = launder(dl0), kcl = launder(kcl0);
+    // The buffer's place (a multiple of 256 bytes, which the exclusive-ors stay below) goes into the lane's offset. Two
+    // addresses of one offset: reads of both tiles from one would be merged, and their halves copied apart.
+    static_assert(BK % 256 == 0 && BV % 256 == 0, "tiles begin at a whole row of banks");
+    const int dlk = launder(dl0 + base + buf * BUF), dlq = launder(dl0 + base + buf * BUF + BK + BV);
+    const int kat = base + buf * BUF, vat = kat + BK, kcl = launder(kcl0 + kat), vcl = vcl0 + vat;
     Frag<T> vf[2];
     auto read_v = [&] {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) vf[s] = TV::col_frag(tv, vcl, s, wave);
+      for (int s = 0; s < 2; ++s) vf[s] = dealt_column<T, LV::DP>(vat, vcl, lane, s, wave);
     };
-    auto read_k = [&](auto x) { return TK::col_frag(tk, kcl, x & 1, x >> 1); };
-    Ring<Frag<T>, AHEAD> kring;
+    // Two of the state's row blocks at a time (the last alone if they are odd), so that neighbouring products do not
+    // wait for one another.
+    constexpr int PAIR = ND % 2 ? 1 : 2;
+    struct KF {
+      Frag<T> x[PAIR];
+    };
+    auto read_k = [&](auto y) {
+      KF f;
+      unrolled<PAIR>([&](auto e) { f.x[e] = dealt_column<T, LK::DP>(kat, kcl, lane, y & 1, (y >> 1) * PAIR + e); });
+      return f;
+    };
+    constexpr int KAHEAD = PAIR == 2 ? 1 : AHEAD;
+    Ring<KF, KAHEAD> kring;
 
     f32x16 o = f32x16{};
     float back = 1.0f;  // fp16: what takes the output out of its unit
     if constexpr (OUT) {
       Ring<KQ, AHEAD> ring;
-      auto read_kq = [&](auto t) { return KQ{DR::read(tk, dlk, t), DR::read(tq, dlq, t)}; };
+      auto read_kq = [&](auto t) { return KQ{DR::read(dlk, t), DR::read(dlq, t)}; };
       first_reads<NT, AHEAD>(ring, read_kq);
       f32x16 p = f32x16{};
-      float mul = 1.0f, front = lam;
+      float mul = 1.0f, front = lam * due;
       if constexpr (F16) {
         float top = 0.0f;
 #pragma unroll
@@ -312,7 +351,7 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
           for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(st[m][r]));
         const int e = 15 - min(max(__builtin_amdgcn_frexp_expf(wave_max(top)), -45), 120);
         mul = __builtin_amdgcn_ldexpf(1.0f, e);
-        front = __builtin_amdgcn_ldexpf(lam, -e - unit);
+        front = __builtin_amdgcn_ldexpf(front, -e - unit);
       }
       // Scores and memory by 16 channels: the pieces of one step's state are made while the products of the
       // step before it run.
@@ -322,11 +361,14 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
         if constexpr (F16) x *= mul;
         Frag<T> sf[NPS];
         split_pieces<T, NPS>(x, sf);
+        // Neighbours do not wait for one another.
+        if constexpr (NPS > 1) o = mma<T>(sf[NPS - 1], f.q, o);
         p = mma<T>(f.k, f.q, p);
-        unrolled<NPS>([&](auto z) { o = mma<T>(sf[NPS - 1 - z], f.q, o); });
+        o = mma<T>(sf[0], f.q, o);
+        if constexpr (sizeof(T) == 2) hold(o);
       });
       read_v();
-      first_reads<2 * ND, AHEAD>(kring, read_k);
+      first_reads<2 * ND / PAIR, KAHEAD>(kring, read_k);
 #pragma unroll
       for (int r = 0; r < 16; ++r) p[r] *= pw[r];
       if constexpr (F16) {
@@ -352,10 +394,11 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
       }
     } else {
       read_v();
-      first_reads<2 * ND, AHEAD>(kring, read_k);
+      first_reads<2 * ND / PAIR, KAHEAD>(kring, read_k);
     }
 
-    // The state behind the tile.
+    // The state behind the tile. st holds it over `due`, the decay that it has not been multiplied with yet:
+    // that is done when it falls below 2^-20, and what is added in between is divided by it.
     f32x8 x[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -363,29 +406,39 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[s][j] *= gam[8 * s + j];
     }
-    float keep = whole;
+    float keep = due * whole, f = 1.0f;
+    bool now = keep < 0x1p-20f;
     if constexpr (F16) {
       float top = 0.0f;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[s][j]));
-      const int next = 15 - min(max(__builtin_amdgcn_frexp_expf(wave_max(top)), -45), 60);
-      const float f = __builtin_amdgcn_ldexpf(1.0f, next);
-      keep = __builtin_amdgcn_ldexpf(whole, next - unit);
-      unit = next;
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[s][j] *= f;
+      top = wave_max(top);
+      const int e = min(max(__builtin_amdgcn_frexp_expf(top), -45), 60), over = __builtin_amdgcn_frexp_expf(top / keep) + unit;
+      now = now || over > 15 || over < 5;
+      if (now) keep = __builtin_amdgcn_ldexpf(keep, 15 - e - unit), unit = 15 - e;
+      f = __builtin_amdgcn_ldexpf(1.0f, unit);
     }
+    if (now) {
+#pragma unroll
+      for (int m = 0; m < ND; ++m) st[m] *= keep;
+      due = 1.0f;
+    } else {
+      due = keep;
+      f /= keep;
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) x[s] *= f;
     Frag<T> xf[2][NPV];
 #pragma unroll
     for (int s = 0; s < 2; ++s) split_pieces<T, NPV>(x[s], xf[s]);
-    read_and_use<2 * ND, AHEAD>(kring, read_k, [&](auto y, const Frag<T>& kf) {
-      constexpr int m = y >> 1, s = y & 1;
-      if constexpr (s == 0) st[m] *= keep;
-      unrolled<NPV>([&](auto z) { st[m] = mma<T>(kf, xf[s][NPV - 1 - z], st[m]); });
+    read_and_use<2 * ND / PAIR, KAHEAD>(kring, read_k, [&](auto y, const KF& kf) {
+      constexpr int m = (y >> 1) * PAIR, s = y & 1;
+      unrolled<NPV * PAIR>([&](auto z) {
+        constexpr int e = z % PAIR;
+        st[m + e] = mma<T>(kf.x[e], xf[s][NPV - 1 - z / PAIR], st[m + e]);
+      });
     });
 
     land();  // the next tile; in front of the stores, so that they are not waited for
@@ -393,8 +446,23 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
       if (n || (rev ? i < short_ : i >= ahead)) {
         if (wide && !jb.outF32) {
           T* to = (T*)jb.out + off;
+          if constexpr (sizeof(T) == 2) {
+            // The halves of a lane pair exchange four channels of every sixteen: 16 adjacent bytes each.
 #pragma unroll
-          for (int u = 0; u < 4; ++u) store4<T>(to + 8 * u, 0, 4, o[4 * u] * back, o[4 * u + 1] * back, o[4 * u + 2] * back, o[4 * u + 3] * back);
+            for (int u = 0; u < 4; u += 2) {
+              u32x4 w;
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const auto y = __builtin_amdgcn_permlane32_swap(pack2<T>(o[4 * u + 2 * e] * back, o[4 * u + 2 * e + 1] * back),
+                                                                pack2<T>(o[4 * u + 4 + 2 * e] * back, o[4 * u + 5 + 2 * e] * back), false, false);
+                w[e] = y[0], w[2 + e] = y[1];
+              }
+              __builtin_memcpy(to + 8 * u + 4 * h, &w, 16);
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) store4<T>(to + 8 * u, 0, 4, o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+          }
         } else {
           const int left = dv - 32 * wave - 4 * h;
 #pragma unroll
@@ -417,7 +485,7 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
     to = jb.seg + ((int64_t)bh * a.nseg + seg) * dk * dv;
   }
   if (to && c < dv) {
-    const float f = F16 ? __builtin_amdgcn_ldexpf(1.0f, -unit) : 1.0f;
+    const float f = F16 ? __builtin_amdgcn_ldexpf(due, -unit) : due;
 #pragma unroll
     for (int m = 0; m < ND; ++m)
 #pragma unroll
