@@ -27,8 +27,9 @@
 // A run's first tile may be short, the others are whole: forwards the tiles end where the sequence does,
 // backwards they begin where it does. Only a (c) and the query's power a^(c-1-i) or a^(i+1) know of it.
 //
-// Where heads are few, a sequence is cut into segments: their own states first (the kernel without OUT), those
-// joined in order (decay_join_kernel), then every segment from the state in front of it.
+// Where heads are few, a sequence is cut into segments, in one of two ways. Long ones: the segments' own states first
+// (the kernel without OUT), those joined in order (decay_join_kernel), then every segment from the state in front of
+// it. Short ones: every segment runs through all tiles in front of it for the state alone, in the one launch.
 #pragma once
 
 #include "attn_common.h"
@@ -48,7 +49,7 @@ struct DecayJob {
   int64_t qs[3], ks[3], vs[3], os[3]; // element strides of batch, head, token
   int qg, kg, vg;                     // query heads per head of q, k, v
   int dk, dv;
-  int reverse, outF32, firstT;        // firstT: first is [dv][dk]
+  int reverse, outF32, firstT, segT;  // firstT, segT: first, seg is [dv][dk]; segT: and another job's
   int modeQ, modeK, modeV;            // LoadMode, kPlain or kAsync
   float sp, so, sk;                   // scales of the scores, of the state's part and of what is added to the state
 };
@@ -58,6 +59,7 @@ struct DecayArgs {
   const float* logDecay;
   const int32_t* lengths;
   int B, H, N, jobs, nseg, segTiles;
+  int prefix;  // every segment forms the state in front of it by itself; otherwise decay_join_kernel has
 };
 
 // Pieces that a value is carried in.
@@ -136,28 +138,24 @@ template <typename T, int DC, int THREADS> struct DecayLoader {
     const uint32_t rowBytes = (uint32_t)stride * (uint32_t)sizeof(T);
     const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tile;
     const int wave = uniform(threadIdx.x >> 6);
-    if (__builtin_expect(mode == kAsync && hi - lo == kDecayTile && D == DP, 1)) {
-      // The loop's ordinary case: no branch between its loads.
+    if (mode == kAsync) {
+      // What is not loaded keeps the zeros that the kernel begins with: columns behind D never are, rows outside lack in a run's first
+      // tile alone.
+      const bool whole = hi - lo == kDecayTile;
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
         const int s = i * THREADS + (int)threadIdx.x;
         if (CHUNKS % THREADS != 0 && i * THREADS + wave * 64 >= CHUNKS) break;
         const int r = s / L::CPR, c = (s % L::CPR) ^ L::swz(r);
-        load_to_lds<16>(first, (uint32_t)r * rowBytes + (uint32_t)c * 16, to + (i * THREADS + wave * 64) * 16);
-      }
-      return;
-    }
-#pragma unroll 1
-    for (int i = 0; i < NIT; ++i) {
-      const int s = i * THREADS + (int)threadIdx.x;
-      if (CHUNKS % THREADS != 0 && i * THREADS + wave * 64 >= CHUNKS) break;
-      const int r = s / L::CPR, c = (s % L::CPR) ^ L::swz(r);
-      if (mode == kAsync) {
-        if (r >= lo && r < hi && c * L::CE < D)
+        if ((whole || (r >= lo && r < hi)) && (D == DP || c * L::CE < D))
           load_to_lds<16>(first, (uint32_t)r * rowBytes + (uint32_t)c * 16, to + (i * THREADS + wave * 64) * 16);
-        else if (c * L::CE < DC)
-          *(u32x4*)(tile + s * 16) = (u32x4){0, 0, 0, 0};
-      } else {
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < NIT; ++i) {
+        const int s = i * THREADS + (int)threadIdx.x;
+        if (CHUNKS % THREADS != 0 && i * THREADS + wave * 64 >= CHUNKS) break;
+        const int r = s / L::CPR, c = (s % L::CPR) ^ L::swz(r);
         *(u32x4*)(tile + s * 16) = load_chunk<T>(first + (int64_t)r * stride, r >= lo && r < hi, c * L::CE, D);
       }
     }
@@ -241,6 +239,12 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
   const int len = uniform(decay_length(a, b));
   int begin, end;
   decay_segment(a, len, seg, rev, &begin, &end);
+  int pre = 0;  // tiles that are run for the state alone
+  if (OUT && a.prefix && end > begin) {
+    pre = (rev ? len - end : begin) / TILE + ((rev ? len - end : begin) % TILE != 0);
+    if (rev) end = len;
+    else begin = 0;
+  }
   const int tiles = (end - begin + TILE - 1) / TILE;
   const int short_ = end - begin - (tiles - 1) * TILE;  // tokens of the tile that is run first
   const int dk = jb.dk, dv = jb.dv;
@@ -258,18 +262,23 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
     char* to = smem + buf * BUF;
     LK::fill(to, kp + (int64_t)at * jb.ks[2], jb.ks[2], lo, hi, dk, jb.modeK);
     LV::fill(to + BK, vp + (int64_t)at * jb.vs[2], jb.vs[2], lo, hi, dv, jb.modeV);
-    if constexpr (OUT) LK::fill(to + BK + BV, qp + (int64_t)at * jb.qs[2], jb.qs[2], lo, hi, dk, jb.modeQ);
+    if (OUT && n >= pre) LK::fill(to + BK + BV, qp + (int64_t)at * jb.qs[2], jb.qs[2], lo, hi, dk, jb.modeQ);
   };
+  if (tiles && (short_ < TILE || dk < LK::DP || dv < LV::DP)) {
+    for (int x = threadIdx.x * 16; x < 2 * BUF; x += THREADS * 16) *(u32x4*)(smem + x) = (u32x4){0, 0, 0, 0};
+    __syncthreads();
+  }
   if (tiles) fill(0, 0);
 
   // The state's rows 32 m + 8 (r / 4) + 4 h + r % 4 of column c.
   f32x16 st[ND];
 #pragma unroll
   for (int m = 0; m < ND; ++m) st[m] = f32x16{};
-  const float* from = !OUT ? nullptr : a.nseg > 1 ? jb.seg + ((int64_t)bh * a.nseg + seg) * dk * dv
+  const bool joined = a.nseg > 1 && !a.prefix;
+  const float* from = !OUT ? nullptr : joined ? jb.seg + ((int64_t)bh * a.nseg + seg) * dk * dv
                                      : jb.first ? jb.first + (int64_t)bh * dk * dv : nullptr;
   if (from && c < dv) {
-    const bool tr = a.nseg == 1 && jb.firstT;
+    const bool tr = joined ? jb.segT : jb.firstT;
 #pragma unroll
     for (int m = 0; m < ND; ++m)
 #pragma unroll
@@ -337,7 +346,8 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
 
     f32x16 o = f32x16{};
     float back = 1.0f;  // fp16: what takes the output out of its unit
-    if constexpr (OUT) {
+    const bool full = OUT && n >= pre;
+    if (full) {
       Ring<KQ, AHEAD> ring;
       auto read_kq = [&](auto t) { return KQ{DR::read(dlk, t), DR::read(dlq, t)}; };
       first_reads<NT, AHEAD>(ring, read_kq);
@@ -443,7 +453,7 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) de
 
     land();  // the next tile; in front of the stores, so that they are not waited for
     if constexpr (OUT) {
-      if (n || (rev ? i < short_ : i >= ahead)) {
+      if (full && (n || (rev ? i < short_ : i >= ahead))) {
         if (wide && !jb.outF32) {
           T* to = (T*)jb.out + off;
           if constexpr (sizeof(T) == 2) {

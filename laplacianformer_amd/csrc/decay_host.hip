@@ -153,13 +153,33 @@ int load_mode(const void* p, const int64_t* strides, int64_t d, int64_t size) {
              : kPlain;
 }
 
-// How many segments to cut the sequences of `runs` (runs of the operator times sequences times heads) into.
-void plan_segments(DecayArgs& a, int64_t runs, int dv) {
+// Into how many segments the sequences of `runs` (runs of the operator times sequences times heads) are cut, and
+// how their states are found: the least of what the busiest SIMD takes. A wave alone takes tf us for a tile (one
+// launch of 4 tiles against one of 1, one head: bf16 1.2 and 2.1 at 32 and 128 key channels, fp16 1.6 and 2.5, fp32
+// 2.8 and 7.4), ts for its state alone (one launch of 15 tiles in 15 segments: bf16 0.8 to 1.1, fp32 0.9 to 1.5), and
+// 3 us to begin. A SIMD holds two waves, which take one and a half times as long together (fp32, whose products
+// fill it alone, 1.9). Segments joined in launches of their own cost two more, 10 us, and four passes
+// over their states at 4 TB/s.
+void plan_segments(int dtype, DecayArgs& a, int64_t runs, int dk, int dv) {
+  const bool f32 = dtype == LFAMD_F32;
   const int64_t tiles = ((int64_t)a.N + kDecayTile - 1) / kDecayTile;
-  const int64_t want = (int64_t)num_cus() * (decay_value_dim(dv) == 128 ? 2 : decay_value_dim(dv) == 64 ? 4 : 8);
-  int64_t n = std::max<int64_t>(1, std::min<int64_t>({want / std::max<int64_t>(runs, 1), tiles / 4, 64}));
-  a.segTiles = (int)std::max<int64_t>(1, (tiles + n - 1) / n);
-  a.nseg = (int)std::max<int64_t>(1, (tiles + a.segTiles - 1) / a.segTiles);
+  const double width = decay_key_dim(dk);
+  const double tf = f32 ? 1.3 + 0.047 * width : (dtype == LFAMD_F16 ? 1.3 : 0.85) + 0.0095 * width;
+  const double ts = (f32 ? 0.35 : 0.58) * tf;
+  const double waves = (double)runs * (decay_value_dim(dv) / 32) / (4.0 * num_cus());
+  double least = 0.0;
+  for (int64_t n = 1; n <= 64 && n <= std::max<int64_t>(tiles, 1); ++n) {
+    const int64_t seg = std::max<int64_t>(1, (tiles + n - 1) / n);
+    if (n > 1 && (tiles + seg - 1) / seg != n) continue;  // fewer segments do the same
+    const int64_t w = std::max<int64_t>(1, (int64_t)ceil(waves * (double)n));
+    const double share = (double)(w / 2) * (f32 ? 1.9 : 1.5) + (double)(w % 2);
+    // The last segment has most in front of it.
+    const double prefix = ((double)(tiles - seg) * ts + (double)seg * tf + 3.0) * share;
+    const double joined = n == 1 ? prefix : ((double)seg * (tf + ts) + 6.0) * share + 10.0 + (double)(runs * n * dk * dv) * 16.0 / 4e6;
+    if (n > 1 && std::min(prefix, joined) >= least) continue;
+    least = std::min(prefix, joined);
+    a.nseg = (int)n, a.segTiles = (int)seg, a.prefix = n > 1 && prefix <= joined;
+  }
 }
 
 DecayArgs base_args(const lfamd_decay* d) {
@@ -175,11 +195,17 @@ int run_tiles(int dtype, const DecayArgs& a, int out, hipStream_t st) {
 
 // The jobs of `a`, whose channels computed with agree, through their segments.
 int run_jobs(int dtype, const DecayArgs& a, hipStream_t st) {
-  if (a.nseg > 1) {
-    if (int e = run_tiles(dtype, a, 0, st)) return e;
+  if (a.nseg > 1 && !a.prefix) {
+    DecayArgs s = a;  // the jobs whose states are formed
+    s.jobs = 0;
     int most = 0;
-    for (int j = 0; j < a.jobs; ++j) most = std::max(most, a.job[j].dk * a.job[j].dv);
-    decay_join_kernel<<<dim3(a.B * a.H, (most + 255) / 256, a.jobs), dim3(256), 0, st>>>(a);
+    for (int j = 0; j < a.jobs; ++j)
+      if (!a.job[j].segT) {
+        s.job[s.jobs++] = a.job[j];
+        most = std::max(most, a.job[j].dk * a.job[j].dv);
+      }
+    if (int e = run_tiles(dtype, s, 0, st)) return e;
+    decay_join_kernel<<<dim3(s.B * s.H, (most + 255) / 256, s.jobs), dim3(256), 0, st>>>(s);
     if (int e = check_launch("decay_attention")) return e;
   }
   return run_tiles(dtype, a, 1, st);
@@ -198,20 +224,21 @@ struct BackwardPlan {
   size_t segs[3], part[2], total;  // bytes of each run's segments (dq, dk, dv), of the shared heads' parts of dk and dv
 };
 
-BackwardPlan plan_backward(const lfamd_decay* d) {
+BackwardPlan plan_backward(int dtype, const lfamd_decay* d) {
   BackwardPlan p{};
   p.split = decay_key_dim((int)d->key_dim) != decay_key_dim((int)d->value_dim) ||
             decay_value_dim((int)d->key_dim) != decay_value_dim((int)d->value_dim);
   p.shared = d->kv_heads != d->heads;
   p.both = p.own = base_args(d);
   const int64_t bh = d->batch * d->heads;
-  plan_segments(p.both, bh * (p.split ? 2 : 3), (int)d->key_dim);
-  plan_segments(p.own, bh, (int)d->value_dim);
-  if (!p.split) p.own.nseg = p.both.nseg, p.own.segTiles = p.both.segTiles;
+  plan_segments(dtype, p.both, bh * (p.split ? 2 : 3), (int)d->value_dim, (int)d->key_dim);
+  if (p.split) plan_segments(dtype, p.own, bh, (int)d->key_dim, (int)d->value_dim);
+  else p.own.nseg = p.both.nseg, p.own.segTiles = p.both.segTiles, p.own.prefix = p.both.prefix;
   const size_t state = (size_t)bh * d->key_dim * d->value_dim * sizeof(float);
   for (int j = 0; j < 3; ++j) {
-    const int n = j == 2 ? p.own.nseg : p.both.nseg;
-    p.segs[j] = n > 1 ? round16(state * n) : 0;
+    const DecayArgs& a = j == 2 ? p.own : p.both;
+    // dk takes the states that dv forms, transposed, where the two are in one launch.
+    p.segs[j] = a.nseg > 1 && !a.prefix && !(j == 1 && !p.split) ? round16(state * a.nseg) : 0;
     p.total += p.segs[j];
   }
   const size_t rows = (size_t)bh * d->tokens * sizeof(float);
@@ -247,8 +274,8 @@ size_t lfamd_decay_attention_workspace_size(int dtype, const lfamd_decay* desc) 
   bool empty = false;
   if (check_desc("decay_attention", dtype, desc, &empty) || empty) return 0;
   DecayArgs a = base_args(desc);
-  plan_segments(a, desc->batch * desc->heads, (int)desc->value_dim);
-  return a.nseg > 1 ? (size_t)desc->batch * desc->heads * a.nseg * desc->key_dim * desc->value_dim * sizeof(float) : 0;
+  plan_segments(dtype, a, desc->batch * desc->heads, (int)desc->key_dim, (int)desc->value_dim);
+  return a.nseg > 1 && !a.prefix ? (size_t)desc->batch * desc->heads * a.nseg * desc->key_dim * desc->value_dim * sizeof(float) : 0;
 }
 
 int lfamd_decay_attention(int dtype, const lfamd_decay* desc, const void* q, const void* k, const void* v, const float* state,
@@ -260,7 +287,7 @@ int lfamd_decay_attention(int dtype, const lfamd_decay* desc, const void* q, con
   if (desc->tokens && (!q || !k || !v || !out)) return fail(LFAMD_ERR_ARG, "%s: null pointer", who);
   if (int e = check_workspace(who, workspace, workspace_bytes, lfamd_decay_attention_workspace_size(dtype, desc))) return e;
   DecayArgs a = base_args(desc);
-  plan_segments(a, desc->batch * desc->heads, (int)desc->value_dim);
+  plan_segments(dtype, a, desc->batch * desc->heads, (int)desc->key_dim, (int)desc->value_dim);
   const int64_t size = (int64_t)dtype_size(dtype);
   DecayJob& j = a.job[0];
   a.jobs = 1;
@@ -276,7 +303,7 @@ int lfamd_decay_attention(int dtype, const lfamd_decay* desc, const void* q, con
 size_t lfamd_decay_attention_backward_workspace_size(int dtype, const lfamd_decay* desc) {
   bool empty = false;
   if (check_desc("decay_attention backward", dtype, desc, &empty) || empty) return 0;
-  return plan_backward(desc).total;
+  return plan_backward(dtype, desc).total;
 }
 
 int lfamd_decay_attention_backward(int dtype, const lfamd_decay* desc, const void* q, const void* k, const void* v,
@@ -292,7 +319,7 @@ int lfamd_decay_attention_backward(int dtype, const lfamd_decay* desc, const voi
   if (empty || (!kv && !grads->grad_q && !grads->grad_state)) return ok();
   if (desc->tokens == 0 && !grads->grad_state) return ok();
   if (desc->tokens && (!q || !k || !v || !grads->grad_out)) return fail(LFAMD_ERR_ARG, "%s: null pointer", who);
-  BackwardPlan p = plan_backward(desc);
+  BackwardPlan p = plan_backward(dtype, desc);
   if (int e = check_workspace(who, workspace, workspace_bytes, p.total)) return e;
   char* ws = (char*)workspace;
   auto take = [&](size_t n) {
@@ -334,6 +361,7 @@ int lfamd_decay_attention_backward(int dtype, const lfamd_decay* desc, const voi
   if (kv && desc->tokens) {
     DecayJob j = job(V, O, Q, p.shared ? part[0] : grads->grad_k, p.shared ? rows[0] : grads->grad_k_strides, segs[1]);
     j.first = grads->grad_last_state, j.firstT = 1, j.reverse = 1, j.outF32 = p.shared, j.so = 1.0f, j.sk = desc->scale;
+    if (!p.split) j.seg = segs[2], j.segT = 1;
     a.job[a.jobs++] = j;
   }
   if (kv || grads->grad_state) {
