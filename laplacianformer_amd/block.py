@@ -1,7 +1,8 @@
 """Operators of a transformer block around the attention (no counterpart in the
 reference, which ships its two operators only): the norm with the residual's
-addition, rotary positions on the token grid, exact softmax attention, and
-``AttentionBlock``, which joins them with either attention.
+addition, alone or with the norm, gate and scale of the block in front of it, rotary positions
+on the token grid, exact softmax attention, linear attention with a decay for each head, and
+``AttentionBlock``, which joins them with any of the three attentions.
 
 All run on hand-written HIP kernels in float32, float16 and bfloat16 (float64 and CPU
 tensors are refused), take strided inputs where the last dimension's elements are
@@ -159,40 +160,62 @@ class AttentionBlock(torch.nn.Module):
     and k by their tokens' grid positions (rotary), attends, and projects back. It returns
     ``(out, sum)``: the next block's ``(x, residual)``, also under autocast, where out is of 16 bits and the
     sum stays float32 (x and residual of different types are widened to the wider one). ``attention`` is "softmax"
-    (softmax_attention, ``kv_heads`` key heads shared by ``heads`` query heads) or
-    "laplacian" (laplacian_attention with ``pool`` and ``iters``, one key head per query head, a grid of two
-    axes). Caches of keys and the 8-bit norm are for callers of the functions: the block takes neither.
+    (softmax_attention, ``kv_heads`` key heads shared by ``heads`` query heads), "decay" (decay_attention, causal, with
+    shared key heads too; its output, which no softmax has normalised, goes through a norm in front of the projection)
+    or "laplacian" (laplacian_attention with ``pool`` and ``iters``, one key head per query head, a grid of two
+    axes). ``log_decay`` are the heads' values for "decay" (default: log(1 - 2^-n), n from 5 to 12).
+
+    With ``post_norm`` the addition norms x, the block in front's output, with a weight of its own, and
+    ``residual_scale`` and forward's ``gate`` multiply what is added (gated_add_rms_norm). Caches of keys, states and
+    the 8-bit norm are for callers of the functions: the block takes none of them.
     """
 
     def __init__(self, dim: int, heads: int, kv_heads: int | None = None, attention: str = "softmax",
                  positions: bool = True, base: float = 10000.0, causal: bool = False, pool: int = 4, iters: int = 10,
-                 eps: float = 1e-6):
+                 eps: float = 1e-6, post_norm: bool = False, residual_scale: float = 1.0,
+                 log_decay: Sequence[float] | None = None):
         super().__init__()
         kv_heads = heads if kv_heads is None else kv_heads
         if dim % heads or heads % kv_heads:
             raise ValueError("dim must be divisible by heads, and heads by kv_heads")
-        if attention not in ("softmax", "laplacian"):
-            raise ValueError("attention must be 'softmax' or 'laplacian'")
+        if attention not in ("softmax", "laplacian", "decay"):
+            raise ValueError("attention must be 'softmax', 'laplacian' or 'decay'")
         if attention == "laplacian" and (causal or kv_heads != heads):
             raise ValueError("laplacian attention is not causal and shares no key heads")
-        self.heads, self.kv_heads, self.attention, self.causal = heads, kv_heads, attention, causal
+        if log_decay is not None and (attention != "decay" or len(log_decay) != heads):
+            raise ValueError("log_decay takes a value for each head of decay attention")
+        self.heads, self.kv_heads, self.attention = heads, kv_heads, attention
+        self.causal = causal or attention == "decay"
         self.positions, self.base, self.pool, self.iters, self.eps = positions, base, pool, iters, eps
+        self.residual_scale = residual_scale
         d = dim // heads
         self.weight = torch.nn.Parameter(torch.ones(dim))
         self.qkv = torch.nn.Linear(dim, (heads + 2 * kv_heads) * d)
         self.proj = torch.nn.Linear(dim, dim)
+        self.post_weight = torch.nn.Parameter(torch.ones(dim)) if post_norm else None
+        if attention == "decay":
+            if log_decay is None:
+                log_decay = [math.log1p(-2.0 ** -(5 + 7 * h / max(heads - 1, 1))) for h in range(heads)]
+            self.out_weight = torch.nn.Parameter(torch.ones(dim))
+            # No buffer: it stays float32 whatever type the module is taken to.
+            self._log_decay = torch.tensor(list(log_decay), dtype=torch.float32)
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, grid: Sequence[int] | None = None,
                 positions: torch.Tensor | None = None, mask: torch.Tensor | None = None,
-                lengths: torch.Tensor | None = None):
+                lengths: torch.Tensor | None = None, gate: torch.Tensor | None = None):
         """x, residual [B, N, dim]. ``grid``: the token grid, ``positions`` [axes, N] or [axes, B, N] in its
         place. With neither, the tokens of a causal block, or of a batch with ``lengths``, are sequences: one axis,
         whatever N is, so that a prefix has the same positions; else N has to be a square's.
-        ``mask`` and ``lengths`` (int32 [B], the tokens that each sequence has) go to softmax_attention."""
+        ``mask`` and ``lengths`` (int32 [B], the tokens that each sequence has) go to softmax_attention, ``lengths``
+        to decay_attention as well. ``gate`` multiplies what is added to the residual (gated_add_rms_norm's)."""
         B, N, C = x.shape
         d = C // self.heads
         if self.attention == "laplacian" and (mask is not None or lengths is not None):
             raise ValueError("laplacian attention takes neither mask nor lengths")
+        if self.attention == "decay" and mask is not None:
+            raise ValueError("decay attention takes no mask")
+        if gate is not None and residual is None:
+            raise ValueError("a gate is of what is added to a residual, and there is none")
         if grid is None and (self.attention == "laplacian" or self.positions and positions is None):
             side = math.isqrt(N)
             if self.causal or lengths is not None:
@@ -211,7 +234,12 @@ class AttentionBlock(torch.nn.Module):
             if x.dtype != residual.dtype:  # under autocast: a 16-bit projection beside the fp32 stream, which stays fp32
                 wide = torch.promote_types(x.dtype, residual.dtype)
                 x, residual = x.to(wide), residual.to(wide)
-            y, total = add_rms_norm(x, self.weight, residual, eps=self.eps)
+            if self.post_weight is None and gate is None and self.residual_scale == 1.0:
+                y, total = add_rms_norm(x, self.weight, residual, eps=self.eps)
+            else:
+                if gate is not None and gate.dtype != x.dtype:
+                    gate = gate.float()
+                y, total = gated_add_rms_norm(x, self.weight, residual, self.post_weight, gate, self.residual_scale, self.eps)
         qkv = self.qkv(y).view(B, N, self.heads + 2 * self.kv_heads, d).transpose(1, 2)
         q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1)
         if self.positions:
@@ -220,6 +248,11 @@ class AttentionBlock(torch.nn.Module):
             q, k = rotary(q, k, positions, rotary_sections(d, positions.shape[0]), self.base)
         if self.attention == "softmax":
             o = softmax_attention(q, k, v, mask=mask, causal=self.causal, k_lengths=lengths, q_lengths=lengths)
+        elif self.attention == "decay":
+            if self._log_decay.device != x.device:
+                self._log_decay = self._log_decay.to(x.device)
+            o = decay_attention(q, k, v, self._log_decay, lengths=lengths)
+            return self.proj(add_rms_norm(o.transpose(1, 2).reshape(B, N, C), self.out_weight, eps=self.eps)), total
         else:
             o = laplacian_attention(q.contiguous(), k.contiguous(), v.contiguous(), grid=tuple(grid), pool=self.pool,
                                     iters=self.iters)
