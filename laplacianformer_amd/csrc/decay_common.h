@@ -214,7 +214,7 @@ template <typename T, int DK, int DV, bool OUT> constexpr size_t decay_lds() {
 // Grid: jobs x B H x segments. OUT: the outputs; otherwise the segments' own states only. DK, DV: channels
 // computed with; a wave for every 32 of DV.
 template <typename T, int DK, int DV, bool OUT>
-__global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && DK >= 96 ? 1 : 2) decay_kernel(const DecayArgs a) {
+__global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && (DK >= 96 || (DK == 64 && DV == 32)) ? 1 : 2) decay_kernel(const DecayArgs a) {
   constexpr int THREADS = DV * 2, NT = DK / 16, ND = DK / 32, TILE = kDecayTile;
   constexpr int NPP = DecayPieces<T>::P, NPS = DecayPieces<T>::S, NPV = DecayPieces<T>::V;
   constexpr bool F16 = std::is_same<T, f16s>::value;
