@@ -451,15 +451,15 @@ typedef struct {
   float scale;
 } lfamd_decay;
 
-/* state may be NULL (zero), and so may last_state, which takes the state behind the last token and may be
- * state itself. The workspace (16-byte aligned; 0 bytes where the heads alone fill the chip) holds the
+/* state may be NULL (zero), and so may last_state, which takes the state behind the last token; the two must not
+ * overlap (LFAMD_ERR_ARG where they are the same). The workspace (16-byte aligned; 0 bytes where the heads alone fill the chip) holds the
  * states of the segments that long sequences are cut into. Deterministic. */
 size_t lfamd_decay_attention_workspace_size(int dtype, const lfamd_decay* desc);
 int lfamd_decay_attention(int dtype, const lfamd_decay* desc, const void* q, const void* k, const void* v, const float* state,
                           void* out, float* last_state, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients from the forward's inputs; nothing else is kept. grad_last_state NULL: zero. grad_q, grad_k and
- * grad_v together, and grad_state (with the two; fp32, like the states) may be NULL. Deterministic,
+ * grad_v together, and grad_state (with the two; fp32, like the states; not grad_last_state's memory) may be NULL. Deterministic,
  * without atomics; heads that share a key head are added in fp32. log_decay has no gradient. */
 typedef struct {
   const void* grad_out;

@@ -284,6 +284,8 @@ int lfamd_decay_attention(int dtype, const lfamd_decay* desc, const void* q, con
   bool empty = false;
   if (int e = check_desc(who, dtype, desc, &empty)) return e;
   if (empty || (desc->tokens == 0 && !last_state)) return ok();
+  // Segments read the first state while another writes the last one.
+  if (last_state && last_state == state) return fail(LFAMD_ERR_ARG, "%s: last_state must not be state", who);
   if (desc->tokens && (!q || !k || !v || !out)) return fail(LFAMD_ERR_ARG, "%s: null pointer", who);
   if (int e = check_workspace(who, workspace, workspace_bytes, lfamd_decay_attention_workspace_size(dtype, desc))) return e;
   DecayArgs a = base_args(desc);
@@ -316,6 +318,8 @@ int lfamd_decay_attention_backward(int dtype, const lfamd_decay* desc, const voi
   const bool kv = grads->grad_k != nullptr;
   if (kv != (grads->grad_v != nullptr)) return fail(LFAMD_ERR_ARG, "%s: grad_k and grad_v come together", who);
   if (desc->tokens && grads->grad_state && !kv) return fail(LFAMD_ERR_ARG, "%s: grad_state comes with grad_k and grad_v", who);
+  if (grads->grad_state && grads->grad_state == grads->grad_last_state)
+    return fail(LFAMD_ERR_ARG, "%s: grad_state must not be grad_last_state", who);
   if (empty || (!kv && !grads->grad_q && !grads->grad_state)) return ok();
   if (desc->tokens == 0 && !grads->grad_state) return ok();
   if (desc->tokens && (!q || !k || !v || !grads->grad_out)) return fail(LFAMD_ERR_ARG, "%s: null pointer", who);

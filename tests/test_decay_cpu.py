@@ -81,6 +81,9 @@ def test_decay_refusals(lib):
     assert f(long, ws=DUMMY, n=need - 1) == 1
     assert f(long, ws=ctypes.c_void_p(24), n=need) == 1 and b"aligned" in lib.lfamd_last_error()
 
+    assert lib.lfamd_decay_attention(0, ctypes.byref(decay()), DUMMY, DUMMY, DUMMY, DUMMY, DUMMY, DUMMY, NULL, 0, NULL) == 1
+    assert b"last_state" in lib.lfamd_last_error()  # the first state's memory
+
     def b(d, g, dt=0, ws=DUMMY, n=1 << 40):
         return lib.lfamd_decay_attention_backward(dt, ctypes.byref(d), DUMMY, DUMMY, DUMMY, NULL, ctypes.byref(g) if g else None, ws, n, NULL)
 
@@ -89,6 +92,7 @@ def test_decay_refusals(lib):
     assert b(decay(), L.DecayGrads(grad_out=16, grad_k=16)) == 1 and b"together" in lib.lfamd_last_error()
     assert b(decay(), L.DecayGrads(grad_out=16, grad_state=16)) == 1 and b"grad_state" in lib.lfamd_last_error()
     assert b(decay(), L.DecayGrads(grad_q=16)) == 1
+    assert b(decay(), L.DecayGrads(grad_out=16, grad_k=16, grad_v=16, grad_state=32, grad_last_state=32)) == 1
     assert b(decay(), full, ws=NULL) == 1 and b(decay(), full, ws=DUMMY, n=8) == 1  # shared heads: fp32 parts
     assert b(decay(), full, ws=ctypes.c_void_p(24)) == 1
     assert b(decay(), L.DecayGrads()) == 0 and b(decay(batch=0), full) == 0
