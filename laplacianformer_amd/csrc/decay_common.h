@@ -120,10 +120,16 @@ template <typename T> __device__ __forceinline__ f32x8 frag_values(const Frag<T>
   return x;
 }
 
+// The largest of a wave's values, without the LDS that a shuffle goes through (three in a row for each tile in fp16): lanes turned
+// round within 16, then the two exchanges of 16 and of 32 lanes.
+template <int TURN> __device__ __forceinline__ float turned_max(float x) {
+  return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + TURN, 0xf, 0xf, false)));
+}
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int s = 1; s < 32; s <<= 1) x = fmaxf(x, __shfl_xor(x, s));
-  return half_max(x);
+  x = turned_max<1>(turned_max<2>(turned_max<4>(turned_max<8>(x))));
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return half_max(fmaxf(__builtin_bit_cast(float, (uint32_t)p[0]), __builtin_bit_cast(float, (uint32_t)p[1])));
 }
 
 // The tile of tokens t0 .. into LDS: Tile<T, DP>'s layout by THREADS threads, whole waves at a time.
