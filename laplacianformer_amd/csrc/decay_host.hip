@@ -44,24 +44,29 @@ __global__ void __launch_bounds__(256) decay_join_kernel(const DecayArgs a) {
   }
 }
 
-// out[b][hk][n] = sum over the heads that share hk, in order, of part[b][h][n] (fp32), rounded once.
-template <typename T>
-__global__ void __launch_bounds__(256) decay_share_kernel(const float* part, T* out, int64_t s0, int64_t s1, int64_t s2, int B,
-                                                         int Hk, int G, int N, int D) {
-  const int packs = (D + 3) / 4;
+// out[b][hk][n] = sum over the heads that share hk, in order, of part[b][h][n] (fp32), rounded once: dk and dv.
+struct ShareArgs {
+  const float* part[2];
+  void* out[2];
+  int64_t s[2][3];
+  int D[2];
+  int B, Hk, G, N;
+};
+template <typename T> __global__ void __launch_bounds__(256) decay_share_kernel(const ShareArgs a) {
+  const int z = blockIdx.y, D = a.D[z], packs = (D + 3) / 4;
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= (int64_t)B * Hk * N * packs) return;
+  if (at >= (int64_t)a.B * a.Hk * a.N * packs) return;
   const int64_t row = at / packs;
   const int c = (int)(at - row * packs) * 4;
-  const int64_t bh = row / N, n = row - bh * N;
+  const int64_t bh = row / a.N, n = row - bh * a.N;
   float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int g = 0; g < G; ++g) {
-    const float* p = part + ((bh * G + g) * N + n) * D + c;
+  for (int g = 0; g < a.G; ++g) {
+    const float* p = a.part[z] + ((bh * a.G + g) * a.N + n) * D + c;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (c + j < D) x[j] += p[j];
   }
-  store4<T>(out + (bh / Hk) * s0 + (bh % Hk) * s1 + n * s2, c, D, x[0], x[1], x[2], x[3]);
+  store4<T>((T*)a.out[z] + (bh / a.Hk) * a.s[z][0] + (bh % a.Hk) * a.s[z][1] + n * a.s[z][2], c, D, x[0], x[1], x[2], x[3]);
 }
 
 struct StepArgs {
@@ -254,14 +259,6 @@ int check_workspace(const char* who, const void* ws, size_t have, size_t need) {
   return LFAMD_OK;
 }
 
-template <typename T>
-int share_heads(const float* part, void* out, const int64_t* s, const lfamd_decay* d, int64_t D, hipStream_t st) {
-  const int64_t n = d->batch * d->kv_heads * d->tokens * ((D + 3) / 4);
-  decay_share_kernel<T><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(
-      part, (T*)out, s[0], s[1], s[2], (int)d->batch, (int)d->kv_heads, (int)(d->heads / d->kv_heads), (int)d->tokens, (int)D);
-  return check_launch("decay_attention backward");
-}
-
 }  // namespace
 
 }  // namespace lfamd
@@ -380,18 +377,18 @@ int lfamd_decay_attention_backward(int dtype, const lfamd_decay* desc, const voi
   if (p.split && o.jobs)
     if (int e = run_jobs(dtype, o, st)) return e;
   if (p.shared && kv && desc->tokens) {
-    const struct {
-      const float* part;
-      void* out;
-      const int64_t* s;
-      int64_t D;
-    } each[2] = {{part[0], grads->grad_k, grads->grad_k_strides, dk}, {part[1], grads->grad_v, grads->grad_v_strides, dv}};
-    for (const auto& x : each) {
-      const int e = dtype == LFAMD_F32   ? share_heads<float>(x.part, x.out, x.s, desc, x.D, st)
-                    : dtype == LFAMD_F16 ? share_heads<f16s>(x.part, x.out, x.s, desc, x.D, st)
-                                         : share_heads<bf16s>(x.part, x.out, x.s, desc, x.D, st);
-      if (e) return e;
+    ShareArgs h{};
+    h.part[0] = part[0], h.part[1] = part[1], h.out[0] = grads->grad_k, h.out[1] = grads->grad_v;
+    set3(h.s[0], grads->grad_k_strides), set3(h.s[1], grads->grad_v_strides);
+    h.D[0] = dk, h.D[1] = dv, h.B = (int)desc->batch, h.Hk = (int)desc->kv_heads, h.G = G, h.N = (int)desc->tokens;
+    const int64_t packs = desc->batch * desc->kv_heads * desc->tokens * ((std::max(dk, dv) + 3) / 4);
+    const dim3 grid((unsigned)((packs + 255) / 256), 2), t(256);
+    switch (dtype) {
+      case LFAMD_F32: decay_share_kernel<float><<<grid, t, 0, st>>>(h); break;
+      case LFAMD_F16: decay_share_kernel<f16s><<<grid, t, 0, st>>>(h); break;
+      default: decay_share_kernel<bf16s><<<grid, t, 0, st>>>(h); break;
     }
+    return check_launch(who);
   }
   return ok();
 }
