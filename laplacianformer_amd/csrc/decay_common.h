@@ -30,6 +30,13 @@
 // Where heads are few, a sequence is cut into segments, in one of two ways. Long ones: the segments' own states first
 // (the kernel without OUT), those joined in order (decay_join_kernel), then every segment from the state in front of
 // it. Short ones: every segment runs through all tiles in front of it for the state alone, in the one launch.
+//
+// What bounds it (one MI355X, bf16): 32 heads over 8 key heads, 32768 tokens, 128 channels: 276 us for the outputs and
+// 103 for the states (HBM alone: 133 and 26). A wave issues some 530 VALU instructions (192 make the state's pieces, 120
+// the values', 48 the scores') and 52 matrix products for a tile, and the time is the sum of 4 cycles for each of
+// the former and 32 for each of the latter: the two do not overlap, whatever the waves. 64 heads, 16384 tokens, 64 channels:
+// 118 us forward (4.5 TB/s), 330 for the three gradients (1.4 GB, 4.2 TB/s): HBM. P and S in one piece instead of two
+// would take 365 instead of 418 us at the former and 2 % off the latter, for outputs 1.4 times as far off.
 #pragma once
 
 #include "attn_common.h"

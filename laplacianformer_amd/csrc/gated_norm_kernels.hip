@@ -17,6 +17,9 @@
 // dg = c wp A and dwp = c g A, one sum for both. Workgroups (for narrow rows, waves) walk pieces of the rows
 // that share a gate row in a fixed order, and a second kernel adds what they found in order: the same
 // call gives the same bits.
+// Measured on one MI355X: 8 x 2048 x 4096 bf16, a gate per sequence, 113 us forward (537 MB, 4.8 TB/s), 166 backward (805 MB,
+// 4.85 TB/s) and 15 for the partial rows; 64 x 196 x 333 fp32, a gate per channel, 17, 32 and 4 us (rows of 84 vectors
+// in a wave each: their own latencies).
 #include <math.h>
 
 #include <algorithm>
