@@ -155,7 +155,8 @@ template <typename T, int DC, int THREADS> struct DecayLoader {
       // What is not loaded keeps the zeros that the kernel begins with: columns behind D never are, rows outside lack in a run's first
       // tile alone.
       const bool whole = hi - lo == kDecayTile;
-#pragma unroll
+      constexpr int STEPS = sizeof(T) == 4 && NIT > 2 ? 2 : NIT;  // more would hold an address each through the kernel
+#pragma unroll STEPS
       for (int i = 0; i < NIT; ++i) {
         const int s = i * THREADS + (int)threadIdx.x;
         if (CHUNKS % THREADS != 0 && i * THREADS + wave * 64 >= CHUNKS) break;
@@ -231,7 +232,8 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && (DK >= 96 || (DK == 
   constexpr int THREADS = DV * 2, NT = DK / 16, ND = DK / 32, TILE = kDecayTile;
   constexpr int NPP = DecayPieces<T>::P, NPS = DecayPieces<T>::S, NPV = DecayPieces<T>::V;
   constexpr bool F16 = std::is_same<T, f16s>::value;
-  constexpr int AHEAD = sizeof(T) == 2 ? 3 : 1;  // fragment reads in flight in front of their products
+  // Fragment reads in flight in front of their products (fp32: none, its products take long and their fragments registers).
+  constexpr int AHEAD = sizeof(T) == 2 ? 3 : 0;
   using LK = DecayLoader<T, DK, THREADS>;
   using LV = DecayLoader<T, DV, THREADS>;
   using TK = typename LK::L;
@@ -345,7 +347,7 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && (DK >= 96 || (DK == 
     };
     // Two of the state's row blocks at a time (the last alone if they are odd), so that neighbouring products do not
     // wait for one another.
-    constexpr int PAIR = ND % 2 ? 1 : 2;
+    constexpr int PAIR = ND % 2 || sizeof(T) == 4 ? 1 : 2;
     struct KF {
       Frag<T> x[PAIR];
     };
@@ -541,16 +543,23 @@ template <typename T, int DK, int DV, bool OUT> int decay_launch(const DecayArgs
 
 // Channels computed with for `d`: of keys, of values.
 inline int decay_key_dim(int d) { return compute_dim(d); }
-inline int decay_value_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+// (In fp32 few value columns of 128 key channels would take more registers than a workgroup of few waves may be given:
+// its waves for the other columns run empty.)
+inline int decay_value_dim(bool f32, int dk, int dv) {
+  return f32 && decay_key_dim(dk) == 128 ? 128 : dv <= 32 ? 32 : dv <= 64 ? 64 : 128;
+}
 
 template <typename T, bool OUT> int decay_dispatch(const DecayArgs& a, hipStream_t st) {
   auto values = [&](auto dk) {
     constexpr int DK = decltype(dk)::value;
-    switch (decay_value_dim(a.job[0].dv)) {
-      case 32: return decay_launch<T, DK, 32, OUT>(a, st);
-      case 64: return decay_launch<T, DK, 64, OUT>(a, st);
-      default: return decay_launch<T, DK, 128, OUT>(a, st);
+    if constexpr (sizeof(T) == 2 || DK < 128) {
+      switch (decay_value_dim(sizeof(T) == 4, DK, a.job[0].dv)) {
+        case 32: return decay_launch<T, DK, 32, OUT>(a, st);
+        case 64: return decay_launch<T, DK, 64, OUT>(a, st);
+        default: break;
+      }
     }
+    return decay_launch<T, DK, 128, OUT>(a, st);
   };
   switch (decay_key_dim(a.job[0].dk)) {
     case 32: return values(std::integral_constant<int, 32>{});

@@ -172,7 +172,7 @@ void plan_segments(int dtype, DecayArgs& a, int64_t runs, int dk, int dv) {
   const double width = decay_key_dim(dk);
   const double tf = f32 ? 1.3 + 0.047 * width : (dtype == LFAMD_F16 ? 1.3 : 0.85) + 0.0095 * width;
   const double ts = (f32 ? 0.35 : 0.58) * tf;
-  const double waves = (double)runs * (decay_value_dim(dv) / 32) / (4.0 * num_cus());
+  const double waves = (double)runs * (decay_value_dim(f32, dk, dv) / 32) / (4.0 * num_cus());
   double least = 0.0;
   for (int64_t n = 1; n <= 64 && n <= std::max<int64_t>(tiles, 1); ++n) {
     const int64_t seg = std::max<int64_t>(1, (tiles + n - 1) / n);
@@ -232,8 +232,7 @@ struct BackwardPlan {
 
 BackwardPlan plan_backward(int dtype, const lfamd_decay* d) {
   BackwardPlan p{};
-  p.split = decay_key_dim((int)d->key_dim) != decay_key_dim((int)d->value_dim) ||
-            decay_value_dim((int)d->key_dim) != decay_value_dim((int)d->value_dim);
+  p.split = decay_key_dim((int)d->key_dim) != decay_key_dim((int)d->value_dim);
   p.shared = d->kv_heads != d->heads;
   p.both = p.own = base_args(d);
   const int64_t bh = d->batch * d->heads;

@@ -135,9 +135,8 @@ def test_cpu_tensors_raise():
         lf.decay_attention_step(q.requires_grad_(), q, q, lg, torch.zeros(1, 2, 8, 8))
 
 
-# Scratch bytes per lane of the kernels that do not fit their registers (1024 threads have 128 each, two waves of a SIMD 256): (kernel, type, its integer arguments): the most that it may take.
+# Scratch bytes per lane of the kernels that do not fit their registers (1024 threads have 128 each): (kernel, type, its integer arguments): the most that it may take.
 SCRATCH = {
-    ("decay_kernel", "f", (64, 64, 1)): 8, ("decay_kernel", "f", (64, 128, 1)): 52,
     ("gated_add_rms_norm_bwd_kernel", "f", (1024, 2, 0, 1)): 36, ("gated_add_rms_norm_bwd_kernel", "f", (1024, 2, 1, 1)): 108,
     ("gated_add_rms_norm_bwd_kernel", "f", (1024, 2, 1, 0)): 64, ("gated_add_rms_norm_bwd_kernel", "f", (1024, 2, 2, 1)): 24,
     ("gated_add_rms_norm_bwd_kernel", "f16s", (1024, 1, 1, 1)): 60, ("gated_add_rms_norm_bwd_kernel", "bf16s", (1024, 1, 1, 1)): 72,
