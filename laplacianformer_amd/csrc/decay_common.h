@@ -304,20 +304,26 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && (DK >= 96 || (DK == 
   }
 
   // Powers of the decay: of a score's distance (0 outside the triangle), of a token's to the state that it goes
-  // into, of the query's from the state in front, and of a whole tile.
+  // into, of the query's from the state in front, and of a whole tile. A lane forms one and asks the others for the
+  // rest (33 exponentials in each lane took 1 us of a call's 8).
+  const float power = decay_pow(lg, lane);
+  auto power_of = [&](int n) { return __shfl(power, n); };
   auto row_of = [&](int r) { return 8 * (r >> 2) + 4 * h + (r & 3); };
   f32x16 pw, gam;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const int j = row_of(r), n = rev ? j - i : i - j;
-    gam[r] = jb.sk * decay_pow(lg, rev ? j + 1 : TILE - 1 - j);
-    if constexpr (OUT) pw[r] = n < 0 ? 0.0f : jb.sp * decay_pow(lg, n);
+    gam[r] = jb.sk * power_of(rev ? j + 1 : TILE - 1 - j);
+    if constexpr (OUT) {
+      const float x = jb.sp * power_of(max(n, 0));
+      pw[r] = n < 0 ? 0.0f : x;
+    }
   }
   const int ahead = TILE - short_;  // rows that the first tile lacks
-  float lam = jb.so * decay_pow(lg, max(rev ? short_ - 1 - i : i + 1 - ahead, 0));
-  const float lams = jb.so * decay_pow(lg, rev ? TILE - 1 - i : i + 1);
-  float whole = decay_pow64(lg, max(short_, 0));
+  float lam = jb.so * power_of(max(rev ? short_ - 1 - i : i + 1 - ahead, 0));
+  const float lams = jb.so * power_of(rev ? TILE - 1 - i : i + 1);
   const float wholes = decay_pow64(lg, TILE);
+  float whole = short_ == TILE ? wholes : decay_pow64(lg, short_);
 
   const int kcl0 = TK::col_lane(lane), vcl0 = TV::col_lane(lane), dl0 = DR::lane_offset(lane);
   struct KQ {
