@@ -4,7 +4,7 @@ Drop-in for the reference's ``Laplace_subtraction_cuda`` extension: ``ext()``
 returns a module with the same name and exports, backed by hand-written gfx950
 HIP kernels behind the C ABI of ``include/laplacianformer_amd.h``. Beside the
 reference's operators: the attention layer built on them, and the operators of the
-transformer block around it (norm, rotary positions, softmax attention).
+transformer block around it (norms, rotary positions, softmax and decaying linear attention).
 """
 from ._lib import EXT_PATH, LIB_PATH, capi, check, dtype_code, ext
 from .attention import LaplacianAttention, laplacian_attention
