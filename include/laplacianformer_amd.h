@@ -409,7 +409,8 @@ int lfamd_softmax_attention_backward(int dtype, const lfamd_attention* desc, con
  *   sum = residual + scale * gate * z (gate NULL: 1), rs = 1 / sqrt(mean(sum^2) + eps), y = sum * rs * weight,
  * statistics of fp32 values, of the unrounded sum. x and residual [rows][width] with rows x_stride /
  * residual_stride elements apart, y and sum contiguous, the weights [width] and the gate [rows / gate_rows][width]
- * (gate_rows 0: one gate row for all) with rows gate_stride apart; each of them of its own type, dtype or F32.
+ * (gate_rows 0: one gate row for all; of a NULL gate nothing is read, whatever gate_rows is) with rows gate_stride
+ * apart; each of them of its own type, dtype or F32.
  * rstd and post_rstd [rows] fp32 (rs and rx) or NULL: the backward reads them. 1 <= width <= 8192
  * (LFAMD_ERR_UNSUPPORTED beyond), rows below 2^30; scale finite. */
 typedef struct {
