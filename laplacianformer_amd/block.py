@@ -131,8 +131,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     read, give 0, and the state does not see them. ``scale`` (positive) defaults to ``1 / sqrt(d)``.
 
     What is rounded between the products is carried in pieces: results are those of float32 arithmetic, rounded
-    once. Values in front of a length have to be finite: tiles of 32 tokens multiply zeros by
-    them. With autograd (q, k, v and state, through both results), which keeps the inputs alone.
+    once. A NaN or an infinity in v reaches the other tokens of its tile of 32 too, those in front of it among them (zeros are
+    multiplied by it), and in q, k or the output's gradient it does so in the gradients. Scores ``q_i . k_j`` of
+    j <= i have to be in float32's range. With autograd (q, k, v and state, through both results), which keeps the inputs alone.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.shape[-1] else 1.0

@@ -101,6 +101,11 @@ template <> __device__ __forceinline__ float high_half<f16s>(uint32_t w) { retur
 // otherwise, and their operands wait in registers. There is no instruction in it that could read x early.
 __device__ __forceinline__ void hold(f32x16& x) { asm volatile("" : "+v"(x)); }
 
+// x y, but 0 where either is, of infinities and NaN too: v_mul_legacy_f32, one instruction like the product itself. (There is no builtin
+// for it, and inline assembly would have to wait for matrix results by itself.)
+extern "C" __device__ float lfamd_mul_zero(float x, float y) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ float mul_zero(float x, float y) { return lfamd_mul_zero(x, y); }
+
 // Eight values as NP pieces of an operand.
 template <typename T, int NP> __device__ __forceinline__ void split_pieces(f32x8 x, Frag<T> (&f)[NP]) {
   if constexpr (sizeof(T) == 4) {
@@ -401,7 +406,7 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && (DK >= 96 || (DK == 
       read_v();
       first_reads<2 * ND / PAIR, KAHEAD>(kring, read_k);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] *= pw[r];
+      for (int r = 0; r < 16; ++r) p[r] = mul_zero(p[r], pw[r]);
       if constexpr (F16) {
         float top = 0.0f;
 #pragma unroll
