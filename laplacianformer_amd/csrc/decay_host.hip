@@ -79,7 +79,9 @@ struct StepArgs {
   float scale;
 };
 
-// One token: S <- a S + k v^T in place, out = scale S^T q. Memory-bound by the state, read and written once:
+// One token: S <- a S + k v^T in place, out = scale S^T q. Slow heads take it as S + ((a - 1) S + k v^T): an a that is rounded to 32 bits is
+// off by the same 2^-25 at every token, which over the 1 / (1 - a) tokens that the state holds adds up to up to 2e-5 of it at a = 1 - 2^-10,
+// where the roundings themselves come to 8e-7; a - 1 is off by 2^-24 of itself. (Fast heads would cancel S in it.) Memory-bound by the state, read and written once:
 // a workgroup takes 32 value columns of a head's state, a thread four of them (16 bytes) in every 32nd row,
 // all of its rows in flight at once; the rows' shares of out are added in a fixed order. 2048 states of 128 x 128: 56 us,
 // 4.8 TB/s (one that the last level of cache still holds half of: 42); four of 32 x 32: 3.0.
@@ -88,7 +90,9 @@ template <typename T> __global__ void __launch_bounds__(256) decay_step_kernel(c
   const int block = blockIdx.x % a.blocks, bh = blockIdx.x / a.blocks, b = bh / a.H, hq = bh % a.H;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c0 = 32 * block + 4 * (threadIdx.x & 7), row0 = threadIdx.x >> 3;
-  const float lg = a.logDecay[hq], keep = expf(lg);
+  const float lg = a.logDecay[hq];
+  const bool slow = lg > -0.5f;
+  const float factor = slow ? expm1f(lg) : expf(lg);
   const T* q = (const T*)a.q + b * a.qs[0] + hq * a.qs[1];
   const T* k = (const T*)a.k + b * a.ks[0] + (hq / a.G) * a.ks[1];
   const T* v = (const T*)a.v + b * a.vs[0] + (hq / a.G) * a.vs[1];
@@ -109,7 +113,7 @@ template <typename T> __global__ void __launch_bounds__(256) decay_step_kernel(c
     const int r = row0 + 32 * u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      x[u][j] = fmaf(x[u][j], keep, kr[u] * vc[j]);
+      x[u][j] = fmaf(x[u][j], factor, kr[u] * vc[j]) + (slow ? x[u][j] : 0.0f);
       o[j] = fmaf(qr[u], x[u][j], o[j]);
     }
     if (r < a.dk) store4<float>(s + (int64_t)r * a.dv, c0, a.dv, x[u][0], x[u][1], x[u][2], x[u][3]);

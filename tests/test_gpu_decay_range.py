@@ -59,3 +59,58 @@ def test_values_that_are_not_finite(gpu, dtype):
                 ok[1, 1, 43:] = False
             assert not bool(torch.isfinite(out[1, 1, at]).all())
             bc.assert_within(out[ok], ref[ok], bound[ok], (dtype, bad, name))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_steps(gpu, dtype):
+    """4096 tokens one by one: no error of the decay adds up, and the prompt's form ends in the same state.
+
+    With x = 1 - a about 2^-10 and random keys and values a state holds some 1 / (2 x) = 512 tokens' energy. Each token's two
+    roundings are at most 2^-24 of the state and of what is added, rms 2^-24 / sqrt(3), and add up as their squares: sqrt(512) 2^-24 / sqrt(3)
+    = 7.8e-7 of the state's norm, and 2^-24 from the second. A factor a - 1 off by 2^-23 of itself gives 0.7 2^-23. Sum 9.2e-7; a head's norm of
+    256 elements keeps to a tenth of that, twice it is allowed. (A factor a off by half its unit, 2^-25, alone gives
+    0.7 1024 2^-25 = 2.1e-5.)"""
+    import laplacianformer_amd as lf
+
+    print(f"decay many steps {dtype}", flush=True)
+    H, T, d = 32, 4096, 16
+    lg = torch.tensor([-(1.0 + h / 37.0) / 1024 for h in range(H)])
+    K, V = (gen((T, 1, H, 1, d), 420 + i, dtype).to(gpu) for i in range(2))
+    L, state = lg.to(gpu), torch.zeros(1, H, d, d, device=gpu)
+    with torch.no_grad():
+        for t in range(T):
+            lf.decay_attention_step(K[t], K[t], V[t], L, state)
+        k, v = (x[:, 0, :, 0].transpose(0, 1)[None] for x in (K, V))
+        _, last = lf.decay_attention(k, k, v, L, return_state=True)
+    left = torch.exp(lg.double()[:, None] * torch.arange(T - 1, -1, -1).double())
+    k, v = k[0].cpu().double(), v[0].cpu().double()
+    ref = (k * left[..., None]).transpose(-1, -2) @ v
+    for got, name in ((state, "steps"), (last, "prompt")):
+        err = (got[0].cpu().double() - ref).norm(dim=(1, 2)) / ref.norm(dim=(1, 2))
+        assert err.max() <= 1.9e-6, (dtype, name, err.max().item())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_step_decays_around_the_border(gpu, dtype):
+    """The step's two forms of the decay, on both sides of where they meet, and a decay of nothing and of all; bounds as
+    in test_step, where fast heads' states vanish beside what is added to them and in front of them."""
+    import laplacianformer_amd as lf
+
+    lg = torch.tensor([0.0, -1e-7, -0.49, -0.5, -0.51, -3.0, -100.0, -math.inf])
+    H, d, e = len(lg), 20, 36
+    for size in (1e-3, 1.0, 1e6):
+        q, k, v = gen((1, H, 1, d), 430, dtype), gen((1, H, 1, d), 431, dtype), gen((1, H, 1, e), 432, dtype)
+        s0 = gen((1, H, d, e), 433, "f32", size)
+        state = s0.to(gpu)
+        out = lf.decay_attention_step(q.to(gpu), k.to(gpu), v.to(gpu), lg.to(gpu), state, scale=0.2)
+        a, kv = torch.exp(lg.double()).view(1, H, 1, 1), k.double().transpose(-1, -2) * v.double()
+        S, mag = a * s0.double() + kv, a * s0.double().abs() + kv.abs()
+        bc.assert_within(state, S, 6 * bc.U32 * mag, (dtype, size, "state"))
+        ref, m = 0.2 * (q.double() @ S), 0.2 * (q.double().abs() @ mag)
+        c = (d + 16) * bc.U32
+        # Outputs of 0.2 * 20 products with states of up to 4e6: fp16 ends at 65504, and what lies well beyond is an infinity.
+        out, most = out.cpu(), torch.finfo(out.dtype).max
+        fits = ref.abs() < 0.99 * most
+        bound = c * m + bc.unit(TORCH_DT[dtype]) * (ref.abs() + c * m)
+        bc.assert_within(out[fits], ref[fits], bound[fits], (dtype, size, "out"))
+        assert bool(torch.isinf(out[ref.abs() > 1.01 * most]).all())
