@@ -79,8 +79,13 @@ __device__ __forceinline__ int decay_length(const DecayArgs& a, int b) {
 }
 // exp(lg n) for whole n >= 0, of a log_decay of -inf too.
 __device__ __forceinline__ float decay_pow(float lg, int n) { return n == 0 ? 1.0f : expf(lg * (float)n); }
-// The same in 64 bits: the factor of a whole tile or segment, which powers are taken of.
-__device__ __forceinline__ float decay_pow64(float lg, int n) { return n == 0 ? 1.0f : (float)exp((double)lg * (double)n); }
+// The same in 64 bits: the factor of a whole tile or segment, which powers are taken of. A rounding of it to 32 bits would be made in
+// each of them again (2^-25 of the state a tile, over all tiles that it holds), so that low takes what it leaves.
+__device__ __forceinline__ float decay_pow64(float lg, int n, float* low = nullptr) {
+  const double x = n == 0 ? 1.0 : exp((double)lg * (double)n);
+  if (low) *low = (float)(x - (double)(float)x);
+  return (float)x;
+}
 
 // The tokens of a segment of a sequence of len: cut from its end if it is run forwards, from its start if backwards.
 __device__ __forceinline__ void decay_segment(const DecayArgs& a, int len, int seg, bool rev, int* begin, int* end) {
@@ -327,7 +332,8 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && (DK >= 96 || (DK == 
   const int ahead = TILE - short_;  // rows that the first tile lacks
   float lam = jb.so * power_of(max(rev ? short_ - 1 - i : i + 1 - ahead, 0));
   const float lams = jb.so * power_of(rev ? TILE - 1 - i : i + 1);
-  const float wholes = decay_pow64(lg, TILE);
+  float low;  // what wholes leaves of a whole tile's factor; a first tile's is met once
+  const float wholes = decay_pow64(lg, TILE, &low);
   float whole = short_ == TILE ? wholes : decay_pow64(lg, short_);
 
   const int kcl0 = TK::col_lane(lane), vcl0 = TV::col_lane(lane), dl0 = DR::lane_offset(lane);
@@ -442,7 +448,7 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && (DK >= 96 || (DK == 
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[s][j] *= gam[8 * s + j];
     }
-    float keep = due * whole, f = 1.0f;
+    float keep = fmaf(due, whole, n ? due * low : 0.0f), f = 1.0f;
     bool now = keep < 0x1p-20f;
     if constexpr (F16) {
       float top = 0.0f;

@@ -18,7 +18,9 @@ __global__ void __launch_bounds__(256) decay_join_kernel(const DecayArgs a) {
   const int size = jb.dk * jb.dv, e = blockIdx.y * 256 + threadIdx.x, bh = blockIdx.x;
   if (e >= size) return;
   const int b = bh / a.H, len = decay_length(a, b), span = a.segTiles * kDecayTile;
-  const float lg = a.logDecay[bh % a.H], full = decay_pow64(lg, span);
+  const float lg = a.logDecay[bh % a.H];
+  float low;
+  const float full = decay_pow64(lg, span, &low);
   float* p = jb.seg + (int64_t)bh * a.nseg * size + e;
   float s = 0.0f;
   if (jb.first) {
@@ -39,7 +41,7 @@ __global__ void __launch_bounds__(256) decay_join_kernel(const DecayArgs a) {
       int begin, end;
       decay_segment(a, len, at, jb.reverse, &begin, &end);
       p[(int64_t)at * size] = s;
-      s = fmaf(end - begin == span ? full : decay_pow64(lg, end - begin), s, own[u]);
+      s = end - begin == span ? fmaf(full, s, fmaf(low, s, own[u])) : fmaf(decay_pow64(lg, end - begin), s, own[u]);
     }
   }
 }

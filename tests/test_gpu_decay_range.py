@@ -114,3 +114,31 @@ def test_step_decays_around_the_border(gpu, dtype):
         bound = c * m + bc.unit(TORCH_DT[dtype]) * (ref.abs() + c * m)
         bc.assert_within(out[fits], ref[fits], bound[fits], (dtype, size, "out"))
         assert bool(torch.isinf(out[ref.abs() > 1.01 * most]).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_very_slow_heads(gpu, dtype):
+    """Decays of some 2^-15.6 a token over 32768 tokens, in heads enough that no sequence is cut: no error of a whole tile's factor
+    adds up over the 1024 tiles.
+
+    The state grows as the square root of the tokens. A tile goes into it in r = 16 accumulations (fp32; bf16: 2 of each of
+    3 pieces, 6) and one rounding of its factor, each rms 2^-24 / sqrt(3) of the state then, which add up as their squares:
+    sqrt((r + 1) 1024 / 2) 2^-24 / sqrt(3) = 3.2e-6 (2.1e-6) of the last state. One and a half times that is allowed. (A factor off by half
+    its unit, 2^-25, alone gives 2^-25 1024 / sqrt(3) = 1.8e-5.)"""
+    import ctypes
+
+    import laplacianformer_amd as lf
+    import laplacianformer_amd._lib as L
+
+    print(f"decay very slow heads {dtype}", flush=True)
+    H, B, N, d = 32, 128, 32768, 8
+    lg = torch.tensor([-(1.0 + h / 37.0) * 2e-5 for h in range(H)])
+    desc = L.Decay(batch=B, heads=H, kv_heads=H, tokens=N, key_dim=d, value_dim=d, log_decay=16, scale=1.0)
+    assert lf.capi().lfamd_decay_attention_workspace_size(lf.dtype_code(TORCH_DT[dtype]), ctypes.byref(desc)) == 0
+    k, v = (gen((1, H, N, d), 440 + i, dtype).to(gpu) for i in range(2))
+    with torch.no_grad():
+        _, last = lf.decay_attention(k.expand(B, -1, -1, -1), k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1), lg.to(gpu), return_state=True)
+    left = torch.exp(lg.double()[:, None] * torch.arange(N - 1, -1, -1).double())
+    ref = (k[0].cpu().double() * left[..., None]).transpose(-1, -2) @ v[0].cpu().double()
+    err = (last[B // 2].cpu().double() - ref).norm(dim=(1, 2)) / ref.norm(dim=(1, 2))
+    assert err.max() <= (4.8e-6 if dtype == "f32" else 3.2e-6), (dtype, err.max().item())
