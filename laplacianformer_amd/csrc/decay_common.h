@@ -16,7 +16,8 @@
 // the scaled V) is carried in two pieces x = hi + lo (V in bf16 in three), whose products the
 // accumulators add: results have the accuracy of 32-bit arithmetic, the state among them, which is
 // fp32. In fp16 the pieces are scaled by powers of two that keep both ends of the type's range away: P
-// for each query, S and V for each wave and tile.
+// for each query, S for each wave and tile, V for each column (a column of 1e-5 beside one of 600: its state 1e-3 off with one
+// power for the wave, 1e-7 with its own; times the same).
 //
 // The gradients are the same operator on other operands: with g the gradient of out and S^T for S,
 //   dq = run(g, v, k) forwards;   dk = run(v, g, q),  dv = run(k, q, g) backwards in time,
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && (DK >= 96 || (DK == 
   const int64_t step = (rev ? -TILE : TILE) * jb.os[2];
   int64_t off = ooff + (int64_t)(tile_at(0) + i) * jb.os[2] + 32 * wave + 4 * h;
   float due = 1.0f;
-  int unit = 0;  // fp16: st holds the state times 2^unit as well
+  int unit = 0;  // fp16: st holds the state's column times 2^unit as well
   land();
   __syncthreads();
   for (int n = 0; n < tiles; ++n) {
@@ -391,9 +392,11 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && (DK >= 96 || (DK == 
         for (int m = 0; m < ND; ++m)
 #pragma unroll
           for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(st[m][r]));
-        const int e = 15 - min(max(__builtin_amdgcn_frexp_expf(wave_max(top)), -45), 120);
-        mul = __builtin_amdgcn_ldexpf(1.0f, e);
-        front = __builtin_amdgcn_ldexpf(front, -e - unit);
+        // Columns have units of their own, outputs add over key channels alone: one power of two for the wave.
+        const float column = top > 0.0f ? (float)(__builtin_amdgcn_frexp_expf(top) - unit) : -1000.0f;
+        const int e = 15 - min(max((int)wave_max(column), -60), 120);
+        mul = __builtin_amdgcn_ldexpf(1.0f, e - unit);
+        front = __builtin_amdgcn_ldexpf(front, -e);
       }
       // Scores and memory by 16 channels: the pieces of one step's state are made while the products of the
       // step before it run.
@@ -456,10 +459,21 @@ __global__ void __launch_bounds__(DV * 2, sizeof(T) == 4 && (DK >= 96 || (DK == 
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[s][j]));
-      top = wave_max(top);
-      const int e = min(max(__builtin_amdgcn_frexp_expf(top), -45), 60), over = __builtin_amdgcn_frexp_expf(top / keep) + unit;
-      now = now || over > 15 || over < 5;
-      if (now) keep = __builtin_amdgcn_ldexpf(keep, 15 - e - unit), unit = 15 - e;
+      // The lane pair's column: its largest value times 2^unit is to be of 2^8 to 2^15, so that the second piece's step,
+      // 2^-24, is 2^-32 of it or less; a new unit makes it one of 2^11, between the two, if the column's state has room for it.
+      top = half_max(top);
+      const int over = __builtin_amdgcn_frexp_expf(top / keep) + unit;
+      now = __any(now || (top > 0.0f && (over > 15 || over < 9)));
+      if (now) {
+        float most = 0.0f;
+#pragma unroll
+        for (int m = 0; m < ND; ++m)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(st[m][r]));
+        const int room = 100 + unit - __builtin_amdgcn_frexp_expf(half_max(most) * keep);
+        const int to = top > 0.0f ? min(12 - min(max(__builtin_amdgcn_frexp_expf(top), -80), 60), room) : unit;
+        keep = __builtin_amdgcn_ldexpf(keep, to - unit), unit = to;
+      }
       f = __builtin_amdgcn_ldexpf(1.0f, unit);
     }
     if (now) {

@@ -142,3 +142,73 @@ def test_very_slow_heads(gpu, dtype):
     ref = (k[0].cpu().double() * left[..., None]).transpose(-1, -2) @ v[0].cpu().double()
     err = (last[B // 2].cpu().double() - ref).norm(dim=(1, 2)) / ref.norm(dim=(1, 2))
     assert err.max() <= (4.8e-6 if dtype == "f32" else 3.2e-6), (dtype, err.max().item())
+
+
+def _tile_steps(k, v, lg, N):
+    """sum over tiles of a^(tokens behind it) (sum over j of |k_j|) (largest a^(tile's end - j) |v_j|), [B, H, d, e]: what one
+    step of the value operand's second piece, relative to the tile's largest value in the column, comes to in the state."""
+    front = -N % 32
+    K, V = (torch.cat((torch.zeros(*x.shape[:2], front, x.shape[3], dtype=torch.float64), x.double().abs()), 2) for x in (k, v))
+    n = (N + front) // 32
+    K, V = (x.view(*x.shape[:2], n, 32, x.shape[3]) for x in (K, V))
+    inside = dc.powers(lg, 31 - torch.arange(32))[None, :, None, :, None]
+    behind = dc.powers(lg, 32 * (n - 1 - torch.arange(n)))[None, :, :, None, None]
+    return (behind * K.sum(3)[..., :, None] * (inside * V).amax(3)[..., None, :]).sum(2)
+
+
+@pytest.mark.parametrize("N", [20, 32, 64, 75, 200, 2500])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_columns_of_very_different_sizes(gpu, dtype, N):
+    """Value columns of 1 to 1e-5 and an outlier of 600 in the first tile beside them; the states' columns do not see one
+    another, in any type. Bound: decaycheck's with, in fp16, half a step 2^-25 of the value operand's second piece over a largest
+    value of 2^8 in the tile's column, 2^-33 of that."""
+    import laplacianformer_amd as lf
+
+    print(f"decay columns {dtype} {N}", flush=True)
+    B, H, d, e = 1, 4, 24, 40
+    lg = torch.tensor([-2.0 ** -12, -0.03, 0.0, -1.5])
+    q, k, v, g = (gen((B, H, N, x), 450 + i, "f32") for i, x in enumerate((d, d, e, e)))
+    size = torch.logspace(0, -5, 8)[torch.arange(e) % 8]
+    v, g = v * size, g * size.flip(0)
+    v[:, :, 3, 0], g[:, :, -2, 33] = 600.0, -300.0
+    v[:, :, N // 2:, 9] = 0.0
+    q, k, v, g = (x.to(TORCH_DT[dtype]) for x in (q, k, v, g))
+    s0 = gen((B, H, d, e), 455, "f32") * size
+    ref = dc.decay(q, k, v, lg, 0.2, s0, None, g)
+    leaves = [x.to(gpu).requires_grad_() for x in (q, k, v, s0)]
+    out, last = lf.decay_attention(*leaves[:3], lg.to(gpu), state=leaves[3], scale=0.2, return_state=True)
+    grads = torch.autograd.grad(out, leaves, g.to(gpu))
+    extra = {}
+    if dtype == "f16":
+        extra["last"] = 2.0 ** -33 * _tile_steps(k, v, lg, N)
+        # Backwards: the same on the queries and the outputs' gradients, whose tiles begin where the sequence does.
+        a = torch.exp(lg.double())[None, :, None, None]
+        extra["dstate"] = 2.0 ** -33 * 0.2 * a * _tile_steps(q.flip(2), g.flip(2), lg, N)
+    for name, x in zip(("out", "last", "dq", "dk", "dv", "dstate"), (out, last, *grads)):
+        bc.assert_within(x, ref[name][0], ref[name][1] + extra.get(name, 0.0), (dtype, N, name))
+
+
+def test_fp16_states_of_other_sizes_than_the_values(gpu):
+    """fp16: large and small states beside small and large values, zero columns and tiles, and scales far from 1."""
+    import laplacianformer_amd as lf
+
+    lg = torch.tensor([-0.01, -1.0])
+    for ss, vs, scale in ((1e12, 1e-6, 0.1), (1e-12, 3e4, 0.1), (0.0, 6e4, 1e4), (1.0, 1e-4, 1e-8), (1e-20, 1e-3, 1.0)):
+        print("decay fp16 states", ss, vs, scale, flush=True)
+        q, k, v, g = (gen((1, 2, 100, 32), 460 + i, "f32") for i in range(4))
+        k[:, :, 40:80] = 0.0
+        v[:, :, :, 5], v[:, :, 10:70, 6] = 0.0, 0.0
+        q, k, v, g = q.half(), k.half(), (v * vs).clamp(-6e4, 6e4).half(), g.half()
+        s0 = gen((1, 2, 32, 32), 465, "f32") * ss
+        s0[..., 7] = 0.0
+        ref = dc.decay(q, k, v, lg, scale, s0, None, g)
+        leaves = [x.to(gpu).requires_grad_() for x in (q, k, v, s0)]
+        out, last = lf.decay_attention(*leaves[:3], lg.to(gpu), state=leaves[3], scale=scale, return_state=True)
+        grads = torch.autograd.grad(out, leaves, g.to(gpu))
+        step = 2.0 ** -33 * _tile_steps(k, v, lg, 100)
+        bc.assert_within(last, ref["last"][0], ref["last"][1] + step, (ss, vs, scale, "last"))
+        for name, x in zip(("out", "dq", "dk", "dv", "dstate"), (out, *grads)):
+            if ref[name][0].abs().max() < torch.finfo(x.dtype).max:
+                a = torch.exp(lg.double())[None, :, None, None]
+                step = 2.0 ** -33 * scale * a * _tile_steps(q.flip(2), g.flip(2), lg, 100) if name == "dstate" else 0.0
+                bc.assert_within(x, ref[name][0], ref[name][1] + step, (ss, vs, scale, name))
