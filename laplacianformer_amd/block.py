@@ -12,6 +12,7 @@ call gives the same bits. Gradients are of first order (no create_graph); forwar
 from __future__ import annotations
 
 import math
+import warnings
 from typing import Sequence
 
 import torch
@@ -164,7 +165,8 @@ class AttentionBlock(torch.nn.Module):
     (softmax_attention, ``kv_heads`` key heads shared by ``heads`` query heads), "decay" (decay_attention, causal, with
     shared key heads too; its output, which no softmax has normalised, goes through a norm in front of the projection)
     or "laplacian" (laplacian_attention with ``pool`` and ``iters``, one key head per query head, a grid of two
-    axes). ``log_decay`` are the heads' values for "decay" (default: log(1 - 2^-n), n from 5 to 12).
+    axes). ``log_decay`` are the heads' values for "decay" (default: log(1 - 2^-n), n from 5 to 12): a buffer
+    of the state dict, float32 whatever type the module is taken to.
 
     With ``post_norm`` the addition norms x, the block in front's output, with a weight of its own, and
     ``residual_scale`` and forward's ``gate`` multiply what is added (gated_add_rms_norm). Caches of keys, states and
@@ -198,8 +200,24 @@ class AttentionBlock(torch.nn.Module):
             if log_decay is None:
                 log_decay = [math.log1p(-2.0 ** -(5 + 7 * h / max(heads - 1, 1))) for h in range(heads)]
             self.out_weight = torch.nn.Parameter(torch.ones(dim))
-            # No buffer: it stays float32 whatever type the module is taken to.
-            self._log_decay = torch.tensor(list(log_decay), dtype=torch.float32)
+            self.register_buffer("_log_decay", torch.tensor(list(log_decay), dtype=torch.float32))
+
+    def _apply(self, fn, recurse: bool = True):
+        kept = self._buffers.get("_log_decay")
+        super()._apply(fn, recurse)
+        if kept is not None and self._log_decay.dtype != torch.float32:  # half() and the like: it stays float32
+            self._log_decay = kept.to(self._log_decay.device)
+        return self
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        name = prefix + "_log_decay"
+        if "_log_decay" not in self._buffers:
+            return
+        if name in missing_keys:  # saved when the values were in no state dict
+            missing_keys.remove(name)
+            warnings.warn(f"the state dict has no {name}: the block keeps the values that it was built with", stacklevel=2)
+        self._log_decay = self._log_decay.float()  # of an assigned state dict in 16 bits
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, grid: Sequence[int] | None = None,
                 positions: torch.Tensor | None = None, mask: torch.Tensor | None = None,
@@ -250,8 +268,6 @@ class AttentionBlock(torch.nn.Module):
         if self.attention == "softmax":
             o = softmax_attention(q, k, v, mask=mask, causal=self.causal, k_lengths=lengths, q_lengths=lengths)
         elif self.attention == "decay":
-            if self._log_decay.device != x.device:
-                self._log_decay = self._log_decay.to(x.device)
             o = decay_attention(q, k, v, self._log_decay, lengths=lengths)
             return self.proj(add_rms_norm(o.transpose(1, 2).reshape(B, N, C), self.out_weight, eps=self.eps)), total
         else:
