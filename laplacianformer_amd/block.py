@@ -125,8 +125,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     ``[B, H, N, e]``: with ``a = exp(log_decay[h])``, ``S_t = a S_(t-1) + k_t v_t^T``, ``out_t = scale S_t^T q_t``.
 
     H is a multiple of Hk: query head ``h`` reads key head ``h // (H // Hk)``. d and e are at most 128.
-    ``log_decay`` is float32 ``[H]``, at most 0 (-inf: a token sees itself alone), without a gradient; nothing checks
-    its values. ``state`` is the S in front of the first token, float32 ``[B, H, d, e]`` (default: zero);
+    ``log_decay`` is float32 ``[H]``, at most 0 (-inf: a token sees itself alone), without a gradient (one that requires it is
+    refused where gradients are recorded); nothing checks its values. ``state`` is the S in front of the first token, float32 ``[B, H, d, e]`` (default: zero);
     with ``return_state`` the result is ``(out, state behind the last token)``, from which the next
     tokens go on, here or in decay_attention_step. ``lengths`` is int32 ``[B]``: tokens from ``lengths[b]`` on are not
     read, give 0, and the state does not see them. ``scale`` (positive) defaults to ``1 / sqrt(d)``.

@@ -743,7 +743,7 @@ Tensor SoftmaxAttention(const Tensor q, const Tensor k, const Tensor v, const Op
 
 std::vector<Tensor> DecayAttention(const Tensor q, const Tensor k, const Tensor v, const Tensor log_decay, const OptTensor state,
                                    const OptTensor lengths, double scale, bool return_state) {
-  TORCH_CHECK(!log_decay.requires_grad(), "decay_attention: log_decay has no gradient");
+  TORCH_CHECK(!records({&log_decay}), "decay_attention: log_decay has no gradient");
   no_tangent("decay_attention", {&q, &k, &v, &log_decay, if_given(state)});
   if (records({&q, &k, &v, if_given(state)}))
     return DecayAttentionNode::apply(q, k, v, log_decay, state, lengths, scale, return_state);

@@ -212,3 +212,19 @@ def test_fp16_states_of_other_sizes_than_the_values(gpu):
                 a = torch.exp(lg.double())[None, :, None, None]
                 step = 2.0 ** -33 * scale * a * _tile_steps(q.flip(2), g.flip(2), lg, 100) if name == "dstate" else 0.0
                 bc.assert_within(x, ref[name][0], ref[name][1] + step, (ss, vs, scale, name))
+
+
+def test_decays_that_require_a_gradient(gpu):
+    """They have none, which is no reason to refuse a call that records none."""
+    import laplacianformer_amd as lf
+
+    q, lg = torch.randn(1, 2, 5, 8, device=gpu), torch.full((2,), -0.1, device=gpu)
+    want, leaf = lf.decay_attention(q, q, q, lg), lg.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        lf.decay_attention(q, q, q, leaf)
+    with torch.no_grad():
+        assert torch.equal(lf.decay_attention(q, q, q, leaf), want)
+        one = q[:, :, :1]
+        lf.decay_attention_step(one, one, one, leaf, torch.zeros(1, 2, 8, 8, device=gpu))
+    with torch.inference_mode():
+        assert torch.equal(lf.decay_attention(q, q, q, leaf), want)
