@@ -228,3 +228,56 @@ def test_decays_that_require_a_gradient(gpu):
         lf.decay_attention_step(one, one, one, leaf, torch.zeros(1, 2, 8, 8, device=gpu))
     with torch.inference_mode():
         assert torch.equal(lf.decay_attention(q, q, q, leaf), want)
+
+
+def _long(q, k, v, lg, first):
+    """sum over j <= i of a^(i - j) (q_i . k_j) v_j + a^(i + 1) q_i first in 64 bits by chunks, the same of the terms'
+    magnitudes, and the state behind the last token."""
+    out, mag, step = torch.empty_like(v), torch.empty_like(v), 256
+    S, M = first, first.abs()
+    for n in range(0, q.shape[2], step):
+        x, y, z = (t[:, :, n:n + step] for t in (q, k, v))
+        i = torch.arange(x.shape[2])
+        D, ahead = dc.powers(lg, i[:, None] - i)[None], dc.powers(lg, i + 1)[None, ..., None]
+        out[:, :, n:n + step] = ((x @ y.transpose(-1, -2)) * D) @ z + ahead * (x @ S)
+        mag[:, :, n:n + step] = ((x.abs() @ y.abs().transpose(-1, -2)) * D) @ z.abs() + ahead * (x.abs() @ M)
+        y, whole = y * dc.powers(lg, len(i) - 1 - i)[None, ..., None], dc.powers(lg, torch.tensor(len(i)))[None, :, None, None]
+        S, M = whole * S + y.transpose(-1, -2) @ z, whole * M + y.abs().transpose(-1, -2) @ z.abs()
+    return out, mag, S
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads", [1, 24])
+def test_long_gradients(gpu, dtype, heads):
+    """20011 tokens, two query heads to each key head, keys narrower than values, a state and its gradient, in sequences cut into few
+    segments and into many. Bound: test_long's count of additions for one run and the shared heads' one, and decaycheck's pieces; in fp16
+    decaycheck's steps of the largest score and state. States, norm-relative: the slowest head's holds 64 tiles' energy of up to 17 roundings of rms
+    2^-24 / sqrt(3) each, 1.1e-6; 2^-18 is allowed."""
+    import laplacianformer_amd as lf
+
+    H, N, d, e, scale = 2 * heads, 20011, 24, 40, 0.2
+    print(f"decay long gradients {dtype} H{H}", flush=True)
+    lg = torch.tensor(([-2.0 ** -12, -2.0 ** -6, -2.0 ** -9, -0.4] * heads)[:H])
+    q, k, v, g = (gen((1, h, N, x), 470 + i, dtype) for i, (h, x) in enumerate(((H, d), (heads, d), (heads, e), (H, e))))
+    s0, gl = gen((1, H, d, e), 475, "f32"), gen((1, H, d, e), 476, "f32")
+    leaves = [x.to(gpu).requires_grad_() for x in (q, k, v, s0)]
+    res = lf.decay_attention(*leaves[:3], lg.to(gpu), state=leaves[3], scale=scale, return_state=True)
+    grads = torch.autograd.grad(res, leaves, (g.to(gpu), gl.to(gpu)))
+    Q, G = q.double(), g.double()
+    K, V = (x.double().repeat_interleave(2, 1) for x in (k, v))
+    turn = lambda x: x.transpose(-1, -2).contiguous()  # noqa: E731
+    back = lambda x: x.flip(2)  # noqa: E731
+    R = gl.double() * torch.exp(-lg.double())[None, :, None, None] / scale  # a^(N - 1 - i) in place of a^(N - i)
+    ref = {"out": _long(Q, K, V, lg, s0.double()), "dq": _long(G, V, K, lg, turn(s0.double())),
+           "dk": _long(back(V), back(G), back(Q), lg, turn(R)), "dv": _long(back(K), back(Q), back(G), lg, R)}
+    u = bc.unit(TORCH_DT[dtype])
+    c = (64 + 3 * N / 32 + 64 + 2) * bc.U32 + (0.0 if dtype == "f32" else 2 * u * u + 2.0 ** -22)
+    for name, got in zip(("out", "dq", "dk", "dv"), (res[0], *grads[:3])):
+        want, mag, _ = (scale * x for x in ref[name])
+        if name in ("dk", "dv"):
+            want, mag = (back(x).reshape(1, heads, 2, N, -1).sum(2) for x in (want, mag))
+        err = c * mag + (2.0 ** -38 * 64 * mag.amax() if dtype == "f16" else 0.0)
+        bc.assert_within(got, want, err + u * (want.abs() + err), (dtype, H, name))
+    for name, got in (("last", res[1]), ("dstate", grads[3])):
+        want = ref["out"][2] if name == "last" else scale * torch.exp(lg.double())[None, :, None, None] * ref["dv"][2]
+        assert (got.cpu().double() - want).norm() <= 2.0 ** -18 * want.norm(), (dtype, H, name)
