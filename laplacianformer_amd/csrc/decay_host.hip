@@ -81,6 +81,14 @@ struct StepArgs {
   float scale;
 };
 
+// e^x - 1 for |x| < 0.5, its series up to x^9 / 9! (the rest is below 2^-9 / 10! = 2^-30 of it).
+__device__ __forceinline__ float small_expm1(float x) {
+  float y = 1.0f;
+#pragma unroll
+  for (int n = 9; n > 1; --n) y = fmaf(x * (1.0f / (float)n), y, 1.0f);
+  return x * y;
+}
+
 // One token: S <- a S + k v^T in place, out = scale S^T q. Slow heads take it as S + ((a - 1) S + k v^T): an a that is rounded to 32 bits is
 // off by the same 2^-25 at every token, which over the 1 / (1 - a) tokens that the state holds adds up to up to 2e-5 of it at a = 1 - 2^-10,
 // where the roundings themselves come to 8e-7; a - 1 is off by 2^-24 of itself. (Fast heads would cancel S in it.) Memory-bound by the state, read and written once:
@@ -93,8 +101,7 @@ template <typename T> __global__ void __launch_bounds__(256) decay_step_kernel(c
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c0 = 32 * block + 4 * (threadIdx.x & 7), row0 = threadIdx.x >> 3;
   const float lg = a.logDecay[hq];
-  const bool slow = lg > -0.5f;
-  const float factor = slow ? expm1f(lg) : expf(lg);
+  const bool slow = fabsf(lg) < 0.5f;
   const T* q = (const T*)a.q + b * a.qs[0] + hq * a.qs[1];
   const T* k = (const T*)a.k + b * a.ks[0] + (hq / a.G) * a.ks[1];
   const T* v = (const T*)a.v + b * a.vs[0] + (hq / a.G) * a.vs[1];
@@ -109,6 +116,7 @@ template <typename T> __global__ void __launch_bounds__(256) decay_step_kernel(c
     qr[u] = r < a.dk ? to_acc(q[r]) : 0.0f;
     vc[u] = c0 + u < a.dv ? to_acc(v[c0 + u]) : 0.0f;
   }
+  const float factor = slow ? small_expm1(lg) : expf(lg);
   float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
