@@ -131,8 +131,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     tokens go on, here or in decay_attention_step. ``lengths`` is int32 ``[B]``: tokens from ``lengths[b]`` on are not
     read, give 0, and the state does not see them. ``scale`` (positive) defaults to ``1 / sqrt(d)``.
 
-    What is rounded between the products is carried in pieces: results are those of float32 arithmetic, rounded
-    once. A NaN or an infinity in v reaches the other tokens of its tile of 32 too, those in front of it among them (zeros are
+    Scores and states go into the products in two 16-bit pieces: in front of its own rounding an output (a gradient of q, k, v) is
+    off by up to 2^-17 of its terms in bfloat16, 2^-23 in float16, beside float32's additions; where terms cancel, that is of the terms. States
+    take three pieces (float16: two, relative to the largest value of a column in 32 tokens) and are off as float32 sums are. A NaN or an infinity in v reaches the other tokens of its tile of 32 too, those in front of it among them (zeros are
     multiplied by it), and in q, k or the output's gradient it does so in the gradients. Scores ``q_i . k_j`` of
     j <= i have to be in float32's range. With autograd (q, k, v and state, through both results), which keeps the inputs alone.
     """
@@ -169,7 +170,8 @@ class AttentionBlock(torch.nn.Module):
     of the state dict, float32 whatever type the module is taken to.
 
     With ``post_norm`` the addition norms x, the block in front's output, with a weight of its own, and
-    ``residual_scale`` and forward's ``gate`` multiply what is added (gated_add_rms_norm). Caches of keys, states and
+    ``residual_scale`` and forward's ``gate`` multiply what is added (gated_add_rms_norm; with any of the three dim is at most 8192
+    instead of 16384). Caches of keys, states and
     the 8-bit norm are for callers of the functions: the block takes none of them.
     """
 

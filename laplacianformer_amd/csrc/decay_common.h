@@ -14,8 +14,9 @@
 //
 // Operands are of 16 bits where the inputs are, and whatever is rounded in front of a product (P, S,
 // the scaled V) is carried in two pieces x = hi + lo (V in bf16 in three), whose products the
-// accumulators add: results have the accuracy of 32-bit arithmetic, the state among them, which is
-// fp32. In fp16 the pieces are scaled by powers of two that keep both ends of the type's range away: P
+// accumulators add. Two pieces leave 2^-17 of each score and state that an output is formed of in bf16, 2^-23 in
+// fp16, in front of the output's own rounding of 2^-8 or 2^-11; of the values that go into the state, which is fp32, three
+// leave 2^-26 in bf16. In fp16 the pieces are scaled by powers of two that keep both ends of the type's range away: P
 // for each query, S for each wave and tile, V for each column (a column of 1e-5 beside one of 600: its state 1e-3 off with one
 // power for the wave, 1e-7 with its own; times the same).
 //
@@ -34,10 +35,14 @@
 //
 // What bounds it (one MI355X, bf16): 32 heads over 8 key heads, 32768 tokens, 128 channels: 276 us for the outputs and
 // 103 for the states (HBM alone: 133 and 26). A wave issues some 530 VALU instructions (192 make the state's pieces, 120
-// the values', 48 the scores') and 52 matrix products for a tile, and the time is the sum of 4 cycles for each of
-// the former and 32 for each of the latter: the two do not overlap, whatever the waves. 64 heads, 16384 tokens, 64 channels:
+// the values', 48 the scores') and 52 matrix products for a tile, and the time is about the sum of 4 cycles for each of
+// the former and 32 for each of the latter (the SIMDs' matrix cores are busy for 38 % of it, VALU issue for 52 %); why two waves on a SIMD
+// overlap them so little is not known. 64 heads, 16384 tokens, 64 channels:
 // 118 us forward (4.5 TB/s), 330 for the three gradients (1.4 GB, 4.2 TB/s): HBM. P and S in one piece instead of two
-// would take 365 instead of 418 us at the former and 2 % off the latter, for outputs 1.4 times as far off.
+// took 365 instead of 418 us at the former and 2 % off the latter, for outputs 1.4 times as far off. In three bf16 pieces
+// instead of two they take 455 instead of 401 us (whole call), and the latter's training step 709 instead of 652: outputs and gradients are as far
+// off in 64 bits' eyes (1.7e-3, bf16's own rounding) and differ from plain fp32 arithmetic rounded to bf16 by 6e-5 in place of 1e-4 of their norm (what
+// is off by 2^-17 rounds the other way now and then). Two are kept.
 #pragma once
 
 #include "attn_common.h"

@@ -91,7 +91,7 @@ __device__ __forceinline__ float small_expm1(float x) {
 
 // One token: S <- a S + k v^T in place, out = scale S^T q. Slow heads take it as S + ((a - 1) S + k v^T): an a that is rounded to 32 bits is
 // off by the same 2^-25 at every token, which over the 1 / (1 - a) tokens that the state holds adds up to up to 2e-5 of it at a = 1 - 2^-10,
-// where the roundings themselves come to 8e-7; a - 1 is off by 2^-24 of itself. (Fast heads would cancel S in it.) Memory-bound by the state, read and written once:
+// where the roundings themselves come to 6e-7; a - 1 is off by 2^-24 of itself. (Fast heads would cancel S in it.) Memory-bound by the state, read and written once:
 // a workgroup takes 32 value columns of a head's state, a thread four of them (16 bytes) in every 32nd row,
 // all of its rows in flight at once; the rows' shares of out are added in a fixed order. 2048 states of 128 x 128: 56 us,
 // 4.8 TB/s (one that the last level of cache still holds half of: 42); four of 32 x 32: 3.0.
@@ -175,11 +175,14 @@ int load_mode(const void* p, const int64_t* strides, int64_t d, int64_t size) {
 
 // Into how many segments the sequences of `runs` (runs of the operator times sequences times heads) are cut, and
 // how their states are found: the least of what the busiest SIMD takes. A wave alone takes tf us for a tile (one
-// launch of 4 tiles against one of 1, one head: bf16 1.2 and 2.1 at 32 and 128 key channels, fp16 1.6 and 2.5, fp32
-// 2.8 and 7.4), ts for its state alone (one launch of 15 tiles in 15 segments: bf16 0.8 to 1.1, fp32 0.9 to 1.5), and
-// 3 us to begin. A SIMD holds two waves, which take one and a half times as long together (fp32, whose products
+// segment of 15 tiles against one of 1, one head, 32 and 128 key channels: bf16 1.3 and 2.2, fp16 1.5 and 2.45, fp32 3.1 and
+// 8.1), ts for its state alone (15 tiles in 15 segments: bf16 0.74 and 1.1, fp16 0.76 and 1.15, fp32 1.3 and 3.3), and
+// 3 us to begin; the constants below are within a tenth of those, but for fp32's (tf a tenth, ts a quarter less, of kernels before
+// they lost their reads ahead). A SIMD holds two waves, which take one and a half times as long together (fp32, whose products
 // fill it alone, 1.9). Segments joined in launches of their own cost two more, 10 us, and four passes
-// over their states at 4 TB/s.
+// over their states at 4 TB/s; the join's chain is not in it. At most 64 segments, which bounds the workspace and that chain: 256
+// would be faster for few heads and very long sequences (one head, 131072 tokens, 128 channels, bf16: 243 us against 122, fp32 764 against 255; four,
+// 64 channels: 185 against 131) and in fp32 (one head, 32768 tokens, 64 channels: 133 against 87), not for that head in bf16 (66 against 72).
 void plan_segments(int dtype, DecayArgs& a, int64_t runs, int dk, int dv) {
   const bool f32 = dtype == LFAMD_F32;
   const int64_t tiles = ((int64_t)a.N + kDecayTile - 1) / kDecayTile;
